@@ -86,7 +86,8 @@ const char* varq_last_error(void);
 uint64_t varq_launch_count(void);
 
 /* Every wait inside the kernels is bounded; a wait that expires makes the kernel record a
- * non-zero code and drain instead of hanging.  This call waits for all prior work of the current
+ * non-zero code and drain instead of hanging; numbers on the device that lie outside their bounds (varq_paged_batch_t)
+ * leave one, too.  This call waits for all prior work of the current
  * device (cudaDeviceSynchronize), returns the first such code since the last call (0 = none) and
  * clears it.  HOST pointer.  No counterpart in the reference. */
 int varq_device_status(int32_t* status);
@@ -257,6 +258,55 @@ int varq_attn_fwd_qnorm(const varq_tensor_t* q, const varq_tensor_t* k_codes, co
                         int32_t B, int32_t H, int32_t Lq, int32_t Lk, int32_t D,
                         int32_t k_store_bits, int32_t v_store_bits, float softmax_scale, const float* q_mul, float q_eps,
                         const varq_tensor_t* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- paged caches
+ * The quantized K and V of many sequences of different lengths in one pool of pages, for serving.  No counterpart in the
+ * reference, whose caches hold one batch of equally long samples (VAR_Q/quant.py:180-205); quantization is its
+ * symmetric per-token-per-head mode (VAR_Q/quant.py:92-95, 112-121) with each token's own scale.
+ *   k_codes / v_codes : int32 [n_pages][n_heads][page_size][head_dim * bits / 32], packed as everywhere in this library
+ *   k_scale / v_scale : fp32  [n_pages][n_heads][page_size]; value = code * scale
+ * all contiguous and 16-byte aligned.  page_size: a power of two from 16 to 1024; head_dim 64 or 128; bits 2, 4 or 8 for K and V each.
+ * A slot is page * page_size + offset.  What is not written may hold anything: nothing reads it. */
+typedef struct {
+    int32_t *k_codes, *v_codes;
+    float *k_scale, *v_scale;
+    int32_t n_pages, page_size, n_heads, head_dim, k_bits, v_bits;
+} varq_paged_t;
+
+/* Quantize n_tokens rows per head of k and v, descriptors (1, n_tokens, n_heads, head_dim) of one type, into their slots:
+ *   scale = max(amax|x| / (2^(bits-1) - 1), eps), code = rint(x / scale), fp32, true division, half to even.
+ * A negative slot, or one behind the pool, writes nothing (padding tokens).  Slots must differ.  A row that holds a NaN or an infinity is
+ * stored with a NaN scale, so that it reads as NaN throughout. */
+int varq_paged_append(const varq_paged_t* cache, const varq_tensor_t* k, const varq_tensor_t* v, const int64_t* slots, int64_t n_tokens,
+                      float eps, void* stream);
+
+/* k_out, v_out (1, n_tokens, n_heads, head_dim), fp32, fp16 or bf16, both of one type: code * scale of every slot, zeros for a
+ * negative slot or one behind the pool. */
+int varq_paged_read(const varq_paged_t* cache, const int64_t* slots, int64_t n_tokens, const varq_tensor_t* k_out, const varq_tensor_t* v_out,
+                    void* stream);
+
+/* The queries of a batch and where their sequences lie.  Sequence b has kv_lens[b] tokens in the cache, token i of them in page
+ * block_table[b * table_stride + i / page_size]; its queries are rows q_starts[b] .. q_starts[b + 1] - 1 (q_starts[0] = 0, n_seqs + 1
+ * entries), and they are the sequence's last tokens: query i of n stands at position kv_lens[b] - n + i.
+ *   causal = 0 : every query sees the whole sequence
+ *   causal = 1 : a query at position p sees the keys 0 .. p; with window w > 0 the keys p - w + 1 .. p and the first `sinks` keys
+ * Query head i uses head i / (q_heads / n_heads) of the cache.  max_q bounds the queries of a sequence, max_kv is the longest kv_lens (a
+ * hint: it decides how the work is split).
+ * The device checks what the host cannot see: starts, lengths and page numbers outside their bounds are clamped into them and leave a
+ * code (64, 65, 66) for varq_device_status. */
+typedef struct {
+    const int32_t *q_starts, *kv_lens, *block_table;
+    int64_t table_stride, n_queries;
+    int32_t table_pages, n_seqs, q_heads, max_q, max_kv, causal, window, sinks;
+    float softmax_scale;
+} varq_paged_batch_t;
+
+/* out = softmax(q k^T * softmax_scale) v over the pages; q and out (1, n_queries, q_heads, head_dim), fp16 or bf16 (one type).  lse (or
+ * NULL): fp32 [n_queries][q_heads], log of the sum of exponentials.  A query that sees no key gets zeros and -inf.
+ * What a query does not see does not reach its result, whatever it holds. */
+size_t varq_paged_attn_workspace_bytes(const varq_paged_t* cache, const varq_paged_batch_t* batch);
+int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch_t* batch, const varq_tensor_t* q, const varq_tensor_t* out, float* lse,
+                    void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -23,6 +23,7 @@ SYMBOLS = (
     "varq_quant_static_scratch_bytes", "varq_unpack_dequant",
     "varq_attn_workspace_bytes", "varq_attn_fwd", "varq_attn_force_path",
     "varq_qk_norm_stats", "varq_quant_pack_prestats", "varq_attn_fwd_qnorm", "varq_append", "varq_append_workspace_bytes",
+    "varq_paged_append", "varq_paged_read", "varq_paged_attn", "varq_paged_attn_workspace_bytes",
 )
 
 
@@ -44,6 +45,20 @@ class AppendJob(ctypes.Structure):
     _fields_ = [("x", Tensor), ("bits", ctypes.c_int32), ("store_bits", ctypes.c_int32), ("eps", ctypes.c_float),
                 ("token0", ctypes.c_int32), ("row0", ctypes.c_int32), ("_pad", ctypes.c_int32), ("codes", Tensor), ("p", QParams),
                 ("row_of_token", ctypes.c_void_p), ("row_begin", ctypes.c_void_p)]
+
+
+class Paged(ctypes.Structure):
+    _fields_ = [("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("n_pages", ctypes.c_int32), ("page_size", ctypes.c_int32), ("n_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("k_bits", ctypes.c_int32), ("v_bits", ctypes.c_int32)]
+
+
+class PagedBatch(ctypes.Structure):
+    _fields_ = [("q_starts", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p), ("block_table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64), ("n_queries", ctypes.c_int64),
+                ("table_pages", ctypes.c_int32), ("n_seqs", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("max_q", ctypes.c_int32),
+                ("max_kv", ctypes.c_int32), ("causal", ctypes.c_int32), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32),
+                ("softmax_scale", ctypes.c_float)]
 
 
 _lib = None
@@ -91,6 +106,15 @@ def _declare(lib):
     lib.varq_append.argtypes = [ctypes.POINTER(AppendJob), i32, i32, i32, i32, i32, f32, vp, sz, vp]
     lib.varq_attn_fwd_qnorm.restype = i32
     lib.varq_attn_fwd_qnorm.argtypes = [T, T, T, Q, Q, i32, i32, i32, i32, i32, i32, i32, f32, vp, f32, T, vp, sz, vp]
+    P, B = ctypes.POINTER(Paged), ctypes.POINTER(PagedBatch)
+    lib.varq_paged_append.restype = i32
+    lib.varq_paged_append.argtypes = [P, T, T, vp, i64, f32, vp]
+    lib.varq_paged_read.restype = i32
+    lib.varq_paged_read.argtypes = [P, vp, i64, T, T, vp]
+    lib.varq_paged_attn_workspace_bytes.restype = sz
+    lib.varq_paged_attn_workspace_bytes.argtypes = [P, B]
+    lib.varq_paged_attn.restype = i32
+    lib.varq_paged_attn.argtypes = [P, B, T, T, vp, vp, sz, vp]
     return lib
 
 

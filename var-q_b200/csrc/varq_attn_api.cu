@@ -1,5 +1,6 @@
 // C entry points of attention over the packed cache: argument checks and kernel selection.
 #include "varq_attn.cuh"
+#include "varq_paged.cuh"
 
 using namespace varq;
 
@@ -155,6 +156,7 @@ extern "C" int varq_device_status(int32_t* status) {
     if (!status) return fail(VARQ_ERR_ARG, "varq_device_status: null pointer");
     int v = 0;
     if (int rc = attn_tc_status(&v)) return rc;
+    if (int rc = paged_status(&v)) return rc;
     *status = v;
     return VARQ_OK;
 }

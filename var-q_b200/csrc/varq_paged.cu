@@ -1,0 +1,342 @@
+// Writing tokens into a paged cache and reading them back.
+//
+// Append: a row (token, head) of K or V becomes D codes and one scale,
+//   scale = max(amax|x| / (2^(bits-1) - 1), eps),   code = rint(x / scale) to even,
+// with the bits of a true fp32 division.  Eight values per lane, 8 or 16 lanes per row, the row read once and held in registers.  Rounding
+// without a division per value: y = x * (1 / scale) is within 2^-22 |y| of the quotient and |y| <= 127.5, so rint(y) is the code unless y lies
+// within 2^-14 of a half; a lane that holds such a value divides its eight.  A row with a NaN or an infinity has a NaN scale and zero codes:
+// whoever reads it gets NaN, as from arithmetic on the values themselves, and whoever does not see it loses nothing.
+// Read: code * scale, converted to the output's type once.
+#include "varq_attn.cuh"
+#include "varq_paged.cuh"
+#include "varq_quant.cuh"
+
+namespace varq {
+namespace {
+
+struct AppendArgs {
+    PagedView c;
+    const void *k, *v;
+    long long ks_t, ks_h, vs_t, vs_h;
+    const long long* slots;
+    uint32_t rows;                     // tokens x heads
+    FastDiv heads;
+    float eps;
+};
+struct ReadArgs {
+    PagedView c;
+    void *k, *v;
+    long long ks_t, ks_h, vs_t, vs_h;
+    const long long* slots;
+    uint32_t rows;
+    FastDiv heads;
+};
+
+constexpr int ROW_THREADS = 256;
+
+// codes of eight values in the low bytes' order of a row: 64, 32 or 16 bits
+__device__ __forceinline__ void store_codes(int32_t* pool, long long word0, int lane, int bits, const int (&q)[8]) {
+    if (bits == 8) {
+        uint32_t w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            w[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040), 0x5410);
+        *reinterpret_cast<uint2*>(pool + word0 + 2 * lane) = make_uint2(w[0], w[1]);
+    } else if (bits == 4) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w |= (uint32_t)(q[i] & 15) << (4 * i);
+        pool[word0 + lane] = (int32_t)w;
+    } else {
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w |= (uint32_t)(q[i] & 3) << (2 * i);
+        reinterpret_cast<unsigned short*>(pool + word0)[lane] = (unsigned short)w;
+    }
+}
+__device__ __forceinline__ void load_codes(const int32_t* pool, long long word0, int lane, int bits, uint32_t (&w)[2]) {
+    if (bits == 8) {
+        const uint2 x = __ldg(reinterpret_cast<const uint2*>(pool + word0 + 2 * lane));
+        w[0] = x.x; w[1] = x.y;
+    } else {
+        w[0] = bits == 4 ? (uint32_t)__ldg(pool + word0 + lane) : __ldg(reinterpret_cast<const unsigned short*>(pool + word0) + lane);
+        w[1] = 0;
+    }
+}
+// signed fields -> fp32: 0x4B000000 | u is 2^23 + u
+__device__ __forceinline__ void codes_to_float(const uint32_t (&w)[2], int bits, float (&f)[8]) {
+    if (bits == 8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(__byte_perm(w[i >> 2] ^ 0x80808080u, 0x4B000000u, 0x7540 | (i & 3))) - 8388736.f;
+    } else {
+        const uint32_t flip = bits == 4 ? 0x88888888u : 0xAAAAu, mask = (1u << bits) - 1u;
+        const float base = 8388608.f + (float)(1 << (bits - 1));
+        const uint32_t u = w[0] ^ flip;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(((u >> (bits * i)) & mask) | 0x4B000000u) - base;
+    }
+}
+
+template <typename T, int D, int U, bool VEC>
+__global__ void __launch_bounds__(ROW_THREADS) paged_append_kernel(AppendArgs a) {
+    constexpr int LPR = D / 8, RPB = ROW_THREADS / LPR;
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & (LPR - 1), page_mask = (1 << a.c.page_shift) - 1;
+    const bool is_v = blockIdx.y != 0;
+    const T* x = reinterpret_cast<const T*>(is_v ? a.v : a.k);
+    const long long st = is_v ? a.vs_t : a.ks_t, sh = is_v ? a.vs_h : a.ks_h;
+    const int bits = is_v ? a.c.vb : a.c.kb, words = D * bits / 32;
+    int32_t* pool = is_v ? a.c.vc : a.c.kc;
+    float* scales = is_v ? a.c.vs : a.c.ks;
+    const long long n_slots = (long long)a.c.n_pages << a.c.page_shift;
+    const float top = (float)((1 << (bits - 1)) - 1);
+    const uint32_t row0 = blockIdx.x * (RPB * U) + threadIdx.x / LPR;
+    float f[U][8];
+    long long at[U];                   // row of the pools, negative: not written
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t row = row0 + u * RPB;
+        at[u] = -1;
+        if (row < a.rows) {
+            const uint32_t t = a.heads.div(row), h = row - t * a.heads.d;
+            const long long slot = __ldg(a.slots + t);
+            if (slot >= 0 && slot < n_slots) {
+                at[u] = (((slot >> a.c.page_shift) * a.c.H + h) << a.c.page_shift) + (slot & page_mask);
+                const T* p = x + t * st + h * sh + lane * 8;
+                if constexpr (VEC) { Vec8<T> r; r.load(p); r.get(f[u]); }
+                else load_vals<T, 8, false>(p, f[u], 8);
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        uint32_t hi = 0;               // order of the absolute values, NaN above infinity
+        if (at[u] >= 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) hi = max(hi, __float_as_uint(f[u][i]) & 0x7fffffffu);
+        }
+#pragma unroll
+        for (int z = LPR / 2; z; z >>= 1) hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, z));
+        if (at[u] < 0) continue;
+        int q[8];
+        float scale;
+        if (hi >= 0x7f800000u) {
+            scale = __uint_as_float(0x7fffffffu);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[i] = 0;
+        } else {
+            scale = fmaxf(__fdiv_rn(__uint_as_float(hi), top), a.eps);
+            const float r = __frcp_rn(scale);
+            float far = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float y = f[u][i] * r, z = y + Q_MAGIC;
+                q[i] = (int)__float_as_uint(z);                          // the integer in the low bits, sign included
+                far = fmaxf(far, fabsf(y - (z - Q_MAGIC)));
+            }
+            if (far > 0.5f - 1.f / 16384.f) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) q[i] = (int)__float_as_uint(rintf(__fdiv_rn(f[u][i], scale)) + Q_MAGIC);
+            }
+        }
+        store_codes(pool, at[u] * words, lane, bits, q);
+        if (lane == 0) scales[at[u]] = scale;
+    }
+}
+
+template <typename T, int D, int U, bool VEC>
+__global__ void __launch_bounds__(ROW_THREADS) paged_read_kernel(ReadArgs a) {
+    constexpr int LPR = D / 8, RPB = ROW_THREADS / LPR;
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & (LPR - 1), page_mask = (1 << a.c.page_shift) - 1;
+    const bool is_v = blockIdx.y != 0;
+    T* out = reinterpret_cast<T*>(is_v ? a.v : a.k);
+    const long long st = is_v ? a.vs_t : a.ks_t, sh = is_v ? a.vs_h : a.ks_h;
+    const int bits = is_v ? a.c.vb : a.c.kb, words = D * bits / 32;
+    const int32_t* pool = is_v ? a.c.vc : a.c.kc;
+    const float* scales = is_v ? a.c.vs : a.c.ks;
+    const long long n_slots = (long long)a.c.n_pages << a.c.page_shift;
+    const uint32_t row0 = blockIdx.x * (RPB * U) + threadIdx.x / LPR;
+    if (!out) return;
+    uint32_t w[U][2], t[U], h[U];
+    float s[U];
+    bool there[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t row = min(row0 + u * RPB, a.rows - 1);
+        t[u] = a.heads.div(row); h[u] = row - t[u] * a.heads.d;
+        const long long slot = __ldg(a.slots + t[u]);
+        there[u] = slot >= 0 && slot < n_slots;
+        w[u][0] = w[u][1] = 0; s[u] = 0.f;
+        if (there[u]) {
+            const long long at = (((slot >> a.c.page_shift) * a.c.H + h[u]) << a.c.page_shift) + (slot & page_mask);
+            load_codes(pool, at * words, lane, bits, w[u]);
+            s[u] = __ldg(scales + at);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (row0 + u * RPB >= a.rows) break;
+        float f[8];
+        codes_to_float(w[u], bits, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = there[u] ? f[i] * s[u] : 0.f;
+        store_vals<T, 8, VEC>(out + t[u] * st + h[u] * sh + lane * 8, f, 8);
+    }
+}
+
+bool rows_aligned16(const void* p, long long st, long long sh, int es) {
+    return aligned16(p) && (st * es) % 16 == 0 && (sh * es) % 16 == 0;
+}
+
+int check_cache(const char* who, const varq_paged_t* c, PagedView& v) {
+    if (!c) return fail(VARQ_ERR_ARG, "%s: null cache", who);
+    if (c->n_pages < 1 || c->n_heads < 1) return fail(VARQ_ERR_ARG, "%s: %d pages, %d heads", who, c->n_pages, c->n_heads);
+    if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)))
+        return fail(VARQ_ERR_ARG, "%s: a page holds 16, 32, ... 1024 tokens (got %d)", who, c->page_size);
+    if (c->head_dim != 64 && c->head_dim != 128) return fail(VARQ_ERR_UNSUPPORTED, "%s: head_dim %d is not 64 or 128", who, c->head_dim);
+    if ((c->k_bits != 2 && c->k_bits != 4 && c->k_bits != 8) || (c->v_bits != 2 && c->v_bits != 4 && c->v_bits != 8))
+        return fail(VARQ_ERR_ARG, "%s: bits must be 2, 4 or 8 (got %d, %d)", who, c->k_bits, c->v_bits);
+    if (!c->k_codes || !c->v_codes || !c->k_scale || !c->v_scale) return fail(VARQ_ERR_ARG, "%s: null pool", who);
+    if (!aligned16(c->k_codes) || !aligned16(c->v_codes) || !aligned16(c->k_scale) || !aligned16(c->v_scale)) return fail(VARQ_ERR_ARG, "%s: pools must start on a 16-byte boundary", who);
+    v.kc = c->k_codes; v.vc = c->v_codes; v.ks = c->k_scale; v.vs = c->v_scale;
+    v.n_pages = c->n_pages; v.page_shift = 0;
+    while ((1 << v.page_shift) < c->page_size) ++v.page_shift;
+    v.H = c->n_heads; v.D = c->head_dim; v.kb = c->k_bits; v.vb = c->v_bits;
+    return VARQ_OK;
+}
+int check_rows(const char* who, const PagedView& c, long long n) {
+    if (n < 0) return fail(VARQ_ERR_ARG, "%s: %lld tokens", who, n);
+    if (n * c.H >= 0x7fffffffLL) return fail(VARQ_ERR_UNSUPPORTED, "%s: %lld tokens of %d heads are 2^31 rows or more", who, n, c.H);
+    return VARQ_OK;
+}
+
+// Rows per thread: four keep enough bytes in flight for a long call (32768 tokens of 8 heads), one spreads a short call over the SMs
+template <typename A, typename K1, typename K4>
+int launch_rows(K1 one, K4 four, const A& a, int D, cudaStream_t st) {
+    const uint32_t rpb = ROW_THREADS / (D / 8);
+    if (a.rows >= 4ull * rpb * sm_count() * 4) VARQ_CUDA_TRY(launch_pdl(four, dim3((a.rows + 4 * rpb - 1) / (4 * rpb), 2), ROW_THREADS, 0, st, 1, a));
+    else VARQ_CUDA_TRY(launch_pdl(one, dim3((a.rows + rpb - 1) / rpb, 2), ROW_THREADS, 0, st, 1, a));
+    count_launches(1);
+    return VARQ_OK;
+}
+template <typename T> int run_append(const AppendArgs& a, bool vec, cudaStream_t st) {
+    if (a.c.D == 64) return vec ? launch_rows(paged_append_kernel<T, 64, 1, true>, paged_append_kernel<T, 64, 4, true>, a, 64, st)
+                                : launch_rows(paged_append_kernel<T, 64, 1, false>, paged_append_kernel<T, 64, 4, false>, a, 64, st);
+    return vec ? launch_rows(paged_append_kernel<T, 128, 1, true>, paged_append_kernel<T, 128, 4, true>, a, 128, st)
+               : launch_rows(paged_append_kernel<T, 128, 1, false>, paged_append_kernel<T, 128, 4, false>, a, 128, st);
+}
+template <typename T> int run_read(const ReadArgs& a, bool vec, cudaStream_t st) {
+    if (a.c.D == 64) return vec ? launch_rows(paged_read_kernel<T, 64, 1, true>, paged_read_kernel<T, 64, 4, true>, a, 64, st)
+                                : launch_rows(paged_read_kernel<T, 64, 1, false>, paged_read_kernel<T, 64, 4, false>, a, 64, st);
+    return vec ? launch_rows(paged_read_kernel<T, 128, 1, true>, paged_read_kernel<T, 128, 4, true>, a, 128, st)
+               : launch_rows(paged_read_kernel<T, 128, 1, false>, paged_read_kernel<T, 128, 4, false>, a, 128, st);
+}
+
+__device__ int g_paged_status = 0;
+
+}  // namespace
+
+int* paged_status_word() {
+    void* p = nullptr;
+    if (cudaGetSymbolAddress(&p, g_paged_status) != cudaSuccess) return nullptr;
+    return reinterpret_cast<int*>(p);
+}
+int paged_status(int* out) {
+    int v = 0;
+    VARQ_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_paged_status, sizeof(int)));
+    if (v != 0) {
+        const int zero = 0;
+        VARQ_CUDA_TRY(cudaMemcpyToSymbol(g_paged_status, &zero, sizeof(int)));
+    }
+    if (*out == 0) *out = v;
+    return VARQ_OK;
+}
+
+}  // namespace varq
+
+using namespace varq;
+
+extern "C" int varq_paged_append(const varq_paged_t* cache, const varq_tensor_t* k, const varq_tensor_t* v, const int64_t* slots, int64_t n_tokens,
+                                 float eps, void* stream) {
+    AppendArgs a;
+    if (int rc = check_cache("varq_paged_append", cache, a.c)) return rc;
+    if (int rc = check_rows("varq_paged_append", a.c, n_tokens)) return rc;
+    if (!k || !v) return fail(VARQ_ERR_ARG, "varq_paged_append: null descriptor");
+    if (!dtype_ok(k->dtype) || k->dtype != v->dtype) return fail(VARQ_ERR_ARG, "varq_paged_append: K and V must have one type, fp32, fp16 or bf16");
+    if (!(eps >= 1e-30f && eps < 1e30f)) return fail(VARQ_ERR_ARG, "varq_paged_append: eps must lie in [1e-30, 1e30)");
+    if (n_tokens == 0) return VARQ_OK;
+    if (!k->ptr || !v->ptr || !slots) return fail(VARQ_ERR_ARG, "varq_paged_append: null pointer");
+    const int es = dtype_size(k->dtype);
+    if ((uintptr_t)k->ptr % es || (uintptr_t)v->ptr % es || (uintptr_t)slots % 8) return fail(VARQ_ERR_ARG, "varq_paged_append: misaligned pointer");
+    a.k = k->ptr; a.v = v->ptr;
+    a.ks_t = k->stride_l; a.ks_h = k->stride_h; a.vs_t = v->stride_l; a.vs_h = v->stride_h;
+    a.slots = reinterpret_cast<const long long*>(slots);
+    a.rows = (uint32_t)(n_tokens * a.c.H);
+    a.heads = FastDiv((uint32_t)a.c.H);
+    a.eps = eps;
+    const bool vec = rows_aligned16(k->ptr, a.ks_t, a.ks_h, es) && rows_aligned16(v->ptr, a.vs_t, a.vs_h, es);
+    const cudaStream_t st = (cudaStream_t)stream;
+    return k->dtype == VARQ_F32 ? run_append<float>(a, vec, st) : k->dtype == VARQ_F16 ? run_append<__half>(a, vec, st) : run_append<__nv_bfloat16>(a, vec, st);
+}
+
+extern "C" int varq_paged_read(const varq_paged_t* cache, const int64_t* slots, int64_t n_tokens, const varq_tensor_t* k_out,
+                               const varq_tensor_t* v_out, void* stream) {
+    ReadArgs a;
+    if (int rc = check_cache("varq_paged_read", cache, a.c)) return rc;
+    if (int rc = check_rows("varq_paged_read", a.c, n_tokens)) return rc;
+    if (!k_out || !v_out) return fail(VARQ_ERR_ARG, "varq_paged_read: null descriptor");
+    if (!dtype_ok(k_out->dtype) || k_out->dtype != v_out->dtype) return fail(VARQ_ERR_ARG, "varq_paged_read: K and V must have one type, fp32, fp16 or bf16");
+    if (n_tokens == 0) return VARQ_OK;
+    if (!k_out->ptr || !v_out->ptr || !slots) return fail(VARQ_ERR_ARG, "varq_paged_read: null pointer");
+    const int es = dtype_size(k_out->dtype);
+    if ((uintptr_t)k_out->ptr % es || (uintptr_t)v_out->ptr % es || (uintptr_t)slots % 8) return fail(VARQ_ERR_ARG, "varq_paged_read: misaligned pointer");
+    a.k = k_out->ptr; a.v = v_out->ptr;
+    a.ks_t = k_out->stride_l; a.ks_h = k_out->stride_h; a.vs_t = v_out->stride_l; a.vs_h = v_out->stride_h;
+    a.slots = reinterpret_cast<const long long*>(slots);
+    a.rows = (uint32_t)(n_tokens * a.c.H);
+    a.heads = FastDiv((uint32_t)a.c.H);
+    const bool vec = rows_aligned16(a.k, a.ks_t, a.ks_h, es) && rows_aligned16(a.v, a.vs_t, a.vs_h, es);
+    const cudaStream_t st = (cudaStream_t)stream;
+    return k_out->dtype == VARQ_F32 ? run_read<float>(a, vec, st) : k_out->dtype == VARQ_F16 ? run_read<__half>(a, vec, st) : run_read<__nv_bfloat16>(a, vec, st);
+}
+
+extern "C" size_t varq_paged_attn_workspace_bytes(const varq_paged_t* cache, const varq_paged_batch_t* batch) {
+    (void)cache; (void)batch;
+    return 0;
+}
+
+extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch_t* batch, const varq_tensor_t* q, const varq_tensor_t* out, float* lse,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+    PagedAttnArgs a;
+    (void)workspace; (void)workspace_bytes;
+    if (int rc = check_cache("varq_paged_attn", cache, a.c)) return rc;
+    if (!batch || !q || !out) return fail(VARQ_ERR_ARG, "varq_paged_attn: null descriptor");
+    if (batch->n_seqs < 0 || batch->n_queries < 0 || batch->max_q < 0 || batch->max_kv < 0 || batch->table_pages < 0)
+        return fail(VARQ_ERR_ARG, "varq_paged_attn: negative size");
+    if (batch->q_heads < 1 || batch->q_heads % a.c.H) return fail(VARQ_ERR_ARG, "varq_paged_attn: %d query heads over %d heads of the cache", batch->q_heads, a.c.H);
+    if ((q->dtype != VARQ_F16 && q->dtype != VARQ_BF16) || out->dtype != q->dtype)
+        return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_attn: queries and outputs are fp16 or bf16, both of one type");
+    if (batch->window < 0 || batch->sinks < 0) return fail(VARQ_ERR_ARG, "varq_paged_attn: window %d, sinks %d", batch->window, batch->sinks);
+    if (batch->window && !batch->causal) return fail(VARQ_ERR_ARG, "varq_paged_attn: a window needs causal attention");
+    if (batch->sinks && !batch->window) return fail(VARQ_ERR_ARG, "varq_paged_attn: sinks need a window");
+    if (!(batch->softmax_scale > 0.f && batch->softmax_scale < 1e30f)) return fail(VARQ_ERR_ARG, "varq_paged_attn: softmax_scale must be positive and finite");
+    if (batch->n_seqs > 65535) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_attn: %d sequences (65535 at most)", batch->n_seqs);
+    if (batch->n_queries >= (1ll << 31)) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_attn: 2^31 query tokens or more");
+    if (batch->n_queries == 0 || batch->n_seqs == 0 || batch->max_q == 0) return VARQ_OK;
+    if (!q->ptr || !out->ptr || !batch->q_starts || !batch->kv_lens || (batch->table_pages && !batch->block_table)) return fail(VARQ_ERR_ARG, "varq_paged_attn: null pointer");
+    if (((uintptr_t)q->ptr | (uintptr_t)out->ptr) % 2 || ((uintptr_t)batch->q_starts | (uintptr_t)batch->kv_lens | (uintptr_t)batch->block_table | (uintptr_t)lse) % 4)
+        return fail(VARQ_ERR_ARG, "varq_paged_attn: misaligned pointer");
+    a.q = q->ptr; a.dtype = q->dtype; a.qs_t = q->stride_l; a.qs_h = q->stride_h;
+    a.out = out->ptr; a.os_t = out->stride_l; a.os_h = out->stride_h;
+    a.lse = lse;
+    a.q_starts = batch->q_starts; a.kv_lens = batch->kv_lens; a.table = batch->block_table;
+    a.table_stride = batch->table_stride; a.table_pages = batch->table_pages;
+    a.B = batch->n_seqs; a.T = (int)batch->n_queries; a.Hq = batch->q_heads; a.G = a.Hq / a.c.H;
+    a.max_q = (int)(batch->max_q < batch->n_queries ? batch->max_q : batch->n_queries); a.max_kv = batch->max_kv;
+    a.scale_log2 = batch->softmax_scale * 1.4426950408889634f;
+    a.causal = batch->causal != 0; a.window = batch->window; a.sinks = batch->sinks;
+    return paged_attn_simple_run(a, (cudaStream_t)stream);
+}

@@ -1,0 +1,73 @@
+// What the kernels over a paged cache share: where a token's codes lie, what a sequence holds, which keys a query sees.
+#pragma once
+#include "varq_common.cuh"
+
+namespace varq {
+
+// Division of numbers below 2^31 by one that is fixed for a launch: multiply by ceil(2^(32 + s) / d) - 2^32, add, shift (Granlund and
+// Montgomery, "Division by invariant integers using multiplication").
+struct FastDiv {
+    uint32_t d, m, s;
+    explicit FastDiv(uint32_t d_ = 1) : d(d_), s(0) {
+        while ((1ull << s) < d) ++s;
+        m = (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1);
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return (uint32_t)(((unsigned long long)__umulhi(n, m) + n) >> s); }
+};
+
+// The pools: codes [page][head][offset][words of a row], scales [page][head][offset]
+struct PagedView {
+    int32_t *kc, *vc;
+    float *ks, *vs;
+    int n_pages, page_shift, H, D, kb, vb;
+};
+
+struct PagedAttnArgs {
+    PagedView c;
+    const void* q; int dtype; long long qs_t, qs_h;
+    void* out; long long os_t, os_h;
+    float* lse;                        // [T][Hq] or null
+    const int32_t *q_starts, *kv_lens, *table;
+    long long table_stride; int table_pages;
+    int B, T, Hq, G;                   // sequences, query tokens of all of them, query heads, query heads per head of the cache
+    int max_q, max_kv;
+    float scale_log2;                  // softmax_scale * log2(e)
+    int causal, window, sinks;         // window 0: none
+};
+
+// First thing that was wrong with numbers that only the device sees (lengths, starts, page numbers): the access is clamped into the
+// tensors' bounds and the code is kept for varq_device_status.
+enum PagedStatus : int { PAGED_BAD_STARTS = 64, PAGED_BAD_LENGTH = 65, PAGED_BAD_PAGE = 66 };
+int* paged_status_word();              // its device address; null if it cannot be had
+int paged_status(int* out);            // its value where *out is 0; clears it
+
+// Sequence b: its first query token, number of queries, tokens in the cache
+struct PagedSeq { int q0, nq, kv; };
+__device__ __forceinline__ PagedSeq paged_seq(const PagedAttnArgs& a, int b, int* status) {
+    const int s0 = __ldg(a.q_starts + b), s1 = __ldg(a.q_starts + b + 1), kv = __ldg(a.kv_lens + b);
+    PagedSeq s;
+    s.q0 = min(max(s0, 0), a.T);
+    s.nq = min(min(max(s1, s.q0), a.T) - s.q0, a.max_q);
+    s.kv = (int)min((long long)max(kv, 0), (long long)a.table_pages << a.c.page_shift);
+    if (s.q0 != s0 || s.nq != s1 - s0) atomicCAS(status, 0, PAGED_BAD_STARTS);
+    if (s.kv != kv) atomicCAS(status, 0, PAGED_BAD_LENGTH);
+    return s;
+}
+__device__ __forceinline__ int paged_page(const PagedAttnArgs& a, int p, int* status) {
+    if ((unsigned)p < (unsigned)a.c.n_pages) return p;
+    atomicCAS(status, 0, PAGED_BAD_PAGE);
+    return 0;
+}
+
+// Keys that a query at position p sees: [0, min(sinks, hi)) and [lo, hi); none where hi <= 0
+struct PagedSpan { int lo, hi; };
+__device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, int p, int kv) {
+    PagedSpan s;
+    s.hi = a.causal ? min(p + 1, kv) : kv;
+    s.lo = a.window ? max(p - a.window + 1, 0) : 0;
+    return s;
+}
+
+int paged_attn_simple_run(const PagedAttnArgs& a, cudaStream_t st);
+
+}  // namespace varq

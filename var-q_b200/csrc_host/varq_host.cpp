@@ -391,6 +391,151 @@ PyObject* py_dequant(PyObject*, PyObject* const* a, Py_ssize_t n) {
     GUARD_END
 }
 
+// ---------------------------------------------------------------- paged caches
+// The checks of these calls stand here alone: there is no Python form behind them.
+struct Refuse : std::runtime_error { PyObject* type; Refuse(PyObject* t, const std::string& m) : std::runtime_error("[VAR-Q] " + m), type(t) {} };
+#define GUARD_PAGED_END } catch (const Refuse& e) { PyErr_SetString(e.type, e.what()); return nullptr; } \
+    catch (const std::exception& e) { if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what()); return nullptr; }
+void need(bool ok, const char* what) { if (!ok) throw Refuse(PyExc_ValueError, what); }
+const at::Tensor& tensor_arg(PyObject* o, const char* name) {
+    if (!THPVariable_Check(o)) throw Refuse(PyExc_TypeError, std::string(name) + " must be a tensor");
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (!t.is_cuda()) throw Refuse(PyExc_RuntimeError, std::string(name) + " must be a CUDA tensor: this build runs on the GPU only (no CPU fallback exists)");
+    return t;
+}
+const at::Tensor& on_device(const at::Tensor& t, const at::Tensor& like, const char* name) {
+    if (t.device() != like.device()) throw Refuse(PyExc_ValueError, std::string(name) + " is on another device than the cache");
+    return t;
+}
+long long int_arg(PyObject* o, long long lo, long long hi, const char* name) {
+    const long long v = PyLong_AsLongLong(o);
+    if (v == -1 && PyErr_Occurred()) throw std::runtime_error("");
+    if (v < lo || v > hi) throw Refuse(PyExc_ValueError, std::string(name) + " is out of range");
+    return v;
+}
+// a[0..3] the pools, a[4] head_dim
+varq_paged_t paged_desc(PyObject* const* a, const at::Tensor*& kc) {
+    static const char* const names[4] = {"k_codes", "v_codes", "k_scale", "v_scale"};
+    const at::Tensor* t[4];
+    for (int i = 0; i < 4; ++i) {
+        t[i] = &tensor_arg(a[i], names[i]);
+        need(t[i]->is_contiguous() && t[i]->dim() == (i < 2 ? 4 : 3) && t[i]->scalar_type() == (i < 2 ? at::kInt : at::kFloat),
+             "the pools are contiguous int32 codes [pages, heads, page_size, words] and fp32 scales [pages, heads, page_size]");
+        on_device(*t[i], *t[0], names[i]);
+        for (int d = 0; d < 3; ++d) need(t[i]->size(d) == t[0]->size(d) && t[i]->size(d) <= INT32_MAX, "the pools differ in pages, heads or page size");
+    }
+    const long long D = int_arg(a[4], 1, 4096, "head_dim");
+    varq_paged_t c;
+    c.k_codes = t[0]->data_ptr<int32_t>(); c.v_codes = t[1]->data_ptr<int32_t>();
+    c.k_scale = t[2]->data_ptr<float>(); c.v_scale = t[3]->data_ptr<float>();
+    c.n_pages = (int)t[0]->size(0); c.n_heads = (int)t[0]->size(1); c.page_size = (int)t[0]->size(2); c.head_dim = (int)D;
+    c.k_bits = (int)(t[0]->size(3) * 32 / D); c.v_bits = (int)(t[1]->size(3) * 32 / D);
+    need(c.k_bits * D == t[0]->size(3) * 32 && c.v_bits * D == t[1]->size(3) * 32, "words per row do not match head_dim");
+    kc = t[0];
+    return c;
+}
+const int64_t* slots_arg(PyObject* o, const at::Tensor& like, long long& n) {
+    const at::Tensor& s = on_device(tensor_arg(o, "slots"), like, "slots");
+    need(s.dim() == 1 && s.scalar_type() == at::kLong && (s.is_contiguous() || s.numel() == 0), "slots must be a contiguous int64 vector");
+    n = s.size(0);
+    return s.data_ptr<int64_t>();
+}
+// [tokens, heads, head_dim] with any strides in front of a contiguous head_dim
+varq_tensor_t rows_desc(const at::Tensor& x) { return {x.data_ptr(), dtype_code(x.scalar_type()), 0, 0, x.stride(0), x.stride(1)}; }
+PyObject* make_pair(const at::Tensor& a, const at::Tensor& b) {
+    PyObject *x = THPVariable_Wrap(a), *y = x ? THPVariable_Wrap(b) : nullptr;
+    PyObject* r = y ? PyTuple_Pack(2, x, y) : nullptr;
+    Py_XDECREF(x); Py_XDECREF(y);
+    return r;
+}
+// paged_append(k_codes, v_codes, k_scale, v_scale, head_dim, k, v, slots, eps)
+PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    GUARD_BEGIN
+    if (!want(n, 9)) return nullptr;
+    const at::Tensor* kc;
+    const varq_paged_t c = paged_desc(a, kc);
+    const at::Tensor *x[2] = {&on_device(tensor_arg(a[5], "k"), *kc, "k"), &on_device(tensor_arg(a[6], "v"), *kc, "v")};
+    long long tokens;
+    const int64_t* slots = slots_arg(a[7], *kc, tokens);
+    for (const at::Tensor* t : x) {
+        need(t->dim() == 3 && t->size(0) == tokens && t->size(1) == c.n_heads && t->size(2) == c.head_dim, "k and v must be [tokens, heads, head_dim] of the cache, a slot per token");
+        need(t->stride(2) == 1 || t->numel() == 0, "the last dimension of k and v must be contiguous");
+        need(dtype_code(t->scalar_type()) >= 0 && t->scalar_type() == x[0]->scalar_type(), "k and v must have one type: float32, float16 or bfloat16");
+    }
+    const double eps = PyFloat_AsDouble(a[8]);
+    if (PyErr_Occurred()) return nullptr;
+    const c10::DeviceIndex dev = kc->device().index();
+    const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, dev));
+    const varq_tensor_t kd = rows_desc(*x[0]), vd = rows_desc(*x[1]);
+    const int rc = varq_paged_append(&c, &kd, &vd, slots, tokens, (float)eps, c10::cuda::getCurrentCUDAStream(dev).stream());
+    if (rc != VARQ_OK) return raise(rc);
+    Py_RETURN_NONE;
+    GUARD_PAGED_END
+}
+// paged_read(k_codes, v_codes, k_scale, v_scale, head_dim, slots, dtype) -> (k, v)
+PyObject* py_paged_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    GUARD_BEGIN
+    if (!want(n, 7)) return nullptr;
+    const at::Tensor* kc;
+    const varq_paged_t c = paged_desc(a, kc);
+    long long tokens;
+    const int64_t* slots = slots_arg(a[5], *kc, tokens);
+    if (!THPDtype_Check(a[6])) throw Refuse(PyExc_TypeError, "dtype must be a torch.dtype");
+    const at::ScalarType s = reinterpret_cast<THPDtype*>(a[6])->scalar_type;
+    need(dtype_code(s) >= 0, "dtype must be float32, float16 or bfloat16");
+    const c10::DeviceIndex dev = kc->device().index();
+    const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, dev));
+    const at::Tensor k = empty({tokens, c.n_heads, c.head_dim}, s, dev), v = empty({tokens, c.n_heads, c.head_dim}, s, dev);
+    const varq_tensor_t kd = rows_desc(k), vd = rows_desc(v);
+    const int rc = varq_paged_read(&c, slots, tokens, &kd, &vd, c10::cuda::getCurrentCUDAStream(dev).stream());
+    return rc == VARQ_OK ? make_pair(k, v) : raise(rc);
+    GUARD_PAGED_END
+}
+// paged_attend(k_codes, v_codes, k_scale, v_scale, head_dim, q, block_table, kv_lens, q_starts, max_q, max_kv, softmax_scale, causal, window or None, sinks,
+//              return_lse) -> out or (out, lse)
+PyObject* py_paged_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    GUARD_BEGIN
+    if (!want(n, 16)) return nullptr;
+    const at::Tensor* kc;
+    const varq_paged_t c = paged_desc(a, kc);
+    const at::Tensor &q = on_device(tensor_arg(a[5], "q"), *kc, "q"), &table = on_device(tensor_arg(a[6], "block_table"), *kc, "block_table"),
+                     &lens = on_device(tensor_arg(a[7], "kv_lens"), *kc, "kv_lens"), &starts = on_device(tensor_arg(a[8], "q_starts"), *kc, "q_starts");
+    need(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16, "q must be float16 or bfloat16");
+    need(q.dim() == 3 && q.size(2) == c.head_dim && q.size(1) > 0 && q.size(1) <= INT32_MAX, "q must be [tokens, query heads, head_dim] with the cache's head_dim");
+    need(q.stride(2) == 1 || q.numel() == 0, "the last dimension of q must be contiguous");
+    need(lens.dim() == 1 && lens.scalar_type() == at::kInt && lens.is_contiguous(), "kv_lens must be a contiguous int32 vector");
+    need(starts.dim() == 1 && starts.scalar_type() == at::kInt && starts.is_contiguous() && starts.size(0) == lens.size(0) + 1,
+         "q_starts must be a contiguous int32 vector with one entry more than kv_lens");
+    need(table.dim() == 2 && table.scalar_type() == at::kInt && table.size(0) == lens.size(0) && (table.stride(1) == 1 || table.size(1) < 2) && table.size(1) <= INT32_MAX,
+         "block_table must be int32 [sequences, pages] with contiguous rows");
+    varq_paged_batch_t b;
+    b.q_starts = starts.data_ptr<int32_t>(); b.kv_lens = lens.data_ptr<int32_t>(); b.block_table = table.data_ptr<int32_t>();
+    b.table_stride = table.stride(0); b.n_queries = q.size(0); b.table_pages = (int)table.size(1);
+    need(lens.size(0) <= INT32_MAX, "too many sequences");
+    b.n_seqs = (int)lens.size(0); b.q_heads = (int)q.size(1);
+    b.max_q = (int)int_arg(a[9], 0, INT32_MAX, "max_q"); b.max_kv = (int)int_arg(a[10], 0, INT32_MAX, "max_kv");
+    const double scale = PyFloat_AsDouble(a[11]);
+    if (PyErr_Occurred()) return nullptr;
+    b.softmax_scale = (float)scale;
+    const int causal = PyObject_IsTrue(a[12]), with_lse = PyObject_IsTrue(a[15]);
+    if (causal < 0 || with_lse < 0) return nullptr;
+    b.causal = causal;
+    b.window = a[13] == Py_None ? 0 : (int)int_arg(a[13], 1, INT32_MAX, "window");
+    b.sinks = (int)int_arg(a[14], 0, INT32_MAX, "sinks");
+    const c10::DeviceIndex dev = kc->device().index();
+    const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, dev));
+    const at::Tensor out = empty({q.size(0), q.size(1), q.size(2)}, q.scalar_type(), dev);
+    at::Tensor lse;
+    if (with_lse) lse = empty({q.size(0), q.size(1)}, at::kFloat, dev);
+    const varq_tensor_t qd = rows_desc(q), od = rows_desc(out);
+    const size_t ws = varq_paged_attn_workspace_bytes(&c, &b);
+    const at::Tensor buf = scratch(ws, dev);
+    const int rc = varq_paged_attn(&c, &b, &qd, &od, with_lse ? lse.data_ptr<float>() : nullptr, scratch_ptr(buf), ws, c10::cuda::getCurrentCUDAStream(dev).stream());
+    if (rc != VARQ_OK) return raise(rc);
+    return with_lse ? make_pair(out, lse) : THPVariable_Wrap(out);
+    GUARD_PAGED_END
+}
+
 // ---------------------------------------------------------------- attributes
 enum Field : long { F_BITS, F_METHOD, F_PACK, F_SYM, F_REDUCE, F_GROUP, F_MAX, F_DEBUG, F_FMT, F_EPS, F_SHAPE, F_PEND, F_LAST, F_META,
                     F_WORDS, F_NB, F_NH, F_NG, F_LCAP, F_RCAP, F_NTOK, F_NROWS, F_T0 };
@@ -501,6 +646,10 @@ PyMethodDef methods[] = {
     FAST("step_normalised", py_step_normalised, "step_normalised(q, k, v, scale_mul, k_cache, v_cache, scale, out_dtype, eps) -> Tensor or None"),
     FAST("use_var_q", py_use, "use_var_q(cache, item) -> Tensor or None"),
     FAST("dequant", py_dequant, "dequant(cache, which) -> Tensor or None"),
+    FAST("paged_append", py_paged_append, "paged_append(k_codes, v_codes, k_scale, v_scale, head_dim, k, v, slots, eps)"),
+    FAST("paged_read", py_paged_read, "paged_read(k_codes, v_codes, k_scale, v_scale, head_dim, slots, dtype) -> (k, v)"),
+    FAST("paged_attend", py_paged_attend, "paged_attend(k_codes, v_codes, k_scale, v_scale, head_dim, q, block_table, kv_lens, q_starts, max_q, max_kv, "
+         "softmax_scale, causal, window, sinks, return_lse) -> out or (out, lse)"),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Host path of the VAR_Q package.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

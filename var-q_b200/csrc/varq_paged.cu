@@ -245,6 +245,7 @@ int* paged_status_word() {
     return reinterpret_cast<int*>(p);
 }
 int paged_status(int* out) {
+    if (int rc = paged_attn_tc_status(out)) return rc;
     int v = 0;
     VARQ_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_paged_status, sizeof(int)));
     if (v != 0) {
@@ -303,15 +304,48 @@ extern "C" int varq_paged_read(const varq_paged_t* cache, const int64_t* slots, 
     return k_out->dtype == VARQ_F32 ? run_read<float>(a, vec, st) : k_out->dtype == VARQ_F16 ? run_read<__half>(a, vec, st) : run_read<__nv_bfloat16>(a, vec, st);
 }
 
+namespace {
+
+// How a call is shared out
+struct AttnPlan {
+    bool tc;
+    int splits, tiles_per_split;       // tiles of 16 keys (decode kernel)
+};
+AttnPlan plan_attn(int B, int H, int G, int max_q, int max_kv, int window, int sinks) {
+    AttnPlan p;
+    const long long rows = (long long)max_q * G;
+    const long long span = window && (long long)window + max_q + sinks < max_kv ? (long long)window + max_q + sinks : max_kv;      // keys of a CTA, about
+    p.tc = rows > 16;
+    const long long units = p.tc ? 128 : 16, tiles = (span + units - 1) / units > 0 ? (span + units - 1) / units : 1;
+    const long long base = (long long)B * H * (p.tc ? (rows + 255) / 256 : 1), room = (long long)sm_count() * (p.tc ? 1 : 3);
+    // the number of parts that makes the waves of CTAs shortest, a CTA costing its tiles and a fixed part (set-up and merging)
+    const long long fixed = p.tc ? 4 : 16, least = p.tc ? 2 : 16;
+    long long best = 0;
+    p.splits = 1;
+    for (long long s = 1; s == 1 || (s <= tiles / least && s <= 256); ++s) {
+        const long long cost = (base * s + room - 1) / room * ((tiles + s - 1) / s + fixed + (s > 1 ? fixed : 0));
+        if (best == 0 || cost < best) { best = cost; p.splits = (int)s; }
+        if (base * s > 8 * room) break;
+    }
+    p.tiles_per_split = (int)((tiles + p.splits - 1) / p.splits);
+    return p;
+}
+size_t part_floats(const AttnPlan& p, long long n_queries, int q_heads, int D) { return p.splits > 1 ? (size_t)p.splits * n_queries * q_heads * (D + 2) : 0; }
+
+}  // namespace
+
 extern "C" size_t varq_paged_attn_workspace_bytes(const varq_paged_t* cache, const varq_paged_batch_t* batch) {
-    (void)cache; (void)batch;
-    return 0;
+    if (!cache || !batch || cache->n_heads < 1 || batch->q_heads < cache->n_heads || batch->n_seqs < 1 || batch->n_queries < 1 || batch->max_q < 1 || batch->max_kv < 0 ||
+        batch->window < 0 || batch->sinks < 0 || cache->head_dim < 1)
+        return 0;
+    const int max_q = (int)(batch->max_q < batch->n_queries ? batch->max_q : batch->n_queries);
+    const AttnPlan p = plan_attn(batch->n_seqs, cache->n_heads, batch->q_heads / cache->n_heads, max_q, batch->max_kv, batch->window, batch->sinks);
+    return part_floats(p, batch->n_queries, batch->q_heads, cache->head_dim) * sizeof(float);
 }
 
 extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch_t* batch, const varq_tensor_t* q, const varq_tensor_t* out, float* lse,
                                void* workspace, size_t workspace_bytes, void* stream) {
     PagedAttnArgs a;
-    (void)workspace; (void)workspace_bytes;
     if (int rc = check_cache("varq_paged_attn", cache, a.c)) return rc;
     if (!batch || !q || !out) return fail(VARQ_ERR_ARG, "varq_paged_attn: null descriptor");
     if (batch->n_seqs < 0 || batch->n_queries < 0 || batch->max_q < 0 || batch->max_kv < 0 || batch->table_pages < 0)
@@ -338,5 +372,12 @@ extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch
     a.max_q = (int)(batch->max_q < batch->n_queries ? batch->max_q : batch->n_queries); a.max_kv = batch->max_kv;
     a.scale_log2 = batch->softmax_scale * 1.4426950408889634f;
     a.causal = batch->causal != 0; a.window = batch->window; a.sinks = batch->sinks;
-    return paged_attn_simple_run(a, (cudaStream_t)stream);
+    const AttnPlan p = plan_attn(a.B, a.c.H, a.G, a.max_q, a.max_kv, a.window, a.sinks);
+    const size_t need = part_floats(p, a.T, a.Hq, a.c.D) * sizeof(float);
+    if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+        return fail(VARQ_ERR_WORKSPACE, "varq_paged_attn: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
+    float *ws_o = reinterpret_cast<float*>(workspace), *ws_ml = ws_o + (size_t)p.splits * a.T * a.Hq * a.c.D;
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (int rc = p.tc ? paged_attn_tc_run(a, p.splits, ws_o, ws_ml, st) : paged_attn_decode_run(a, p.splits, p.tiles_per_split, ws_o, ws_ml, st)) return rc;
+    return p.splits > 1 ? paged_attn_merge_run(a, p.splits, ws_o, ws_ml, st) : VARQ_OK;
 }

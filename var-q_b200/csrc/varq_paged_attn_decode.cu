@@ -1,0 +1,398 @@
+// Attention of a few query rows (eight or sixteen per CTA) over a paged cache: warp-level tensor-core instructions fed straight from the pages.
+//
+// The work is to stream the codes once, so the kernel is built around instructions per key.  A warp takes 16 keys at a time, which lie in one page;
+// mma.sync m16n8k16 takes the codes as its A operand, and every thread unpacks whole words that it loaded itself:
+//   S^T = K Q^T     thread (g, c) (g = lane / 4, c = lane % 4) holds keys g and g + 8 and a quarter of the head_dim, contiguous in memory (the order
+//                   of the contraction index is free as long as Q follows it); the eight columns are query rows (token, head of the group);
+//   O^T = V^T P^T   thread (g, c) holds an eighth of the head_dim of keys 2c, 2c + 1, 2c + 8, 2c + 9; pairs of keys are joined by byte
+//                   permutes, and P^T is the transpose of S^T's fragment (movmatrix).
+// As in the chunk kernel the V scale goes into the exponent: x = S * (K scale * factor of the row) + log2(V scale), P = 2^(x - m) in fp16,
+// l += P / V scale in fp32; the reference m is raised only when an x passes it by more than 8.  Queries are fp16 times a power of two per row, exact
+// but for elements 2^-22 times smaller than the row's largest.  Warps and CTAs (key ranges) are merged by the log-sum-exp rule.
+#include <cfloat>
+#include <type_traits>
+
+#include "varq_attn.cuh"
+#include "varq_codes.cuh"
+#include "varq_paged.cuh"
+
+namespace varq {
+namespace {
+
+constexpr int PD_WARPS = 4, PD_KEYS = 16;
+constexpr float PD_LAZY = 8.f;
+
+__device__ __forceinline__ void pd_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pd_transpose(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ float pd_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <int BITS> __host__ __device__ constexpr uint32_t pd_neg_base(int cls) {      // fp16 pairs of -(1024 / 2^p + bias), by class of bit position
+    return BITS == 8 ? 0xE480E480u : BITS == 4 ? (cls == 0 ? 0xE408E408u : 0xD480D480u)
+                                               : (cls == 0 ? 0xE402E402u : cls == 1 ? 0xDC08DC08u : cls == 2 ? 0xD420D420u : 0xCC80CC80u);
+}
+template <int BITS> __device__ __forceinline__ void pd_codes(const uint32_t* w, uint32_t (&h)[8], const CodeMagic<BITS>& cm) {
+    Item<BITS>::raw(w, h, cm);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = Item<BITS>::minus_zp(h[i], i, pd_neg_base<BITS>(i % Item<BITS>::CLS));
+}
+template <int BYTES> struct PdRaw {        // `BYTES` of a row (two bytes: the low half of one word)
+    static constexpr int NW = BYTES < 4 ? 1 : BYTES / 4;
+    uint32_t w[NW];
+    __device__ __forceinline__ void load(const unsigned char* p) {
+        if constexpr (BYTES == 2) w[0] = __ldg(reinterpret_cast<const unsigned short*>(p));
+        else if constexpr (BYTES == 4) w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+        else if constexpr (BYTES == 8) { const uint2 v = __ldg(reinterpret_cast<const uint2*>(p)); w[0] = v.x; w[1] = v.y; }
+        else {
+#pragma unroll
+            for (int i = 0; i < BYTES / 16; ++i) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+                w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+            }
+        }
+    }
+};
+// the words of two keys -> words that unpack to pairs (first key, second key) of one head_dim element each, in element order
+template <int BITS, int NW> __device__ __forceinline__ void pd_join(const uint32_t (&a)[NW], const uint32_t (&b)[NW], uint32_t (&o)[2 * NW]) {
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+        o[2 * i] = __byte_perm(a[i], b[i], BITS == 8 ? 0x5140 : 0x5410);
+        o[2 * i + 1] = __byte_perm(a[i], b[i], BITS == 8 ? 0x7362 : 0x7632);
+    }
+}
+
+template <int KB, int VB, int D, int NT>
+__global__ void __launch_bounds__(PD_WARPS * 32, NT > 1 && D == 128 ? 2 : (KB == 8 || VB == 8 || NT > 1) ? 3 : 4)
+paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int tiles_per_split, float* ws_o, float* ws_ml, int* status) {
+    constexpr int KBYTES = D / 4 * KB / 8, VBYTES = D / 8 * VB / 8;       // of a row and thread
+    constexpr unsigned KROW = D * KB / 8, VROW = D * VB / 8;
+    constexpr int ITEMS = D / 64, KSTEPS = D / 16, MT = D / 16, ROWS = 8 * NT;
+    __shared__ float s_part[PD_WARPS][ROWS][D + 2];
+
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+    const int split = (int)(blockIdx.x % (unsigned)splits);
+    const unsigned item = blockIdx.x / (unsigned)splits;
+    const int rt = (int)(item % (unsigned)n_rowtiles), bh = (int)(item / (unsigned)n_rowtiles), b = bh / a.c.H, h = bh - b * a.c.H;
+    const PagedSeq seq = paged_seq(a, b, status);
+    const int rows = seq.nq * a.G, row0 = rt * ROWS, p_first = seq.kv - seq.nq;
+    if (row0 >= rows) return;
+
+    // ---- the 16-key tiles: first tokens, then the window (or everything)
+    const int t0 = row0 / a.G, t1 = (min(row0 + ROWS, rows) - 1) / a.G;
+    const int hi = max(a.causal ? min(seq.kv, p_first + t1 + 1) : seq.kv, 0), lo = a.window ? max(p_first + t0 - a.window + 1, 0) & ~(PD_KEYS - 1) : 0;
+    const int ns = min((a.sinks + PD_KEYS - 1) / PD_KEYS, lo / PD_KEYS), n_tiles = hi > 0 ? ns + (max(hi - lo, 0) + PD_KEYS - 1) / PD_KEYS : 0;
+    const int begin = (int)min((long long)split * tiles_per_split, (long long)n_tiles), end = split == splits - 1 ? n_tiles : min(begin + tiles_per_split, n_tiles);
+    const int all_hi = a.causal ? min(p_first + t0 + 1, seq.kv) : seq.kv, all_lo = a.window ? p_first + t1 - a.window + 1 : 0;      // what every row sees
+    auto key_of = [&](int i) { return i < ns ? i * PD_KEYS : lo + (i - ns) * PD_KEYS; };
+
+    // ---- Q fragments: column g is row t * 8 + g, scaled by a power of two to use fp16's range
+    uint32_t qf[NT][KSTEPS][2];
+    float qfac[NT][2];                 // of this thread's two score columns: softmax scale in the log2 domain / power of two
+    int col_hi[NT][2], col_lo[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        float v[D / 4], mx = 0.f;
+        const int row = row0 + t * 8 + g, token = row / a.G, head = h * a.G + row - token * a.G;
+#pragma unroll
+        for (int j = 0; j < D / 4; j += 8) {
+            float e[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (row < rows) load_q8(a.q, a.dtype, (long long)(seq.q0 + token) * a.qs_t + head * a.qs_h + c * (D / 4) + j, e);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { v[j + i] = e[i]; mx = fmaxf(mx, fabsf(e[i])); }
+        }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1)); mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        // 2^(8 - exponent of the largest element), inside fp32's range
+        const int ex = min(max((int)(__float_as_uint(mx) >> 23), 40), 240);
+        const float f = __uint_as_float((uint32_t)(262 - ex) << 23), fi = __uint_as_float((uint32_t)(ex - 8) << 23);
+#pragma unroll
+        for (int s = 0; s < KSTEPS; ++s)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int p = 2 * s + r, d = (p >> 3) * 16;
+                const __half2 hh = __floats2half2_rn(v[d + code_at(KB, 2 * (p & 7))] * f, v[d + code_at(KB, 2 * (p & 7) + 1)] * f);
+                qf[t][s][r] = *reinterpret_cast<const uint32_t*>(&hh);
+            }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r2 = row0 + t * 8 + 2 * c + e;
+            qfac[t][e] = __shfl_sync(0xffffffffu, fi, (2 * c + e) * 4) * a.scale_log2;
+            const PagedSpan s = paged_span(a, p_first + r2 / a.G, seq.kv);
+            col_hi[t][e] = r2 < rows ? s.hi : seq.kv; col_lo[t][e] = r2 < rows ? s.lo : 0;
+        }
+    }
+
+    float o[NT][MT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) { o[t][i][0] = 0.f; o[t][i][1] = 0.f; o[t][i][2] = 0.f; o[t][i][3] = 0.f; }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) { m[t][e] = -1e30f; l[t][e] = 0.f; }
+    }
+    CodeMagic<KB> kmagic;
+    CodeMagic<VB> vmagic;
+    kmagic.init();
+    vmagic.init();
+    const int32_t* table = a.table + b * a.table_stride;
+    const int page_mask = (1 << a.c.page_shift) - 1;
+    const unsigned char *kbase = reinterpret_cast<const unsigned char*>(a.c.kc) + c * KBYTES + g * KROW;
+    const unsigned char *vbase = reinterpret_cast<const unsigned char*>(a.c.vc) + g * VBYTES + 2 * c * VROW;
+    const float *ksc = a.c.ks + g, *vsc = a.c.vs + g;
+    struct Tile {
+        PdRaw<KBYTES> k[2];                // keys g, g + 8
+        PdRaw<VBYTES> v[4];                // keys 2c, 2c + 1, 2c + 8, 2c + 9
+        float ks[2], vs[2];                // of keys g, g + 8
+    };
+    auto page_of = [&](int i) { return __ldg(table + (key_of(i) >> a.c.page_shift)); };
+    auto fetch = [&](Tile& t, int i, int page) {       // whole tiles: a page's rows behind the sequence's end may be loaded, not used
+        const long long at = (((long long)paged_page(a, page, status) * a.c.H + h) << a.c.page_shift) + (key_of(i) & page_mask);
+        const unsigned char *kp = kbase + at * KROW, *vp = vbase + at * VROW;
+        t.k[0].load(kp);
+        t.k[1].load(kp + 8 * KROW);
+        t.v[0].load(vp);
+        t.v[1].load(vp + VROW);
+        t.v[2].load(vp + 8 * VROW);
+        t.v[3].load(vp + 9 * VROW);
+        t.ks[0] = __ldg(ksc + at); t.ks[1] = __ldg(ksc + at + 8);
+        t.vs[0] = __ldg(vsc + at); t.vs[1] = __ldg(vsc + at + 8);
+    };
+    auto process = [&](const Tile& cur, int k0, auto masked_) {
+        constexpr bool MASKED = decltype(masked_)::value;
+        float s[NT][4];
+        {
+            float s2[NT][2][4];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int z = 0; z < 2; ++z) { s2[t][z][0] = 0.f; s2[t][z][1] = 0.f; s2[t][z][2] = 0.f; s2[t][z][3] = 0.f; }
+#pragma unroll
+            for (int it = 0; it < ITEMS; ++it) {
+                uint32_t ka[8], kb[8];
+                pd_codes<KB>(cur.k[0].w + it * Item<KB>::NW, ka, kmagic);
+                pd_codes<KB>(cur.k[1].w + it * Item<KB>::NW, kb, kmagic);
+#pragma unroll
+                for (int s4 = 0; s4 < 4; ++s4) {
+                    const uint32_t af[4] = {ka[2 * s4], kb[2 * s4], ka[2 * s4 + 1], kb[2 * s4 + 1]};
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) pd_mma(s2[t][s4 & 1], af, qf[t][it * 4 + s4][0], qf[t][it * 4 + s4][1]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[t][i] = s2[t][0][i] + s2[t][1][i];
+        }
+        uint32_t pf[NT][2];
+        float lv[2], rv[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            lv[r] = __log2f(cur.vs[r]);
+            rv[r] = __fdividef(1.f, cur.vs[r]);
+            if (MASKED && !(cur.vs[r] <= FLT_MAX && cur.vs[r] > 0.f)) rv[r] = 1.f;      // what is not seen has weight 0, and 0 times its inverse has to be 0
+        }
+        bool over = false;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float x = fmaf(cur.ks[r], s[t][2 * r + e] * qfac[t][e], lv[r]);
+                    if (MASKED) {
+                        const int key = k0 + g + 8 * r;
+                        if (!(key < col_hi[t][e] && (key >= col_lo[t][e] || key < a.sinks))) x = -INFINITY;
+                    }
+                    s[t][2 * r + e] = x;
+                    over = over | (x > m[t][e] + PD_LAZY);
+                }
+        if (__any_sync(0xffffffffu, over)) {
+            // rare after the first tile: new references, the same in every lane of a row, and everything accumulated is rescaled
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float x = fmaxf(s[t][e], s[t][2 + e]);
+#pragma unroll
+                    for (int z = 4; z < 32; z <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, z));
+                    const float mn = fmaxf(m[t][e], x), alpha = pd_ex2(m[t][e] - mn);
+                    m[t][e] = mn;
+                    l[t][e] *= alpha;
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) { o[t][i][e] *= alpha; o[t][i][2 + e] *= alpha; }
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float p0 = pd_ex2(s[t][2 * r] - m[t][0]), p1 = pd_ex2(s[t][2 * r + 1] - m[t][1]);
+                l[t][0] = fmaf(p0, rv[r], l[t][0]); l[t][1] = fmaf(p1, rv[r], l[t][1]);
+                const __half2 hh = __floats2half2_rn(p0, p1);
+                pf[t][r] = pd_transpose(*reinterpret_cast<const uint32_t*>(&hh));
+            }
+        uint32_t ja[2 * PdRaw<VBYTES>::NW], jb[2 * PdRaw<VBYTES>::NW];
+        pd_join<VB>(cur.v[0].w, cur.v[1].w, ja);
+        pd_join<VB>(cur.v[2].w, cur.v[3].w, jb);
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it) {
+            uint32_t va[8], vb_[8];
+            pd_codes<VB>(ja + it * Item<VB>::NW, va, vmagic);
+            pd_codes<VB>(jb + it * Item<VB>::NW, vb_, vmagic);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t af[4] = {va[2 * i], va[2 * i + 1], vb_[2 * i], vb_[2 * i + 1]};
+#pragma unroll
+                for (int t = 0; t < NT; ++t) pd_mma(o[t][it * 4 + i], af, pf[t][0], pf[t][1]);
+            }
+        }
+    };
+    auto step = [&](const Tile& t, int i) {
+        const int k0 = key_of(i);
+        if (k0 + PD_KEYS > all_hi || (k0 < all_lo && k0 + PD_KEYS > a.sinks)) process(t, k0, std::true_type());
+        else process(t, k0, std::false_type());
+    };
+    // two buffers that take turns, the next tile's rows in flight, the page number of the one behind it as well
+    Tile ta, tb;
+    int i = begin + warp, page = i < end ? page_of(i) : 0;
+    if (i < end) fetch(ta, i, page);
+    if (i + PD_WARPS < end) page = page_of(i + PD_WARPS);
+#pragma unroll 1
+    while (i < end) {
+        if (i + PD_WARPS < end) fetch(tb, i + PD_WARPS, page);
+        if (i + 2 * PD_WARPS < end) page = page_of(i + 2 * PD_WARPS);
+        step(ta, i);
+        i += PD_WARPS;
+        if (i >= end) break;
+        if (i + PD_WARPS < end) fetch(ta, i + PD_WARPS, page);
+        if (i + 2 * PD_WARPS < end) page = page_of(i + 2 * PD_WARPS);
+        step(tb, i);
+        i += PD_WARPS;
+    }
+    // ---- a warp's partial result
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int z = 4; z < 32; z <<= 1) l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], z);
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int z = 0; z < 4; ++z)      // row g (z < 2) or g + 8 of row tile j = elements 2 j, 2 j + 1 of this thread's eighth of the head_dim
+                s_part[warp][t * 8 + 2 * c + (z & 1)][g * (D / 8) + 2 * j + (z >> 1)] = o[t][j][z];
+        if (g == 0) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                s_part[warp][t * 8 + 2 * c + e][D] = m[t][e];
+                s_part[warp][t * 8 + 2 * c + e][D + 1] = l[t][e];
+            }
+        }
+    }
+    __syncthreads();
+    // ---- merge the warps, then write the output or this split's part
+    const long long n_rows = (long long)a.T * a.Hq;
+    for (int j = threadIdx.x; j < ROWS * D; j += PD_WARPS * 32) {
+        const int r = j / D, d = j - r * D, row = row0 + r;
+        if (row >= rows) break;
+        float M = -FLT_MAX;
+#pragma unroll
+        for (int w = 0; w < PD_WARPS; ++w) M = fmaxf(M, s_part[w][r][D]);
+        float num = 0.f, den = 0.f;
+#pragma unroll
+        for (int w = 0; w < PD_WARPS; ++w) {
+            const float wt = pd_ex2(s_part[w][r][D] - M);
+            num = fmaf(wt, s_part[w][r][d], num);
+            den = fmaf(wt, s_part[w][r][D + 1], den);
+        }
+        const int token = row / a.G, head = h * a.G + row - token * a.G;
+        const long long out_row = (long long)(seq.q0 + token) * a.Hq + head;
+        if (splits == 1) {
+            store_o_elem(a.out, a.dtype, (long long)(seq.q0 + token) * a.os_t + head * a.os_h + d, den != 0.f ? num / den : 0.f);
+            if (d == 0 && a.lse) a.lse[out_row] = den != 0.f ? (M + __log2f(den)) * 0.6931471805599453f : -INFINITY;
+        } else {
+            ws_o[(split * n_rows + out_row) * D + d] = num;
+            if (d == 0) *reinterpret_cast<float2*>(ws_ml + (split * n_rows + out_row) * 2) = make_float2(M, den);
+        }
+    }
+}
+
+// One warp per output row: the splits' numerators and sums, by the log-sum-exp rule, in the splits' order
+template <int D>
+__global__ void __launch_bounds__(128) paged_attn_merge_kernel(PagedAttnArgs a, int splits, const float* ws_o, const float* ws_ml) {
+    constexpr int V = D / 32;
+    pdl_trigger();
+    pdl_wait();
+    const long long n_rows = (long long)a.T * a.Hq, row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= n_rows) return;
+    float M = -FLT_MAX;
+    for (int s = lane; s < splits; s += 32) M = fmaxf(M, ws_ml[(s * n_rows + row) * 2]);
+#pragma unroll
+    for (int z = 16; z; z >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, z));
+    float num[V], den = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) num[i] = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+        const float2 ml = *reinterpret_cast<const float2*>(ws_ml + (s * n_rows + row) * 2);
+        const float w = pd_ex2(ml.x - M);
+        den = fmaf(w, ml.y, den);
+        const float* o = ws_o + (s * n_rows + row) * D + lane * V;
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            const float2 x = *reinterpret_cast<const float2*>(o + i);
+            num[i] = fmaf(w, x.x, num[i]); num[i + 1] = fmaf(w, x.y, num[i + 1]);
+        }
+    }
+    const long long token = row / a.Hq;
+    const int head = (int)(row - token * a.Hq);
+    const float inv = den != 0.f ? 1.f / den : 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) store_o_elem(a.out, a.dtype, token * a.os_t + head * a.os_h + lane * V + i, num[i] * inv);
+    if (lane == 0 && a.lse) a.lse[row] = den != 0.f ? (M + __log2f(den)) * 0.6931471805599453f : -INFINITY;
+}
+
+template <int KB, int VB, int D>
+int launch(const PagedAttnArgs& a, int splits, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st) {
+    const long long rows = (long long)a.max_q * a.G;
+    const int nt = rows <= 8 ? 1 : 2, n_rowtiles = (int)((rows + 8 * nt - 1) / (8 * nt));
+    const long long blocks = (long long)a.B * a.c.H * n_rowtiles * splits;
+    if (blocks > 0x7fffffffLL) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_attn: more than 2^31 thread blocks");
+    VARQ_CUDA_TRY(nt == 1 ? launch_pdl(paged_attn_decode_kernel<KB, VB, D, 1>, (unsigned)blocks, PD_WARPS * 32, 0, st, 1, a, n_rowtiles, splits, tiles_per_split, ws_o, ws_ml, paged_status_word())
+                          : launch_pdl(paged_attn_decode_kernel<KB, VB, D, 2>, (unsigned)blocks, PD_WARPS * 32, 0, st, 1, a, n_rowtiles, splits, tiles_per_split, ws_o, ws_ml, paged_status_word()));
+    count_launches(1);
+    return VARQ_OK;
+}
+
+}  // namespace
+
+int paged_attn_decode_run(const PagedAttnArgs& a, int splits, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st) {
+#define GO(K_, V_) \
+    if (a.c.kb == K_ && a.c.vb == V_) return a.c.D == 64 ? launch<K_, V_, 64>(a, splits, tiles_per_split, ws_o, ws_ml, st) : launch<K_, V_, 128>(a, splits, tiles_per_split, ws_o, ws_ml, st);
+    GO(8, 8) GO(8, 4) GO(8, 2) GO(4, 8) GO(4, 4) GO(4, 2) GO(2, 8) GO(2, 4) GO(2, 2)
+#undef GO
+    return fail(VARQ_ERR_ARG, "varq_paged_attn: bits must be 2, 4 or 8");
+}
+
+int paged_attn_merge_run(const PagedAttnArgs& a, int splits, const float* ws_o, const float* ws_ml, cudaStream_t st) {
+    const long long blocks = ((long long)a.T * a.Hq + 3) / 4;
+    if (blocks > 0x7fffffffLL) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_attn: more than 2^31 thread blocks");
+    VARQ_CUDA_TRY(a.c.D == 64 ? launch_pdl(paged_attn_merge_kernel<64>, (unsigned)blocks, 128, 0, st, 1, a, splits, ws_o, ws_ml)
+                              : launch_pdl(paged_attn_merge_kernel<128>, (unsigned)blocks, 128, 0, st, 1, a, splits, ws_o, ws_ml));
+    count_launches(1);
+    return VARQ_OK;
+}
+
+}  // namespace varq

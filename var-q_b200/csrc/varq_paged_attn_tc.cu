@@ -1,0 +1,495 @@
+// Attention of a chunk over a paged cache on the 5th-generation tensor cores (tcgen05 + TMEM).
+//
+// One CTA = one (sequence, head of the cache) x 256 query rows, two tiles of 128; a row is a (token, query head of the group) pair, so query
+// heads that share a head of the cache share its converted tiles.  It walks over tiles of 128 keys; a tile of first tokens (sinks) and the window
+// are lists of tiles one behind the other.  Per key tile and query tile
+//   S = Q K^T       Q fp16 in shared memory, K integer codes as exact fp16; S fp32 in tensor memory
+//   x = S a_j + b_j with a_j = K scale * softmax_scale * log2 e and b_j = log2 of the V scale
+//   P = 2^(x - m)   fp16, written over S in tensor memory, = weight * V scale relative to the row's reference m
+//   l += P / V scale in fp32, from the unrounded P;      O += P V, V integer codes as exact fp16, O fp32 in tensor memory
+// and at the end out = O / l, log-sum-exp = (m + log2 l) ln 2.  The reference m is that of weight times V scale, which is what bounds O.  It is raised only when an x
+// passes it by more than 8: the tile is then computed again against the new one, O and l rescaled.  fp16 queries are exact, and so are bf16
+// queries of usual size; a row whose largest element lies outside [2^-4, 2^15) is scaled by a power of two (then S a_j takes a factor).
+// Warps: 0-3 and 4-7 softmax of the two query tiles, a thread per row; 8-11 and 12-15 convert K and V: packed rows come straight from the pages
+// into registers, a tile ahead, and go to 128B-swizzled fp16 tiles in shared memory, scales to the tables a, b, 1 / V scale; warp 16 issues the products.
+// While one query tile is in its softmax the tensor pipe works for the other.
+// Every wait is bounded: on expiry the kernel records a status code and all roles drain out.
+#include "varq_attn_tc.cuh"
+#include "varq_paged.cuh"
+
+namespace varq {
+namespace {
+
+constexpr int PT_M = 128, PT_N = 128;
+constexpr float PT_LAZY = 8.f;
+
+template <int D> struct PtPlan {
+    static constexpr int KST = 2, VST = 2, TS = 4;                 // stages of K and V, tables (a table outlives its K stage by a tile)
+    static constexpr int Q_BYTES = PT_M * D * 2, T_BYTES = PT_N * D * 2;
+    static constexpr int TAB_FLOATS = 3 * PT_N;
+    static constexpr int OFF_Q = 0, OFF_K = OFF_Q + 2 * Q_BYTES, OFF_V = OFF_K + KST * T_BYTES, OFF_TAB = OFF_V + VST * T_BYTES;
+    static constexpr int OFF_BAR = OFF_TAB + TS * TAB_FLOATS * 4, N_BARS = 2 * KST + 2 * VST + TS + 9;
+    static constexpr int OFF_MISC = OFF_BAR + N_BARS * 8, SMEM = OFF_MISC + 16 + 1024;
+    static constexpr int COL_S = 0, COL_O = 2 * PT_N, TMEM_COLS = 512;
+    static_assert(COL_O + 2 * D <= TMEM_COLS && SMEM <= 227 * 1024, "plan");
+    static constexpr int THREADS = 640, REGS = 96, REGS_SOFT = 168, REGS_CONV = 56, REGS_MISC = 32;
+    static_assert(256 * REGS_SOFT + 256 * REGS_CONV + 128 * REGS_MISC <= THREADS * REGS, "register plan");
+};
+
+// 16-byte chunk `ch` (eight head_dim values) of row `r` in a 128B-swizzled tile of 128 rows: blocks of 64 columns
+__device__ __forceinline__ uint32_t pt_chunk(int r, int ch) {
+    return (uint32_t)((ch >> 3) * (128 * 128) + (r >> 3) * 1024 + (r & 7) * 128 + (((ch & 7) ^ (r & 7)) << 4));
+}
+// D[tmem] (+)= A[smem] B[smem]
+__device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <int BITS> __host__ __device__ constexpr uint32_t pt_neg_base(int cls) {      // fp16 pairs of -(1024 / 2^p + bias), by class of bit position
+    return BITS == 8 ? 0xE480E480u : BITS == 4 ? (cls == 0 ? 0xE408E408u : 0xD480D480u)
+                                               : (cls == 0 ? 0xE402E402u : cls == 1 ? 0xDC08DC08u : cls == 2 ? 0xD420D420u : 0xCC80CC80u);
+}
+
+// The key tiles of a CTA: `ns` tiles of first tokens, then those from `lo` on
+struct PtTiles {
+    int ns, lo, n;
+    __device__ __forceinline__ int key(int i) const { return i < ns ? i * PT_N : lo + (i - ns) * PT_N; }
+};
+
+// one of the two 16-element halves of a query row's 32, packed fp16 in element order -> operand order of codes of `kb` bits
+__device__ __forceinline__ void q_operand_order(uint32_t (&w)[8], int kb) {
+    if (kb == 8) return;
+    uint32_t o[8];
+    if (kb == 4) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                o[4 * i + 2 * j] = __byte_perm(w[4 * i + j], w[4 * i + 2 + j], 0x5410);
+                o[4 * i + 2 * j + 1] = __byte_perm(w[4 * i + j], w[4 * i + 2 + j], 0x7632);
+            }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { o[2 * j] = __byte_perm(w[j], w[4 + j], 0x5410); o[2 * j + 1] = __byte_perm(w[j], w[4 + j], 0x7632); }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = o[i];
+}
+
+template <int D>
+__global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(PagedAttnArgs a, int n_qblocks, int splits, float* ws_o, float* ws_ml, int* status) {
+    using P = PtPlan<D>;
+    constexpr int KST = P::KST, VST = P::VST, TS = P::TS;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + P::OFF_BAR);
+    uint64_t *bar_k = bars, *bar_kf = bar_k + KST, *bar_v = bar_kf + KST, *bar_vf = bar_v + VST, *bar_tab = bar_vf + VST;   // written, free; tables written
+    uint64_t *bar_q = bar_tab + TS, *bar_s = bar_q + 2, *bar_p = bar_s + 2, *bar_o = bar_p + 2, *bar_end = bar_o + 2;      // [2]: by query tile
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + P::OFF_MISC);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + P::OFF_MISC + 8);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+    if (warp == 17) {
+        if (lane < P::N_BARS) {
+            const int i = lane;
+            const bool by_128 = i < KST || (i >= 2 * KST && i < 2 * KST + VST) || (i >= 2 * KST + 2 * VST + TS && i < 2 * KST + 2 * VST + TS + 2) ||
+                                (i >= 2 * KST + 2 * VST + TS + 4 && i < 2 * KST + 2 * VST + TS + 6);
+            const bool by_256 = i >= 2 * KST + 2 * VST && i < 2 * KST + 2 * VST + TS;
+            mbar_init(&bars[i], by_128 ? 128u : by_256 ? 256u : 1u);
+        }
+        if (lane == 0) *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 16) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)P::TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pdl_wait();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    pdl_trigger();       // behind the allocation: a CTA of a next launch must not take tensor memory that one of this launch still asks for
+    const uint32_t tmem_base = *tmem_slot;
+
+    // ---- what this CTA does: late query blocks, which see the most keys, first
+    const int split = (int)(blockIdx.x % (unsigned)splits);
+    const unsigned item = blockIdx.x / (unsigned)splits, heads = (unsigned)(a.B * a.c.H);
+    const int bh = (int)(item % heads), qb = n_qblocks - 1 - (int)(item / heads), b = bh / a.c.H, h = bh - b * a.c.H;
+    const PagedSeq seq = paged_seq(a, b, status);
+    const int rows = seq.nq * a.G, row0 = qb * (2 * PT_M);                   // rows of the (sequence, head); first one of this CTA
+    const int p_first = seq.kv - seq.nq;                                     // position of the first query
+    PtTiles tiles;
+    int n_t[2], tile0 = 0;                                                   // key tiles of the two query tiles
+    {
+        const int t0 = row0 / a.G, t1 = (min(row0 + 2 * PT_M, rows) - 1) / a.G, t_mid = (min(row0 + PT_M, rows) - 1) / a.G;
+        const int hi = max(a.causal ? min(seq.kv, p_first + t1 + 1) : seq.kv, 0), hi0 = max(a.causal ? min(seq.kv, p_first + t_mid + 1) : seq.kv, 0);
+        tiles.lo = a.window ? max(p_first + t0 - a.window + 1, 0) & ~(PT_N - 1) : 0;
+        tiles.ns = min((a.sinks + PT_N - 1) / PT_N, tiles.lo / PT_N);
+        const int n = hi > 0 ? tiles.ns + (max(hi - tiles.lo, 0) + PT_N - 1) / PT_N : 0, n0 = hi0 > 0 ? tiles.ns + (max(hi0 - tiles.lo, 0) + PT_N - 1) / PT_N : 0;
+        tile0 = (int)((long long)n * split / splits);
+        tiles.n = row0 < rows ? (int)((long long)n * (split + 1) / splits) - tile0 : 0;
+        n_t[0] = min(max(n0 - tile0, 0), tiles.n);
+        n_t[1] = row0 + PT_M < rows ? tiles.n : 0;
+    }
+    const int n_all = max(n_t[0], n_t[1]);
+    const int page_mask = (1 << a.c.page_shift) - 1;
+    const int32_t* table = a.table + b * a.table_stride;
+
+    if (warp < 8) {
+        // =============================================================== softmax, epilogue
+        set_registers<P::REGS_SOFT, P::REGS>();
+        const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane, row = row0 + t * PT_M + r;
+        const bool live = row < rows;
+        const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16), col_s = lane_base + P::COL_S + t * PT_N, col_o = lane_base + P::COL_O + t * D;
+        if (row0 + t * PT_M < rows) {
+            const int token = live ? row / a.G : 0, head = h * a.G + (live ? row - token * a.G : 0);
+            // ---- queries -> fp16 in shared memory, in the order in which the codes of K are unpacked
+            float q_factor = 1.f;
+            {
+                uint4 raw[D / 8];
+                const long long off = (long long)(seq.q0 + token) * a.qs_t + head * a.qs_h;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) raw[i] = live ? load_q16<2>(a.q, off + 8 * i) : make_uint4(0, 0, 0, 0);
+                float f = 1.f;
+                if (a.dtype == VARQ_BF16) {
+                    uint32_t top = 0;                                        // bits of the largest absolute value
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i) {
+                        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) top = max(top, max(w[j] & 0x7fffu, (w[j] >> 16) & 0x7fffu));
+                    }
+                    const int ex = (int)(top >> 7);                          // exponent: 2^(ex - 127)
+                    if (top && (ex < 123 || ex > 141)) {                     // -> largest element in [2^8, 2^9); NaN and infinity stay what they are
+                        const int e = min(max(ex, 40), 240);
+                        f = __uint_as_float((uint32_t)(262 - e) << 23);
+                        q_factor = __uint_as_float((uint32_t)(e - 8) << 23);
+                    }
+                }
+                unsigned char* qs = smem + P::OFF_Q + t * P::Q_BYTES;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    uint32_t w[8] = {raw[2 * i].x, raw[2 * i].y, raw[2 * i].z, raw[2 * i].w, raw[2 * i + 1].x, raw[2 * i + 1].y, raw[2 * i + 1].z, raw[2 * i + 1].w};
+                    if (a.dtype == VARQ_BF16) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) w[j] = pack_half2(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xffff0000u) * f);
+                    }
+                    q_operand_order(w, a.c.kb);
+                    sts128(qs + pt_chunk(r, 2 * i), w[0], w[1], w[2], w[3]);
+                    sts128(qs + pt_chunk(r, 2 * i + 1), w[4], w[5], w[6], w[7]);
+                }
+            }
+            fence_async_smem();
+            mbar_arrive(&bar_q[t]);
+            const bool scaled = __any_sync(0xffffffffu, q_factor != 1.f);
+            const PagedSpan span = paged_span(a, p_first + token, seq.kv);
+            // keys between which every row of the query tile sees everything
+            const int tl = min(row0 + t * PT_M + PT_M, rows) - 1, all_hi = a.causal ? p_first + (row0 + t * PT_M) / a.G + 1 : 0x7fffffff,
+                      all_lo = a.window ? p_first + tl / a.G - a.window + 1 : 0;
+            float m = -1e30f, l = 0.f;
+            bool ok = true;
+            const int n = n_t[t];
+#pragma unroll 1
+            for (int j = 0; j < n; ++j) {
+                const int key0 = tiles.key(tile0 + j);
+                ok = mbar_wait(&bar_tab[j % TS], (j / TS) & 1, abort_flag, 201) && mbar_wait(&bar_s[t], j & 1, abort_flag, 202);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                const float* tab = reinterpret_cast<const float*>(smem + P::OFF_TAB) + (j % TS) * P::TAB_FLOATS;
+                uint32_t pk[PT_N / 2];
+                float2 sum;
+                float top;
+                auto pass = [&](auto masked_, auto scaled_) {
+                    constexpr bool MASKED = decltype(masked_)::value != 0, SCALED = decltype(scaled_)::value != 0;
+                    sum = make_float2(0.f, 0.f);
+                    top = -INFINITY;
+                    const float2 nm = make_float2(-m, -m), qf = make_float2(q_factor, q_factor);
+#pragma unroll
+                    for (int c = 0; c < PT_N / 32; ++c) {
+                        uint32_t s[32];
+                        tmem_ld32(col_s + c * 32, s);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 ta = *reinterpret_cast<const float4*>(tab + c * 32 + i), tb = *reinterpret_cast<const float4*>(tab + PT_N + c * 32 + i),
+                                         tc = *reinterpret_cast<const float4*>(tab + 2 * PT_N + c * 32 + i);
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                float2 x = make_float2(__uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1]));
+                                if (SCALED) { x.x *= qf.x; x.y *= qf.y; }
+                                x = fma2(x, e ? make_float2(ta.z, ta.w) : make_float2(ta.x, ta.y), e ? make_float2(tb.z, tb.w) : make_float2(tb.x, tb.y));
+                                if (MASKED) {
+                                    const int k = key0 + c * 32 + i + 2 * e;
+                                    x.x = k < span.hi && (k >= span.lo || k < a.sinks) ? x.x : -INFINITY;
+                                    x.y = k + 1 < span.hi && (k + 1 >= span.lo || k + 1 < a.sinks) ? x.y : -INFINITY;
+                                }
+                                top = fmaxf(top, fmaxf(x.x, x.y));
+                                x = add2(x, nm);
+                                const float2 p = make_float2(ex2(x.x), ex2(x.y));
+                                sum = fma2(p, e ? make_float2(tc.z, tc.w) : make_float2(tc.x, tc.y), sum);
+                                pk[(c * 32 + i) / 2 + e] = pack_half2(p.x, p.y);
+                            }
+                        }
+                    }
+                };
+                const bool masked = key0 + PT_N > all_hi || (key0 < all_lo && key0 + PT_N > a.sinks);
+                auto compute = [&]() {
+                    if (scaled) { if (masked) pass(IntC<1>(), IntC<1>()); else pass(IntC<0>(), IntC<1>()); }
+                    else if (masked) pass(IntC<1>(), IntC<0>());
+                    else pass(IntC<0>(), IntC<0>());
+                };
+                compute();
+                if (__any_sync(0xffffffffu, top > m + PT_LAZY)) {
+                    const float mn = top > m + PT_LAZY ? top : m, alpha = ex2(m - mn);
+                    m = mn;
+                    l *= alpha;
+                    if (j > 0) {                     // the products of the tiles before are complete: S came behind them
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(col_o + c, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            tmem_st32(col_o + c, o);
+                        }
+                    }
+                    compute();
+                }
+                l += sum.x + sum.y;
+                tmem_st32(col_s, pk);
+                tmem_st32(col_s + 32, pk + 32);
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(&bar_p[t]);
+            }
+            // ---- O / l, or this split's part
+            if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bar_o[t], 0, abort_flag, 203));
+            tc_fence_after();
+            if (ok) {
+                const float inv = l != 0.f ? 1.f / l : 0.f;       // (a NaN stays one)
+                const long long out_row = (long long)(seq.q0 + token) * a.Hq + head, n_rows = (long long)a.T * a.Hq;
+                const long long oo = (long long)(seq.q0 + token) * a.os_t + head * a.os_h;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    float v[32];
+                    if (n > 0) { tmem_ld32(col_o + c, o); tmem_wait_ld(); }
+                    else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = 0u;
+                    }
+                    if (a.c.vb == 8) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]);
+                    } else if (a.c.vb == 4) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[(i & 16) + code_pos(4, i & 15)]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[(i & 16) + code_pos(2, i & 15)]);
+                    }
+                    if (!live) continue;
+                    if (splits == 1) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] *= inv;
+                        store_o_row32(a.out, a.dtype, oo + c, v);
+                    } else {
+                        store_o_row32(ws_o, VARQ_F32, (split * n_rows + out_row) * D + c, v);
+                    }
+                }
+                if (live && splits > 1) *reinterpret_cast<float2*>(ws_ml + (split * n_rows + out_row) * 2) = make_float2(m, l);
+                if (live && splits == 1 && a.lse) a.lse[out_row] = l != 0.f ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY;
+            }
+        }
+    } else if (warp < 16) {
+        // =============================================================== converters
+        set_registers<P::REGS_CONV, P::REGS>();
+        const bool is_k = warp < 12;
+        const int ptid = tid - (is_k ? 256 : 384), it = ptid & 3, kq = ptid >> 2;       // 16-code item of a 64-column block; keys kq, kq + 32, ...
+        const int32_t* pool = is_k ? a.c.kc : a.c.vc;
+        const float* scales = is_k ? a.c.ks : a.c.vs;
+        unsigned char* stages = smem + (is_k ? P::OFF_K : P::OFF_V);
+        uint64_t *full = is_k ? bar_k : bar_v, *freed = is_k ? bar_kf : bar_vf;
+        auto loop = [&](auto bits_) {
+            constexpr int BITS = decltype(bits_)::value, NW = BITS / 2, WORDS = D * BITS / 32, NB = D / 64;
+            CodeMagic<BITS> magic;
+            magic.init();
+            int pg[4];
+            uint32_t w[4][NB][NW];
+            float sc;
+            auto fetch_pages = [&](int i) {
+                const int key0 = tiles.key(tile0 + i) + kq;
+#pragma unroll
+                for (int p = 0; p < 4; ++p) pg[p] = key0 + 32 * p < seq.kv ? __ldg(table + ((key0 + 32 * p) >> a.c.page_shift)) : -1;
+            };
+            auto fetch_rows = [&](int i) {
+                const int key0 = tiles.key(tile0 + i) + kq;
+                sc = 0.f;
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    const int key = key0 + 32 * p;
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int z = 0; z < NW; ++z) w[p][nb][z] = 0u;
+                    if (key < seq.kv) {
+                        const long long at = (((long long)paged_page(a, pg[p], status) * a.c.H + h) << a.c.page_shift) + (key & page_mask);
+                        const int32_t* src = pool + at * WORDS + it * NW;
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            if constexpr (NW == 4) {
+                                const uint4 x = __ldg(reinterpret_cast<const uint4*>(src + nb * 4 * NW));
+                                w[p][nb][0] = x.x; w[p][nb][1] = x.y; w[p][nb][2] = x.z; w[p][nb][3] = x.w;
+                            } else if constexpr (NW == 2) {
+                                const uint2 x = __ldg(reinterpret_cast<const uint2*>(src + nb * 4 * NW));
+                                w[p][nb][0] = x.x; w[p][nb][1] = x.y;
+                            } else w[p][nb][0] = (uint32_t)__ldg(src + nb * 4 * NW);
+                        }
+                        if (it == p) sc = __ldg(scales + at);
+                    }
+                }
+            };
+            if (n_all > 0) { fetch_pages(0); fetch_rows(0); }
+            if (n_all > 1) fetch_pages(1);
+#pragma unroll 1
+            for (int j = 0; j < n_all; ++j) {
+                const int st = j % 2;
+                if (j >= 2 && !mbar_wait(&freed[st], ((j >> 1) - 1) & 1, abort_flag, is_k ? 204 : 205)) break;
+                unsigned char* tile = stages + st * P::T_BYTES;
+                float* tab = reinterpret_cast<float*>(smem + P::OFF_TAB) + (j % TS) * P::TAB_FLOATS;
+                {
+                    const int k = kq + 32 * it;
+                    const bool there = tiles.key(tile0 + j) + k < seq.kv;
+                    if (is_k) tab[k] = there ? sc * a.scale_log2 : 0.f;
+                    else {                                      // a scale that is no number spoils the rows that see it, and no other: 0 * its inverse must be 0
+                        const bool fine = sc <= FLT_MAX;
+                        tab[PT_N + k] = there ? (fine ? __log2f(sc) : sc - sc) : -INFINITY;
+                        tab[2 * PT_N + k] = there && fine ? __fdividef(1.f, sc) : there ? 1.f : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int p = 0; p < 4; ++p)
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        uint32_t hw[8];
+                        Item<BITS>::raw(w[p][nb], hw, magic);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) hw[i] = Item<BITS>::minus_zp(hw[i], i, pt_neg_base<BITS>(i % Item<BITS>::CLS));
+                        const int key = kq + 32 * p;
+                        sts128(tile + pt_chunk(key, nb * 8 + 2 * it), hw[0], hw[1], hw[2], hw[3]);
+                        sts128(tile + pt_chunk(key, nb * 8 + 2 * it + 1), hw[4], hw[5], hw[6], hw[7]);
+                    }
+                fence_async_smem();
+                mbar_arrive(&full[st]);
+                mbar_arrive(&bar_tab[j % TS]);
+                if (j + 1 < n_all) fetch_rows(j + 1);
+                if (j + 2 < n_all) fetch_pages(j + 2);
+            }
+        };
+        const int bits = is_k ? a.c.kb : a.c.vb;
+        if (bits == 8) loop(IntC<8>()); else if (bits == 4) loop(IntC<4>()); else loop(IntC<2>());
+    } else {
+        set_registers<P::REGS_MISC, P::REGS>();
+        if (warp == 16) {
+            // =============================================================== products (the whole warp waits; one elected lane issues)
+            constexpr uint32_t IDESC_S = instr_desc(PT_M, PT_N, 0), IDESC_O = instr_desc(PT_M, D, 1);
+            const uint64_t qd = smem_desc(smem_u32(smem + P::OFF_Q), 16, 1024), kd = smem_desc(smem_u32(smem + P::OFF_K), 16, 1024);
+            const uint64_t vd = smem_desc(smem_u32(smem + P::OFF_V), PT_N * 128, 1024);
+            bool ok = true;
+            auto issue_s = [&](int t, int j) {
+                const uint64_t ad = qd + (uint64_t)((t * P::Q_BYTES) >> 4), bd = kd + (uint64_t)(((j % KST) * P::T_BYTES) >> 4);
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint64_t step = (uint64_t)(((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4);
+                    tc_mma_ss(tmem_base + P::COL_S + t * PT_N, ad + step, bd + step, IDESC_S, kk ? 1u : 0u);
+                }
+                tc_commit(&bar_s[t]);
+            };
+            auto issue_o = [&](int t, int j) {
+                const uint64_t bd = vd + (uint64_t)(((j % VST) * P::T_BYTES) >> 4);
+#pragma unroll
+                for (int kk = 0; kk < PT_N / 16; ++kk)
+                    tc_mma_ts(tmem_base + P::COL_O + t * D, tmem_base + P::COL_S + t * PT_N + kk * 8, bd + (uint64_t)((kk * 2048) >> 4), IDESC_O, j || kk ? 1u : 0u);
+            };
+            for (int t = 0; t < 2 && ok; ++t)
+                if (n_t[t] > 0) {
+                    ok = mbar_wait_warp(&bar_q[t], 0, abort_flag, 206) && mbar_wait_warp(&bar_k[0], 0, abort_flag, 207);
+                    tc_fence_after();
+                    if (ok) issue_s(t, 0);
+                }
+            if (ok && n_all > 0) tc_commit(&bar_kf[0]);
+#pragma unroll 1
+            for (int j = 0; j < n_all && ok; ++j) {
+                if (!(ok = mbar_wait_warp(&bar_v[j % VST], (j / VST) & 1, abort_flag, 208))) break;
+                if (j + 1 < n_all && !(ok = mbar_wait_warp(&bar_k[(j + 1) % KST], ((j + 1) / KST) & 1, abort_flag, 209))) break;
+#pragma unroll 1
+                for (int t = 0; t < 2; ++t) {
+                    if (j >= n_t[t]) continue;
+                    if (!(ok = mbar_wait_warp(&bar_p[t], j & 1, abort_flag, 210))) break;
+                    tc_fence_after();
+                    issue_o(t, j);
+                    if (j + 1 < n_t[t]) issue_s(t, j + 1);
+                    else tc_commit(&bar_o[t]);
+                }
+                tc_commit(&bar_vf[j % VST]);
+                if (j + 1 < n_all) tc_commit(&bar_kf[(j + 1) % KST]);
+            }
+            // nothing of this CTA may be in flight when its memory goes
+            tc_commit(bar_end);
+            for (uint32_t i = 0; i < TC_SPIN_LIMIT && !__all_sync(0xffffffffu, mbar_try(bar_end, 0)); ++i) {}
+        }
+    }
+    __syncthreads();
+    if (warp == 16) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)P::TMEM_COLS) : "memory");
+    }
+}
+
+template <int D> int launch_tc(const PagedAttnArgs& a, int n_qblocks, int splits, float* ws_o, float* ws_ml, cudaStream_t st) {
+    using P = PtPlan<D>;
+    static bool configured[64] = {false};
+    int dev = 0;
+    VARQ_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        VARQ_CUDA_TRY(cudaFuncSetAttribute(paged_attn_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, P::SMEM));
+        if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
+    const long long blocks = (long long)a.B * a.c.H * n_qblocks * splits;
+    if (blocks > 0x7fffffffLL) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_attn: more than 2^31 thread blocks");
+    VARQ_CUDA_TRY(launch_pdl(paged_attn_tc_kernel<D>, (unsigned)blocks, P::THREADS, P::SMEM, st, 1, a, n_qblocks, splits, ws_o, ws_ml, paged_status_word()));
+    count_launches(1);
+    return VARQ_OK;
+}
+
+}  // namespace
+
+int paged_attn_tc_run(const PagedAttnArgs& a, int splits, float* ws_o, float* ws_ml, cudaStream_t st) {
+    const int n_qblocks = (int)(((long long)a.max_q * a.G + 2 * PT_M - 1) / (2 * PT_M));
+    return a.c.D == 64 ? launch_tc<64>(a, n_qblocks, splits, ws_o, ws_ml, st) : launch_tc<128>(a, n_qblocks, splits, ws_o, ws_ml, st);
+}
+int paged_attn_tc_status(int* out) { return tc_file_status(out); }
+
+}  // namespace varq

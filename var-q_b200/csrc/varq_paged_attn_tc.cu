@@ -32,7 +32,7 @@ template <int D> struct PtPlan {
     static constexpr int OFF_MISC = OFF_BAR + N_BARS * 8, SMEM = OFF_MISC + 16 + 1024;
     static constexpr int COL_S = 0, COL_O = 2 * PT_N, TMEM_COLS = 512;
     static_assert(COL_O + 2 * D <= TMEM_COLS && SMEM <= 227 * 1024, "plan");
-    static constexpr int THREADS = 640, REGS = 96, REGS_SOFT = 168, REGS_CONV = 56, REGS_MISC = 32;
+    static constexpr int THREADS = 640, REGS = 96, REGS_SOFT = 136, REGS_CONV = 72, REGS_MISC = 64;
     static_assert(256 * REGS_SOFT + 256 * REGS_CONV + 128 * REGS_MISC <= THREADS * REGS, "register plan");
 };
 
@@ -61,9 +61,22 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
+// waits for the loads from tensor memory in flight; what was loaded into `r` is not used before
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                   "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :: "memory");
+}
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+// one arrival for a warp, behind what all its lanes did
+__device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
 }
 template <int BITS> __host__ __device__ constexpr uint32_t pt_neg_base(int cls) {      // fp16 pairs of -(1024 / 2^p + bias), by class of bit position
     return BITS == 8 ? 0xE480E480u : BITS == 4 ? (cls == 0 ? 0xE408E408u : 0xD480D480u)
@@ -112,10 +125,10 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
     if (warp == 17) {
         if (lane < P::N_BARS) {
             const int i = lane;
-            const bool by_128 = i < KST || (i >= 2 * KST && i < 2 * KST + VST) || (i >= 2 * KST + 2 * VST + TS && i < 2 * KST + 2 * VST + TS + 2) ||
-                                (i >= 2 * KST + 2 * VST + TS + 4 && i < 2 * KST + 2 * VST + TS + 6);
-            const bool by_256 = i >= 2 * KST + 2 * VST && i < 2 * KST + 2 * VST + TS;
-            mbar_init(&bars[i], by_128 ? 128u : by_256 ? 256u : 1u);
+            const bool by_4 = i < KST || (i >= 2 * KST && i < 2 * KST + VST) || (i >= 2 * KST + 2 * VST + TS && i < 2 * KST + 2 * VST + TS + 2) ||
+                              (i >= 2 * KST + 2 * VST + TS + 4 && i < 2 * KST + 2 * VST + TS + 6);         // warps that arrive
+            const bool by_8 = i >= 2 * KST + 2 * VST && i < 2 * KST + 2 * VST + TS;
+            mbar_init(&bars[i], by_4 ? 4u : by_8 ? 8u : 1u);
         }
         if (lane == 0) *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -200,7 +213,7 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                 }
             }
             fence_async_smem();
-            mbar_arrive(&bar_q[t]);
+            warp_arrive(&bar_q[t], lane);
             const bool scaled = __any_sync(0xffffffffu, q_factor != 1.f);
             const PagedSpan span = paged_span(a, p_first + token, seq.kv);
             // keys between which every row of the query tile sees everything
@@ -217,72 +230,95 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                 if (!ok) break;
                 tc_fence_after();
                 const float* tab = reinterpret_cast<const float*>(smem + P::OFF_TAB) + (j % TS) * P::TAB_FLOATS;
-                uint32_t pk[PT_N / 2];
-                float2 sum;
-                float top;
-                auto pass = [&](auto masked_, auto scaled_) {
-                    constexpr bool MASKED = decltype(masked_)::value != 0, SCALED = decltype(scaled_)::value != 0;
-                    sum = make_float2(0.f, 0.f);
-                    top = -INFINITY;
-                    const float2 nm = make_float2(-m, -m), qf = make_float2(q_factor, q_factor);
+                const bool special = scaled || key0 + PT_N > all_hi || (key0 < all_lo && key0 + PT_N > a.sinks);
+                float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+                // a chunk of 32 scores -> 16 columns of P, over scores that are read already
+                auto chunk = [&](uint32_t (&s)[32], int c, auto special_) {
+                    constexpr bool SPECIAL = decltype(special_)::value != 0;
+                    const float *ta = tab + c * 32, *tb = ta + PT_N, *tc = tb + PT_N;
+                    float2 x[16];
+                    float top0 = -INFINITY, top1 = -INFINITY;
 #pragma unroll
-                    for (int c = 0; c < PT_N / 32; ++c) {
-                        uint32_t s[32];
-                        tmem_ld32(col_s + c * 32, s);
-                        tmem_wait_ld();
+                    for (int i = 0; i < 16; i += 2) {
+                        const float4 va = *reinterpret_cast<const float4*>(ta + 2 * i), vb = *reinterpret_cast<const float4*>(tb + 2 * i);
+                        x[i] = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+                        x[i + 1] = make_float2(__uint_as_float(s[2 * i + 2]), __uint_as_float(s[2 * i + 3]));
+                        if (SPECIAL) { x[i].x *= q_factor; x[i].y *= q_factor; x[i + 1].x *= q_factor; x[i + 1].y *= q_factor; }
+                        x[i] = fma2(x[i], make_float2(va.x, va.y), make_float2(vb.x, vb.y));
+                        x[i + 1] = fma2(x[i + 1], make_float2(va.z, va.w), make_float2(vb.z, vb.w));
+                        if (SPECIAL) {
+                            const int k = key0 + c * 32 + 2 * i;
+                            auto sees = [&](int key) { return key < span.hi && (key >= span.lo || key < a.sinks); };
+                            x[i].x = sees(k) ? x[i].x : -INFINITY; x[i].y = sees(k + 1) ? x[i].y : -INFINITY;
+                            x[i + 1].x = sees(k + 2) ? x[i + 1].x : -INFINITY; x[i + 1].y = sees(k + 3) ? x[i + 1].y : -INFINITY;
+                        }
+                        top0 = fmaxf(top0, fmaxf(x[i].x, x[i].y));
+                        top1 = fmaxf(top1, fmaxf(x[i + 1].x, x[i + 1].y));
+                    }
+                    top0 = fmaxf(top0, top1);
+                    if (__any_sync(0xffffffffu, top0 > m + PT_LAZY)) {
+                        const float mn = top0 > m + PT_LAZY ? top0 : m, alpha = ex2(m - mn);
+                        m = mn;
+                        l *= alpha;
+                        sum0.x *= alpha; sum0.y *= alpha; sum1.x *= alpha; sum1.y *= alpha;
+                        const __half2 ah = __float2half2_rn(alpha);
+                        const uint32_t au = *reinterpret_cast<const uint32_t*>(&ah);
+                        tmem_wait_st();
+#pragma unroll 1
+                        for (int z = 0; z < c; ++z) {             // P of the tile's chunks before this one
+                            uint32_t o[16];
+                            tmem_ld16(col_s + 16 * z, o);
+                            tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            const float4 ta = *reinterpret_cast<const float4*>(tab + c * 32 + i), tb = *reinterpret_cast<const float4*>(tab + PT_N + c * 32 + i),
-                                         tc = *reinterpret_cast<const float4*>(tab + 2 * PT_N + c * 32 + i);
+                            for (int i = 0; i < 16; ++i) o[i] = h2_mul(o[i], au);
+                            tmem_st16(col_s + 16 * z, o);
+                        }
+                        if (j > 0) {                              // the products of the tiles before are complete: S came behind them
+#pragma unroll 1
+                            for (int z = 0; z < D; z += 16) {
+                                uint32_t o[16];
+                                tmem_ld16(col_o + z, o);
+                                tmem_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                float2 x = make_float2(__uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1]));
-                                if (SCALED) { x.x *= qf.x; x.y *= qf.y; }
-                                x = fma2(x, e ? make_float2(ta.z, ta.w) : make_float2(ta.x, ta.y), e ? make_float2(tb.z, tb.w) : make_float2(tb.x, tb.y));
-                                if (MASKED) {
-                                    const int k = key0 + c * 32 + i + 2 * e;
-                                    x.x = k < span.hi && (k >= span.lo || k < a.sinks) ? x.x : -INFINITY;
-                                    x.y = k + 1 < span.hi && (k + 1 >= span.lo || k + 1 < a.sinks) ? x.y : -INFINITY;
-                                }
-                                top = fmaxf(top, fmaxf(x.x, x.y));
-                                x = add2(x, nm);
-                                const float2 p = make_float2(ex2(x.x), ex2(x.y));
-                                sum = fma2(p, e ? make_float2(tc.z, tc.w) : make_float2(tc.x, tc.y), sum);
-                                pk[(c * 32 + i) / 2 + e] = pack_half2(p.x, p.y);
+                                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                                tmem_st16(col_o + z, o);
                             }
                         }
                     }
-                };
-                const bool masked = key0 + PT_N > all_hi || (key0 < all_lo && key0 + PT_N > a.sinks);
-                auto compute = [&]() {
-                    if (scaled) { if (masked) pass(IntC<1>(), IntC<1>()); else pass(IntC<0>(), IntC<1>()); }
-                    else if (masked) pass(IntC<1>(), IntC<0>());
-                    else pass(IntC<0>(), IntC<0>());
-                };
-                compute();
-                if (__any_sync(0xffffffffu, top > m + PT_LAZY)) {
-                    const float mn = top > m + PT_LAZY ? top : m, alpha = ex2(m - mn);
-                    m = mn;
-                    l *= alpha;
-                    if (j > 0) {                     // the products of the tiles before are complete: S came behind them
-#pragma unroll 1
-                        for (int c = 0; c < D; c += 32) {
-                            uint32_t o[32];
-                            tmem_ld32(col_o + c, o);
-                            tmem_wait_ld();
+                    const float2 nm = make_float2(-m, -m);
+                    uint32_t pk[16];
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                            tmem_st32(col_o + c, o);
-                        }
+                    for (int i = 0; i < 16; i += 2) {
+                        const float4 vc = *reinterpret_cast<const float4*>(tc + 2 * i);
+                        x[i] = add2(x[i], nm);
+                        x[i + 1] = add2(x[i + 1], nm);
+                        x[i].x = ex2(x[i].x); x[i].y = ex2(x[i].y); x[i + 1].x = ex2(x[i + 1].x); x[i + 1].y = ex2(x[i + 1].y);
+                        sum0 = fma2(x[i], make_float2(vc.x, vc.y), sum0);
+                        sum1 = fma2(x[i + 1], make_float2(vc.z, vc.w), sum1);
+                        pk[i] = pack_half2(x[i].x, x[i].y);
+                        pk[i + 1] = pack_half2(x[i + 1].x, x[i + 1].y);
                     }
-                    compute();
-                }
-                l += sum.x + sum.y;
-                tmem_st32(col_s, pk);
-                tmem_st32(col_s + 32, pk + 32);
+                    tmem_st16(col_s + 16 * c, pk);
+                };
+                auto tile = [&](auto special_) {
+                    uint32_t s0[32], s1[32];
+                    tmem_ld32(col_s, s0);
+                    tmem_wait_ld32(s0);
+#pragma unroll 1
+                    for (int c = 0; c < PT_N / 32; c += 2) {      // the next chunk's scores in flight
+                        tmem_ld32(col_s + 32 * c + 32, s1);
+                        chunk(s0, c, special_);
+                        tmem_wait_ld32(s1);
+                        if (c + 2 < PT_N / 32) tmem_ld32(col_s + 32 * c + 64, s0);
+                        chunk(s1, c + 1, special_);
+                        tmem_wait_ld32(s0);
+                    }
+                };
+                if (special) tile(IntC<1>()); else tile(IntC<0>());
+                l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(&bar_p[t]);
+                warp_arrive(&bar_p[t], lane);
             }
             // ---- O / l, or this split's part
             if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bar_o[t], 0, abort_flag, 203));
@@ -402,8 +438,8 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                         sts128(tile + pt_chunk(key, nb * 8 + 2 * it + 1), hw[4], hw[5], hw[6], hw[7]);
                     }
                 fence_async_smem();
-                mbar_arrive(&full[st]);
-                mbar_arrive(&bar_tab[j % TS]);
+                warp_arrive(&full[st], lane);
+                warp_arrive(&bar_tab[j % TS], lane);
                 if (j + 1 < n_all) fetch_rows(j + 1);
                 if (j + 2 < n_all) fetch_pages(j + 2);
             }

@@ -201,6 +201,8 @@ int check_cache(const char* who, const varq_paged_t* c, PagedView& v) {
         return fail(VARQ_ERR_ARG, "%s: bits must be 2, 4 or 8 (got %d, %d)", who, c->k_bits, c->v_bits);
     if (!c->k_codes || !c->v_codes || !c->k_scale || !c->v_scale) return fail(VARQ_ERR_ARG, "%s: null pool", who);
     if (!aligned16(c->k_codes) || !aligned16(c->v_codes) || !aligned16(c->k_scale) || !aligned16(c->v_scale)) return fail(VARQ_ERR_ARG, "%s: pools must start on a 16-byte boundary", who);
+    if ((unsigned long long)c->n_pages * c->n_heads * c->page_size >= (1ull << 32))
+        return fail(VARQ_ERR_UNSUPPORTED, "%s: %d pages of %d tokens and %d heads are 2^32 rows or more", who, c->n_pages, c->page_size, c->n_heads);
     v.kc = c->k_codes; v.vc = c->v_codes; v.ks = c->k_scale; v.vs = c->v_scale;
     v.n_pages = c->n_pages; v.page_shift = 0;
     while ((1 << v.page_shift) < c->page_size) ++v.page_shift;

@@ -29,7 +29,7 @@ template <int D> struct PtPlan {
     static constexpr int TAB_FLOATS = 3 * PT_N;
     static constexpr int OFF_Q = 0, OFF_K = OFF_Q + 2 * Q_BYTES, OFF_V = OFF_K + KST * T_BYTES, OFF_TAB = OFF_V + VST * T_BYTES;
     static constexpr int OFF_BAR = OFF_TAB + TS * TAB_FLOATS * 4, N_BARS = 2 * KST + 2 * VST + TS + 9;
-    static constexpr int OFF_MISC = OFF_BAR + N_BARS * 8, SMEM = OFF_MISC + 16 + 1024;
+    static constexpr int OFF_QF = (OFF_BAR + N_BARS * 8 + 15) / 16 * 16, OFF_MISC = OFF_QF + 2 * PT_M * 4, SMEM = OFF_MISC + 16 + 1024;
     static constexpr int COL_S = 0, COL_O = 2 * PT_N, TMEM_COLS = 512;
     static_assert(COL_O + 2 * D <= TMEM_COLS && SMEM <= 227 * 1024, "plan");
     static constexpr int THREADS = 640, REGS = 96, REGS_SOFT = 136, REGS_CONV = 72, REGS_MISC = 64;
@@ -60,6 +60,20 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
         : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
+}
+// 16 rows x 32 columns: thread (g, c) = (lane / 4, lane % 4) gets columns 2c, 2c + 1 of every eight, of row g (r[4n], r[4n + 1]) and row g + 8
+__device__ __forceinline__ void tmem_ld_16x256(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr) : "memory");
+}
+// 16 rows x 16 columns: column c of every four, of row g (r[2n]) and row g + 8 (r[2n + 1])
+__device__ __forceinline__ void tmem_st_16x128(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 // waits for the loads from tensor memory in flight; what was loaded into `r` is not used before
 __device__ __forceinline__ void tmem_wait_ld32(uint32_t (&r)[32]) {
@@ -215,13 +229,25 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
             fence_async_smem();
             warp_arrive(&bar_q[t], lane);
             const bool scaled = __any_sync(0xffffffffu, q_factor != 1.f);
-            const PagedSpan span = paged_span(a, p_first + token, seq.kv);
+            if (scaled) reinterpret_cast<float*>(smem + P::OFF_QF)[t * PT_M + r] = q_factor;
+            __syncwarp();
             // keys between which every row of the query tile sees everything
             const int tl = min(row0 + t * PT_M + PT_M, rows) - 1, all_hi = a.causal ? p_first + (row0 + t * PT_M) / a.G + 1 : 0x7fffffff,
                       all_lo = a.window ? p_first + tl / a.G - a.window + 1 : 0;
-            float m = -1e30f, l = 0.f;
+            // A thread holds, of every eight columns of S, two of the rows g, g + 8, g + 16, g + 24 of its warp's 32 (g = lane / 4): it needs a quarter of
+            // the keys' tables and uses an entry for four rows
+            const int g = lane >> 2, cq = lane & 3;
+            float m[4] = {0.f, 0.f, 0.f, 0.f};
+            float2 l[4] = {};
+            unsigned unset = 15u;                                           // rows that have no reference yet: they have seen no key
             bool ok = true;
             const int n = n_t[t];
+            auto by_lane = [&](const float (&v)[4]) {                        // rows g + 8 i of a thread -> row `lane`
+                float o = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { const float x = __shfl_sync(0xffffffffu, v[i], (lane & 7) * 4); o = (lane >> 3) == i ? x : o; }
+                return o;
+            };
 #pragma unroll 1
             for (int j = 0; j < n; ++j) {
                 const int key0 = tiles.key(tile0 + j);
@@ -230,101 +256,146 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                 if (!ok) break;
                 tc_fence_after();
                 const float* tab = reinterpret_cast<const float*>(smem + P::OFF_TAB) + (j % TS) * P::TAB_FLOATS;
-                const bool special = scaled || key0 + PT_N > all_hi || (key0 < all_lo && key0 + PT_N > a.sinks);
-                float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
-                // a chunk of 32 scores -> 16 columns of P, over scores that are read already
-                auto chunk = [&](uint32_t (&s)[32], int c, auto special_) {
-                    constexpr bool SPECIAL = decltype(special_)::value != 0;
-                    const float *ta = tab + c * 32, *tb = ta + PT_N, *tc = tb + PT_N;
-                    float2 x[16];
+                const bool masked = key0 + PT_N > all_hi || (key0 < all_lo && key0 + PT_N > a.sinks);
+                // a chunk of 32 scores per row: x - m in place; references raised where an x passes its own by more than 8
+                auto scores = [&](uint32_t (&s)[32], int c) {
+                    if (scaled) {
+                        const float* qf = reinterpret_cast<const float*>(smem + P::OFF_QF) + t * PT_M + quarter * 32 + g;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * qf[8 * ((i >> 4) * 2 + ((i >> 1) & 1))]);
+                    }
                     float top0 = -INFINITY, top1 = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        const float4 va = *reinterpret_cast<const float4*>(ta + 2 * i), vb = *reinterpret_cast<const float4*>(tb + 2 * i);
-                        x[i] = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
-                        x[i + 1] = make_float2(__uint_as_float(s[2 * i + 2]), __uint_as_float(s[2 * i + 3]));
-                        if (SPECIAL) { x[i].x *= q_factor; x[i].y *= q_factor; x[i + 1].x *= q_factor; x[i + 1].y *= q_factor; }
-                        x[i] = fma2(x[i], make_float2(va.x, va.y), make_float2(vb.x, vb.y));
-                        x[i + 1] = fma2(x[i + 1], make_float2(va.z, va.w), make_float2(vb.z, vb.w));
-                        if (SPECIAL) {
-                            const int k = key0 + c * 32 + 2 * i;
-                            auto sees = [&](int key) { return key < span.hi && (key >= span.lo || key < a.sinks); };
-                            x[i].x = sees(k) ? x[i].x : -INFINITY; x[i].y = sees(k + 1) ? x[i].y : -INFINITY;
-                            x[i + 1].x = sees(k + 2) ? x[i + 1].x : -INFINITY; x[i + 1].y = sees(k + 3) ? x[i + 1].y : -INFINITY;
+                    for (int v = 0; v < 4; ++v) {
+                        const float4 ab = *reinterpret_cast<const float4*>(tab + (c * 16 + v * 4 + cq) * 4);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t* w = &s[(i >> 1) * 16 + v * 4 + (i & 1) * 2];
+                            float2 x = fma2(make_float2(__uint_as_float(w[0]), __uint_as_float(w[1])), make_float2(ab.x, ab.y), make_float2(ab.z, ab.w));
+                            x = add2(x, make_float2(-m[i], -m[i]));
+                            w[0] = __float_as_uint(x.x); w[1] = __float_as_uint(x.y);
                         }
-                        top0 = fmaxf(top0, fmaxf(x[i].x, x[i].y));
-                        top1 = fmaxf(top1, fmaxf(x[i + 1].x, x[i + 1].y));
                     }
-                    top0 = fmaxf(top0, top1);
-                    if (__any_sync(0xffffffffu, top0 > m + PT_LAZY)) {
-                        const float mn = top0 > m + PT_LAZY ? top0 : m, alpha = ex2(m - mn);
-                        m = mn;
-                        l *= alpha;
-                        sum0.x *= alpha; sum0.y *= alpha; sum1.x *= alpha; sum1.y *= alpha;
-                        const __half2 ah = __float2half2_rn(alpha);
-                        const uint32_t au = *reinterpret_cast<const uint32_t*>(&ah);
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const PagedSpan sp = paged_span(a, p_first + min(row0 + t * PT_M + quarter * 32 + g + 8 * i, rows - 1) / a.G, seq.kv);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const int k = key0 + c * 32 + (e >> 1) * 8 + 2 * cq + (e & 1);
+                                uint32_t& w = s[(i >> 1) * 16 + (e >> 1) * 4 + (i & 1) * 2 + (e & 1)];
+                                if (k >= sp.hi || (k < sp.lo && k >= a.sinks)) w = 0xff800000u;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        top0 = fmaxf(top0, fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 1])));
+                        top1 = fmaxf(top1, fmaxf(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])));
+                    }
+                    if (__any_sync(0xffffffffu, unset != 0u || fmaxf(top0, top1) > PT_LAZY)) {
+                        float alpha[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float up = -INFINITY;                            // how far the row's largest x is above its reference
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) up = fmaxf(up, __uint_as_float(s[(i >> 1) * 16 + (e >> 1) * 4 + (i & 1) * 2 + (e & 1)]));
+                            up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 1));
+                            up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 2));
+                            const bool first = (unset >> i & 1u) && up > -INFINITY;
+                            up = first || (up > PT_LAZY && !(unset >> i & 1u)) ? up : 0.f;
+                            alpha[i] = first ? 1.f : ex2(-up);               // (nothing is accumulated where the reference is the first)
+                            if (first) unset &= ~(1u << i);
+                            m[i] += up;
+                            l[i].x *= alpha[i]; l[i].y *= alpha[i];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                uint32_t& w = s[(i >> 1) * 16 + (e >> 1) * 4 + (i & 1) * 2 + (e & 1)];
+                                w = __float_as_uint(__uint_as_float(w) - up);
+                            }
+                        }
+                        const float al = by_lane(alpha);
+                        const __half2 ah = __float2half2_rn(al);
                         tmem_wait_st();
 #pragma unroll 1
-                        for (int z = 0; z < c; ++z) {             // P of the tile's chunks before this one
+                        for (int z = 0; z < c; ++z) {                        // P of the tile's chunks before this one
                             uint32_t o[16];
                             tmem_ld16(col_s + 16 * z, o);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = h2_mul(o[i], au);
+                            for (int i = 0; i < 16; ++i) o[i] = h2_mul(o[i], *reinterpret_cast<const uint32_t*>(&ah));
                             tmem_st16(col_s + 16 * z, o);
                         }
-                        if (j > 0) {                              // the products of the tiles before are complete: S came behind them
+                        if (j > 0) {                                         // the products of the tiles before are complete: S came behind them
 #pragma unroll 1
                             for (int z = 0; z < D; z += 16) {
                                 uint32_t o[16];
                                 tmem_ld16(col_o + z, o);
                                 tmem_wait_ld();
 #pragma unroll
-                                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
                                 tmem_st16(col_o + z, o);
                             }
                         }
                     }
-                    const float2 nm = make_float2(-m, -m);
+                };
+                // P of a chunk: 16 columns over scores that are read already
+                auto weights = [&](uint32_t (&s)[32], int c) {
                     uint32_t pk[16];
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        const float4 vc = *reinterpret_cast<const float4*>(tc + 2 * i);
-                        x[i] = add2(x[i], nm);
-                        x[i + 1] = add2(x[i + 1], nm);
-                        x[i].x = ex2(x[i].x); x[i].y = ex2(x[i].y); x[i + 1].x = ex2(x[i + 1].x); x[i + 1].y = ex2(x[i + 1].y);
-                        sum0 = fma2(x[i], make_float2(vc.x, vc.y), sum0);
-                        sum1 = fma2(x[i + 1], make_float2(vc.z, vc.w), sum1);
-                        pk[i] = pack_half2(x[i].x, x[i].y);
-                        pk[i + 1] = pack_half2(x[i + 1].x, x[i + 1].y);
+                    for (int v = 0; v < 4; ++v) {
+                        const float2 vc = *reinterpret_cast<const float2*>(tab + 2 * PT_N + c * 32 + v * 8 + 2 * cq);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t* w = &s[(i >> 1) * 16 + v * 4 + (i & 1) * 2];
+                            const float2 p = make_float2(ex2(__uint_as_float(w[0])), ex2(__uint_as_float(w[1])));
+                            l[i] = fma2(p, vc, l[i]);
+                            pk[(i >> 1) * 8 + v * 2 + (i & 1)] = pack_half2(p.x, p.y);
+                        }
                     }
-                    tmem_st16(col_s + 16 * c, pk);
+                    tmem_st_16x128(col_s + 16 * c, pk);
+                    tmem_st_16x128(col_s + 16 * c + (16u << 16), pk + 8);
                 };
-                auto tile = [&](auto special_) {
-                    uint32_t s0[32], s1[32];
-                    tmem_ld32(col_s, s0);
-                    tmem_wait_ld32(s0);
+                uint32_t s0[32], s1[32];
+                auto load = [&](uint32_t (&s)[32], int c) {
+                    tmem_ld_16x256(col_s + 32 * c, s);
+                    tmem_ld_16x256(col_s + 32 * c + (16u << 16), s + 16);
+                };
+                load(s0, 0);
+                tmem_wait_ld32(s0);
+                scores(s0, 0);
 #pragma unroll 1
-                    for (int c = 0; c < PT_N / 32; c += 2) {      // the next chunk's scores in flight
-                        tmem_ld32(col_s + 32 * c + 32, s1);
-                        chunk(s0, c, special_);
-                        tmem_wait_ld32(s1);
-                        if (c + 2 < PT_N / 32) tmem_ld32(col_s + 32 * c + 64, s0);
-                        chunk(s1, c + 1, special_);
-                        tmem_wait_ld32(s0);
-                    }
-                };
-                if (special) tile(IntC<1>()); else tile(IntC<0>());
-                l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
+                for (int c = 0; c < PT_N / 32; c += 2) {          // the next chunk's scores in flight
+                    load(s1, c + 1);
+                    weights(s0, c);
+                    tmem_wait_ld32(s1);
+                    scores(s1, c + 1);
+                    if (c + 2 < PT_N / 32) load(s0, c + 2);
+                    weights(s1, c + 1);
+                    if (c + 2 < PT_N / 32) { tmem_wait_ld32(s0); scores(s0, c + 2); }
+                }
                 tmem_wait_st();
                 tc_fence_before();
                 warp_arrive(&bar_p[t], lane);
+            }
+            float row_l, row_m;
+            {
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[i] = l[i].x + l[i].y;
+                    v[i] += __shfl_xor_sync(0xffffffffu, v[i], 1);
+                    v[i] += __shfl_xor_sync(0xffffffffu, v[i], 2);
+                    if (unset >> i & 1u) m[i] = -1e30f;
+                }
+                row_l = by_lane(v);
+                row_m = by_lane(m);
             }
             // ---- O / l, or this split's part
             if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bar_o[t], 0, abort_flag, 203));
             tc_fence_after();
             if (ok) {
-                const float inv = l != 0.f ? 1.f / l : 0.f;       // (a NaN stays one)
+                const float inv = row_l != 0.f ? 1.f / row_l : 0.f;       // (a NaN stays one)
                 const long long out_row = (long long)(seq.q0 + token) * a.Hq + head, n_rows = (long long)a.T * a.Hq;
                 const long long oo = (long long)(seq.q0 + token) * a.os_t + head * a.os_h;
 #pragma unroll 1
@@ -355,8 +426,8 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                         store_o_row32(ws_o, VARQ_F32, (split * n_rows + out_row) * D + c, v);
                     }
                 }
-                if (live && splits > 1) *reinterpret_cast<float2*>(ws_ml + (split * n_rows + out_row) * 2) = make_float2(m, l);
-                if (live && splits == 1 && a.lse) a.lse[out_row] = l != 0.f ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY;
+                if (live && splits > 1) *reinterpret_cast<float2*>(ws_ml + (split * n_rows + out_row) * 2) = make_float2(row_m, row_l);
+                if (live && splits == 1 && a.lse) a.lse[out_row] = row_l != 0.f ? (row_m + __log2f(row_l)) * 0.6931471805599453f : -INFINITY;
             }
         }
     } else if (warp < 16) {
@@ -372,75 +443,83 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
             constexpr int BITS = decltype(bits_)::value, NW = BITS / 2, WORDS = D * BITS / 32, NB = D / 64;
             CodeMagic<BITS> magic;
             magic.init();
-            int pg[4];
-            uint32_t w[4][NB][NW];
-            float sc;
+            uint32_t row[4], w[4][NB][NW];
+            float sc = 0.f;
+            const unsigned char* base = reinterpret_cast<const unsigned char*>(pool) + it * (NW * 4);
             auto fetch_pages = [&](int i) {
                 const int key0 = tiles.key(tile0 + i) + kq;
 #pragma unroll
-                for (int p = 0; p < 4; ++p) pg[p] = key0 + 32 * p < seq.kv ? __ldg(table + ((key0 + 32 * p) >> a.c.page_shift)) : -1;
-            };
-            auto fetch_rows = [&](int i) {
-                const int key0 = tiles.key(tile0 + i) + kq;
-                sc = 0.f;
-#pragma unroll
                 for (int p = 0; p < 4; ++p) {
                     const int key = key0 + 32 * p;
+                    row[p] = key < seq.kv ? (uint32_t)__ldg(table + (key >> a.c.page_shift)) : 0u;
+                }
+            };
+            auto fetch_rows = [&](int i, int p0, int p1) {
+                const int key0 = tiles.key(tile0 + i) + kq;
 #pragma unroll
-                    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                        for (int z = 0; z < NW; ++z) w[p][nb][z] = 0u;
+                for (int p = p0; p < p1; ++p) {
+                    const int key = key0 + 32 * p;
                     if (key < seq.kv) {
-                        const long long at = (((long long)paged_page(a, pg[p], status) * a.c.H + h) << a.c.page_shift) + (key & page_mask);
-                        const int32_t* src = pool + at * WORDS + it * NW;
+                        const uint32_t at = (((uint32_t)paged_page(a, (int)row[p], status) * a.c.H + h) << a.c.page_shift) + (key & page_mask);
+                        const unsigned char* src = base + (size_t)at * (WORDS * 4);
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb) {
                             if constexpr (NW == 4) {
-                                const uint4 x = __ldg(reinterpret_cast<const uint4*>(src + nb * 4 * NW));
+                                const uint4 x = __ldg(reinterpret_cast<const uint4*>(src + nb * 64));
                                 w[p][nb][0] = x.x; w[p][nb][1] = x.y; w[p][nb][2] = x.z; w[p][nb][3] = x.w;
                             } else if constexpr (NW == 2) {
-                                const uint2 x = __ldg(reinterpret_cast<const uint2*>(src + nb * 4 * NW));
+                                const uint2 x = __ldg(reinterpret_cast<const uint2*>(src + nb * 32));
                                 w[p][nb][0] = x.x; w[p][nb][1] = x.y;
-                            } else w[p][nb][0] = (uint32_t)__ldg(src + nb * 4 * NW);
+                            } else w[p][nb][0] = __ldg(reinterpret_cast<const uint32_t*>(src + nb * 16));
                         }
                         if (it == p) sc = __ldg(scales + at);
                     }
                 }
             };
-            if (n_all > 0) { fetch_pages(0); fetch_rows(0); }
-            if (n_all > 1) fetch_pages(1);
-#pragma unroll 1
-            for (int j = 0; j < n_all; ++j) {
-                const int st = j % 2;
-                if (j >= 2 && !mbar_wait(&freed[st], ((j >> 1) - 1) & 1, abort_flag, is_k ? 204 : 205)) break;
-                unsigned char* tile = stages + st * P::T_BYTES;
-                float* tab = reinterpret_cast<float*>(smem + P::OFF_TAB) + (j % TS) * P::TAB_FLOATS;
-                {
-                    const int k = kq + 32 * it;
-                    const bool there = tiles.key(tile0 + j) + k < seq.kv;
-                    if (is_k) tab[k] = there ? sc * a.scale_log2 : 0.f;
-                    else {                                      // a scale that is no number spoils the rows that see it, and no other: 0 * its inverse must be 0
-                        const bool fine = sc <= FLT_MAX;
-                        tab[PT_N + k] = there ? (fine ? __log2f(sc) : sc - sc) : -INFINITY;
-                        tab[2 * PT_N + k] = there && fine ? __fdividef(1.f, sc) : there ? 1.f : 0.f;
-                    }
-                }
+            auto convert = [&](unsigned char* tile, int p0, int p1) {
 #pragma unroll
-                for (int p = 0; p < 4; ++p)
+                for (int p = p0; p < p1; ++p)
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
                         uint32_t hw[8];
                         Item<BITS>::raw(w[p][nb], hw, magic);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) hw[i] = Item<BITS>::minus_zp(hw[i], i, pt_neg_base<BITS>(i % Item<BITS>::CLS));
-                        const int key = kq + 32 * p;
-                        sts128(tile + pt_chunk(key, nb * 8 + 2 * it), hw[0], hw[1], hw[2], hw[3]);
-                        sts128(tile + pt_chunk(key, nb * 8 + 2 * it + 1), hw[4], hw[5], hw[6], hw[7]);
+                        const uint32_t at = pt_chunk(kq, 2 * it) + nb * (128 * 128) + p * (32 * 128);
+                        sts128(tile + at, hw[0], hw[1], hw[2], hw[3]);
+                        sts128(tile + (at ^ 16u), hw[4], hw[5], hw[6], hw[7]);
                     }
+            };
+            // keys behind the sequence's end keep the words of an earlier tile (any codes are finite); their table entries hide them
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int z = 0; z < NW; ++z) w[p][nb][z] = 0u;
+            if (n_all > 0) { fetch_pages(0); fetch_rows(0, 0, 4); }
+            if (n_all > 1) fetch_pages(1);
+#pragma unroll 1
+            for (int j = 0; j < n_all; ++j) {
+                const int st = j % 2, k = kq + 32 * it;
+                if (j >= 2 && !mbar_wait(&freed[st], ((j >> 1) - 1) & 1, abort_flag, is_k ? 204 : 205)) break;
+                unsigned char* tile = stages + st * P::T_BYTES;
+                float* tab = reinterpret_cast<float*>(smem + P::OFF_TAB) + (j % TS) * P::TAB_FLOATS;
+                float* tab_a = tab + (k >> 1) * 4 + (k & 1);
+                const bool there = tiles.key(tile0 + j) + k < seq.kv;
+                if (is_k) tab_a[0] = there ? sc * a.scale_log2 : 0.f;
+                else {                                      // a scale that is no number spoils the rows that see it, and no other: 0 * its inverse must be 0
+                    const bool fine = sc <= FLT_MAX;
+                    tab_a[2] = there ? (fine ? __log2f(sc) : sc - sc) : -INFINITY;
+                    tab[2 * PT_N + k] = there && fine ? __fdividef(1.f, sc) : there ? 1.f : 0.f;
+                }
+                convert(tile, 0, 2);
+                if (j + 1 < n_all) fetch_rows(j + 1, 0, 2);
+                convert(tile, 2, 4);
                 fence_async_smem();
                 warp_arrive(&full[st], lane);
                 warp_arrive(&bar_tab[j % TS], lane);
-                if (j + 1 < n_all) fetch_rows(j + 1);
+                if (j + 1 < n_all) fetch_rows(j + 1, 2, 4);
                 if (j + 2 < n_all) fetch_pages(j + 2);
             }
         };

@@ -49,18 +49,14 @@ __device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint
         "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
+// pairs of fp32 in one 64-bit register
+using pair = unsigned long long;
+__device__ __forceinline__ pair pair_of(float x, float y) { pair d; asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y)); return d; }
+__device__ __forceinline__ float pair_x(pair p) { float x, y; asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); return x; }
+__device__ __forceinline__ float pair_y(pair p) { float x, y; asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); return y; }
+__device__ __forceinline__ pair fma2(pair a, pair b, pair c) { pair d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c)); return d; }
+__device__ __forceinline__ pair add2(pair a, pair b) { pair d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
+__device__ __forceinline__ pair mul2(pair a, pair b) { pair d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
 // 16 rows x 32 columns: thread (g, c) = (lane / 4, lane % 4) gets columns 2c, 2c + 1 of every eight, of row g (r[4n], r[4n + 1]) and row g + 8
 __device__ __forceinline__ void tmem_ld_16x256(uint32_t taddr, uint32_t* r) {
     asm volatile(
@@ -75,14 +71,8 @@ __device__ __forceinline__ void tmem_st_16x128(uint32_t taddr, const uint32_t* r
         "tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
         ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
-// waits for the loads from tensor memory in flight; what was loaded into `r` is not used before
-__device__ __forceinline__ void tmem_wait_ld32(uint32_t (&r)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
-                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
-                   "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-                 :: "memory");
-}
+// what a load from tensor memory left, behind the wait for it (volatile: not moved in front of that)
+__device__ __forceinline__ pair tmem_pair(uint32_t lo, uint32_t hi) { pair d; asm volatile("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi)); return d; }
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -237,8 +227,11 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
             // A thread holds, of every eight columns of S, two of the rows g, g + 8, g + 16, g + 24 of its warp's 32 (g = lane / 4): it needs a quarter of
             // the keys' tables and uses an entry for four rows
             const int g = lane >> 2, cq = lane & 3;
-            float m[4] = {0.f, 0.f, 0.f, 0.f};
-            float2 l[4] = {};
+            int pos[4];                                                     // positions of the four rows' tokens
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pos[i] = p_first + min(row0 + t * PT_M + quarter * 32 + g + 8 * i, rows - 1) / a.G;
+            pair nm[4] = {0ull, 0ull, 0ull, 0ull};                          // minus the reference, twice
+            pair l[4] = {0ull, 0ull, 0ull, 0ull};
             unsigned unset = 15u;                                           // rows that have no reference yet: they have seen no key
             bool ok = true;
             const int n = n_t[t];
@@ -258,40 +251,45 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                 const float* tab = reinterpret_cast<const float*>(smem + P::OFF_TAB) + (j % TS) * P::TAB_FLOATS;
                 const bool masked = key0 + PT_N > all_hi || (key0 < all_lo && key0 + PT_N > a.sinks);
                 // a chunk of 32 scores per row: x - m in place; references raised where an x passes its own by more than 8
-                auto scores = [&](uint32_t (&s)[32], int c) {
+                pair x[16];                                      // [half of the rows][eight columns][row g, g + 8]
+                auto scores = [&](const uint32_t (&s)[32], int c) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = tmem_pair(s[2 * i], s[2 * i + 1]);
                     if (scaled) {
                         const float* qf = reinterpret_cast<const float*>(smem + P::OFF_QF) + t * PT_M + quarter * 32 + g;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * qf[8 * ((i >> 4) * 2 + ((i >> 1) & 1))]);
+                        for (int i = 0; i < 16; ++i) { const float f = qf[8 * ((i >> 3) * 2 + (i & 1))]; x[i] = mul2(x[i], pair_of(f, f)); }
                     }
-                    float top0 = -INFINITY, top1 = -INFINITY;
 #pragma unroll
                     for (int v = 0; v < 4; ++v) {
-                        const float4 ab = *reinterpret_cast<const float4*>(tab + (c * 16 + v * 4 + cq) * 4);
+                        const ulonglong2 ab = *reinterpret_cast<const ulonglong2*>(tab + (c * 16 + v * 4 + cq) * 4);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            uint32_t* w = &s[(i >> 1) * 16 + v * 4 + (i & 1) * 2];
-                            float2 x = fma2(make_float2(__uint_as_float(w[0]), __uint_as_float(w[1])), make_float2(ab.x, ab.y), make_float2(ab.z, ab.w));
-                            x = add2(x, make_float2(-m[i], -m[i]));
-                            w[0] = __float_as_uint(x.x); w[1] = __float_as_uint(x.y);
+                            pair& y = x[(i >> 1) * 8 + v * 2 + (i & 1)];
+                            y = add2(fma2(y, ab.x, ab.y), nm[i]);
                         }
                     }
                     if (masked) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const PagedSpan sp = paged_span(a, p_first + min(row0 + t * PT_M + quarter * 32 + g + 8 * i, rows - 1) / a.G, seq.kv);
+                            const PagedSpan sp = paged_span(a, pos[i], seq.kv);
+                            // bit k: this thread's column 2c + k of the 32 is seen
+                            auto below = [](int k) { return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1u; };
+                            const int c0 = key0 + 32 * c + 2 * cq;
+                            const uint32_t sees = below(sp.hi - c0) & (~below(sp.lo - c0) | below(a.sinks - c0));
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const int k = key0 + c * 32 + (e >> 1) * 8 + 2 * cq + (e & 1);
-                                uint32_t& w = s[(i >> 1) * 16 + (e >> 1) * 4 + (i & 1) * 2 + (e & 1)];
-                                if (k >= sp.hi || (k < sp.lo && k >= a.sinks)) w = 0xff800000u;
+                            for (int v = 0; v < 4; ++v) {
+                                pair& y = x[(i >> 1) * 8 + v * 2 + (i & 1)];
+                                y = pair_of(sees >> (8 * v) & 1u ? pair_x(y) : -INFINITY, sees >> (8 * v + 1) & 1u ? pair_y(y) : -INFINITY);
                             }
                         }
+                        asm volatile("" ::: "memory");          // one copy of what follows, not one per branch
                     }
+                    float top0 = -INFINITY, top1 = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        top0 = fmaxf(top0, fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 1])));
-                        top1 = fmaxf(top1, fmaxf(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])));
+                    for (int i = 0; i < 16; i += 2) {
+                        top0 = fmaxf(top0, fmaxf(pair_x(x[i]), pair_y(x[i])));
+                        top1 = fmaxf(top1, fmaxf(pair_x(x[i + 1]), pair_y(x[i + 1])));
                     }
                     if (__any_sync(0xffffffffu, unset != 0u || fmaxf(top0, top1) > PT_LAZY)) {
                         float alpha[4];
@@ -299,20 +297,17 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                         for (int i = 0; i < 4; ++i) {
                             float up = -INFINITY;                            // how far the row's largest x is above its reference
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) up = fmaxf(up, __uint_as_float(s[(i >> 1) * 16 + (e >> 1) * 4 + (i & 1) * 2 + (e & 1)]));
+                            for (int v = 0; v < 4; ++v) { const pair y = x[(i >> 1) * 8 + v * 2 + (i & 1)]; up = fmaxf(up, fmaxf(pair_x(y), pair_y(y))); }
                             up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 1));
                             up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 2));
                             const bool first = (unset >> i & 1u) && up > -INFINITY;
                             up = first || (up > PT_LAZY && !(unset >> i & 1u)) ? up : 0.f;
                             alpha[i] = first ? 1.f : ex2(-up);               // (nothing is accumulated where the reference is the first)
                             if (first) unset &= ~(1u << i);
-                            m[i] += up;
-                            l[i].x *= alpha[i]; l[i].y *= alpha[i];
+                            nm[i] = add2(nm[i], pair_of(-up, -up));
+                            l[i] = mul2(l[i], pair_of(alpha[i], alpha[i]));
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                uint32_t& w = s[(i >> 1) * 16 + (e >> 1) * 4 + (i & 1) * 2 + (e & 1)];
-                                w = __float_as_uint(__uint_as_float(w) - up);
-                            }
+                            for (int v = 0; v < 4; ++v) { pair& y = x[(i >> 1) * 8 + v * 2 + (i & 1)]; y = add2(y, pair_of(-up, -up)); }
                         }
                         const float al = by_lane(alpha);
                         const __half2 ah = __float2half2_rn(al);
@@ -340,39 +335,30 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                     }
                 };
                 // P of a chunk: 16 columns over scores that are read already
-                auto weights = [&](uint32_t (&s)[32], int c) {
+                auto weights = [&](int c) {
                     uint32_t pk[16];
 #pragma unroll
                     for (int v = 0; v < 4; ++v) {
-                        const float2 vc = *reinterpret_cast<const float2*>(tab + 2 * PT_N + c * 32 + v * 8 + 2 * cq);
+                        const pair vc = *reinterpret_cast<const pair*>(tab + 2 * PT_N + c * 32 + v * 8 + 2 * cq);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const uint32_t* w = &s[(i >> 1) * 16 + v * 4 + (i & 1) * 2];
-                            const float2 p = make_float2(ex2(__uint_as_float(w[0])), ex2(__uint_as_float(w[1])));
-                            l[i] = fma2(p, vc, l[i]);
-                            pk[(i >> 1) * 8 + v * 2 + (i & 1)] = pack_half2(p.x, p.y);
+                            const pair y = x[(i >> 1) * 8 + v * 2 + (i & 1)];
+                            const float p0 = ex2(pair_x(y)), p1 = ex2(pair_y(y));
+                            l[i] = fma2(pair_of(p0, p1), vc, l[i]);
+                            pk[(i >> 1) * 8 + v * 2 + (i & 1)] = pack_half2(p0, p1);
                         }
                     }
                     tmem_st_16x128(col_s + 16 * c, pk);
                     tmem_st_16x128(col_s + 16 * c + (16u << 16), pk + 8);
                 };
-                uint32_t s0[32], s1[32];
-                auto load = [&](uint32_t (&s)[32], int c) {
+#pragma unroll 1
+                for (int c = 0; c < PT_N / 32; ++c) {
+                    uint32_t s[32];
                     tmem_ld_16x256(col_s + 32 * c, s);
                     tmem_ld_16x256(col_s + 32 * c + (16u << 16), s + 16);
-                };
-                load(s0, 0);
-                tmem_wait_ld32(s0);
-                scores(s0, 0);
-#pragma unroll 1
-                for (int c = 0; c < PT_N / 32; c += 2) {          // the next chunk's scores in flight
-                    load(s1, c + 1);
-                    weights(s0, c);
-                    tmem_wait_ld32(s1);
-                    scores(s1, c + 1);
-                    if (c + 2 < PT_N / 32) load(s0, c + 2);
-                    weights(s1, c + 1);
-                    if (c + 2 < PT_N / 32) { tmem_wait_ld32(s0); scores(s0, c + 2); }
+                    tmem_wait_ld();
+                    scores(s, c);
+                    weights(c);
                 }
                 tmem_wait_st();
                 tc_fence_before();
@@ -380,13 +366,13 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
             }
             float row_l, row_m;
             {
-                float v[4];
+                float v[4], m[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    v[i] = l[i].x + l[i].y;
+                    v[i] = pair_x(l[i]) + pair_y(l[i]);
                     v[i] += __shfl_xor_sync(0xffffffffu, v[i], 1);
                     v[i] += __shfl_xor_sync(0xffffffffu, v[i], 2);
-                    if (unset >> i & 1u) m[i] = -1e30f;
+                    m[i] = unset >> i & 1u ? -1e30f : -pair_x(nm[i]);
                 }
                 row_l = by_lane(v);
                 row_m = by_lane(m);
@@ -476,6 +462,7 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                     }
                 }
             };
+            const uint32_t d0 = pt_chunk(kq, 2 * it), d1 = pt_chunk(kq, 2 * it + 1);
             auto convert = [&](unsigned char* tile, int p0, int p1) {
 #pragma unroll
                 for (int p = p0; p < p1; ++p)
@@ -485,9 +472,8 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                         Item<BITS>::raw(w[p][nb], hw, magic);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) hw[i] = Item<BITS>::minus_zp(hw[i], i, pt_neg_base<BITS>(i % Item<BITS>::CLS));
-                        const uint32_t at = pt_chunk(kq, 2 * it) + nb * (128 * 128) + p * (32 * 128);
-                        sts128(tile + at, hw[0], hw[1], hw[2], hw[3]);
-                        sts128(tile + (at ^ 16u), hw[4], hw[5], hw[6], hw[7]);
+                        sts128(tile + d0 + nb * (128 * 128) + p * (32 * 128), hw[0], hw[1], hw[2], hw[3]);
+                        sts128(tile + d1 + nb * (128 * 128) + p * (32 * 128), hw[4], hw[5], hw[6], hw[7]);
                     }
             };
             // keys behind the sequence's end keep the words of an earlier tile (any codes are finite); their table entries hide them
@@ -514,12 +500,11 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                     tab[2 * PT_N + k] = there && fine ? __fdividef(1.f, sc) : there ? 1.f : 0.f;
                 }
                 convert(tile, 0, 2);
-                if (j + 1 < n_all) fetch_rows(j + 1, 0, 2);
                 convert(tile, 2, 4);
                 fence_async_smem();
                 warp_arrive(&full[st], lane);
                 warp_arrive(&bar_tab[j % TS], lane);
-                if (j + 1 < n_all) fetch_rows(j + 1, 2, 4);
+                if (j + 1 < n_all) fetch_rows(j + 1, 0, 4);
                 if (j + 2 < n_all) fetch_pages(j + 2);
             }
         };

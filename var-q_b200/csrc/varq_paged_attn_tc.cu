@@ -71,8 +71,16 @@ __device__ __forceinline__ void tmem_st_16x128(uint32_t taddr, const uint32_t* r
         "tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
         ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
-// what a load from tensor memory left, behind the wait for it (volatile: not moved in front of that)
-__device__ __forceinline__ pair tmem_pair(uint32_t lo, uint32_t hi) { pair d; asm volatile("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi)); return d; }
+// waits for the loads from tensor memory in flight, and keeps the use of what they left in `r` behind that
+__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                   "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]),
+                   "+r"(r[31])
+                 :: "memory");
+}
+__device__ __forceinline__ pair pair_of_bits(uint32_t x, uint32_t y) { pair d; asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(x), "r"(y)); return d; }
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -249,117 +257,112 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                 if (!ok) break;
                 tc_fence_after();
                 const float* tab = reinterpret_cast<const float*>(smem + P::OFF_TAB) + (j % TS) * P::TAB_FLOATS;
-                const bool masked = key0 + PT_N > all_hi || (key0 < all_lo && key0 + PT_N > a.sinks);
-                // a chunk of 32 scores per row: x - m in place; references raised where an x passes its own by more than 8
-                pair x[16];                                      // [half of the rows][eight columns][row g, g + 8]
-                auto scores = [&](const uint32_t (&s)[32], int c) {
+                // Two forms of a tile, so that the usual one carries neither masks nor factors: as branches inside they cost 10 % of a long call
+                auto tile = [&](auto special_) {
+                    constexpr bool SPECIAL = decltype(special_)::value != 0;
+#pragma unroll 1
+                    for (int c = 0; c < PT_N / 32; ++c) {
+                        pair x[16];                              // x - m of 32 columns: [half of the rows][eight columns][row g, g + 8]
+                        bool again = true;
+#pragma unroll 1
+                        while (true) {
+                            uint32_t s[32];
+                            tmem_ld_16x256(col_s + 32 * c, s);
+                            tmem_ld_16x256(col_s + 32 * c + (16u << 16), s + 16);
+                            tmem_loaded(s);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = tmem_pair(s[2 * i], s[2 * i + 1]);
-                    if (scaled) {
-                        const float* qf = reinterpret_cast<const float*>(smem + P::OFF_QF) + t * PT_M + quarter * 32 + g;
+                            for (int i = 0; i < 16; ++i) x[i] = pair_of_bits(s[2 * i], s[2 * i + 1]);
+                            if (SPECIAL && scaled) {
+                                const float* qf = reinterpret_cast<const float*>(smem + P::OFF_QF) + t * PT_M + quarter * 32 + g;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) { const float f = qf[8 * ((i >> 3) * 2 + (i & 1))]; x[i] = mul2(x[i], pair_of(f, f)); }
-                    }
-#pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        const ulonglong2 ab = *reinterpret_cast<const ulonglong2*>(tab + (c * 16 + v * 4 + cq) * 4);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            pair& y = x[(i >> 1) * 8 + v * 2 + (i & 1)];
-                            y = add2(fma2(y, ab.x, ab.y), nm[i]);
-                        }
-                    }
-                    if (masked) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const PagedSpan sp = paged_span(a, pos[i], seq.kv);
-                            // bit k: this thread's column 2c + k of the 32 is seen
-                            auto below = [](int k) { return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1u; };
-                            const int c0 = key0 + 32 * c + 2 * cq;
-                            const uint32_t sees = below(sp.hi - c0) & (~below(sp.lo - c0) | below(a.sinks - c0));
+                                for (int i = 0; i < 16; ++i) { const float f = qf[8 * ((i >> 3) * 2 + (i & 1))]; x[i] = mul2(x[i], pair_of(f, f)); }
+                            }
 #pragma unroll
                             for (int v = 0; v < 4; ++v) {
-                                pair& y = x[(i >> 1) * 8 + v * 2 + (i & 1)];
-                                y = pair_of(sees >> (8 * v) & 1u ? pair_x(y) : -INFINITY, sees >> (8 * v + 1) & 1u ? pair_y(y) : -INFINITY);
+                                const ulonglong2 ab = *reinterpret_cast<const ulonglong2*>(tab + (c * 16 + v * 4 + cq) * 4);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) { pair& y = x[(i >> 1) * 8 + v * 2 + (i & 1)]; y = add2(fma2(y, ab.x, ab.y), nm[i]); }
                             }
-                        }
-                        asm volatile("" ::: "memory");          // one copy of what follows, not one per branch
-                    }
-                    float top0 = -INFINITY, top1 = -INFINITY;
+                            if (SPECIAL) {
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        top0 = fmaxf(top0, fmaxf(pair_x(x[i]), pair_y(x[i])));
-                        top1 = fmaxf(top1, fmaxf(pair_x(x[i + 1]), pair_y(x[i + 1])));
-                    }
-                    if (__any_sync(0xffffffffu, unset != 0u || fmaxf(top0, top1) > PT_LAZY)) {
-                        float alpha[4];
+                                for (int i = 0; i < 4; ++i) {
+                                    const PagedSpan sp = paged_span(a, pos[i], seq.kv);
+                                    // bit k: this thread's column 2c + k of the 32 is seen
+                                    auto below = [](int k) { return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1u; };
+                                    const int c0 = key0 + 32 * c + 2 * cq;
+                                    const uint32_t sees = below(sp.hi - c0) & (~below(sp.lo - c0) | below(a.sinks - c0));
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float up = -INFINITY;                            // how far the row's largest x is above its reference
+                                    for (int v = 0; v < 4; ++v) {
+                                        pair& y = x[(i >> 1) * 8 + v * 2 + (i & 1)];
+                                        y = pair_of(sees >> (8 * v) & 1u ? pair_x(y) : -INFINITY, sees >> (8 * v + 1) & 1u ? pair_y(y) : -INFINITY);
+                                    }
+                                }
+                            }
+                            float top0 = -INFINITY, top1 = -INFINITY;
 #pragma unroll
-                            for (int v = 0; v < 4; ++v) { const pair y = x[(i >> 1) * 8 + v * 2 + (i & 1)]; up = fmaxf(up, fmaxf(pair_x(y), pair_y(y))); }
-                            up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 1));
-                            up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 2));
-                            const bool first = (unset >> i & 1u) && up > -INFINITY;
-                            up = first || (up > PT_LAZY && !(unset >> i & 1u)) ? up : 0.f;
-                            alpha[i] = first ? 1.f : ex2(-up);               // (nothing is accumulated where the reference is the first)
-                            if (first) unset &= ~(1u << i);
-                            nm[i] = add2(nm[i], pair_of(-up, -up));
-                            l[i] = mul2(l[i], pair_of(alpha[i], alpha[i]));
+                            for (int i = 0; i < 16; i += 2) {
+                                top0 = fmaxf(top0, fmaxf(pair_x(x[i]), pair_y(x[i])));
+                                top1 = fmaxf(top1, fmaxf(pair_x(x[i + 1]), pair_y(x[i + 1])));
+                            }
+                            if (!again || !__any_sync(0xffffffffu, unset != 0u || fmaxf(top0, top1) > PT_LAZY)) break;
+                            // new references, then the chunk once more: changed in place, x would be copied on the way that is always taken
+                            again = false;
+                            float alpha[4];
 #pragma unroll
-                            for (int v = 0; v < 4; ++v) { pair& y = x[(i >> 1) * 8 + v * 2 + (i & 1)]; y = add2(y, pair_of(-up, -up)); }
-                        }
-                        const float al = by_lane(alpha);
-                        const __half2 ah = __float2half2_rn(al);
-                        tmem_wait_st();
+                            for (int i = 0; i < 4; ++i) {
+                                float up = -INFINITY;                        // how far the row's largest x is above its reference
+#pragma unroll
+                                for (int v = 0; v < 4; ++v) { const pair y = x[(i >> 1) * 8 + v * 2 + (i & 1)]; up = fmaxf(up, fmaxf(pair_x(y), pair_y(y))); }
+                                up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 1));
+                                up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 2));
+                                const bool first = (unset >> i & 1u) && up > -INFINITY;
+                                up = first || (up > PT_LAZY && !(unset >> i & 1u)) ? up : 0.f;
+                                alpha[i] = first ? 1.f : ex2(-up);           // (nothing is accumulated where the reference is the first)
+                                if (first) unset &= ~(1u << i);
+                                nm[i] = add2(nm[i], pair_of(-up, -up));
+                                l[i] = mul2(l[i], pair_of(alpha[i], alpha[i]));
+                            }
+                            const float al = by_lane(alpha);
+                            const __half2 ah = __float2half2_rn(al);
+                            tmem_wait_st();
 #pragma unroll 1
-                        for (int z = 0; z < c; ++z) {                        // P of the tile's chunks before this one
-                            uint32_t o[16];
-                            tmem_ld16(col_s + 16 * z, o);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = h2_mul(o[i], *reinterpret_cast<const uint32_t*>(&ah));
-                            tmem_st16(col_s + 16 * z, o);
-                        }
-                        if (j > 0) {                                         // the products of the tiles before are complete: S came behind them
-#pragma unroll 1
-                            for (int z = 0; z < D; z += 16) {
+                            for (int z = 0; z < c; ++z) {                    // P of the tile's chunks before this one
                                 uint32_t o[16];
-                                tmem_ld16(col_o + z, o);
+                                tmem_ld16(col_s + 16 * z, o);
                                 tmem_wait_ld();
 #pragma unroll
-                                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
-                                tmem_st16(col_o + z, o);
+                                for (int i = 0; i < 16; ++i) o[i] = h2_mul(o[i], *reinterpret_cast<const uint32_t*>(&ah));
+                                tmem_st16(col_s + 16 * z, o);
+                            }
+                            if (j > 0) {                                     // the products of the tiles before are complete: S came behind them
+#pragma unroll 1
+                                for (int z = 0; z < D; z += 16) {
+                                    uint32_t o[16];
+                                    tmem_ld16(col_o + z, o);
+                                    tmem_wait_ld();
+#pragma unroll
+                                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
+                                    tmem_st16(col_o + z, o);
+                                }
                             }
                         }
-                    }
-                };
-                // P of a chunk: 16 columns over scores that are read already
-                auto weights = [&](int c) {
-                    uint32_t pk[16];
+                        uint32_t pk[16];                         // P of the chunk: 16 columns over scores that are read already
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        const pair vc = *reinterpret_cast<const pair*>(tab + 2 * PT_N + c * 32 + v * 8 + 2 * cq);
+                        for (int v = 0; v < 4; ++v) {
+                            const pair vc = *reinterpret_cast<const pair*>(tab + 2 * PT_N + c * 32 + v * 8 + 2 * cq);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const pair y = x[(i >> 1) * 8 + v * 2 + (i & 1)];
-                            const float p0 = ex2(pair_x(y)), p1 = ex2(pair_y(y));
-                            l[i] = fma2(pair_of(p0, p1), vc, l[i]);
-                            pk[(i >> 1) * 8 + v * 2 + (i & 1)] = pack_half2(p0, p1);
+                            for (int i = 0; i < 4; ++i) {
+                                const pair y = x[(i >> 1) * 8 + v * 2 + (i & 1)];
+                                const float p0 = ex2(pair_x(y)), p1 = ex2(pair_y(y));
+                                l[i] = fma2(pair_of(p0, p1), vc, l[i]);
+                                pk[(i >> 1) * 8 + v * 2 + (i & 1)] = pack_half2(p0, p1);
+                            }
                         }
+                        tmem_st_16x128(col_s + 16 * c, pk);
+                        tmem_st_16x128(col_s + 16 * c + (16u << 16), pk + 8);
                     }
-                    tmem_st_16x128(col_s + 16 * c, pk);
-                    tmem_st_16x128(col_s + 16 * c + (16u << 16), pk + 8);
                 };
-#pragma unroll 1
-                for (int c = 0; c < PT_N / 32; ++c) {
-                    uint32_t s[32];
-                    tmem_ld_16x256(col_s + 32 * c, s);
-                    tmem_ld_16x256(col_s + 32 * c + (16u << 16), s + 16);
-                    tmem_wait_ld();
-                    scores(s, c);
-                    weights(c);
-                }
+                if (scaled || key0 + PT_N > all_hi || (key0 < all_lo && key0 + PT_N > a.sinks)) tile(IntC<1>()); else tile(IntC<0>());
                 tmem_wait_st();
                 tc_fence_before();
                 warp_arrive(&bar_p[t], lane);
@@ -429,24 +432,25 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
             constexpr int BITS = decltype(bits_)::value, NW = BITS / 2, WORDS = D * BITS / 32, NB = D / 64;
             CodeMagic<BITS> magic;
             magic.init();
-            uint32_t row[4], w[4][NB][NW];
-            float sc = 0.f;
+            uint32_t w[4][NB][NW];
+            int page = 0;                              // of key kq + 32 * it of the next tile
+            float sc = 0.f;                            // that key's scale
             const unsigned char* base = reinterpret_cast<const unsigned char*>(pool) + it * (NW * 4);
             auto fetch_pages = [&](int i) {
-                const int key0 = tiles.key(tile0 + i) + kq;
+                const int key = tiles.key(tile0 + i) + kq + 32 * it;
+                page = key < seq.kv ? __ldg(table + (key >> a.c.page_shift)) : -1;
+            };
+            auto fetch_rows = [&](int i) {             // a lane of four looks up one of their four keys
+                const int key = tiles.key(tile0 + i) + kq + 32 * it;
+                uint32_t own = ~0u;
+                if (key < seq.kv) {
+                    own = (uint32_t)((paged_page(a, page, status) * a.c.H + h) << a.c.page_shift) + (key & page_mask);
+                    sc = __ldg(scales + own);
+                }
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
-                    const int key = key0 + 32 * p;
-                    row[p] = key < seq.kv ? (uint32_t)__ldg(table + (key >> a.c.page_shift)) : 0u;
-                }
-            };
-            auto fetch_rows = [&](int i, int p0, int p1) {
-                const int key0 = tiles.key(tile0 + i) + kq;
-#pragma unroll
-                for (int p = p0; p < p1; ++p) {
-                    const int key = key0 + 32 * p;
-                    if (key < seq.kv) {
-                        const uint32_t at = (((uint32_t)paged_page(a, (int)row[p], status) * a.c.H + h) << a.c.page_shift) + (key & page_mask);
+                    const uint32_t at = __shfl_sync(0xffffffffu, own, p, 4);
+                    if (at != ~0u) {
                         const unsigned char* src = base + (size_t)at * (WORDS * 4);
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb) {
@@ -458,14 +462,13 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                                 w[p][nb][0] = x.x; w[p][nb][1] = x.y;
                             } else w[p][nb][0] = __ldg(reinterpret_cast<const uint32_t*>(src + nb * 16));
                         }
-                        if (it == p) sc = __ldg(scales + at);
                     }
                 }
             };
             const uint32_t d0 = pt_chunk(kq, 2 * it), d1 = pt_chunk(kq, 2 * it + 1);
-            auto convert = [&](unsigned char* tile, int p0, int p1) {
+            auto convert = [&](unsigned char* tile) {
 #pragma unroll
-                for (int p = p0; p < p1; ++p)
+                for (int p = 0; p < 4; ++p)
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
                         uint32_t hw[8];
@@ -483,7 +486,7 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                     for (int z = 0; z < NW; ++z) w[p][nb][z] = 0u;
-            if (n_all > 0) { fetch_pages(0); fetch_rows(0, 0, 4); }
+            if (n_all > 0) { fetch_pages(0); fetch_rows(0); }
             if (n_all > 1) fetch_pages(1);
 #pragma unroll 1
             for (int j = 0; j < n_all; ++j) {
@@ -499,12 +502,11 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                     tab_a[2] = there ? (fine ? __log2f(sc) : sc - sc) : -INFINITY;
                     tab[2 * PT_N + k] = there && fine ? __fdividef(1.f, sc) : there ? 1.f : 0.f;
                 }
-                convert(tile, 0, 2);
-                convert(tile, 2, 4);
+                convert(tile);
                 fence_async_smem();
                 warp_arrive(&full[st], lane);
                 warp_arrive(&bar_tab[j % TS], lane);
-                if (j + 1 < n_all) fetch_rows(j + 1, 0, 4);
+                if (j + 1 < n_all) fetch_rows(j + 1);
                 if (j + 2 < n_all) fetch_pages(j + 2);
             }
         };

@@ -218,7 +218,8 @@ int varq_unpack_dequant(const varq_tensor_t* codes, int32_t B, int32_t L, int32_
  * CUDA-core kernel, the streaming CUDA-core kernel, the tcgen05 tensor-core kernel, the warp-level tensor-core
  * kernel of the early scales (MID), that of a few queries over a long cache (DECODE) or the fp32 kernel of the first scales (EARLY).
  * A pinned kernel that cannot take a call (shape, layout, grouping) yields to the
- * next one in the automatic order and finally to the general kernel.  For tests and measurements that compare the kernels on
+ * next one in the automatic order and finally to the general kernel.  TC and DECODE pin the kernel of varq_paged_attn, too, which take
+ * every call of it.  For tests and measurements that compare the kernels on
  * one input; no counterpart in the reference. */
 #define VARQ_ATTN_PATH_AUTO   0
 #define VARQ_ATTN_PATH_SMALL  1

@@ -7,6 +7,7 @@ using namespace varq;
 // Kernel choice pinned by varq_attn_force_path (0 = automatic).  A test hook, not a fallback switch: a pinned
 // kernel that cannot take the call still yields to the general CUDA-core kernel.
 static int g_forced_path = 0;
+int varq::forced_attn_path() { return g_forced_path; }
 
 static bool words_aligned16(const varq_tensor_t* t, int words) {
     return (words % 4 == 0) && aligned16(t->ptr) && (t->stride_b % 4 == 0) && (t->stride_l % 4 == 0) &&

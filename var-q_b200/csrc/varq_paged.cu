@@ -313,13 +313,13 @@ struct AttnPlan {
     bool tc;
     int splits, tiles_per_split;       // tiles of 16 keys (decode kernel)
 };
-AttnPlan plan_attn(int B, int H, int G, int max_q, int max_kv, int window, int sinks) {
+AttnPlan plan_attn(int B, int H, int D, int G, int max_q, int max_kv, int window, int sinks) {
     AttnPlan p;
     const long long rows = (long long)max_q * G;
     const long long span = window && (long long)window + max_q + sinks < max_kv ? (long long)window + max_q + sinks : max_kv;      // keys of a CTA, about
-    p.tc = rows > 16;
+    p.tc = forced_attn_path() == VARQ_ATTN_PATH_TC || (forced_attn_path() != VARQ_ATTN_PATH_DECODE && rows > (D == 64 ? 80 : 48));
     const long long units = p.tc ? 128 : 16, tiles = (span + units - 1) / units > 0 ? (span + units - 1) / units : 1;
-    const long long base = (long long)B * H * (p.tc ? (rows + 255) / 256 : 1), room = (long long)sm_count() * (p.tc ? 1 : 3);
+    const long long base = (long long)B * H * (p.tc ? (rows + 255) / 256 : (rows + 15) / 16), room = (long long)sm_count() * (p.tc ? 1 : 3);
     // the number of parts that makes the waves of CTAs shortest, a CTA costing its tiles and a fixed part (set-up and merging)
     const long long fixed = p.tc ? 4 : 16, least = p.tc ? 2 : 16;
     long long best = 0;
@@ -341,7 +341,7 @@ extern "C" size_t varq_paged_attn_workspace_bytes(const varq_paged_t* cache, con
         batch->window < 0 || batch->sinks < 0 || cache->head_dim < 1)
         return 0;
     const int max_q = (int)(batch->max_q < batch->n_queries ? batch->max_q : batch->n_queries);
-    const AttnPlan p = plan_attn(batch->n_seqs, cache->n_heads, batch->q_heads / cache->n_heads, max_q, batch->max_kv, batch->window, batch->sinks);
+    const AttnPlan p = plan_attn(batch->n_seqs, cache->n_heads, cache->head_dim, batch->q_heads / cache->n_heads, max_q, batch->max_kv, batch->window, batch->sinks);
     return part_floats(p, batch->n_queries, batch->q_heads, cache->head_dim) * sizeof(float);
 }
 
@@ -374,7 +374,7 @@ extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch
     a.max_q = (int)(batch->max_q < batch->n_queries ? batch->max_q : batch->n_queries); a.max_kv = batch->max_kv;
     a.scale_log2 = batch->softmax_scale * 1.4426950408889634f;
     a.causal = batch->causal != 0; a.window = batch->window; a.sinks = batch->sinks;
-    const AttnPlan p = plan_attn(a.B, a.c.H, a.G, a.max_q, a.max_kv, a.window, a.sinks);
+    const AttnPlan p = plan_attn(a.B, a.c.H, a.c.D, a.G, a.max_q, a.max_kv, a.window, a.sinks);
     const size_t need = part_floats(p, a.T, a.Hq, a.c.D) * sizeof(float);
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
         return fail(VARQ_ERR_WORKSPACE, "varq_paged_attn: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);

@@ -73,5 +73,6 @@ int paged_attn_tc_run(const PagedAttnArgs& a, int splits, float* ws_o, float* ws
 int paged_attn_decode_run(const PagedAttnArgs& a, int splits, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st);
 int paged_attn_merge_run(const PagedAttnArgs& a, int splits, const float* ws_o, const float* ws_ml, cudaStream_t st);
 int paged_attn_tc_status(int* out);
+int forced_attn_path();                // varq_attn_force_path
 
 }  // namespace varq

@@ -1,7 +1,9 @@
 // Attention of a few query rows (eight or sixteen per CTA) over a paged cache: warp-level tensor-core instructions fed straight from the pages.
 //
-// The work is to stream the codes once, so the kernel is built around instructions per key.  A warp takes 16 keys at a time, which lie in one page;
-// mma.sync m16n8k16 takes the codes as its A operand, and every thread unpacks whole words that it loaded itself:
+// The work is to stream the codes once, so the kernel is built around instructions per key and bytes in flight.  A warp takes 16 keys at a time, which lie
+// in one page, 16 rows one behind the other: its lanes copy them (cp.async, 16 bytes each) to a ring of its own in shared memory, several tiles ahead.  The
+// 16-byte chunks of a row are permuted by the row's number, so that the fragments below come out without bank conflicts.
+// mma.sync m16n8k16 takes the codes as its A operand, and every thread unpacks whole words:
 //   S^T = K Q^T     thread (g, c) (g = lane / 4, c = lane % 4) holds keys g and g + 8 and a quarter of the head_dim, contiguous in memory (the order
 //                   of the contraction index is free as long as Q follows it); the eight columns are query rows (token, head of the group);
 //   O^T = V^T P^T   thread (g, c) holds an eighth of the head_dim of keys 2c, 2c + 1, 2c + 8, 2c + 9; pairs of keys are joined by byte
@@ -46,21 +48,39 @@ template <int BITS> __device__ __forceinline__ void pd_codes(const uint32_t* w, 
 #pragma unroll
     for (int i = 0; i < 8; ++i) h[i] = Item<BITS>::minus_zp(h[i], i, pd_neg_base<BITS>(i % Item<BITS>::CLS));
 }
-template <int BYTES> struct PdRaw {        // `BYTES` of a row (two bytes: the low half of one word)
+template <int BYTES> struct PdRaw {        // `BYTES` of a row in shared memory (two bytes: the low half of one word)
     static constexpr int NW = BYTES < 4 ? 1 : BYTES / 4;
     uint32_t w[NW];
-    __device__ __forceinline__ void load(const unsigned char* p) {
-        if constexpr (BYTES == 2) w[0] = __ldg(reinterpret_cast<const unsigned short*>(p));
-        else if constexpr (BYTES == 4) w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-        else if constexpr (BYTES == 8) { const uint2 v = __ldg(reinterpret_cast<const uint2*>(p)); w[0] = v.x; w[1] = v.y; }
-        else {
+};
+// A tile of 16 rows of RB bytes in shared memory: chunk of 16 bytes `ch` of row `r`
+template <int RB> __device__ __forceinline__ int pd_chunk(int r, int ch) { return r * RB + ((RB == 128 ? ch ^ (r & 7) : RB == 64 ? ch ^ ((r >> 1) & 3) : ch) << 4); }
+template <int RB, int BYTES> __device__ __forceinline__ void pd_read(PdRaw<BYTES>& o, const unsigned char* tile, int r, int part) {      // part: in units of BYTES
+    if constexpr (BYTES == 32) {
 #pragma unroll
-            for (int i = 0; i < BYTES / 16; ++i) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
-                w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-            }
+        for (int i = 0; i < 2; ++i) {
+            const uint4 v = *reinterpret_cast<const uint4*>(tile + pd_chunk<RB>(r, 2 * part + i));
+            o.w[4 * i] = v.x; o.w[4 * i + 1] = v.y; o.w[4 * i + 2] = v.z; o.w[4 * i + 3] = v.w;
         }
+    } else {
+        const unsigned char* p = tile + pd_chunk<RB>(r, part * BYTES / 16) + (part * BYTES & 15);
+        if constexpr (BYTES == 16) { const uint4 v = *reinterpret_cast<const uint4*>(p); o.w[0] = v.x; o.w[1] = v.y; o.w[2] = v.z; o.w[3] = v.w; }
+        else if constexpr (BYTES == 8) { const uint2 v = *reinterpret_cast<const uint2*>(p); o.w[0] = v.x; o.w[1] = v.y; }
+        else if constexpr (BYTES == 4) o.w[0] = *reinterpret_cast<const uint32_t*>(p);
+        else o.w[0] = *reinterpret_cast<const unsigned short*>(p);
     }
+}
+template <int RB> __device__ __forceinline__ void pd_copy(unsigned char* tile, const unsigned char* src, int lane) {      // 16 rows, contiguous in memory
+#pragma unroll
+    for (int i = 0; i < (RB + 31) / 32; ++i) {
+        const int ch = lane + 32 * i;                       // of 16 * RB / 16 = RB
+        if (RB >= 32 || ch < RB)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(tile + pd_chunk<RB>(ch / (RB / 16), ch % (RB / 16)))), "l"(src + ch * 16) : "memory");
+    }
+}
+template <int KB, int VB, int D> struct PdPlan {
+    static constexpr int KROW = D * KB / 8, VROW = D * VB / 8, TILE = 16 * (KROW + VROW) + 128;      // rows, then 16 scales of K and of V
+    static constexpr int ST = TILE > 3000 ? 4 : TILE > 1500 ? 5 : 6;                                 // tiles of a warp's ring
+    static constexpr int SMEM = PD_WARPS * ST * TILE;
 };
 // the words of two keys -> words that unpack to pairs (first key, second key) of one head_dim element each, in element order
 template <int BITS, int NW> __device__ __forceinline__ void pd_join(const uint32_t (&a)[NW], const uint32_t (&b)[NW], uint32_t (&o)[2 * NW]) {
@@ -72,12 +92,14 @@ template <int BITS, int NW> __device__ __forceinline__ void pd_join(const uint32
 }
 
 template <int KB, int VB, int D, int NT>
-__global__ void __launch_bounds__(PD_WARPS * 32, NT > 1 && D == 128 ? 2 : (KB == 8 || VB == 8 || NT > 1) ? 3 : 4)
+__global__ void __launch_bounds__(PD_WARPS * 32, NT > 1 ? (D == 128 ? 3 : 4) : D == 128 ? (KB == 8 && VB == 8 ? 3 : 4) : 5)
 paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int tiles_per_split, float* ws_o, float* ws_ml, int* status) {
+    using P = PdPlan<KB, VB, D>;
     constexpr int KBYTES = D / 4 * KB / 8, VBYTES = D / 8 * VB / 8;       // of a row and thread
-    constexpr unsigned KROW = D * KB / 8, VROW = D * VB / 8;
+    constexpr int KROW = P::KROW, VROW = P::VROW, ST = P::ST;
     constexpr int ITEMS = D / 64, KSTEPS = D / 16, MT = D / 16, ROWS = 8 * NT;
-    __shared__ float s_part[PD_WARPS][ROWS][D + 2];
+    extern __shared__ __align__(128) unsigned char pd_smem[];
+    float (*s_part)[ROWS][D + 2] = reinterpret_cast<float (*)[ROWS][D + 2]>(pd_smem);      // behind the last use of the rings
 
     pdl_trigger();
     pdl_wait();
@@ -147,26 +169,44 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int tiles_
     vmagic.init();
     const int32_t* table = a.table + b * a.table_stride;
     const int page_mask = (1 << a.c.page_shift) - 1;
-    const unsigned char *kbase = reinterpret_cast<const unsigned char*>(a.c.kc) + c * KBYTES + g * KROW;
-    const unsigned char *vbase = reinterpret_cast<const unsigned char*>(a.c.vc) + g * VBYTES + 2 * c * VROW;
-    const float *ksc = a.c.ks + g, *vsc = a.c.vs + g;
+    unsigned char* ring = pd_smem + warp * (ST * P::TILE);
+    // A warp takes the tiles begin + warp, + PD_WARPS, ...: `n` of them.  Lane x keeps the page of tile (x mod 32) of the next 32.
+    const int n = begin + warp < end ? (end - begin - warp + PD_WARPS - 1) / PD_WARPS : 0;
+    int pages = 0;
+    auto request = [&](int i) {                  // tile i of the warp, into its place in the ring; an empty group behind the last
+        if (i < n) {
+            const int key = key_of(begin + warp + i * PD_WARPS);
+            if ((i & 31) == 0) {
+                const int mine = i + lane;
+                pages = mine < n ? __ldg(table + (key_of(begin + warp + mine * PD_WARPS) >> a.c.page_shift)) : 0;
+            }
+            const int page = paged_page(a, __shfl_sync(0xffffffffu, pages, i & 31), status);
+            const uint32_t at = (uint32_t)((page * a.c.H + h) << a.c.page_shift) + (key & page_mask);      // whole tiles: a page's rows behind the sequence's end may be
+            unsigned char* t = ring + (i % ST) * P::TILE;                                                  // copied, not used
+            pd_copy<KROW>(t, reinterpret_cast<const unsigned char*>(a.c.kc) + (size_t)at * KROW, lane);
+            pd_copy<VROW>(t + 16 * KROW, reinterpret_cast<const unsigned char*>(a.c.vc) + (size_t)at * VROW, lane);
+            if (lane < 8) {
+                const float* src = (lane < 4 ? a.c.ks : a.c.vs) + at + (lane & 3) * 4;
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(t + 16 * (KROW + VROW) + lane * 16)), "l"(src) : "memory");
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
     struct Tile {
         PdRaw<KBYTES> k[2];                // keys g, g + 8
         PdRaw<VBYTES> v[4];                // keys 2c, 2c + 1, 2c + 8, 2c + 9
         float ks[2], vs[2];                // of keys g, g + 8
     };
-    auto page_of = [&](int i) { return __ldg(table + (key_of(i) >> a.c.page_shift)); };
-    auto fetch = [&](Tile& t, int i, int page) {       // whole tiles: a page's rows behind the sequence's end may be loaded, not used
-        const long long at = (((long long)paged_page(a, page, status) * a.c.H + h) << a.c.page_shift) + (key_of(i) & page_mask);
-        const unsigned char *kp = kbase + at * KROW, *vp = vbase + at * VROW;
-        t.k[0].load(kp);
-        t.k[1].load(kp + 8 * KROW);
-        t.v[0].load(vp);
-        t.v[1].load(vp + VROW);
-        t.v[2].load(vp + 8 * VROW);
-        t.v[3].load(vp + 9 * VROW);
-        t.ks[0] = __ldg(ksc + at); t.ks[1] = __ldg(ksc + at + 8);
-        t.vs[0] = __ldg(vsc + at); t.vs[1] = __ldg(vsc + at + 8);
+    auto read = [&](Tile& t, int i) {
+        const unsigned char *p = ring + (i % ST) * P::TILE, *pv = p + 16 * KROW;
+        const float* ps = reinterpret_cast<const float*>(p + 16 * (KROW + VROW));
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            pd_read<KROW>(t.k[r], p, g + 8 * r, c);
+            t.ks[r] = ps[g + 8 * r]; t.vs[r] = ps[16 + g + 8 * r];
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) pd_read<VROW>(t.v[r], pv, 2 * c + (r & 1) + 8 * (r >> 1), g);
     };
     auto process = [&](const Tile& cur, int k0, auto masked_) {
         constexpr bool MASKED = decltype(masked_)::value;
@@ -258,28 +298,21 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int tiles_
             }
         }
     };
-    auto step = [&](const Tile& t, int i) {
-        const int k0 = key_of(i);
+#pragma unroll 1
+    for (int i = 0; i < ST - 1; ++i) request(i);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
+        __syncwarp();                            // all lanes' copies of tile i are there, and all lanes are done with tile i - 1
+        Tile t;
+        read(t, i);
+        request(i + ST - 1);
+        const int k0 = key_of(begin + warp + i * PD_WARPS);
         if (k0 + PD_KEYS > all_hi || (k0 < all_lo && k0 + PD_KEYS > a.sinks)) process(t, k0, std::true_type());
         else process(t, k0, std::false_type());
-    };
-    // two buffers that take turns, the next tile's rows in flight, the page number of the one behind it as well
-    Tile ta, tb;
-    int i = begin + warp, page = i < end ? page_of(i) : 0;
-    if (i < end) fetch(ta, i, page);
-    if (i + PD_WARPS < end) page = page_of(i + PD_WARPS);
-#pragma unroll 1
-    while (i < end) {
-        if (i + PD_WARPS < end) fetch(tb, i + PD_WARPS, page);
-        if (i + 2 * PD_WARPS < end) page = page_of(i + 2 * PD_WARPS);
-        step(ta, i);
-        i += PD_WARPS;
-        if (i >= end) break;
-        if (i + PD_WARPS < end) fetch(ta, i + PD_WARPS, page);
-        if (i + 2 * PD_WARPS < end) page = page_of(i + 2 * PD_WARPS);
-        step(tb, i);
-        i += PD_WARPS;
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
     // ---- a warp's partial result
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -364,16 +397,28 @@ __global__ void __launch_bounds__(128) paged_attn_merge_kernel(PagedAttnArgs a, 
     if (lane == 0 && a.lse) a.lse[row] = den != 0.f ? (M + __log2f(den)) * 0.6931471805599453f : -INFINITY;
 }
 
-template <int KB, int VB, int D>
-int launch(const PagedAttnArgs& a, int splits, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st) {
+template <int KB, int VB, int D, int NT>
+int launch_nt(const PagedAttnArgs& a, int splits, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st) {
+    constexpr int PART = PD_WARPS * 8 * NT * (D + 2) * 4, SMEM = PdPlan<KB, VB, D>::SMEM > PART ? PdPlan<KB, VB, D>::SMEM : PART;
     const long long rows = (long long)a.max_q * a.G;
-    const int nt = rows <= 8 ? 1 : 2, n_rowtiles = (int)((rows + 8 * nt - 1) / (8 * nt));
+    const int n_rowtiles = (int)((rows + 8 * NT - 1) / (8 * NT));
     const long long blocks = (long long)a.B * a.c.H * n_rowtiles * splits;
     if (blocks > 0x7fffffffLL) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_attn: more than 2^31 thread blocks");
-    VARQ_CUDA_TRY(nt == 1 ? launch_pdl(paged_attn_decode_kernel<KB, VB, D, 1>, (unsigned)blocks, PD_WARPS * 32, 0, st, 1, a, n_rowtiles, splits, tiles_per_split, ws_o, ws_ml, paged_status_word())
-                          : launch_pdl(paged_attn_decode_kernel<KB, VB, D, 2>, (unsigned)blocks, PD_WARPS * 32, 0, st, 1, a, n_rowtiles, splits, tiles_per_split, ws_o, ws_ml, paged_status_word()));
+    static bool configured[64] = {false};
+    int dev = 0;
+    VARQ_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        VARQ_CUDA_TRY(cudaFuncSetAttribute(paged_attn_decode_kernel<KB, VB, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+        if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
+    VARQ_CUDA_TRY(launch_pdl(paged_attn_decode_kernel<KB, VB, D, NT>, (unsigned)blocks, PD_WARPS * 32, SMEM, st, 1, a, n_rowtiles, splits, tiles_per_split, ws_o, ws_ml,
+                             paged_status_word()));
     count_launches(1);
     return VARQ_OK;
+}
+template <int KB, int VB, int D>
+int launch(const PagedAttnArgs& a, int splits, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st) {
+    return (long long)a.max_q * a.G <= 8 ? launch_nt<KB, VB, D, 1>(a, splits, tiles_per_split, ws_o, ws_ml, st) : launch_nt<KB, VB, D, 2>(a, splits, tiles_per_split, ws_o, ws_ml, st);
 }
 
 }  // namespace

@@ -2,12 +2,14 @@
 //
 // Append: a row (token, head) of K or V becomes D codes and one scale,
 //   scale = max(amax|x| / (2^(bits-1) - 1), eps),   code = rint(x / scale) to even,
-// with the bits of a true fp32 division.  Eight values per lane, 8 or 16 lanes per row, the row read once and held in registers.  Rounding
-// without a division per value: y = x * (1 / scale) is within 2^-22 |y| of the quotient and |y| <= 127.5, so rint(y) is the code unless y lies
-// within 2^-14 of a half; a lane that holds such a value divides its eight.  A row with a NaN or an infinity has a NaN scale and zero codes:
-// whoever reads it gets NaN, as from arithmetic on the values themselves, and whoever does not see it loses nothing.
+// with the bits of a true fp32 division.  Two pieces of eight values per lane, 4 or 8 lanes per row, the row read once and held in registers.  Rounding
+// without a division per value: with r = 1 / scale the quotient lies between x r (1 - 2^-22) and x r (1 + 2^-22); each end is rounded by one multiply-add with
+// 1.5 * 2^23, which leaves the integer in the low mantissa bits, and where the two agree on all of a lane's values those are the codes.  Else the lane divides.
+// A row with a NaN or an infinity has a NaN scale and zero codes: whoever reads it gets NaN, as from arithmetic on the values themselves, and whoever does
+// not see it loses nothing.
 // Read: code * scale, converted to the output's type once.
 #include "varq_attn.cuh"
+#include "varq_codes.cuh"
 #include "varq_paged.cuh"
 #include "varq_quant.cuh"
 
@@ -34,52 +36,101 @@ struct ReadArgs {
 
 constexpr int ROW_THREADS = 256;
 
-// codes of eight values in the low bytes' order of a row: 64, 32 or 16 bits
-__device__ __forceinline__ void store_codes(int32_t* pool, long long word0, int lane, int bits, const int (&q)[8]) {
+// codes of eight values (fp32 with the code in the low mantissa bits) as piece `ch` of a row: 64, 32 or 16 bits
+__device__ __forceinline__ void store_codes(int32_t* row, int ch, int bits, const uint32_t (&q)[8]) {
     if (bits == 8) {
         uint32_t w[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
             w[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040), 0x5410);
-        *reinterpret_cast<uint2*>(pool + word0 + 2 * lane) = make_uint2(w[0], w[1]);
+        reinterpret_cast<uint2*>(row)[ch] = make_uint2(w[0], w[1]);
     } else if (bits == 4) {
         uint32_t w = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w |= (uint32_t)(q[i] & 15) << (4 * i);
-        pool[word0 + lane] = (int32_t)w;
+        for (int i = 0; i < 8; ++i) w |= (q[i] & 15u) << (4 * i);
+        row[ch] = (int32_t)w;
     } else {
         uint32_t w = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w |= (uint32_t)(q[i] & 3) << (2 * i);
-        reinterpret_cast<unsigned short*>(pool + word0)[lane] = (unsigned short)w;
+        for (int i = 0; i < 8; ++i) w |= (q[i] & 3u) << (2 * i);
+        reinterpret_cast<unsigned short*>(row)[ch] = (unsigned short)w;
     }
 }
-__device__ __forceinline__ void load_codes(const int32_t* pool, long long word0, int lane, int bits, uint32_t (&w)[2]) {
+__device__ __forceinline__ void load_codes(const int32_t* row, int ch, int bits, uint32_t (&w)[2]) {
     if (bits == 8) {
-        const uint2 x = __ldg(reinterpret_cast<const uint2*>(pool + word0 + 2 * lane));
+        const uint2 x = __ldg(reinterpret_cast<const uint2*>(row) + ch);
         w[0] = x.x; w[1] = x.y;
     } else {
-        w[0] = bits == 4 ? (uint32_t)__ldg(pool + word0 + lane) : __ldg(reinterpret_cast<const unsigned short*>(pool + word0) + lane);
+        w[0] = bits == 4 ? (uint32_t)__ldg(row + ch) : __ldg(reinterpret_cast<const unsigned short*>(row) + ch);
         w[1] = 0;
     }
 }
-// signed fields -> fp32: 0x4B000000 | u is 2^23 + u
+// signed fields -> fp32: 0x4B000000 | u is 2^23 + u; narrow ones by way of exact fp16 pairs
 __device__ __forceinline__ void codes_to_float(const uint32_t (&w)[2], int bits, float (&f)[8]) {
     if (bits == 8) {
+        const uint32_t a = w[0] ^ 0x80808080u, b = w[1] ^ 0x80808080u;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(__byte_perm(w[i >> 2] ^ 0x80808080u, 0x4B000000u, 0x7540 | (i & 3))) - 8388736.f;
+        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(__byte_perm(i < 4 ? a : b, 0x4B000000u, 0x7540 | (i & 3))) - 8388736.f;
+    } else if (bits == 4) {                                  // pairs (i, i + 4): 1024 + u, or 1024 + 16 u
+        const uint32_t u = w[0] ^ 0x88888888u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t x = i < 2 ? u : u >> 8;
+            const uint32_t h = i & 1 ? h2_fma((x & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u) : h2_add((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u);
+            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
+            f[i] = v.x; f[i + 4] = v.y;
+        }
     } else {
-        const uint32_t flip = bits == 4 ? 0x88888888u : 0xAAAAu, mask = (1u << bits) - 1u;
-        const float base = 8388608.f + (float)(1 << (bits - 1));
-        const uint32_t u = w[0] ^ flip;
+        const uint32_t u = w[0] ^ 0xAAAAu;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(((u >> (bits * i)) & mask) | 0x4B000000u) - base;
+        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(((u >> (2 * i)) & 3u) | 0x4B000000u) - 8388610.f;
     }
+}
+
+// eight consecutive values of a row, packed as they come, and their largest absolute value as bits (order of the absolute values, NaN above infinity)
+template <typename T, bool VEC> struct Piece {
+    Vec8<T> r;
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (VEC) r.load(p);
+        else {
+            T e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = p[i];
+            if constexpr (sizeof(T) == 4) { r.a = make_float4(e[0], e[1], e[2], e[3]); r.b = make_float4(e[4], e[5], e[6], e[7]); }
+            else r.r = *reinterpret_cast<const uint4*>(e);
+        }
+    }
+    __device__ __forceinline__ uint32_t top() const {       // 16-bit types: of the even and the odd values, side by side
+        if constexpr (sizeof(T) == 4) {
+            float v[8];
+            r.get(v);
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+            return m;
+        } else {
+            return __vmaxu2(__vmaxu2(r.r.x & 0x7fff7fffu, r.r.y & 0x7fff7fffu), __vmaxu2(r.r.z & 0x7fff7fffu, r.r.w & 0x7fff7fffu));
+        }
+    }
+};
+template <typename T> __device__ __forceinline__ uint32_t merge_top(uint32_t a, uint32_t b) { return sizeof(T) == 4 ? max(a, b) : __vmaxu2(a, b); }
+template <typename T> __device__ __forceinline__ float top_value(uint32_t m) {                 // the value itself
+    if constexpr (sizeof(T) == 4) return __uint_as_float(m);
+    else {
+        const unsigned short b = (unsigned short)max(m & 0xffffu, m >> 16);
+        return to_f32<T>(*reinterpret_cast<const T*>(&b));
+    }
+}
+__device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
 }
 
 template <typename T, int D, int U, bool VEC>
 __global__ void __launch_bounds__(ROW_THREADS) paged_append_kernel(AppendArgs a) {
-    constexpr int LPR = D / 8, RPB = ROW_THREADS / LPR;
+    constexpr int LPR = D / 16, RPB = ROW_THREADS / LPR;
     pdl_trigger();
     pdl_wait();
     const int lane = threadIdx.x & (LPR - 1), page_mask = (1 << a.c.page_shift) - 1;
@@ -90,64 +141,66 @@ __global__ void __launch_bounds__(ROW_THREADS) paged_append_kernel(AppendArgs a)
     int32_t* pool = is_v ? a.c.vc : a.c.kc;
     float* scales = is_v ? a.c.vs : a.c.ks;
     const long long n_slots = (long long)a.c.n_pages << a.c.page_shift;
-    const float top = (float)((1 << (bits - 1)) - 1);
+    const float most = (float)((1 << (bits - 1)) - 1);
     const uint32_t row0 = blockIdx.x * (RPB * U) + threadIdx.x / LPR;
-    float f[U][8];
-    long long at[U];                   // row of the pools, negative: not written
+    Piece<T, VEC> f[U][2];
+    uint32_t at[U];                    // row of the pools
+    bool there[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const uint32_t row = row0 + u * RPB;
-        at[u] = -1;
+        there[u] = false;
         if (row < a.rows) {
             const uint32_t t = a.heads.div(row), h = row - t * a.heads.d;
             const long long slot = __ldg(a.slots + t);
             if (slot >= 0 && slot < n_slots) {
-                at[u] = (((slot >> a.c.page_shift) * a.c.H + h) << a.c.page_shift) + (slot & page_mask);
+                there[u] = true;
+                at[u] = (((uint32_t)(slot >> a.c.page_shift) * a.c.H + h) << a.c.page_shift) + ((uint32_t)slot & page_mask);
                 const T* p = x + t * st + h * sh + lane * 8;
-                if constexpr (VEC) { Vec8<T> r; r.load(p); r.get(f[u]); }
-                else load_vals<T, 8, false>(p, f[u], 8);
+                f[u][0].load(p);
+                f[u][1].load(p + D / 2);
             }
         }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        uint32_t hi = 0;               // order of the absolute values, NaN above infinity
-        if (at[u] >= 0) {
+        uint32_t m = there[u] ? merge_top<T>(f[u][0].top(), f[u][1].top()) : 0u;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) hi = max(hi, __float_as_uint(f[u][i]) & 0x7fffffffu);
-        }
+        for (int z = LPR / 2; z; z >>= 1) m = merge_top<T>(m, __shfl_xor_sync(0xffffffffu, m, z));
+        if (!there[u]) continue;
+        const float top = top_value<T>(m);
+        const bool fine = top <= 3.402823466e38f;
+        const float scale = fine ? fmaxf(__fdiv_rn(top, most), a.eps) : __uint_as_float(0x7fffffffu), r = __frcp_rn(scale);
+        const float lo = r * (1.f - 0x1p-22f), hi = r * (1.f + 0x1p-22f);
+        int32_t* out = pool + (size_t)at[u] * words;
 #pragma unroll
-        for (int z = LPR / 2; z; z >>= 1) hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, z));
-        if (at[u] < 0) continue;
-        int q[8];
-        float scale;
-        if (hi >= 0x7f800000u) {
-            scale = __uint_as_float(0x7fffffffu);
+        for (int e = 0; e < 2; ++e) {
+            float v[8];
+            uint32_t q[8], differ = 0;
+            f[u][e].r.get(v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] = 0;
-        } else {
-            scale = fmaxf(__fdiv_rn(__uint_as_float(hi), top), a.eps);
-            const float r = __frcp_rn(scale);
-            float far = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float y = f[u][i] * r, z = y + Q_MAGIC;
-                q[i] = (int)__float_as_uint(z);                          // the integer in the low bits, sign included
-                far = fmaxf(far, fabsf(y - (z - Q_MAGIC)));
+            for (int i = 0; i < 8; i += 2) {
+                const float2 x2 = make_float2(v[i], v[i + 1]), magic = make_float2(Q_MAGIC, Q_MAGIC);
+                const float2 y = fma_pair(x2, make_float2(lo, lo), magic), z = fma_pair(x2, make_float2(hi, hi), magic);
+                q[i] = __float_as_uint(y.x); q[i + 1] = __float_as_uint(y.y);
+                differ |= (q[i] ^ __float_as_uint(z.x)) | (q[i + 1] ^ __float_as_uint(z.y));
             }
-            if (far > 0.5f - 1.f / 16384.f) {
+            if (!fine) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) q[i] = (int)__float_as_uint(rintf(__fdiv_rn(f[u][i], scale)) + Q_MAGIC);
+                for (int i = 0; i < 8; ++i) q[i] = 0u;
+            } else if (differ) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(rintf(__fdiv_rn(v[i], scale)) + Q_MAGIC);
             }
+            store_codes(out, lane + e * LPR, bits, q);
         }
-        store_codes(pool, at[u] * words, lane, bits, q);
         if (lane == 0) scales[at[u]] = scale;
     }
 }
 
 template <typename T, int D, int U, bool VEC>
 __global__ void __launch_bounds__(ROW_THREADS) paged_read_kernel(ReadArgs a) {
-    constexpr int LPR = D / 8, RPB = ROW_THREADS / LPR;
+    constexpr int LPR = D / 16, RPB = ROW_THREADS / LPR;
     pdl_trigger();
     pdl_wait();
     const int lane = threadIdx.x & (LPR - 1), page_mask = (1 << a.c.page_shift) - 1;
@@ -159,31 +212,36 @@ __global__ void __launch_bounds__(ROW_THREADS) paged_read_kernel(ReadArgs a) {
     const float* scales = is_v ? a.c.vs : a.c.ks;
     const long long n_slots = (long long)a.c.n_pages << a.c.page_shift;
     const uint32_t row0 = blockIdx.x * (RPB * U) + threadIdx.x / LPR;
-    if (!out) return;
-    uint32_t w[U][2], t[U], h[U];
+    uint32_t w[U][2][2];
+    T* to[U];
     float s[U];
     bool there[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const uint32_t row = min(row0 + u * RPB, a.rows - 1);
-        t[u] = a.heads.div(row); h[u] = row - t[u] * a.heads.d;
-        const long long slot = __ldg(a.slots + t[u]);
+        const uint32_t row = min(row0 + u * RPB, a.rows - 1), t = a.heads.div(row), h = row - t * a.heads.d;
+        const long long slot = __ldg(a.slots + t);
         there[u] = slot >= 0 && slot < n_slots;
-        w[u][0] = w[u][1] = 0; s[u] = 0.f;
+        to[u] = out + t * st + h * sh + lane * 8;
+        w[u][0][0] = w[u][0][1] = w[u][1][0] = w[u][1][1] = 0; s[u] = 0.f;
         if (there[u]) {
-            const long long at = (((slot >> a.c.page_shift) * a.c.H + h[u]) << a.c.page_shift) + (slot & page_mask);
-            load_codes(pool, at * words, lane, bits, w[u]);
+            const uint32_t at = (((uint32_t)(slot >> a.c.page_shift) * a.c.H + h) << a.c.page_shift) + ((uint32_t)slot & page_mask);
+            const int32_t* p = pool + (size_t)at * words;
+            load_codes(p, lane, bits, w[u][0]);
+            load_codes(p, lane + LPR, bits, w[u][1]);
             s[u] = __ldg(scales + at);
         }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         if (row0 + u * RPB >= a.rows) break;
-        float f[8];
-        codes_to_float(w[u], bits, f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = there[u] ? f[i] * s[u] : 0.f;
-        store_vals<T, 8, VEC>(out + t[u] * st + h[u] * sh + lane * 8, f, 8);
+        for (int e = 0; e < 2; ++e) {
+            float f[8];
+            codes_to_float(w[u][e], bits, f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = there[u] ? f[i] * s[u] : 0.f;
+            store_vals<T, 8, VEC>(to[u] + e * (D / 2), f, 8);
+        }
     }
 }
 
@@ -215,26 +273,26 @@ int check_rows(const char* who, const PagedView& c, long long n) {
     return VARQ_OK;
 }
 
-// Rows per thread: four keep enough bytes in flight for a long call (32768 tokens of 8 heads), one spreads a short call over the SMs
-template <typename A, typename K1, typename K4>
-int launch_rows(K1 one, K4 four, const A& a, int D, cudaStream_t st) {
-    const uint32_t rpb = ROW_THREADS / (D / 8);
-    if (a.rows >= 4ull * rpb * sm_count() * 4) VARQ_CUDA_TRY(launch_pdl(four, dim3((a.rows + 4 * rpb - 1) / (4 * rpb), 2), ROW_THREADS, 0, st, 1, a));
+// Rows per thread: several keep enough bytes in flight for a long call, one spreads a short call over the SMs
+template <int U, typename A, typename K1, typename KU>
+int launch_rows(K1 one, KU several, const A& a, int D, cudaStream_t st) {
+    const uint32_t rpb = ROW_THREADS / (D / 16);
+    if (a.rows >= 4ull * U * rpb * sm_count()) VARQ_CUDA_TRY(launch_pdl(several, dim3((a.rows + U * rpb - 1) / (U * rpb), 2), ROW_THREADS, 0, st, 1, a));
     else VARQ_CUDA_TRY(launch_pdl(one, dim3((a.rows + rpb - 1) / rpb, 2), ROW_THREADS, 0, st, 1, a));
     count_launches(1);
     return VARQ_OK;
 }
+template <typename T, int D, bool VEC> int run_append(const AppendArgs& a, cudaStream_t st) {
+    return launch_rows<2>(paged_append_kernel<T, D, 1, VEC>, paged_append_kernel<T, D, 2, VEC>, a, D, st);
+}
 template <typename T> int run_append(const AppendArgs& a, bool vec, cudaStream_t st) {
-    if (a.c.D == 64) return vec ? launch_rows(paged_append_kernel<T, 64, 1, true>, paged_append_kernel<T, 64, 4, true>, a, 64, st)
-                                : launch_rows(paged_append_kernel<T, 64, 1, false>, paged_append_kernel<T, 64, 4, false>, a, 64, st);
-    return vec ? launch_rows(paged_append_kernel<T, 128, 1, true>, paged_append_kernel<T, 128, 4, true>, a, 128, st)
-               : launch_rows(paged_append_kernel<T, 128, 1, false>, paged_append_kernel<T, 128, 4, false>, a, 128, st);
+    return a.c.D == 64 ? (vec ? run_append<T, 64, true>(a, st) : run_append<T, 64, false>(a, st)) : (vec ? run_append<T, 128, true>(a, st) : run_append<T, 128, false>(a, st));
+}
+template <typename T, int D, bool VEC> int run_read(const ReadArgs& a, cudaStream_t st) {
+    return launch_rows<4>(paged_read_kernel<T, D, 1, VEC>, paged_read_kernel<T, D, 4, VEC>, a, D, st);
 }
 template <typename T> int run_read(const ReadArgs& a, bool vec, cudaStream_t st) {
-    if (a.c.D == 64) return vec ? launch_rows(paged_read_kernel<T, 64, 1, true>, paged_read_kernel<T, 64, 4, true>, a, 64, st)
-                                : launch_rows(paged_read_kernel<T, 64, 1, false>, paged_read_kernel<T, 64, 4, false>, a, 64, st);
-    return vec ? launch_rows(paged_read_kernel<T, 128, 1, true>, paged_read_kernel<T, 128, 4, true>, a, 128, st)
-               : launch_rows(paged_read_kernel<T, 128, 1, false>, paged_read_kernel<T, 128, 4, false>, a, 128, st);
+    return a.c.D == 64 ? (vec ? run_read<T, 64, true>(a, st) : run_read<T, 64, false>(a, st)) : (vec ? run_read<T, 128, true>(a, st) : run_read<T, 128, false>(a, st));
 }
 
 __device__ int g_paged_status = 0;

@@ -2,6 +2,8 @@
 
 The definition is elementwise fp32 arithmetic with true division (scale = max(amax / (2^(bits-1) - 1), 1e-12), code = round half to even),
 so nothing may differ: there is no tolerance in this file.  Values in 16 bits are one rounding of the fp32 product."""
+import math
+
 import pytest
 import torch
 
@@ -109,6 +111,24 @@ def test_ties_and_their_neighbours(bits):
     k = torch.stack(rows).unsqueeze(1)
     cache = PagedCache(4, 16, 1, 64, bits, bits)
     slots = torch.arange(len(rows))
+    cache.append(k.to(DEV), (-k).to(DEV), slots.to(DEV))
+    check(cache, k, -k, slots)
+
+
+@pytest.mark.parametrize("bits", [8, 4, 2])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_scales_of_every_magnitude(bits, dtype):
+    """rows from the smallest to the largest numbers of the type, with every leading pattern of the largest value: the scale's division has to round as it should"""
+    g = torch.Generator().manual_seed(bits)
+    info = torch.finfo(dtype)
+    lo, hi = math.log2(info.tiny), math.log2(info.max)
+    T = 4096
+    size = 2.0 ** (torch.rand((T, 1, 1), generator=g, dtype=torch.float64) * (hi - lo) + lo)
+    k = (torch.rand((T, 1, 64), generator=g, dtype=torch.float64) * 2 - 1) * size
+    k = k.clamp(-info.max, info.max).to(dtype)
+    k[0, 0, 0], k[1, 0, 1], k[2] = info.max, -info.max, 0.0
+    cache = PagedCache(T // 16, 16, 1, 64, bits, bits)
+    slots = torch.arange(T)
     cache.append(k.to(DEV), (-k).to(DEV), slots.to(DEV))
     check(cache, k, -k, slots)
 

@@ -21,8 +21,7 @@ from .quant import _host
 
 
 def _native():
-    _cabi.lib()                          # says what to build if nothing is
-    return _host
+    return _host if _host is not None else _cabi.lib()                    # which says what to build
 
 
 class PagedCache:

@@ -3,8 +3,9 @@
 // Append: a row (token, head) of K or V becomes D codes and one scale,
 //   scale = max(amax|x| / (2^(bits-1) - 1), eps),   code = rint(x / scale) to even,
 // with the bits of a true fp32 division.  Two pieces of eight values per lane, 4 or 8 lanes per row, the row read once and held in registers.  Rounding
-// without a division per value: with r = 1 / scale the quotient lies between x r (1 - 2^-22) and x r (1 + 2^-22); each end is rounded by one multiply-add with
+// without a division per value: with r = 1 / scale the quotient lies between x r (1 - 2^-21) and x r (1 + 2^-21); each end is rounded by one multiply-add with
 // 1.5 * 2^23, which leaves the integer in the low mantissa bits, and where the two agree on all of a lane's values those are the codes.  Else the lane divides.
+// The scale's own division by 1, 7 or 127 is Markstein's: with c = RN(1 / d) and q = RN(a c), RN(q + RN(a - q d) c) is RN(a / d), the remainder being exact.
 // A row with a NaN or an infinity has a NaN scale and zero codes: whoever reads it gets NaN, as from arithmetic on the values themselves, and whoever does
 // not see it loses nothing.
 // Read: code * scale, converted to the output's type once.
@@ -38,22 +39,20 @@ constexpr int ROW_THREADS = 256;
 
 // codes of eight values (fp32 with the code in the low mantissa bits) as piece `ch` of a row: 64, 32 or 16 bits
 __device__ __forceinline__ void store_codes(int32_t* row, int ch, int bits, const uint32_t (&q)[8]) {
+    uint32_t w[2];                     // a byte each
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        w[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040), 0x5410);
     if (bits == 8) {
-        uint32_t w[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            w[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040), 0x5410);
         reinterpret_cast<uint2*>(row)[ch] = make_uint2(w[0], w[1]);
-    } else if (bits == 4) {
-        uint32_t w = 0;
+    } else if (bits == 4) {            // two in a byte: in bytes 0 and 2
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w |= (q[i] & 15u) << (4 * i);
-        row[ch] = (int32_t)w;
-    } else {
-        uint32_t w = 0;
+        for (int i = 0; i < 2; ++i) { w[i] &= 0x0f0f0f0fu; w[i] |= w[i] >> 4; }
+        row[ch] = (int32_t)__byte_perm(w[0], w[1], 0x6420);
+    } else {                           // four in a byte: in byte 0
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w |= (q[i] & 3u) << (2 * i);
-        reinterpret_cast<unsigned short*>(row)[ch] = (unsigned short)w;
+        for (int i = 0; i < 2; ++i) { w[i] &= 0x03030303u; w[i] |= w[i] >> 6; w[i] |= w[i] >> 12; }
+        reinterpret_cast<unsigned short*>(row)[ch] = (unsigned short)__byte_perm(w[0], w[1], 0x0040);
     }
 }
 __device__ __forceinline__ void load_codes(const int32_t* row, int ch, int bits, uint32_t (&w)[2]) {
@@ -141,7 +140,7 @@ __global__ void __launch_bounds__(ROW_THREADS) paged_append_kernel(AppendArgs a)
     int32_t* pool = is_v ? a.c.vc : a.c.kc;
     float* scales = is_v ? a.c.vs : a.c.ks;
     const long long n_slots = (long long)a.c.n_pages << a.c.page_shift;
-    const float most = (float)((1 << (bits - 1)) - 1);
+    const float most = (float)((1 << (bits - 1)) - 1), inv = bits == 8 ? 1.f / 127.f : bits == 4 ? 1.f / 7.f : 1.f;
     const uint32_t row0 = blockIdx.x * (RPB * U) + threadIdx.x / LPR;
     Piece<T, VEC> f[U][2];
     uint32_t at[U];                    // row of the pools
@@ -153,7 +152,7 @@ __global__ void __launch_bounds__(ROW_THREADS) paged_append_kernel(AppendArgs a)
         if (row < a.rows) {
             const uint32_t t = a.heads.div(row), h = row - t * a.heads.d;
             const long long slot = __ldg(a.slots + t);
-            if (slot >= 0 && slot < n_slots) {
+            if ((unsigned long long)slot < (unsigned long long)n_slots) {
                 there[u] = true;
                 at[u] = (((uint32_t)(slot >> a.c.page_shift) * a.c.H + h) << a.c.page_shift) + ((uint32_t)slot & page_mask);
                 const T* p = x + t * st + h * sh + lane * 8;
@@ -170,13 +169,16 @@ __global__ void __launch_bounds__(ROW_THREADS) paged_append_kernel(AppendArgs a)
         if (!there[u]) continue;
         const float top = top_value<T>(m);
         const bool fine = top <= 3.402823466e38f;
-        const float scale = fine ? fmaxf(__fdiv_rn(top, most), a.eps) : __uint_as_float(0x7fffffffu), r = __frcp_rn(scale);
-        const float lo = r * (1.f - 0x1p-22f), hi = r * (1.f + 0x1p-22f);
+        const float quot = top * inv, scale = fine ? fmaxf(fmaf(fmaf(-quot, most, top), inv, quot), a.eps) : __uint_as_float(0x7fffffffu);
+        float r;                                             // within 2^-23, as long as it is a normal number
+        asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(scale));
+        const float lo = r * (1.f - 0x1p-21f), hi = r * (1.f + 0x1p-21f);
+        const uint32_t small = scale > 0x1p125f ? 1u : 0u;
         int32_t* out = pool + (size_t)at[u] * words;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             float v[8];
-            uint32_t q[8], differ = 0;
+            uint32_t q[8], differ = small;
             f[u][e].r.get(v);
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
@@ -220,7 +222,7 @@ __global__ void __launch_bounds__(ROW_THREADS) paged_read_kernel(ReadArgs a) {
     for (int u = 0; u < U; ++u) {
         const uint32_t row = min(row0 + u * RPB, a.rows - 1), t = a.heads.div(row), h = row - t * a.heads.d;
         const long long slot = __ldg(a.slots + t);
-        there[u] = slot >= 0 && slot < n_slots;
+        there[u] = (unsigned long long)slot < (unsigned long long)n_slots;
         to[u] = out + t * st + h * sh + lane * 8;
         w[u][0][0] = w[u][0][1] = w[u][1][0] = w[u][1][1] = 0; s[u] = 0.f;
         if (there[u]) {
@@ -289,7 +291,7 @@ template <typename T> int run_append(const AppendArgs& a, bool vec, cudaStream_t
     return a.c.D == 64 ? (vec ? run_append<T, 64, true>(a, st) : run_append<T, 64, false>(a, st)) : (vec ? run_append<T, 128, true>(a, st) : run_append<T, 128, false>(a, st));
 }
 template <typename T, int D, bool VEC> int run_read(const ReadArgs& a, cudaStream_t st) {
-    return launch_rows<4>(paged_read_kernel<T, D, 1, VEC>, paged_read_kernel<T, D, 4, VEC>, a, D, st);
+    return launch_rows<2>(paged_read_kernel<T, D, 1, VEC>, paged_read_kernel<T, D, 2, VEC>, a, D, st);
 }
 template <typename T> int run_read(const ReadArgs& a, bool vec, cudaStream_t st) {
     return a.c.D == 64 ? (vec ? run_read<T, 64, true>(a, st) : run_read<T, 64, false>(a, st)) : (vec ? run_read<T, 128, true>(a, st) : run_read<T, 128, false>(a, st));
@@ -300,8 +302,13 @@ __device__ int g_paged_status = 0;
 }  // namespace
 
 int* paged_status_word() {
+    static int* known[64] = {nullptr};                       // per device; the address of a variable of the module does not change
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
+    if (dev >= 0 && dev < 64 && known[dev]) return known[dev];
     void* p = nullptr;
     if (cudaGetSymbolAddress(&p, g_paged_status) != cudaSuccess) return nullptr;
+    if (dev >= 0 && dev < 64) known[dev] = reinterpret_cast<int*>(p);
     return reinterpret_cast<int*>(p);
 }
 int paged_status(int* out) {

@@ -375,29 +375,34 @@ namespace {
 
 // How a call is shared out
 struct AttnPlan {
-    bool tc;
+    bool tc, cluster;                  // kernel; its parts meet in clusters, not in the workspace
     int splits, tiles_per_split;       // tiles of 16 keys (decode kernel)
 };
-AttnPlan plan_attn(int B, int H, int D, int G, int max_q, int max_kv, int window, int sinks) {
+AttnPlan plan_attn(const varq_paged_t* c, const varq_paged_batch_t* b) {
     AttnPlan p;
-    const long long rows = (long long)max_q * G;
-    const long long span = window && (long long)window + max_q + sinks < max_kv ? (long long)window + max_q + sinks : max_kv;      // keys of a CTA, about
+    const int max_q = (int)(b->max_q < b->n_queries ? b->max_q : b->n_queries), D = c->head_dim;
+    const long long rows = (long long)max_q * (b->q_heads / c->n_heads);
+    const long long seen = (long long)b->window + max_q + b->sinks, span = b->window && seen < b->max_kv ? seen : b->max_kv;      // keys of a CTA, about
     p.tc = forced_attn_path() == VARQ_ATTN_PATH_TC || (forced_attn_path() != VARQ_ATTN_PATH_DECODE && rows > (D == 64 ? 80 : 48));
-    const long long units = p.tc ? 128 : 16, tiles = (span + units - 1) / units > 0 ? (span + units - 1) / units : 1;
-    const long long base = (long long)B * H * (p.tc ? (rows + 255) / 256 : (rows + 15) / 16), room = (long long)sm_count() * (p.tc ? 1 : 3);
-    // the number of parts that makes the waves of CTAs shortest, a CTA costing its tiles and a fixed part (set-up and merging)
-    const long long fixed = p.tc ? 4 : 16, least = p.tc ? 2 : 16;
+    const long long unit = p.tc ? 128 : 16, tiles = span > unit ? (span + unit - 1) / unit : 1;
+    const int resident = p.tc ? 1 : rows > 8 ? (D == 128 ? 3 : 4) : D == 64 ? 5 : c->k_bits == 8 && c->v_bits == 8 ? 3 : 4;       // CTAs per SM
+    const long long base = (long long)b->n_seqs * c->n_heads * (p.tc ? (rows + 255) / 256 : (rows + 15) / 16), room = (long long)sm_count() * resident;
+    // the number of parts that makes the waves of CTAs shortest, a CTA costing its tiles and a fixed part, parts in the workspace those, the second launch, too
+    const long long fixed = p.tc ? 4 : 16, least = p.tc ? 2 : 4, merge = p.tc ? 4 : 24;
     long long best = 0;
-    p.splits = 1;
+    p.splits = 1; p.cluster = false;
     for (long long s = 1; s == 1 || (s <= tiles / least && s <= 256); ++s) {
-        const long long cost = (base * s + room - 1) / room * ((tiles + s - 1) / s + fixed + (s > 1 ? fixed : 0));
-        if (best == 0 || cost < best) { best = cost; p.splits = (int)s; }
+        const bool near = !p.tc && s <= PAGED_CLUSTER && base * s <= room;
+        const long long cost = (base * s + room - 1) / room * ((tiles + s - 1) / s + fixed) + (s > 1 && !near ? merge : 0);
+        if (best == 0 || cost < best) { best = cost; p.splits = (int)s; p.cluster = s > 1 && near; }
         if (base * s > 8 * room) break;
     }
     p.tiles_per_split = (int)((tiles + p.splits - 1) / p.splits);
     return p;
 }
-size_t part_floats(const AttnPlan& p, long long n_queries, int q_heads, int D) { return p.splits > 1 ? (size_t)p.splits * n_queries * q_heads * (D + 2) : 0; }
+size_t part_floats(const AttnPlan& p, const varq_paged_t* c, const varq_paged_batch_t* b) {
+    return p.splits > 1 && !p.cluster ? (size_t)p.splits * b->n_queries * b->q_heads * (c->head_dim + 2) : 0;
+}
 
 }  // namespace
 
@@ -405,9 +410,7 @@ extern "C" size_t varq_paged_attn_workspace_bytes(const varq_paged_t* cache, con
     if (!cache || !batch || cache->n_heads < 1 || batch->q_heads < cache->n_heads || batch->n_seqs < 1 || batch->n_queries < 1 || batch->max_q < 1 || batch->max_kv < 0 ||
         batch->window < 0 || batch->sinks < 0 || cache->head_dim < 1)
         return 0;
-    const int max_q = (int)(batch->max_q < batch->n_queries ? batch->max_q : batch->n_queries);
-    const AttnPlan p = plan_attn(batch->n_seqs, cache->n_heads, cache->head_dim, batch->q_heads / cache->n_heads, max_q, batch->max_kv, batch->window, batch->sinks);
-    return part_floats(p, batch->n_queries, batch->q_heads, cache->head_dim) * sizeof(float);
+    return part_floats(plan_attn(cache, batch), cache, batch) * sizeof(float);
 }
 
 extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch_t* batch, const varq_tensor_t* q, const varq_tensor_t* out, float* lse,
@@ -439,12 +442,12 @@ extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch
     a.max_q = (int)(batch->max_q < batch->n_queries ? batch->max_q : batch->n_queries); a.max_kv = batch->max_kv;
     a.scale_log2 = batch->softmax_scale * 1.4426950408889634f;
     a.causal = batch->causal != 0; a.window = batch->window; a.sinks = batch->sinks;
-    const AttnPlan p = plan_attn(a.B, a.c.H, a.c.D, a.G, a.max_q, a.max_kv, a.window, a.sinks);
-    const size_t need = part_floats(p, a.T, a.Hq, a.c.D) * sizeof(float);
+    const AttnPlan p = plan_attn(cache, batch);
+    const size_t need = part_floats(p, cache, batch) * sizeof(float);
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
         return fail(VARQ_ERR_WORKSPACE, "varq_paged_attn: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
     float *ws_o = reinterpret_cast<float*>(workspace), *ws_ml = ws_o + (size_t)p.splits * a.T * a.Hq * a.c.D;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (int rc = p.tc ? paged_attn_tc_run(a, p.splits, ws_o, ws_ml, st) : paged_attn_decode_run(a, p.splits, p.tiles_per_split, ws_o, ws_ml, st)) return rc;
-    return p.splits > 1 ? paged_attn_merge_run(a, p.splits, ws_o, ws_ml, st) : VARQ_OK;
+    if (int rc = p.tc ? paged_attn_tc_run(a, p.splits, ws_o, ws_ml, st) : paged_attn_decode_run(a, p.splits, p.cluster, p.tiles_per_split, ws_o, ws_ml, st)) return rc;
+    return need ? paged_attn_merge_run(a, p.splits, ws_o, ws_ml, st) : VARQ_OK;
 }

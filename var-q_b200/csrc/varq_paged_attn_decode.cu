@@ -10,7 +10,10 @@
 //                   permutes, and P^T is the transpose of S^T's fragment (movmatrix).
 // As in the chunk kernel the V scale goes into the exponent: x = S * (K scale * factor of the row) + log2(V scale), P = 2^(x - m) in fp16,
 // l += P / V scale in fp32; the reference m is raised only when an x passes it by more than 8.  Queries are fp16 times a power of two per row, exact
-// but for elements 2^-22 times smaller than the row's largest.  Warps and CTAs (key ranges) are merged by the log-sum-exp rule.
+// but for elements 2^-22 times smaller than the row's largest.  Warps and CTAs (key ranges) are merged by the log-sum-exp rule: where all CTAs are resident
+// at once, up to eight of a row tile are a cluster and read one another's shared memory; else they leave parts in the workspace for a second launch.
+#include <cooperative_groups.h>
+
 #include <cfloat>
 #include <type_traits>
 
@@ -93,7 +96,7 @@ template <int BITS, int NW> __device__ __forceinline__ void pd_join(const uint32
 
 template <int KB, int VB, int D, int NT>
 __global__ void __launch_bounds__(PD_WARPS * 32, NT > 1 ? (D == 128 ? 3 : 4) : D == 128 ? (KB == 8 && VB == 8 ? 3 : 4) : 5)
-paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int tiles_per_split, float* ws_o, float* ws_ml, int* status) {
+paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, int* status) {
     using P = PdPlan<KB, VB, D>;
     constexpr int KBYTES = D / 4 * KB / 8, VBYTES = D / 8 * VB / 8;       // of a row and thread
     constexpr int KROW = P::KROW, VROW = P::VROW, ST = P::ST;
@@ -334,8 +337,14 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int tiles_
         }
     }
     __syncthreads();
-    // ---- merge the warps, then write the output or this split's part
+    // ---- merge the warps, then write the output, meet the cluster, or leave this split's part
     const long long n_rows = (long long)a.T * a.Hq;
+    auto finish = [&](int row, int d, float num, float den, float M) {
+        const int token = row / a.G, head = h * a.G + row - token * a.G;
+        store_o_elem(a.out, a.dtype, (long long)(seq.q0 + token) * a.os_t + head * a.os_h + d, den != 0.f ? num / den : 0.f);
+        if (d == 0 && a.lse) a.lse[(long long)(seq.q0 + token) * a.Hq + head] = den != 0.f ? (M + __log2f(den)) * 0.6931471805599453f : -INFINITY;
+    };
+    float (*s_cta)[D + 2] = reinterpret_cast<float (*)[D + 2]>(pd_smem + PD_WARPS * ROWS * (D + 2) * 4);
     for (int j = threadIdx.x; j < ROWS * D; j += PD_WARPS * 32) {
         const int r = j / D, d = j - r * D, row = row0 + r;
         if (row >= rows) break;
@@ -349,46 +358,80 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int tiles_
             num = fmaf(wt, s_part[w][r][d], num);
             den = fmaf(wt, s_part[w][r][D + 1], den);
         }
-        const int token = row / a.G, head = h * a.G + row - token * a.G;
-        const long long out_row = (long long)(seq.q0 + token) * a.Hq + head;
-        if (splits == 1) {
-            store_o_elem(a.out, a.dtype, (long long)(seq.q0 + token) * a.os_t + head * a.os_h + d, den != 0.f ? num / den : 0.f);
-            if (d == 0 && a.lse) a.lse[out_row] = den != 0.f ? (M + __log2f(den)) * 0.6931471805599453f : -INFINITY;
+        if (splits == 1) finish(row, d, num, den, M);
+        else if (in_cluster) {
+            s_cta[r][d] = num;
+            if (d == 0) { s_cta[r][D] = M; s_cta[r][D + 1] = den; }
         } else {
+            const int token = row / a.G, head = h * a.G + row - token * a.G;
+            const long long out_row = (long long)(seq.q0 + token) * a.Hq + head;
             ws_o[(split * n_rows + out_row) * D + d] = num;
             if (d == 0) *reinterpret_cast<float2*>(ws_ml + (split * n_rows + out_row) * 2) = make_float2(M, den);
         }
     }
+    if (in_cluster) {
+        const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+        cluster.sync();
+        for (int j = threadIdx.x + split * (PD_WARPS * 32); j < ROWS * D; j += splits * (PD_WARPS * 32)) {      // the CTAs share out the elements
+            const int r = j / D, d = j - r * D;
+            if (row0 + r >= rows) break;
+            float M = -FLT_MAX, num = 0.f, den = 0.f;
+            for (int s = 0; s < splits; ++s) M = fmaxf(M, cluster.map_shared_rank(&s_cta[r][D], s)[0]);
+            for (int s = 0; s < splits; ++s) {
+                const float* p = cluster.map_shared_rank(&s_cta[r][0], s);
+                const float wt = pd_ex2(p[D] - M);
+                num = fmaf(wt, p[d], num);
+                den = fmaf(wt, p[D + 1], den);
+            }
+            finish(row0 + r, d, num, den, M);
+        }
+        cluster.sync();                          // nobody leaves while its shared memory is read
+    }
 }
 
-// One warp per output row: the splits' numerators and sums, by the log-sum-exp rule, in the splits' order
-template <int D>
+// W warps per output row (more where there are many splits): the splits' numerators and sums, by the log-sum-exp rule, always in the same order
+template <int D, int W>
 __global__ void __launch_bounds__(128) paged_attn_merge_kernel(PagedAttnArgs a, int splits, const float* ws_o, const float* ws_ml) {
     constexpr int V = D / 32;
+    __shared__ float part[4][D + 1];
     pdl_trigger();
     pdl_wait();
-    const long long n_rows = (long long)a.T * a.Hq, row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (row >= n_rows) return;
-    float M = -FLT_MAX;
-    for (int s = lane; s < splits; s += 32) M = fmaxf(M, ws_ml[(s * n_rows + row) * 2]);
-#pragma unroll
-    for (int z = 16; z; z >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, z));
-    float num[V], den = 0.f;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w0 = warp % W;
+    const long long n_rows = (long long)a.T * a.Hq, row = (long long)blockIdx.x * (4 / W) + warp / W;
+    float num[V], den = 0.f, M = -FLT_MAX;
 #pragma unroll
     for (int i = 0; i < V; ++i) num[i] = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
-        const float2 ml = *reinterpret_cast<const float2*>(ws_ml + (s * n_rows + row) * 2);
-        const float w = pd_ex2(ml.x - M);
-        den = fmaf(w, ml.y, den);
-        const float* o = ws_o + (s * n_rows + row) * D + lane * V;
+    if (row < n_rows) {
+        for (int s = lane; s < splits; s += 32) M = fmaxf(M, ws_ml[(s * n_rows + row) * 2]);
 #pragma unroll
-        for (int i = 0; i < V; i += 2) {
-            const float2 x = *reinterpret_cast<const float2*>(o + i);
-            num[i] = fmaf(w, x.x, num[i]); num[i + 1] = fmaf(w, x.y, num[i + 1]);
+        for (int z = 16; z; z >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, z));
+#pragma unroll 8
+        for (int s = w0; s < splits; s += W) {
+            const float2 ml = *reinterpret_cast<const float2*>(ws_ml + (s * n_rows + row) * 2);
+            const float w = pd_ex2(ml.x - M);
+            den = fmaf(w, ml.y, den);
+            const float* o = ws_o + (s * n_rows + row) * D + lane * V;
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+                const float2 x = *reinterpret_cast<const float2*>(o + i);
+                num[i] = fmaf(w, x.x, num[i]); num[i + 1] = fmaf(w, x.y, num[i + 1]);
+            }
         }
     }
+    if constexpr (W > 1) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) part[warp][lane * V + i] = num[i];
+        if (lane == 0) part[warp][D] = den;
+        __syncthreads();
+        if (w0) return;
+#pragma unroll
+        for (int w = 1; w < W; ++w) {
+            den += part[warp + w][D];
+#pragma unroll
+            for (int i = 0; i < V; ++i) num[i] += part[warp + w][lane * V + i];
+        }
+    }
+    if (row >= n_rows) return;
     const long long token = row / a.Hq;
     const int head = (int)(row - token * a.Hq);
     const float inv = den != 0.f ? 1.f / den : 0.f;
@@ -398,8 +441,8 @@ __global__ void __launch_bounds__(128) paged_attn_merge_kernel(PagedAttnArgs a, 
 }
 
 template <int KB, int VB, int D, int NT>
-int launch_nt(const PagedAttnArgs& a, int splits, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st) {
-    constexpr int PART = PD_WARPS * 8 * NT * (D + 2) * 4, SMEM = PdPlan<KB, VB, D>::SMEM > PART ? PdPlan<KB, VB, D>::SMEM : PART;
+int launch_nt(const PagedAttnArgs& a, int splits, bool in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st) {
+    constexpr int PART = (PD_WARPS + 1) * 8 * NT * (D + 2) * 4, SMEM = PdPlan<KB, VB, D>::SMEM > PART ? PdPlan<KB, VB, D>::SMEM : PART;
     const long long rows = (long long)a.max_q * a.G;
     const int n_rowtiles = (int)((rows + 8 * NT - 1) / (8 * NT));
     const long long blocks = (long long)a.B * a.c.H * n_rowtiles * splits;
@@ -411,31 +454,33 @@ int launch_nt(const PagedAttnArgs& a, int splits, int tiles_per_split, float* ws
         VARQ_CUDA_TRY(cudaFuncSetAttribute(paged_attn_decode_kernel<KB, VB, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
-    VARQ_CUDA_TRY(launch_pdl(paged_attn_decode_kernel<KB, VB, D, NT>, (unsigned)blocks, PD_WARPS * 32, SMEM, st, 1, a, n_rowtiles, splits, tiles_per_split, ws_o, ws_ml,
+    VARQ_CUDA_TRY(launch_pdl(paged_attn_decode_kernel<KB, VB, D, NT>, (unsigned)blocks, PD_WARPS * 32, SMEM, st, in_cluster ? splits : 1, a, n_rowtiles, splits, in_cluster, tiles_per_split, ws_o, ws_ml,
                              paged_status_word()));
     count_launches(1);
     return VARQ_OK;
 }
 template <int KB, int VB, int D>
-int launch(const PagedAttnArgs& a, int splits, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st) {
-    return (long long)a.max_q * a.G <= 8 ? launch_nt<KB, VB, D, 1>(a, splits, tiles_per_split, ws_o, ws_ml, st) : launch_nt<KB, VB, D, 2>(a, splits, tiles_per_split, ws_o, ws_ml, st);
+int launch(const PagedAttnArgs& a, int splits, bool in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st) {
+    return (long long)a.max_q * a.G <= 8 ? launch_nt<KB, VB, D, 1>(a, splits, in_cluster, tiles_per_split, ws_o, ws_ml, st) : launch_nt<KB, VB, D, 2>(a, splits, in_cluster, tiles_per_split, ws_o, ws_ml, st);
 }
 
 }  // namespace
 
-int paged_attn_decode_run(const PagedAttnArgs& a, int splits, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st) {
+int paged_attn_decode_run(const PagedAttnArgs& a, int splits, bool in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st) {
 #define GO(K_, V_) \
-    if (a.c.kb == K_ && a.c.vb == V_) return a.c.D == 64 ? launch<K_, V_, 64>(a, splits, tiles_per_split, ws_o, ws_ml, st) : launch<K_, V_, 128>(a, splits, tiles_per_split, ws_o, ws_ml, st);
+    if (a.c.kb == K_ && a.c.vb == V_) return a.c.D == 64 ? launch<K_, V_, 64>(a, splits, in_cluster, tiles_per_split, ws_o, ws_ml, st) : launch<K_, V_, 128>(a, splits, in_cluster, tiles_per_split, ws_o, ws_ml, st);
     GO(8, 8) GO(8, 4) GO(8, 2) GO(4, 8) GO(4, 4) GO(4, 2) GO(2, 8) GO(2, 4) GO(2, 2)
 #undef GO
     return fail(VARQ_ERR_ARG, "varq_paged_attn: bits must be 2, 4 or 8");
 }
 
 int paged_attn_merge_run(const PagedAttnArgs& a, int splits, const float* ws_o, const float* ws_ml, cudaStream_t st) {
-    const long long blocks = ((long long)a.T * a.Hq + 3) / 4;
+    const int w = splits > 8 ? 4 : 1;
+    const long long blocks = ((long long)a.T * a.Hq * w + 3) / 4;
     if (blocks > 0x7fffffffLL) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_attn: more than 2^31 thread blocks");
-    VARQ_CUDA_TRY(a.c.D == 64 ? launch_pdl(paged_attn_merge_kernel<64>, (unsigned)blocks, 128, 0, st, 1, a, splits, ws_o, ws_ml)
-                              : launch_pdl(paged_attn_merge_kernel<128>, (unsigned)blocks, 128, 0, st, 1, a, splits, ws_o, ws_ml));
+#define GO(D_, W_) if (a.c.D == D_ && w == W_) VARQ_CUDA_TRY(launch_pdl(paged_attn_merge_kernel<D_, W_>, (unsigned)blocks, 128, 0, st, 1, a, splits, ws_o, ws_ml));
+    GO(64, 1) GO(64, 4) GO(128, 1) GO(128, 4)
+#undef GO
     count_launches(1);
     return VARQ_OK;
 }

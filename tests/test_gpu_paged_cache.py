@@ -285,3 +285,54 @@ def test_page_table_with_a_cache():
     cache.append(x.to(DEV), x.to(DEV), table.extend(["c"], [48], DEV))
     check(cache, x, x, table.slots("c", "cpu"))
     check(cache, torch.cat(kept["b"]), -torch.cat(kept["b"]), table.slots("b", "cpu"))
+
+
+@pytest.mark.parametrize("T", [1, 7, 300])
+@pytest.mark.parametrize("kb,vb", [(8, 4), (2, 8)])
+def test_nothing_is_written_outside(T, kb, vb):
+    """pools, values, outputs and log-sums carved out of larger buffers whose rest has to stay as it is"""
+    H, D, page, pages, G = 3, 64, 16, 24, 2
+    lib = _cabi.lib()
+    guard = 12345.0
+
+    def carved(shape, dtype):
+        n = int(torch.Size(shape).numel())
+        big = torch.full((n + 256,), guard, dtype=torch.float32, device=DEV).to(dtype)
+        return big, big[128:128 + n].view(shape)
+
+    shape = (pages, H, page)
+    bigs, pools = zip(carved((*shape, D * kb // 32), torch.int32), carved((*shape, D * vb // 32), torch.int32), carved(shape, torch.float32), carved(shape, torch.float32))
+    cache = PagedCache.over(*pools, D)
+    slots = torch.randperm(pages * page)[:T]
+    slots[T // 2] = pages * page - 1 if pages * page - 1 not in slots else slots[T // 2]
+    k, v = torch.randn((T, H, D)), torch.randn((T, H, D))
+    cache.append(k.to(DEV), v.to(DEV), slots.to(DEV))
+    check(cache, k, v, slots)
+    read = [carved((T, H, D), torch.float16) for _ in range(2)]
+    desc = [_cabi.Tensor(t.data_ptr(), _cabi.F16, 0, 0, H * D, D) for _, t in read]
+    c = _cabi.Paged(*(p.data_ptr() for p in pools), pages, page, H, D, kb, vb)
+    s = slots.to(DEV)
+    _cabi.check(lib.varq_paged_read(c, s.data_ptr(), T, *desc, _cabi.stream_ptr(DEV)))
+    assert torch.equal(read[0][1], cache.read(s, torch.float16)[0]) and torch.equal(read[1][1], cache.read(s, torch.float16)[1])
+    # attention: a sequence over the first pages
+    full = torch.arange(pages * page)
+    x = torch.randn((pages * page, H, D), device=DEV)
+    cache.append(x, x, full.to(DEV))
+    n = min(T + 20, pages * page)
+    q = torch.randn((T, H * G, D), device=DEV).half()
+    table = torch.arange(pages, dtype=torch.int32, device=DEV).view(1, -1)
+    lens, starts = (torch.tensor(z, dtype=torch.int32, device=DEV) for z in ([n], [0, T]))
+    big_o, out = carved((T, H * G, D), torch.float16)
+    big_l, lse = carved((T, H * G), torch.float32)
+    od, qd = (_cabi.Tensor(t.data_ptr(), _cabi.F16, 0, 0, H * G * D, D) for t in (out, q))
+    b = _cabi.PagedBatch(starts.data_ptr(), lens.data_ptr(), table.data_ptr(), pages, T, pages, 1, H * G, T, n, 1, 0, 0, 0.125)
+    need = lib.varq_paged_attn_workspace_bytes(c, b)
+    ws = torch.full((need + 512,), 77, dtype=torch.uint8, device=DEV)
+    _cabi.check(lib.varq_paged_attn(c, b, qd, od, lse.data_ptr(), ws.data_ptr() + 256, need, _cabi.stream_ptr(DEV)))
+    ref = cache.attend(q, table, lens, starts, T, n, 0.125, return_lse=True)
+    assert torch.equal(out, ref[0]) and torch.equal(lse, ref[1])
+    assert (ws[:256] == 77).all() and (ws[256 + need:] == 77).all()
+    for big, t in list(zip(bigs, pools)) + read + [(big_o, out), (big_l, lse)]:
+        edge = torch.cat([big[:128], big[128 + t.numel():]])
+        assert torch.equal(edge, torch.full_like(edge, guard))
+    assert lib.varq_paged_attn(c, b, qd, od, lse.data_ptr(), None, need - 1, _cabi.stream_ptr(DEV)) == (_cabi.ERR_WORKSPACE if need else 0)

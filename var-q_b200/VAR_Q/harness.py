@@ -8,6 +8,9 @@ only that skeleton with randomly initialised torch layers of the same shapes: La
 ``VAR_Q.hooks.install``) -> LayerNorm -> 4x MLP per block, a random token map per scale in place of sampling and
 embedding.  It exists to time the hot path where it runs in practice -- between GEMMs, launched from Python or
 replayed as one CUDA graph -- not to generate images.
+
+``StandInDecoder`` is the same for serving: a causal decoder skeleton over paged caches, whose sequences come, are prefilled chunk by chunk next to
+others that decode token by token, and go.
 """
 import math
 from typing import Optional, Sequence
@@ -15,6 +18,7 @@ from typing import Optional, Sequence
 import torch
 
 from .hooks import install
+from .paged import PagedCache, PageTable
 
 
 class StandInSelfAttention(torch.nn.Module):
@@ -86,3 +90,50 @@ class StandInVAR(torch.nn.Module):
         g = torch.Generator(device=device).manual_seed(seed)
         return [torch.randn((2 * batch, p * p, self.width), generator=g, device=device, dtype=torch.float32).to(dtype)
                 for p in self.patch_nums]
+
+
+class StandInDecoderBlock(torch.nn.Module):
+    def __init__(self, width: int, heads: int, kv_heads: int, head_dim: int, cache: PagedCache, window: Optional[int], sinks: int):
+        super().__init__()
+        self.heads, self.kv_heads, self.head_dim, self.cache, self.window, self.sinks = heads, kv_heads, head_dim, cache, window, sinks
+        self.ln1, self.ln2 = torch.nn.LayerNorm(width), torch.nn.LayerNorm(width)
+        self.qkv = torch.nn.Linear(width, (heads + 2 * kv_heads) * head_dim, bias=False)
+        self.proj = torch.nn.Linear(heads * head_dim, width, bias=False)
+        self.fc1, self.fc2 = torch.nn.Linear(width, 4 * width), torch.nn.Linear(4 * width, width)
+
+    def forward(self, x, slots, batch):
+        # q, k and v stay views of the fused activation: the operators read them with their strides
+        q, k, v = self.qkv(self.ln1(x)).unflatten(-1, (-1, self.head_dim)).split((self.heads, self.kv_heads, self.kv_heads), 1)
+        self.cache.append(k, v, slots)
+        out = self.cache.attend(q, *batch, 1.0 / math.sqrt(self.head_dim), window=self.window, sinks=self.sinks)
+        x = x + self.proj(out.flatten(1))
+        return x + self.fc2(torch.nn.functional.gelu(self.fc1(self.ln2(x)), approximate='tanh'))
+
+
+class StandInDecoder(torch.nn.Module):
+    """``step`` advances any mix of sequences by any number of tokens each; one ``PageTable`` serves all layers, each of which has a cache of its own."""
+
+    def __init__(self, depth: int = 4, width: int = 1024, heads: int = 16, kv_heads: int = 4, head_dim: int = 64, num_pages: int = 256, page_size: int = 64,
+                 k_bits: int = 8, v_bits: int = 8, window: Optional[int] = None, sinks: int = 0, device="cuda"):
+        super().__init__()
+        self.table, self.device_ = PageTable(num_pages, page_size), device
+        caches = [PagedCache(num_pages, page_size, kv_heads, head_dim, k_bits, v_bits, device) for _ in range(depth)]
+        self.blocks = torch.nn.ModuleList(StandInDecoderBlock(width, heads, kv_heads, head_dim, c, window, sinks) for c in caches)
+        self.to(device)
+
+    @torch.inference_mode()
+    def step(self, seqs: Sequence, xs: Sequence[torch.Tensor]) -> Sequence[torch.Tensor]:
+        """``xs[i]`` ``[n_i, width]``: the next inputs of ``seqs[i]`` (new sequences are taken in).  Returns their hidden states."""
+        for s in seqs:
+            if s not in self.table:
+                self.table.add(s)
+        counts = [x.size(0) for x in xs]
+        slots = self.table.extend(seqs, counts, self.device_)
+        batch = self.table.batch(seqs, counts, self.device_)
+        x = torch.cat(list(xs))
+        for b in self.blocks:
+            x = b(x, slots, batch)
+        return x.split(counts)
+
+    def finish(self, seq) -> None:
+        self.table.remove(seq)

@@ -103,6 +103,9 @@ class PageTable:
     def free_pages(self) -> int:
         return len(self._free)
 
+    def __contains__(self, seq) -> bool:
+        return seq in self._pages
+
     def add(self, seq) -> None:
         """A new, empty sequence."""
         if seq in self._pages:

@@ -393,7 +393,7 @@ AttnPlan plan_attn(const varq_paged_t* c, const varq_paged_batch_t* b) {
     p.splits = 1; p.cluster = false;
     for (long long s = 1; s == 1 || (s <= tiles / least && s <= 256); ++s) {
         const bool near = !p.tc && s <= PAGED_CLUSTER && base * s <= room;
-        const long long cost = (base * s + room - 1) / room * ((tiles + s - 1) / s + fixed) + (s > 1 && !near ? merge : 0);
+        const long long cost = (base * s + room - 1) / room * ((tiles + s - 1) / s + fixed + (s > 1 && p.tc ? fixed : 0)) + (s > 1 && !near ? merge : 0);
         if (best == 0 || cost < best) { best = cost; p.splits = (int)s; p.cluster = s > 1 && near; }
         if (base * s > 8 * room) break;
     }

@@ -20,25 +20,31 @@
 namespace varq {
 namespace {
 
-constexpr int PT_M = 128, PT_N = 128;
+constexpr int PT_M = 128, PT_N = 64;
 constexpr float PT_LAZY = 8.f;
 
 template <int D> struct PtPlan {
-    static constexpr int KST = 2, VST = 2, TS = 4;                 // stages of K and V, tables (a table outlives its K stage by a tile)
+    static constexpr int SB = D == 64 ? 3 : 2;                     // score tiles per query tile
+    static constexpr int KST = 4, VST = 4, TS = 8;                 // stages of K and V; tables: a table is read until its P is written, SB tiles behind its K
     static constexpr int Q_BYTES = PT_M * D * 2, T_BYTES = PT_N * D * 2;
     static constexpr int TAB_FLOATS = 3 * PT_N;
     static constexpr int OFF_Q = 0, OFF_K = OFF_Q + 2 * Q_BYTES, OFF_V = OFF_K + KST * T_BYTES, OFF_TAB = OFF_V + VST * T_BYTES;
-    static constexpr int OFF_BAR = OFF_TAB + TS * TAB_FLOATS * 4, N_BARS = 2 * KST + 2 * VST + TS + 9;
-    static constexpr int OFF_QF = (OFF_BAR + N_BARS * 8 + 15) / 16 * 16, OFF_MISC = OFF_QF + 2 * PT_M * 4, SMEM = OFF_MISC + 16 + 1024;
-    static constexpr int COL_S = 0, COL_O = 2 * PT_N, TMEM_COLS = 512;
-    static_assert(COL_O + 2 * D <= TMEM_COLS && SMEM <= 227 * 1024, "plan");
-    static constexpr int THREADS = 640, REGS = 96, REGS_SOFT = 136, REGS_CONV = 72, REGS_MISC = 64;
-    static_assert(256 * REGS_SOFT + 256 * REGS_CONV + 128 * REGS_MISC <= THREADS * REGS, "register plan");
+    // barriers: K, V written and free; tables written; queries; S, P of every score tile; O (a ring of four tiles); end
+    static constexpr int B_K = 0, B_KF = B_K + KST, B_V = B_KF + KST, B_VF = B_V + VST, B_TAB = B_VF + VST, B_Q = B_TAB + TS, B_S = B_Q + 2, B_P = B_S + 2 * SB,
+                         B_O = B_P + 2 * SB, B_END = B_O + 8, N_BARS = B_END + 2;
+    static constexpr int OFF_BAR = OFF_TAB + TS * TAB_FLOATS * 4;
+    static constexpr int OFF_QF = (OFF_BAR + N_BARS * 8 + 15) / 16 * 16;              // factors of the queries [2][128]
+    static constexpr int OFF_XCH = OFF_QF + 2 * PT_M * 4, OFF_MISC = OFF_XCH + 2 * 2 * PT_M * 4, SMEM = OFF_MISC + 16 + 1024;      // a value per row and column half
+    static constexpr int COL_O = 0, COL_S = 2 * D, TMEM_COLS = 512;
+    static_assert(COL_S + 2 * SB * PT_N <= TMEM_COLS && SMEM <= 227 * 1024 && TS >= KST + SB, "plan");
+    static constexpr int SOFT = 8, K_WARP0 = SOFT, V_WARP0 = K_WARP0 + 4, MMA_WARP = V_WARP0 + 4, THREADS = (MMA_WARP + 4) * 32;
+    static constexpr int REGS = 96, REGS_SOFT = 152, REGS_CONV = 64, REGS_MISC = 48;
+    static_assert(SOFT * 32 * REGS_SOFT + 256 * REGS_CONV + 128 * REGS_MISC <= THREADS * REGS, "register plan");
 };
 
-// 16-byte chunk `ch` (eight head_dim values) of row `r` in a 128B-swizzled tile of 128 rows: blocks of 64 columns
-__device__ __forceinline__ uint32_t pt_chunk(int r, int ch) {
-    return (uint32_t)((ch >> 3) * (128 * 128) + (r >> 3) * 1024 + (r & 7) * 128 + (((ch & 7) ^ (r & 7)) << 4));
+// 16-byte chunk `ch` (eight head_dim values) of row `r` in a 128B-swizzled tile of ROWS rows: blocks of 64 columns
+template <int ROWS> __device__ __forceinline__ uint32_t pt_chunk(int r, int ch) {
+    return (uint32_t)((ch >> 3) * (ROWS * 128) + (r >> 3) * 1024 + (r & 7) * 128 + (((ch & 7) ^ (r & 7)) << 4));
 }
 // D[tmem] (+)= A[smem] B[smem]
 __device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -124,28 +130,24 @@ __device__ __forceinline__ void q_operand_order(uint32_t (&w)[8], int kb) {
 template <int D>
 __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(PagedAttnArgs a, int n_qblocks, int splits, float* ws_o, float* ws_ml, int* status) {
     using P = PtPlan<D>;
-    constexpr int KST = P::KST, VST = P::VST, TS = P::TS;
+    constexpr int KST = P::KST, VST = P::VST, TS = P::TS, SB = P::SB;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + P::OFF_BAR);
-    uint64_t *bar_k = bars, *bar_kf = bar_k + KST, *bar_v = bar_kf + KST, *bar_vf = bar_v + VST, *bar_tab = bar_vf + VST;   // written, free; tables written
-    uint64_t *bar_q = bar_tab + TS, *bar_s = bar_q + 2, *bar_p = bar_s + 2, *bar_o = bar_p + 2, *bar_end = bar_o + 2;      // [2]: by query tile
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + P::OFF_MISC);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + P::OFF_MISC + 8);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
-    if (warp == 17) {
-        if (lane < P::N_BARS) {
-            const int i = lane;
-            const bool by_4 = i < KST || (i >= 2 * KST && i < 2 * KST + VST) || (i >= 2 * KST + 2 * VST + TS && i < 2 * KST + 2 * VST + TS + 2) ||
-                              (i >= 2 * KST + 2 * VST + TS + 4 && i < 2 * KST + 2 * VST + TS + 6);         // warps that arrive
-            const bool by_8 = i >= 2 * KST + 2 * VST && i < 2 * KST + 2 * VST + TS;
-            mbar_init(&bars[i], by_4 ? 4u : by_8 ? 8u : 1u);
+    if (warp == P::MMA_WARP + 2) {
+        for (int i = lane; i < P::N_BARS; i += 32) {        // warps that arrive
+            const bool by_8 = i >= P::B_TAB && i < P::B_Q, by_4 = i < P::B_KF || (i >= P::B_V && i < P::B_VF) || (i >= P::B_Q && i < P::B_S) || (i >= P::B_P && i < P::B_O);
+            const bool by_2 = (i >= P::B_KF && i < P::B_V) || (i >= P::B_VF && i < P::B_TAB);
+            mbar_init(&bars[i], by_8 ? 8u : by_4 ? 4u : by_2 ? 2u : 1u);
         }
         if (lane == 0) *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 16) {
+    if (warp == P::MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)P::TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -180,12 +182,12 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
     const int page_mask = (1 << a.c.page_shift) - 1;
     const int32_t* table = a.table + b * a.table_stride;
 
-    if (warp < 8) {
+    if (warp < P::SOFT) {
         // =============================================================== softmax, epilogue
         set_registers<P::REGS_SOFT, P::REGS>();
         const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane, row = row0 + t * PT_M + r;
         const bool live = row < rows;
-        const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16), col_s = lane_base + P::COL_S + t * PT_N, col_o = lane_base + P::COL_O + t * D;
+        const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16), col_s0 = lane_base + P::COL_S + t * (SB * PT_N), col_o = lane_base + P::COL_O + t * D;
         if (row0 + t * PT_M < rows) {
             const int token = live ? row / a.G : 0, head = h * a.G + (live ? row - token * a.G : 0);
             // ---- queries -> fp16 in shared memory, in the order in which the codes of K are unpacked
@@ -220,12 +222,12 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                         for (int j = 0; j < 8; ++j) w[j] = pack_half2(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xffff0000u) * f);
                     }
                     q_operand_order(w, a.c.kb);
-                    sts128(qs + pt_chunk(r, 2 * i), w[0], w[1], w[2], w[3]);
-                    sts128(qs + pt_chunk(r, 2 * i + 1), w[4], w[5], w[6], w[7]);
+                    sts128(qs + pt_chunk<PT_M>(r, 2 * i), w[0], w[1], w[2], w[3]);
+                    sts128(qs + pt_chunk<PT_M>(r, 2 * i + 1), w[4], w[5], w[6], w[7]);
                 }
             }
             fence_async_smem();
-            warp_arrive(&bar_q[t], lane);
+            warp_arrive(&bars[P::B_Q + t], lane);
             const bool scaled = __any_sync(0xffffffffu, q_factor != 1.f);
             if (scaled) reinterpret_cast<float*>(smem + P::OFF_QF)[t * PT_M + r] = q_factor;
             __syncwarp();
@@ -252,101 +254,105 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
 #pragma unroll 1
             for (int j = 0; j < n; ++j) {
                 const int key0 = tiles.key(tile0 + j);
-                ok = mbar_wait(&bar_tab[j % TS], (j / TS) & 1, abort_flag, 201) && mbar_wait(&bar_s[t], j & 1, abort_flag, 202);
+                ok = mbar_wait(&bars[P::B_TAB + j % TS], (j / TS) & 1, abort_flag, 201) && mbar_wait(&bars[P::B_S + t * SB + j % SB], (j / SB) & 1, abort_flag, 202);
+                const uint32_t col_s = col_s0 + (j % SB) * PT_N;
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
                 const float* tab = reinterpret_cast<const float*>(smem + P::OFF_TAB) + (j % TS) * P::TAB_FLOATS;
-                // Two forms of a tile, so that the usual one carries neither masks nor factors: as branches inside they cost 10 % of a long call
+                // Two forms of a tile, so that the usual one carries neither masks nor factors: as branches inside they cost 10 % of a long call.  The scores of a
+                // chunk of 32 keys come with their maximum and the vote on it while the exponentials of the chunk before are at work: alone the chain of load,
+                // maximum, vote and branch takes as long as those (613 cycles a chunk one after the other, 341 so; 280 with two warps on a scheduler, 256 the
+                // exponentials alone).
                 auto tile = [&](auto special_) {
                     constexpr bool SPECIAL = decltype(special_)::value != 0;
-#pragma unroll 1
-                    for (int c = 0; c < PT_N / 32; ++c) {
-                        pair x[16];                              // x - m of 32 columns: [half of the rows][eight columns][row g, g + 8]
-                        bool again = true;
-#pragma unroll 1
-                        while (true) {
-                            uint32_t s[32];
-                            tmem_ld_16x256(col_s + 32 * c, s);
-                            tmem_ld_16x256(col_s + 32 * c + (16u << 16), s + 16);
-                            tmem_loaded(s);
+                    // x - m of 32 columns: [half of the rows][eight columns][row g, g + 8]; true where a row needs another reference
+                    auto scores = [&](pair (&x)[16], int c) -> bool {
+                        uint32_t s[32];
+                        tmem_ld_16x256(col_s + 32 * c, s);
+                        tmem_ld_16x256(col_s + 32 * c + (16u << 16), s + 16);
+                        tmem_loaded(s);
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) x[i] = pair_of_bits(s[2 * i], s[2 * i + 1]);
-                            if (SPECIAL && scaled) {
-                                const float* qf = reinterpret_cast<const float*>(smem + P::OFF_QF) + t * PT_M + quarter * 32 + g;
+                        for (int i = 0; i < 16; ++i) x[i] = pair_of_bits(s[2 * i], s[2 * i + 1]);
+                        if (SPECIAL && scaled) {
+                            const float* qf = reinterpret_cast<const float*>(smem + P::OFF_QF) + t * PT_M + quarter * 32 + g;
 #pragma unroll
-                                for (int i = 0; i < 16; ++i) { const float f = qf[8 * ((i >> 3) * 2 + (i & 1))]; x[i] = mul2(x[i], pair_of(f, f)); }
-                            }
+                            for (int i = 0; i < 16; ++i) { const float f = qf[8 * ((i >> 3) * 2 + (i & 1))]; x[i] = mul2(x[i], pair_of(f, f)); }
+                        }
 #pragma unroll
-                            for (int v = 0; v < 4; ++v) {
-                                const ulonglong2 ab = *reinterpret_cast<const ulonglong2*>(tab + (c * 16 + v * 4 + cq) * 4);
+                        for (int v = 0; v < 4; ++v) {
+                            const ulonglong2 ab = *reinterpret_cast<const ulonglong2*>(tab + (c * 16 + v * 4 + cq) * 4);
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) { pair& y = x[(i >> 1) * 8 + v * 2 + (i & 1)]; y = add2(fma2(y, ab.x, ab.y), nm[i]); }
-                            }
-                            if (SPECIAL) {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const PagedSpan sp = paged_span(a, pos[i], seq.kv);
-                                    // bit k: this thread's column 2c + k of the 32 is seen
-                                    auto below = [](int k) { return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1u; };
-                                    const int c0 = key0 + 32 * c + 2 * cq;
-                                    const uint32_t sees = below(sp.hi - c0) & (~below(sp.lo - c0) | below(a.sinks - c0));
-#pragma unroll
-                                    for (int v = 0; v < 4; ++v) {
-                                        pair& y = x[(i >> 1) * 8 + v * 2 + (i & 1)];
-                                        y = pair_of(sees >> (8 * v) & 1u ? pair_x(y) : -INFINITY, sees >> (8 * v + 1) & 1u ? pair_y(y) : -INFINITY);
-                                    }
-                                }
-                            }
-                            float top0 = -INFINITY, top1 = -INFINITY;
-#pragma unroll
-                            for (int i = 0; i < 16; i += 2) {
-                                top0 = fmaxf(top0, fmaxf(pair_x(x[i]), pair_y(x[i])));
-                                top1 = fmaxf(top1, fmaxf(pair_x(x[i + 1]), pair_y(x[i + 1])));
-                            }
-                            if (!again || !__any_sync(0xffffffffu, unset != 0u || fmaxf(top0, top1) > PT_LAZY)) break;
-                            // new references, then the chunk once more: changed in place, x would be copied on the way that is always taken
-                            again = false;
-                            float alpha[4];
+                            for (int i = 0; i < 4; ++i) { pair& y = x[(i >> 1) * 8 + v * 2 + (i & 1)]; y = add2(fma2(y, ab.x, ab.y), nm[i]); }
+                        }
+                        if (SPECIAL) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                float up = -INFINITY;                        // how far the row's largest x is above its reference
+                                const PagedSpan sp = paged_span(a, pos[i], seq.kv);
+                                // bit k: this thread's column 2c + k of the 32 is seen
+                                auto below = [](int k) { return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1u; };
+                                const int c0 = key0 + 32 * c + 2 * cq;
+                                const uint32_t sees = below(sp.hi - c0) & (~below(sp.lo - c0) | below(a.sinks - c0));
 #pragma unroll
-                                for (int v = 0; v < 4; ++v) { const pair y = x[(i >> 1) * 8 + v * 2 + (i & 1)]; up = fmaxf(up, fmaxf(pair_x(y), pair_y(y))); }
-                                up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 1));
-                                up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 2));
-                                const bool first = (unset >> i & 1u) && up > -INFINITY;
-                                up = first || (up > PT_LAZY && !(unset >> i & 1u)) ? up : 0.f;
-                                alpha[i] = first ? 1.f : ex2(-up);           // (nothing is accumulated where the reference is the first)
-                                if (first) unset &= ~(1u << i);
-                                nm[i] = add2(nm[i], pair_of(-up, -up));
-                                l[i] = mul2(l[i], pair_of(alpha[i], alpha[i]));
-                            }
-                            const float al = by_lane(alpha);
-                            const __half2 ah = __float2half2_rn(al);
-                            tmem_wait_st();
-#pragma unroll 1
-                            for (int z = 0; z < c; ++z) {                    // P of the tile's chunks before this one
-                                uint32_t o[16];
-                                tmem_ld16(col_s + 16 * z, o);
-                                tmem_wait_ld();
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) o[i] = h2_mul(o[i], *reinterpret_cast<const uint32_t*>(&ah));
-                                tmem_st16(col_s + 16 * z, o);
-                            }
-                            if (j > 0) {                                     // the products of the tiles before are complete: S came behind them
-#pragma unroll 1
-                                for (int z = 0; z < D; z += 16) {
-                                    uint32_t o[16];
-                                    tmem_ld16(col_o + z, o);
-                                    tmem_wait_ld();
-#pragma unroll
-                                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
-                                    tmem_st16(col_o + z, o);
+                                for (int v = 0; v < 4; ++v) {
+                                    pair& y = x[(i >> 1) * 8 + v * 2 + (i & 1)];
+                                    y = pair_of(sees >> (8 * v) & 1u ? pair_x(y) : -INFINITY, sees >> (8 * v + 1) & 1u ? pair_y(y) : -INFINITY);
                                 }
                             }
                         }
-                        uint32_t pk[16];                         // P of the chunk: 16 columns over scores that are read already
+                        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) top[i & 3] = fmaxf(top[i & 3], fmaxf(pair_x(x[i]), pair_y(x[i])));
+                        return __any_sync(0xffffffffu, unset != 0u || fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > PT_LAZY) != 0;
+                    };
+                    // new references from the scores of chunk c, whose predecessors are done; the chunk's scores are then computed once more (changed in place they
+                    // would be copied on the way that is always taken)
+                    auto raise = [&](pair (&x)[16], int c) {
+                        float alpha[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float up = -INFINITY;                        // how far the row's largest x is above its reference
+#pragma unroll
+                            for (int v = 0; v < 4; ++v) { const pair y = x[(i >> 1) * 8 + v * 2 + (i & 1)]; up = fmaxf(up, fmaxf(pair_x(y), pair_y(y))); }
+                            up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 1));
+                            up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 2));
+                            const bool first = (unset >> i & 1u) && up > -INFINITY;
+                            up = first || (up > PT_LAZY && !(unset >> i & 1u)) ? up : 0.f;
+                            alpha[i] = first ? 1.f : ex2(-up);           // (nothing is accumulated where the reference is the first)
+                            if (first) unset &= ~(1u << i);
+                            nm[i] = add2(nm[i], pair_of(-up, -up));
+                            l[i] = mul2(l[i], pair_of(alpha[i], alpha[i]));
+                        }
+                        const float al = by_lane(alpha);
+                        const __half2 ah = __float2half2_rn(al);
+                        tmem_wait_st();
+#pragma unroll 1
+                        for (int z = 0; z < c; ++z) {                    // P of the tile's chunks before this one
+                            uint32_t o[16];
+                            tmem_ld16(col_s + 16 * z, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = h2_mul(o[i], *reinterpret_cast<const uint32_t*>(&ah));
+                            tmem_st16(col_s + 16 * z, o);
+                        }
+                        if (j > 0) {                                     // behind the products of the tile before
+                            ok = __all_sync(0xffffffffu, mbar_wait(&bars[P::B_O + 4 * t + ((j - 1) & 3)], ((j - 1) >> 2) & 1, abort_flag, 203));
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int z = 0; z < D && ok; z += 16) {
+                                uint32_t o[16];
+                                tmem_ld16(col_o + z, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
+                                tmem_st16(col_o + z, o);
+                            }
+                        }
+                        scores(x, c);
+                    };
+                    // P of a chunk: 16 columns over scores that are read already
+                    auto weights = [&](const pair (&x)[16], int c) {
+                        uint32_t pk[16];
 #pragma unroll
                         for (int v = 0; v < 4; ++v) {
                             const pair vc = *reinterpret_cast<const pair*>(tab + 2 * PT_N + c * 32 + v * 8 + 2 * cq);
@@ -360,12 +366,19 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                         }
                         tmem_st_16x128(col_s + 16 * c, pk);
                         tmem_st_16x128(col_s + 16 * c + (16u << 16), pk + 8);
-                    }
+                    };
+                    pair xa[16], xb[16];
+                    if (scores(xa, 0)) raise(xa, 0);
+                    const bool other = scores(xb, 1);
+                    weights(xa, 0);
+                    if (other) raise(xb, 1);
+                    weights(xb, 1);
                 };
                 if (scaled || key0 + PT_N > all_hi || (key0 < all_lo && key0 + PT_N > a.sinks)) tile(IntC<1>()); else tile(IntC<0>());
+                if (!ok) break;
                 tmem_wait_st();
                 tc_fence_before();
-                warp_arrive(&bar_p[t], lane);
+                warp_arrive(&bars[P::B_P + t * SB + j % SB], lane);
             }
             float row_l, row_m;
             {
@@ -381,7 +394,7 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                 row_m = by_lane(m);
             }
             // ---- O / l, or this split's part
-            if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bar_o[t], 0, abort_flag, 203));
+            if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars[P::B_O + 4 * t + ((n - 1) & 3)], ((n - 1) >> 2) & 1, abort_flag, 203));
             tc_fence_after();
             if (ok) {
                 const float inv = row_l != 0.f ? 1.f / row_l : 0.f;       // (a NaN stays one)
@@ -419,94 +432,83 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                 if (live && splits == 1 && a.lse) a.lse[out_row] = row_l != 0.f ? (row_m + __log2f(row_l)) * 0.6931471805599453f : -INFINITY;
             }
         }
-    } else if (warp < 16) {
+    } else if (warp < P::MMA_WARP) {
         // =============================================================== converters
         set_registers<P::REGS_CONV, P::REGS>();
-        const bool is_k = warp < 12;
-        const int ptid = tid - (is_k ? 256 : 384), it = ptid & 3, kq = ptid >> 2;       // 16-code item of a 64-column block; keys kq, kq + 32, ...
+        const bool is_k = warp < P::V_WARP0;
+        const int ptid = tid & 127, it = ptid & 3, kq = ptid >> 2;       // 16-code item of a 64-column block; keys kq and kq + 32
         const int32_t* pool = is_k ? a.c.kc : a.c.vc;
         const float* scales = is_k ? a.c.ks : a.c.vs;
         unsigned char* stages = smem + (is_k ? P::OFF_K : P::OFF_V);
-        uint64_t *full = is_k ? bar_k : bar_v, *freed = is_k ? bar_kf : bar_vf;
+        uint64_t *full = bars + (is_k ? P::B_K : P::B_V), *freed = bars + (is_k ? P::B_KF : P::B_VF);
         auto loop = [&](auto bits_) {
             constexpr int BITS = decltype(bits_)::value, NW = BITS / 2, WORDS = D * BITS / 32, NB = D / 64;
             CodeMagic<BITS> magic;
             magic.init();
-            uint32_t w[4][NB][NW];
-            int page = 0;                              // of key kq + 32 * it of the next tile
+            uint32_t w[2][NB][NW];                     // behind a sequence's end: words of an earlier tile (any codes are finite; the tables hide them)
+            const int last_key = max(seq.kv - 1, 0);
+            int page = 0;                              // of key kq + 32 * (it & 1) of the next tile
             float sc = 0.f;                            // that key's scale
             const unsigned char* base = reinterpret_cast<const unsigned char*>(pool) + it * (NW * 4);
+            // Every load is unconditional (keys behind the sequence's end read the pools' first row, and the tables hide them): under a condition its result is
+            // moved into place where the condition ends, which waits for it, and a tile's loads come one after the other
             auto fetch_pages = [&](int i) {
-                const int key = tiles.key(tile0 + i) + kq + 32 * it;
-                page = key < seq.kv ? __ldg(table + (key >> a.c.page_shift)) : -1;
+                const int key = tiles.key(tile0 + i) + kq + 32 * (it & 1);
+                page = __ldg(table + (min(key, last_key) >> a.c.page_shift));
             };
-            auto fetch_rows = [&](int i) {             // a lane of four looks up one of their four keys
-                const int key = tiles.key(tile0 + i) + kq + 32 * it;
-                uint32_t own = ~0u;
-                if (key < seq.kv) {
-                    own = (uint32_t)((paged_page(a, page, status) * a.c.H + h) << a.c.page_shift) + (key & page_mask);
-                    sc = __ldg(scales + own);
-                }
+            auto fetch_rows = [&](int i) {             // the lanes of four look up their two keys
+                const int key = tiles.key(tile0 + i) + kq + 32 * (it & 1);
+                const uint32_t own = key < seq.kv ? (uint32_t)((paged_page(a, page, status) * a.c.H + h) << a.c.page_shift) + (key & page_mask) : 0u;
+                sc = __ldg(scales + own);
 #pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    const uint32_t at = __shfl_sync(0xffffffffu, own, p, 4);
-                    if (at != ~0u) {
-                        const unsigned char* src = base + (size_t)at * (WORDS * 4);
+                for (int p = 0; p < 2; ++p) {
+                    const unsigned char* src = base + (size_t)__shfl_sync(0xffffffffu, own, p, 4) * (WORDS * 4);
 #pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) {
-                            if constexpr (NW == 4) {
-                                const uint4 x = __ldg(reinterpret_cast<const uint4*>(src + nb * 64));
-                                w[p][nb][0] = x.x; w[p][nb][1] = x.y; w[p][nb][2] = x.z; w[p][nb][3] = x.w;
-                            } else if constexpr (NW == 2) {
-                                const uint2 x = __ldg(reinterpret_cast<const uint2*>(src + nb * 32));
-                                w[p][nb][0] = x.x; w[p][nb][1] = x.y;
-                            } else w[p][nb][0] = __ldg(reinterpret_cast<const uint32_t*>(src + nb * 16));
-                        }
+                    for (int nb = 0; nb < NB; ++nb) {
+                        if constexpr (NW == 4) {
+                            const uint4 x = __ldg(reinterpret_cast<const uint4*>(src + nb * 64));
+                            w[p][nb][0] = x.x; w[p][nb][1] = x.y; w[p][nb][2] = x.z; w[p][nb][3] = x.w;
+                        } else if constexpr (NW == 2) {
+                            const uint2 x = __ldg(reinterpret_cast<const uint2*>(src + nb * 32));
+                            w[p][nb][0] = x.x; w[p][nb][1] = x.y;
+                        } else w[p][nb][0] = __ldg(reinterpret_cast<const uint32_t*>(src + nb * 16));
                     }
                 }
             };
-            const uint32_t d0 = pt_chunk(kq, 2 * it), d1 = pt_chunk(kq, 2 * it + 1);
-            auto convert = [&](unsigned char* tile) {
+            const uint32_t d0 = pt_chunk<PT_N>(kq, 2 * it), d1 = pt_chunk<PT_N>(kq, 2 * it + 1);
+            if (n_all > 0) { fetch_pages(0); fetch_rows(0); }
+            if (n_all > 1) fetch_pages(1);
+#pragma unroll 1
+            for (int j = 0; j < n_all; ++j) {
+                const int st = j % KST, k = kq + 32 * it;
+                if (j >= KST && !mbar_wait(&freed[st], (j / KST - 1) & 1, abort_flag, is_k ? 204 : 205)) break;
+                float* tab = reinterpret_cast<float*>(smem + P::OFF_TAB) + (j % TS) * P::TAB_FLOATS;
+                if (it < 2) {
+                    float* tab_a = tab + (k >> 1) * 4 + (k & 1);
+                    const bool there = tiles.key(tile0 + j) + k < seq.kv;
+                    if (is_k) tab_a[0] = there ? sc * a.scale_log2 : 0.f;
+                    else {                                  // a scale that is no number spoils the rows that see it, and no other: 0 * its inverse must be 0
+                        const bool fine = sc <= FLT_MAX;
+                        tab_a[2] = there ? (fine ? __log2f(sc) : sc - sc) : -INFINITY;
+                        tab[2 * PT_N + k] = there && fine ? __fdividef(1.f, sc) : there ? 1.f : 0.f;
+                    }
+                }
+                unsigned char* tile = stages + st * P::T_BYTES;
 #pragma unroll
-                for (int p = 0; p < 4; ++p)
+                for (int p = 0; p < 2; ++p)
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
                         uint32_t hw[8];
                         Item<BITS>::raw(w[p][nb], hw, magic);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) hw[i] = Item<BITS>::minus_zp(hw[i], i, pt_neg_base<BITS>(i % Item<BITS>::CLS));
-                        sts128(tile + d0 + nb * (128 * 128) + p * (32 * 128), hw[0], hw[1], hw[2], hw[3]);
-                        sts128(tile + d1 + nb * (128 * 128) + p * (32 * 128), hw[4], hw[5], hw[6], hw[7]);
+                        sts128(tile + d0 + nb * (PT_N * 128) + p * (32 * 128), hw[0], hw[1], hw[2], hw[3]);
+                        sts128(tile + d1 + nb * (PT_N * 128) + p * (32 * 128), hw[4], hw[5], hw[6], hw[7]);
                     }
-            };
-            // keys behind the sequence's end keep the words of an earlier tile (any codes are finite); their table entries hide them
-#pragma unroll
-            for (int p = 0; p < 4; ++p)
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                    for (int z = 0; z < NW; ++z) w[p][nb][z] = 0u;
-            if (n_all > 0) { fetch_pages(0); fetch_rows(0); }
-            if (n_all > 1) fetch_pages(1);
-#pragma unroll 1
-            for (int j = 0; j < n_all; ++j) {
-                const int st = j % 2, k = kq + 32 * it;
-                if (j >= 2 && !mbar_wait(&freed[st], ((j >> 1) - 1) & 1, abort_flag, is_k ? 204 : 205)) break;
-                unsigned char* tile = stages + st * P::T_BYTES;
-                float* tab = reinterpret_cast<float*>(smem + P::OFF_TAB) + (j % TS) * P::TAB_FLOATS;
-                float* tab_a = tab + (k >> 1) * 4 + (k & 1);
-                const bool there = tiles.key(tile0 + j) + k < seq.kv;
-                if (is_k) tab_a[0] = there ? sc * a.scale_log2 : 0.f;
-                else {                                      // a scale that is no number spoils the rows that see it, and no other: 0 * its inverse must be 0
-                    const bool fine = sc <= FLT_MAX;
-                    tab_a[2] = there ? (fine ? __log2f(sc) : sc - sc) : -INFINITY;
-                    tab[2 * PT_N + k] = there && fine ? __fdividef(1.f, sc) : there ? 1.f : 0.f;
-                }
-                convert(tile);
                 fence_async_smem();
-                warp_arrive(&full[st], lane);
-                warp_arrive(&bar_tab[j % TS], lane);
-                if (j + 1 < n_all) fetch_rows(j + 1);
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(&full[st]); mbar_arrive(&bars[P::B_TAB + j % TS]); }
+                if (j + 1 < n_all) fetch_rows(j + 1);           // behind the fence, which waits for loads on their way
                 if (j + 2 < n_all) fetch_pages(j + 2);
             }
         };
@@ -514,57 +516,52 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
         if (bits == 8) loop(IntC<8>()); else if (bits == 4) loop(IntC<4>()); else loop(IntC<2>());
     } else {
         set_registers<P::REGS_MISC, P::REGS>();
-        if (warp == 16) {
-            // =============================================================== products (the whole warp waits; one elected lane issues)
+        if (warp < P::MMA_WARP + 2) {
+            // =============================================================== products of query tile t (the whole warp waits; one elected lane issues)
+            // S(0) .. S(SB - 1), then for every key tile j: P(j) -> O += P(j) V(j) -> S(j + SB) over the columns of P(j)
             constexpr uint32_t IDESC_S = instr_desc(PT_M, PT_N, 0), IDESC_O = instr_desc(PT_M, D, 1);
-            const uint64_t qd = smem_desc(smem_u32(smem + P::OFF_Q), 16, 1024), kd = smem_desc(smem_u32(smem + P::OFF_K), 16, 1024);
+            const int t = warp - P::MMA_WARP, n = n_t[t];
+            const uint64_t qd = smem_desc(smem_u32(smem + P::OFF_Q + t * P::Q_BYTES), 16, 1024), kd = smem_desc(smem_u32(smem + P::OFF_K), 16, 1024);
             const uint64_t vd = smem_desc(smem_u32(smem + P::OFF_V), PT_N * 128, 1024);
+            const uint32_t col_s = tmem_base + P::COL_S + t * (SB * PT_N), col_o = tmem_base + P::COL_O + t * D;
             bool ok = true;
-            auto issue_s = [&](int t, int j) {
-                const uint64_t ad = qd + (uint64_t)((t * P::Q_BYTES) >> 4), bd = kd + (uint64_t)(((j % KST) * P::T_BYTES) >> 4);
+            auto issue_s = [&](int j) {
+                if (!(ok = mbar_wait_warp(&bars[P::B_K + j % KST], (j / KST) & 1, abort_flag, 207))) return;
+                tc_fence_after();
+                if (j < n) {
+                    const uint64_t bd = kd + (uint64_t)(((j % KST) * P::T_BYTES) >> 4);
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint64_t step = (uint64_t)(((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4);
-                    tc_mma_ss(tmem_base + P::COL_S + t * PT_N, ad + step, bd + step, IDESC_S, kk ? 1u : 0u);
+                    for (int kk = 0; kk < D / 16; ++kk)
+                        tc_mma_ss(col_s + (j % SB) * PT_N, qd + (uint64_t)(((kk >> 2) * (PT_M * 128) + (kk & 3) * 32) >> 4),
+                                  bd + (uint64_t)(((kk >> 2) * (PT_N * 128) + (kk & 3) * 32) >> 4), IDESC_S, kk ? 1u : 0u);
+                    tc_commit(&bars[P::B_S + t * SB + j % SB]);
                 }
-                tc_commit(&bar_s[t]);
+                tc_commit(&bars[P::B_KF + j % KST]);
             };
-            auto issue_o = [&](int t, int j) {
-                const uint64_t bd = vd + (uint64_t)(((j % VST) * P::T_BYTES) >> 4);
-#pragma unroll
-                for (int kk = 0; kk < PT_N / 16; ++kk)
-                    tc_mma_ts(tmem_base + P::COL_O + t * D, tmem_base + P::COL_S + t * PT_N + kk * 8, bd + (uint64_t)((kk * 2048) >> 4), IDESC_O, j || kk ? 1u : 0u);
-            };
-            for (int t = 0; t < 2 && ok; ++t)
-                if (n_t[t] > 0) {
-                    ok = mbar_wait_warp(&bar_q[t], 0, abort_flag, 206) && mbar_wait_warp(&bar_k[0], 0, abort_flag, 207);
-                    tc_fence_after();
-                    if (ok) issue_s(t, 0);
-                }
-            if (ok && n_all > 0) tc_commit(&bar_kf[0]);
+            if (n > 0) ok = mbar_wait_warp(&bars[P::B_Q + t], 0, abort_flag, 206);
+            for (int j = 0; j < SB && j < n_all && ok; ++j) issue_s(j);
 #pragma unroll 1
             for (int j = 0; j < n_all && ok; ++j) {
-                if (!(ok = mbar_wait_warp(&bar_v[j % VST], (j / VST) & 1, abort_flag, 208))) break;
-                if (j + 1 < n_all && !(ok = mbar_wait_warp(&bar_k[(j + 1) % KST], ((j + 1) / KST) & 1, abort_flag, 209))) break;
-#pragma unroll 1
-                for (int t = 0; t < 2; ++t) {
-                    if (j >= n_t[t]) continue;
-                    if (!(ok = mbar_wait_warp(&bar_p[t], j & 1, abort_flag, 210))) break;
+                if (!(ok = mbar_wait_warp(&bars[P::B_V + j % VST], (j / VST) & 1, abort_flag, 208))) break;
+                if (j < n) {
+                    if (!(ok = mbar_wait_warp(&bars[P::B_P + t * SB + j % SB], (j / SB) & 1, abort_flag, 210))) break;
                     tc_fence_after();
-                    issue_o(t, j);
-                    if (j + 1 < n_t[t]) issue_s(t, j + 1);
-                    else tc_commit(&bar_o[t]);
+                    const uint64_t bd = vd + (uint64_t)(((j % VST) * P::T_BYTES) >> 4);
+#pragma unroll
+                    for (int kk = 0; kk < PT_N / 16; ++kk)
+                        tc_mma_ts(col_o, col_s + (j % SB) * PT_N + kk * 8, bd + (uint64_t)((kk * 2048) >> 4), IDESC_O, j || kk ? 1u : 0u);
+                    tc_commit(&bars[P::B_O + 4 * t + (j & 3)]);
                 }
-                tc_commit(&bar_vf[j % VST]);
-                if (j + 1 < n_all) tc_commit(&bar_kf[(j + 1) % KST]);
+                tc_commit(&bars[P::B_VF + j % VST]);
+                if (j + SB < n_all) issue_s(j + SB);
             }
             // nothing of this CTA may be in flight when its memory goes
-            tc_commit(bar_end);
-            for (uint32_t i = 0; i < TC_SPIN_LIMIT && !__all_sync(0xffffffffu, mbar_try(bar_end, 0)); ++i) {}
+            tc_commit(&bars[P::B_END + t]);
+            for (uint32_t i = 0; i < TC_SPIN_LIMIT && !__all_sync(0xffffffffu, mbar_try(&bars[P::B_END + t], 0)); ++i) {}
         }
     }
     __syncthreads();
-    if (warp == 16) {
+    if (warp == P::MMA_WARP) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)P::TMEM_COLS) : "memory");
     }

@@ -1,19 +1,32 @@
 // Attention of a chunk over a paged cache on the 5th-generation tensor cores (tcgen05 + TMEM).
 //
 // One CTA = one (sequence, head of the cache) x 256 query rows, two tiles of 128; a row is a (token, query head of the group) pair, so query
-// heads that share a head of the cache share its converted tiles.  It walks over tiles of 128 keys; a tile of first tokens (sinks) and the window
+// heads that share a head of the cache share its converted tiles.  It walks over tiles of 64 keys; those of first tokens (sinks) and those of the window
 // are lists of tiles one behind the other.  Per key tile and query tile
 //   S = Q K^T       Q fp16 in shared memory, K integer codes as exact fp16; S fp32 in tensor memory
 //   x = S a_j + b_j with a_j = K scale * softmax_scale * log2 e and b_j = log2 of the V scale
 //   P = 2^(x - m)   fp16, written over S in tensor memory, = weight * V scale relative to the row's reference m
 //   l += P / V scale in fp32, from the unrounded P;      O += P V, V integer codes as exact fp16, O fp32 in tensor memory
-// and at the end out = O / l, log-sum-exp = (m + log2 l) ln 2.  The reference m is that of weight times V scale, which is what bounds O.  It is raised only when an x
-// passes it by more than 8: the tile is then computed again against the new one, O and l rescaled.  fp16 queries are exact, and so are bf16
-// queries of usual size; a row whose largest element lies outside [2^-4, 2^15) is scaled by a power of two (then S a_j takes a factor).
-// Warps: 0-3 and 4-7 softmax of the two query tiles, a thread per row; 8-11 and 12-15 convert K and V: packed rows come straight from the pages
-// into registers, a tile ahead, and go to 128B-swizzled fp16 tiles in shared memory, scales to the tables a, b, 1 / V scale; warp 16 issues the products.
-// While one query tile is in its softmax the tensor pipe works for the other.
+// and at the end out = O / l, log-sum-exp = (m + log2 l) ln 2.  P is the operand of a 16-bit product: its rounding (2^-11 relative, of each weight by itself) is
+// the only one to fewer than 32 bits; the codes are exact in fp16.  The reference m is that of weight times V scale, which is what bounds O.  It is raised only
+// when an x passes it by more than 8 (P then stays below 2^8, far from fp16's end): the tile's scores are then taken again against the new one, O and l
+// rescaled.  fp16 queries are exact, and so are bf16 queries of usual size; a row whose largest element lies outside [2^-4, 2^15) is scaled by a power of two
+// (then S a_j takes a factor).
+//
+// Warps: 0-3 and 4-7 softmax of the two query tiles; 8-11 and 12-15 convert K and V: packed rows from shared memory to 128B-swizzled fp16 tiles, scales to the
+// tables a, b, 1 / V scale; 16 and 17 issue the products of the two query tiles; 18 and 19 fetch packed rows and scales of K and V with a bulk copy for every
+// run of keys in one page, RST tiles ahead.  Two or three score tiles per query tile (what tensor memory holds beside O) are in flight, so that a softmax warp
+// finds the next scores there while the tensor pipe works on its weights.
 // Every wait is bounded: on expiry the kernel records a status code and all roles drain out.
+//
+// What bounds it (B200, 1965 MHz): the softmax warps.  At 128 columns and 8-bit codes a tile of 64 keys takes ~2470 cycles of a CTA, of which the exponentials
+// alone are 1024 (8 cycles a warp instruction on each of the four schedulers), the products 2 x 512.  Measured:
+//   2048 queries behind 16384 keys, 32 query / 8 cache heads, 128 columns, 8 bits   740 us   790 TFLOP/s (floor at the measured dense rate 359)
+//   16 sequences, 1024 queries on 2240 keys each, 30 heads, 64 columns, 4 bits       638 us   442 TFLOP/s (half the columns: the same exponentials feed half the products)
+//   4096 queries, window 2048, 128 columns                                          120 us   578 TFLOP/s
+// Tiles tried: 128 keys with one score tile each 784 / 721 / 137 us (the softmax waits for its scores); 64 keys, packed rows straight from the pages into the
+// converters' registers 770 / 680 / 125 us (a converter waits out its loads at the proxy fence, which lets no load pass); bulk copies 740 / 638 / 120 us.
+// Register shares 152 / 64 (softmax / converters) 768 / 638, 144 / 72 740 / 638, 160 / 56 756 / 638 us.
 #include "varq_attn_tc.cuh"
 #include "varq_paged.cuh"
 
@@ -25,20 +38,23 @@ constexpr float PT_LAZY = 8.f;
 
 template <int D> struct PtPlan {
     static constexpr int SB = D == 64 ? 3 : 2;                     // score tiles per query tile
-    static constexpr int KST = 4, VST = 4, TS = 8;                 // stages of K and V; tables: a table is read until its P is written, SB tiles behind its K
-    static constexpr int Q_BYTES = PT_M * D * 2, T_BYTES = PT_N * D * 2;
+    static constexpr int KST = D == 64 ? 4 : 3, VST = KST;         // stages of K and V as fp16
+    static constexpr int RST = D == 64 ? 6 : 3;                    // stages of K and V as they lie in the pages
+    static constexpr int TS = KST + SB;                            // tables: a table is read until its P is written, SB tiles behind its K
+    static constexpr int Q_BYTES = PT_M * D * 2, T_BYTES = PT_N * D * 2, R_BYTES = PT_N * D, RAW_BYTES = R_BYTES + PT_N * 4;     // packed rows, then scales
     static constexpr int TAB_FLOATS = 3 * PT_N;
-    static constexpr int OFF_Q = 0, OFF_K = OFF_Q + 2 * Q_BYTES, OFF_V = OFF_K + KST * T_BYTES, OFF_TAB = OFF_V + VST * T_BYTES;
-    // barriers: K, V written and free; tables written; queries; S, P of every score tile; O (a ring of four tiles); end
-    static constexpr int B_K = 0, B_KF = B_K + KST, B_V = B_KF + KST, B_VF = B_V + VST, B_TAB = B_VF + VST, B_Q = B_TAB + TS, B_S = B_Q + 2, B_P = B_S + 2 * SB,
-                         B_O = B_P + 2 * SB, B_END = B_O + 8, N_BARS = B_END + 2;
+    static constexpr int OFF_Q = 0, OFF_K = OFF_Q + 2 * Q_BYTES, OFF_V = OFF_K + KST * T_BYTES, OFF_RK = OFF_V + VST * T_BYTES, OFF_RV = OFF_RK + RST * RAW_BYTES,
+                         OFF_TAB = OFF_RV + RST * RAW_BYTES;
+    // barriers: K, V written and free; packed K, V there and free; tables written; queries; S, P of every score tile; O (a ring of four tiles); end
+    static constexpr int B_K = 0, B_KF = B_K + KST, B_V = B_KF + KST, B_VF = B_V + VST, B_RK = B_VF + VST, B_RKF = B_RK + RST, B_RV = B_RKF + RST, B_RVF = B_RV + RST,
+                         B_TAB = B_RVF + RST, B_Q = B_TAB + TS, B_S = B_Q + 2, B_P = B_S + 2 * SB, B_O = B_P + 2 * SB, B_END = B_O + 8, N_BARS = B_END + 2;
     static constexpr int OFF_BAR = OFF_TAB + TS * TAB_FLOATS * 4;
     static constexpr int OFF_QF = (OFF_BAR + N_BARS * 8 + 15) / 16 * 16;              // factors of the queries [2][128]
-    static constexpr int OFF_XCH = OFF_QF + 2 * PT_M * 4, OFF_MISC = OFF_XCH + 2 * 2 * PT_M * 4, SMEM = OFF_MISC + 16 + 1024;      // a value per row and column half
+    static constexpr int OFF_MISC = OFF_QF + 2 * PT_M * 4, SMEM = OFF_MISC + 16 + 1024;
     static constexpr int COL_O = 0, COL_S = 2 * D, TMEM_COLS = 512;
-    static_assert(COL_S + 2 * SB * PT_N <= TMEM_COLS && SMEM <= 227 * 1024 && TS >= KST + SB, "plan");
-    static constexpr int SOFT = 8, K_WARP0 = SOFT, V_WARP0 = K_WARP0 + 4, MMA_WARP = V_WARP0 + 4, THREADS = (MMA_WARP + 4) * 32;
-    static constexpr int REGS = 96, REGS_SOFT = 152, REGS_CONV = 64, REGS_MISC = 48;
+    static_assert(COL_S + 2 * SB * PT_N <= TMEM_COLS && SMEM <= 227 * 1024 && OFF_RK % 128 == 0, "plan");
+    static constexpr int SOFT = 8, K_WARP0 = SOFT, V_WARP0 = K_WARP0 + 4, MMA_WARP = V_WARP0 + 4, LOAD_WARP = MMA_WARP + 2, THREADS = (LOAD_WARP + 2) * 32;
+    static constexpr int REGS = 96, REGS_SOFT = 144, REGS_CONV = 72, REGS_MISC = 48;
     static_assert(SOFT * 32 * REGS_SOFT + 256 * REGS_CONV + 128 * REGS_MISC <= THREADS * REGS, "register plan");
 };
 
@@ -58,8 +74,8 @@ __device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint
 // pairs of fp32 in one 64-bit register
 using pair = unsigned long long;
 __device__ __forceinline__ pair pair_of(float x, float y) { pair d; asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y)); return d; }
-__device__ __forceinline__ float pair_x(pair p) { float x, y; asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); return x; }
-__device__ __forceinline__ float pair_y(pair p) { float x, y; asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); return y; }
+__device__ __forceinline__ float pair_x(pair p) { float x; [[maybe_unused]] float y; asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); return x; }
+__device__ __forceinline__ float pair_y(pair p) { [[maybe_unused]] float x; float y; asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); return y; }
 __device__ __forceinline__ pair fma2(pair a, pair b, pair c) { pair d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c)); return d; }
 __device__ __forceinline__ pair add2(pair a, pair b) { pair d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
 __device__ __forceinline__ pair mul2(pair a, pair b) { pair d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
@@ -138,10 +154,12 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + P::OFF_MISC + 8);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
-    if (warp == P::MMA_WARP + 2) {
+    if (warp == P::LOAD_WARP) {
         for (int i = lane; i < P::N_BARS; i += 32) {        // warps that arrive
-            const bool by_8 = i >= P::B_TAB && i < P::B_Q, by_4 = i < P::B_KF || (i >= P::B_V && i < P::B_VF) || (i >= P::B_Q && i < P::B_S) || (i >= P::B_P && i < P::B_O);
-            const bool by_2 = (i >= P::B_KF && i < P::B_V) || (i >= P::B_VF && i < P::B_TAB);
+            auto in = [&](int lo, int hi) { return i >= lo && i < hi; };
+            const bool by_8 = in(P::B_TAB, P::B_Q);
+            const bool by_4 = in(P::B_K, P::B_KF) || in(P::B_V, P::B_VF) || in(P::B_RKF, P::B_RV) || in(P::B_RVF, P::B_TAB) || in(P::B_Q, P::B_S) || in(P::B_P, P::B_O);
+            const bool by_2 = in(P::B_KF, P::B_V) || in(P::B_VF, P::B_RK);
             mbar_init(&bars[i], by_8 ? 8u : by_4 ? 4u : by_2 ? 2u : 1u);
         }
         if (lane == 0) *abort_flag = 0;
@@ -254,10 +272,14 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
 #pragma unroll 1
             for (int j = 0; j < n; ++j) {
                 const int key0 = tiles.key(tile0 + j);
-                ok = mbar_wait(&bars[P::B_TAB + j % TS], (j / TS) & 1, abort_flag, 201) && mbar_wait(&bars[P::B_S + t * SB + j % SB], (j / SB) & 1, abort_flag, 202);
+                {
+                    uint64_t *tab_bar = &bars[P::B_TAB + j % TS], *s_bar = &bars[P::B_S + t * SB + j % SB];
+                    const bool there = mbar_test(tab_bar, (j / TS) & 1) & mbar_test(s_bar, (j / SB) & 1);        // both at once: that is a round trip less
+                    if (!__all_sync(0xffffffffu, there))
+                        ok = mbar_wait_warp(tab_bar, (j / TS) & 1, abort_flag, 201) && mbar_wait_warp(s_bar, (j / SB) & 1, abort_flag, 202);
+                    if (!ok) break;
+                }
                 const uint32_t col_s = col_s0 + (j % SB) * PT_N;
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
                 tc_fence_after();
                 const float* tab = reinterpret_cast<const float*>(smem + P::OFF_TAB) + (j % TS) * P::TAB_FLOATS;
                 // Two forms of a tile, so that the usual one carries neither masks nor factors: as branches inside they cost 10 % of a long call.  The scores of a
@@ -437,52 +459,41 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
         set_registers<P::REGS_CONV, P::REGS>();
         const bool is_k = warp < P::V_WARP0;
         const int ptid = tid & 127, it = ptid & 3, kq = ptid >> 2;       // 16-code item of a 64-column block; keys kq and kq + 32
-        const int32_t* pool = is_k ? a.c.kc : a.c.vc;
-        const float* scales = is_k ? a.c.ks : a.c.vs;
         unsigned char* stages = smem + (is_k ? P::OFF_K : P::OFF_V);
+        const unsigned char* raw_stages = smem + (is_k ? P::OFF_RK : P::OFF_RV);
         uint64_t *full = bars + (is_k ? P::B_K : P::B_V), *freed = bars + (is_k ? P::B_KF : P::B_VF);
+        uint64_t *raw_full = bars + (is_k ? P::B_RK : P::B_RV), *raw_freed = bars + (is_k ? P::B_RKF : P::B_RVF);
         auto loop = [&](auto bits_) {
-            constexpr int BITS = decltype(bits_)::value, NW = BITS / 2, WORDS = D * BITS / 32, NB = D / 64;
+            constexpr int BITS = decltype(bits_)::value, NW = BITS / 2, ROW = D * BITS / 8, NB = D / 64;
             CodeMagic<BITS> magic;
             magic.init();
-            uint32_t w[2][NB][NW];                     // behind a sequence's end: words of an earlier tile (any codes are finite; the tables hide them)
-            const int last_key = max(seq.kv - 1, 0);
-            int page = 0;                              // of key kq + 32 * (it & 1) of the next tile
-            float sc = 0.f;                            // that key's scale
-            const unsigned char* base = reinterpret_cast<const unsigned char*>(pool) + it * (NW * 4);
-            // Every load is unconditional (keys behind the sequence's end read the pools' first row, and the tables hide them): under a condition its result is
-            // moved into place where the condition ends, which waits for it, and a tile's loads come one after the other
-            auto fetch_pages = [&](int i) {
-                const int key = tiles.key(tile0 + i) + kq + 32 * (it & 1);
-                page = __ldg(table + (min(key, last_key) >> a.c.page_shift));
-            };
-            auto fetch_rows = [&](int i) {             // the lanes of four look up their two keys
-                const int key = tiles.key(tile0 + i) + kq + 32 * (it & 1);
-                const uint32_t own = key < seq.kv ? (uint32_t)((paged_page(a, page, status) * a.c.H + h) << a.c.page_shift) + (key & page_mask) : 0u;
-                sc = __ldg(scales + own);
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const unsigned char* src = base + (size_t)__shfl_sync(0xffffffffu, own, p, 4) * (WORDS * 4);
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) {
-                        if constexpr (NW == 4) {
-                            const uint4 x = __ldg(reinterpret_cast<const uint4*>(src + nb * 64));
-                            w[p][nb][0] = x.x; w[p][nb][1] = x.y; w[p][nb][2] = x.z; w[p][nb][3] = x.w;
-                        } else if constexpr (NW == 2) {
-                            const uint2 x = __ldg(reinterpret_cast<const uint2*>(src + nb * 32));
-                            w[p][nb][0] = x.x; w[p][nb][1] = x.y;
-                        } else w[p][nb][0] = __ldg(reinterpret_cast<const uint32_t*>(src + nb * 16));
-                    }
-                }
-            };
+            // Rows of two 64-column blocks: every other group of rows begins with the second, so that the rows that are read together lie in all banks
+            const int nb0 = NB == 2 ? kq >> (BITS == 8 ? 0 : BITS == 4 ? 1 : 2) & 1 : 0;
             const uint32_t d0 = pt_chunk<PT_N>(kq, 2 * it), d1 = pt_chunk<PT_N>(kq, 2 * it + 1);
-            if (n_all > 0) { fetch_pages(0); fetch_rows(0); }
-            if (n_all > 1) fetch_pages(1);
+            int st = 0, rst = 0, ts = 0;
+            uint32_t st_ph = 1, rst_ph = 0;
 #pragma unroll 1
             for (int j = 0; j < n_all; ++j) {
-                const int st = j % KST, k = kq + 32 * it;
-                if (j >= KST && !mbar_wait(&freed[st], (j / KST - 1) & 1, abort_flag, is_k ? 204 : 205)) break;
-                float* tab = reinterpret_cast<float*>(smem + P::OFF_TAB) + (j % TS) * P::TAB_FLOATS;
+                const int k = kq + 32 * it;
+                if (!mbar_wait_warp(&raw_full[rst], rst_ph, abort_flag, is_k ? 211 : 212)) break;
+                const unsigned char* raw = raw_stages + rst * P::RAW_BYTES;
+                uint32_t w[2][NB][NW];                 // rows behind a sequence's end: whatever lay there (any codes are finite; the tables hide them)
+#pragma unroll
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        const unsigned char* src = raw + (kq + 32 * p) * ROW + (nb ^ nb0) * (8 * BITS) + it * (NW * 4);
+                        if constexpr (NW == 4) {
+                            const uint4 x = *reinterpret_cast<const uint4*>(src);
+                            w[p][nb][0] = x.x; w[p][nb][1] = x.y; w[p][nb][2] = x.z; w[p][nb][3] = x.w;
+                        } else if constexpr (NW == 2) {
+                            const uint2 x = *reinterpret_cast<const uint2*>(src);
+                            w[p][nb][0] = x.x; w[p][nb][1] = x.y;
+                        } else w[p][nb][0] = *reinterpret_cast<const uint32_t*>(src);
+                    }
+                const float sc = reinterpret_cast<const float*>(raw + P::R_BYTES)[k & (PT_N - 1)];
+                if (j >= KST && !mbar_wait_warp(&freed[st], st_ph, abort_flag, is_k ? 204 : 205)) break;
+                float* tab = reinterpret_cast<float*>(smem + P::OFF_TAB) + ts * P::TAB_FLOATS;
                 if (it < 2) {
                     float* tab_a = tab + (k >> 1) * 4 + (k & 1);
                     const bool there = tiles.key(tile0 + j) + k < seq.kv;
@@ -502,14 +513,16 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                         Item<BITS>::raw(w[p][nb], hw, magic);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) hw[i] = Item<BITS>::minus_zp(hw[i], i, pt_neg_base<BITS>(i % Item<BITS>::CLS));
-                        sts128(tile + d0 + nb * (PT_N * 128) + p * (32 * 128), hw[0], hw[1], hw[2], hw[3]);
-                        sts128(tile + d1 + nb * (PT_N * 128) + p * (32 * 128), hw[4], hw[5], hw[6], hw[7]);
+                        unsigned char* block = tile + (nb ^ nb0) * (PT_N * 128) + p * (32 * 128);
+                        sts128(block + d0, hw[0], hw[1], hw[2], hw[3]);
+                        sts128(block + d1, hw[4], hw[5], hw[6], hw[7]);
                     }
                 fence_async_smem();
                 __syncwarp();
-                if (lane == 0) { mbar_arrive(&full[st]); mbar_arrive(&bars[P::B_TAB + j % TS]); }
-                if (j + 1 < n_all) fetch_rows(j + 1);           // behind the fence, which waits for loads on their way
-                if (j + 2 < n_all) fetch_pages(j + 2);
+                if (lane == 0) { mbar_arrive(&full[st]); mbar_arrive(&bars[P::B_TAB + ts]); mbar_arrive(&raw_freed[rst]); }
+                if (++st == KST) { st = 0; st_ph ^= 1u; }
+                if (++rst == P::RST) { rst = 0; rst_ph ^= 1u; }
+                if (++ts == TS) ts = 0;
             }
         };
         const int bits = is_k ? a.c.kb : a.c.vb;
@@ -558,6 +571,36 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
             // nothing of this CTA may be in flight when its memory goes
             tc_commit(&bars[P::B_END + t]);
             for (uint32_t i = 0; i < TC_SPIN_LIMIT && !__all_sync(0xffffffffu, mbar_try(&bars[P::B_END + t], 0)); ++i) {}
+        } else {
+            // =============================================================== packed rows and scales of K (V): a bulk copy for every run of keys in one page
+            const bool is_k = warp == P::LOAD_WARP;
+            const int bits = is_k ? a.c.kb : a.c.vb, row = D / 8 * bits, run = min(PT_N, page_mask + 1), last_key = max(seq.kv - 1, 0);
+            const unsigned char* pool = reinterpret_cast<const unsigned char*>(is_k ? a.c.kc : a.c.vc);
+            const float* scales = is_k ? a.c.ks : a.c.vs;
+            unsigned char* raw_stages = smem + (is_k ? P::OFF_RK : P::OFF_RV);
+            uint64_t *raw_full = bars + (is_k ? P::B_RK : P::B_RV), *raw_freed = bars + (is_k ? P::B_RKF : P::B_RVF);
+            auto page_of = [&](int i) { return __ldg(table + (min(tiles.key(tile0 + min(i, n_all - 1)) + lane * run, last_key) >> a.c.page_shift)); };
+            int page = n_all > 0 ? page_of(0) : 0, j = 0;
+#pragma unroll 1
+            for (; j < n_all; ++j) {
+                const int st = j % P::RST, key = tiles.key(tile0 + j) + lane * run;
+                const int next = page_of(j + 1);
+                if (j >= P::RST && !mbar_wait_warp(&raw_freed[st], (j / P::RST - 1) & 1, abort_flag, is_k ? 213 : 214)) break;
+                const bool there = lane * run < PT_N && key < seq.kv;
+                const int runs = __popc(__ballot_sync(0xffffffffu, there));
+                if (lane == 0) mbar_expect_tx(&raw_full[st], (uint32_t)(runs * run * (row + 4)));
+                __syncwarp();
+                if (there) {
+                    const uint32_t own = (uint32_t)((paged_page(a, page, status) * a.c.H + h) << a.c.page_shift) + (key & page_mask);
+                    unsigned char* raw = raw_stages + st * P::RAW_BYTES;
+                    bulk_copy_g2s(raw + lane * run * row, pool + (size_t)own * row, (uint32_t)(run * row), &raw_full[st]);
+                    bulk_copy_g2s(raw + P::R_BYTES + lane * run * 4, scales + own, (uint32_t)(run * 4), &raw_full[st]);
+                }
+                page = next;
+            }
+            // no copy of this CTA may be in flight when its memory goes
+            for (int i = max(j - P::RST, 0); i < j; ++i)
+                for (uint32_t n = 0; n < TC_SPIN_LIMIT && !__all_sync(0xffffffffu, mbar_try(&raw_full[i % P::RST], (i / P::RST) & 1)); ++n) {}
         }
     }
     __syncthreads();

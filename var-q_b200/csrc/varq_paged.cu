@@ -9,6 +9,12 @@
 // A row with a NaN or an infinity has a NaN scale and zero codes: whoever reads it gets NaN, as from arithmetic on the values themselves, and whoever does
 // not see it loses nothing.
 // Read: code * scale, converted to the output's type once.
+//
+// What bounds them (B200): a read its bytes, 32768 tokens of 8 heads x 128 from 8-bit codes to 16-bit values 37 us = 5.5 TB/s (the copy rate is 6.5); an append
+// of the same size the issue of its instructions, 48 us.  Both together: 135 us with eight values a lane and a division and its rounding for each, 93 with sixteen
+// and the bracket, 85 with Markstein's scale and narrow codes merged by the byte (their bytes alone take 52).  On random values at most one lane in five hundred
+// finds its bracket open and divides (16 values, each within 127 * 2^-20 of a tie).  Short calls are a launch's latency: 8 or 999 tokens, written and read
+// back, 7.9 us for both launches.
 #include "varq_attn.cuh"
 #include "varq_codes.cuh"
 #include "varq_paged.cuh"
@@ -275,7 +281,9 @@ int check_rows(const char* who, const PagedView& c, long long n) {
     return VARQ_OK;
 }
 
-// Rows per thread: several keep enough bytes in flight for a long call, one spreads a short call over the SMs
+// Rows per thread: two keep more bytes in flight once the call fills every SM four times over, one spreads a shorter call over the SMs.
+// One / two / four rows, 32768 tokens of 8 heads x 128, 8 bits: append of 16-bit values 56.4 / 50.1 / 59.6 us, of fp32 (half the tokens) 32.0 / 33.5 / 48; read
+// 41.5 / 37.0 / 42.7 us.
 template <int U, typename A, typename K1, typename KU>
 int launch_rows(K1 one, KU several, const A& a, int D, cudaStream_t st) {
     const uint32_t rpb = ROW_THREADS / (D / 16);
@@ -373,7 +381,19 @@ extern "C" int varq_paged_read(const varq_paged_t* cache, const int64_t* slots, 
 
 namespace {
 
-// How a call is shared out
+// How a call is shared out.
+//
+// Kernel: few query rows per head of the cache leave most of the chunk kernel's 256 idle, while the decode kernel reads the keys once for every 16.  They cross
+// where the decode kernel needs a third row tile at head_dim 128, and a sixth at 64 (chunk kernel / decode kernel, us):
+//   128: 24 rows, 64 sequences of 8000 keys 542 / 391; 32 rows, 8 of 1000 24.1 / 20.4; 40 rows, 64 of 8000 542 / 560; 64 rows, 8 of 1000 24.4 / 30.1
+//    64: 40 rows, 32 of 2000 136 / 102; 64 rows 141 / 132; 100 rows, 4 of 300 13.8 / 13.4 (which a larger call would turn round)
+// Parts of the key range: more of them fill the SMs, and each costs a CTA its set-up and, through the workspace, a store and a second launch.  The model below
+// (in tiles; fixed and merge are fits) picked the best or within 2 % of the best of 1 .. 24 parts on 10 of 11 calls that were measured, e.g. 256 queries
+// behind 8192 keys, 8 heads: 1 / 2 / 4 / 8 parts 186 / 117 / 72 / 88 us, picks 4; 2048 behind 16384 740 / 807 / 807 / 943, picks 1.  The one it misses are
+// chunks of 17 to 512 queries behind 0 to 4000 keys, 1 / 2 parts 91 / 77 us, picks 1: only the longest length is known here, and there it is the critical path.
+// Cluster or workspace: parts of the decode kernel that are resident all at once, up to eight of a row tile, meet in a cluster; without a second launch one
+// sequence of 1000 keys takes 8.0 us, with it 12.9.  Where they are not resident, clusters wait for room together: 64 sequences of 8000 keys, 16 heads 284 us
+// in clusters, 259 through the workspace.
 struct AttnPlan {
     bool tc, cluster;                  // kernel; its parts meet in clusters, not in the workspace
     int splits, tiles_per_split;       // tiles of 16 keys (decode kernel)
@@ -383,7 +403,7 @@ AttnPlan plan_attn(const varq_paged_t* c, const varq_paged_batch_t* b) {
     const int max_q = (int)(b->max_q < b->n_queries ? b->max_q : b->n_queries), D = c->head_dim;
     const long long rows = (long long)max_q * (b->q_heads / c->n_heads);
     const long long seen = (long long)b->window + max_q + b->sinks, span = b->window && seen < b->max_kv ? seen : b->max_kv;      // keys of a CTA, about
-    p.tc = forced_attn_path() == VARQ_ATTN_PATH_TC || (forced_attn_path() != VARQ_ATTN_PATH_DECODE && rows > (D == 64 ? 80 : 48));
+    p.tc = forced_attn_path() == VARQ_ATTN_PATH_TC || (forced_attn_path() != VARQ_ATTN_PATH_DECODE && rows > (D == 64 ? 80 : 32));
     const long long unit = p.tc ? 128 : 16, tiles = span > unit ? (span + unit - 1) / unit : 1;
     const int resident = p.tc ? 1 : rows > 8 ? (D == 128 ? 3 : 4) : D == 64 ? 5 : c->k_bits == 8 && c->v_bits == 8 ? 3 : 4;       // CTAs per SM
     const long long base = (long long)b->n_seqs * c->n_heads * (p.tc ? (rows + 255) / 256 : (rows + 15) / 16), room = (long long)sm_count() * resident;

@@ -21,7 +21,7 @@
 //
 // What bounds it (B200, 1965 MHz): the softmax warps.  At 128 columns and 8-bit codes a tile of 64 keys takes ~2470 cycles of a CTA, of which the exponentials
 // alone are 1024 (8 cycles a warp instruction on each of the four schedulers), the products 2 x 512.  Measured:
-//   2048 queries behind 16384 keys, 32 query / 8 cache heads, 128 columns, 8 bits   740 us   790 TFLOP/s (floor at the measured dense rate 359)
+//   2048 queries behind 16384 keys, 32 query / 8 cache heads, 128 columns, 8 bits   740 us   790 TFLOP/s (359 us at the dense rate)
 //   16 sequences, 1024 queries on 2240 keys each, 30 heads, 64 columns, 4 bits       638 us   442 TFLOP/s (half the columns: the same exponentials feed half the products)
 //   4096 queries, window 2048, 128 columns                                          120 us   578 TFLOP/s
 // Tiles tried: 128 keys with one score tile each 784 / 721 / 137 us (the softmax waits for its scores); 64 keys, packed rows straight from the pages into the

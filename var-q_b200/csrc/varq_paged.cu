@@ -391,6 +391,8 @@ namespace {
 // (in tiles; fixed and merge are fits) picked the best or within 2 % of the best of 1 .. 24 parts on 10 of 11 calls that were measured, e.g. 256 queries
 // behind 8192 keys, 8 heads: 1 / 2 / 4 / 8 parts 186 / 117 / 72 / 88 us, picks 4; 2048 behind 16384 740 / 807 / 807 / 943, picks 1.  The one it misses are
 // chunks of 17 to 512 queries behind 0 to 4000 keys, 1 / 2 parts 91 / 77 us, picks 1: only the longest length is known here, and there it is the critical path.
+// Of 11 calls of the decode kernel it misses one by 10 % (24 sequences, 15 rows, a window of 1024: 25.1 us in clusters of two, 22.8 in two parts through the
+// workspace); one query behind 32768 keys takes 313 us in one part, 84 in 4, 31 in 16, 21 in the 54 that it picks.
 // Cluster or workspace: parts of the decode kernel that are resident all at once, up to eight of a row tile, meet in a cluster; without a second launch one
 // sequence of 1000 keys takes 8.0 us, with it 12.9.  Where they are not resident, clusters wait for room together: 64 sequences of 8000 keys, 16 heads 284 us
 // in clusters, 259 through the workspace.

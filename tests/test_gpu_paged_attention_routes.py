@@ -28,6 +28,21 @@ def test_any_number_of_rows(D, kb, vb, counts, G):
     b.check(q, counts, causal=False)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kb,vb", BITS)
+@pytest.mark.parametrize("G,most,n", [(1, 24, 300), (5, 4, 90), (3, 7, 2000)])
+def test_seventeen_to_twenty_four_rows(D, kb, vb, G, most, n):
+    """many sequences with 17 to 24 rows of a head at most: one row tile holds them; some sequences have fewer, or none"""
+    heads = 8
+    kv = [n + 7 * i if i % 4 else i for i in range(8)]
+    counts = [max(most - i, 0) if i != 3 else 0 for i in range(8)]
+    b = Batch(kv, heads, D, kb, vb, page=16, seed=D + kb + most)
+    q = queries(sum(counts), heads * G, D, torch.bfloat16 if G == 5 else torch.float16)
+    b.check(q, counts)
+    b.check(q, counts, causal=False)
+    b.check(q, counts, window=33, sinks=5)
+
+
 @pytest.mark.parametrize("window,sinks", [(1, 0), (3, 1), (17, 5), (64, 64), (127, 0), (200, 130)])
 @pytest.mark.parametrize("c", [1, 9, 150])
 def test_windows(window, sinks, c):

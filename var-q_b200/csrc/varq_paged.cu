@@ -384,9 +384,13 @@ namespace {
 // How a call is shared out.
 //
 // Kernel: few query rows per head of the cache leave most of the chunk kernel's 256 idle, while the decode kernel reads the keys once for every 16.  They cross
-// where the decode kernel needs a third row tile at head_dim 128, and a sixth at 64 (chunk kernel / decode kernel, us):
+// where the decode kernel needs a third row tile at head_dim 128, and a sixth at 64 (chunk kernel / decode kernel of 16 rows a CTA, us):
 //   128: 24 rows, 64 sequences of 8000 keys 542 / 391; 32 rows, 8 of 1000 24.1 / 20.4; 40 rows, 64 of 8000 542 / 560; 64 rows, 8 of 1000 24.4 / 30.1
 //    64: 40 rows, 32 of 2000 136 / 102; 64 rows 141 / 132; 100 rows, 4 of 300 13.8 / 13.4 (which a larger call would turn round)
+// Rows of a decode CTA: 17 to 24 rows in one CTA unpack the keys once, in two of 16 twice, but side by side.  Two / one, us: 24 rows, 64 sequences of 8000 keys, 8 heads
+// 391 / 303; 20 rows, 24 sequences, a window of 1024 32.0 / 28.9; 24 rows, 8 sequences of 1000 20.4 / 19.1; with fewer sequences and heads than a quarter of the SMs 24
+// rows, 1 sequence of 1000 11.6 / 14.4; 20 rows, 2 of 3000 18.1 / 18.8; at 64 columns, 2 of 4000, 2 bits 15.2 / 15.4.  Two of 24 for 40 rows at 64 columns, instead of three
+// of 16: 115 and 102.
 // Parts of the key range: more of them fill the SMs, and each costs a CTA its set-up and, through the workspace, a store and a second launch.  The model below
 // (in tiles; fixed and merge are fits) picked the best or within 2 % of the best of 1 .. 24 parts on 10 of 11 calls that were measured, e.g. 256 queries
 // behind 8192 keys, 8 heads: 1 / 2 / 4 / 8 parts 186 / 117 / 72 / 88 us, picks 4; 2048 behind 16384 740 / 807 / 807 / 943, picks 1.  The one it misses are
@@ -398,6 +402,7 @@ namespace {
 // in clusters, 259 through the workspace.
 struct AttnPlan {
     bool tc, cluster;                  // kernel; its parts meet in clusters, not in the workspace
+    int rows;                          // query rows of a CTA (decode kernel)
     int splits, tiles_per_split;       // tiles of 16 keys (decode kernel)
 };
 AttnPlan plan_attn(const varq_paged_t* c, const varq_paged_batch_t* b) {
@@ -406,9 +411,10 @@ AttnPlan plan_attn(const varq_paged_t* c, const varq_paged_batch_t* b) {
     const long long rows = (long long)max_q * (b->q_heads / c->n_heads);
     const long long seen = (long long)b->window + max_q + b->sinks, span = b->window && seen < b->max_kv ? seen : b->max_kv;      // keys of a CTA, about
     p.tc = forced_attn_path() == VARQ_ATTN_PATH_TC || (forced_attn_path() != VARQ_ATTN_PATH_DECODE && rows > (D == 64 ? 80 : 32));
+    p.rows = rows <= 8 ? 8 : rows > 16 && rows <= 24 && 4ll * b->n_seqs * c->n_heads >= sm_count() ? 24 : 16;
     const long long unit = p.tc ? 128 : 16, tiles = span > unit ? (span + unit - 1) / unit : 1;
-    const int resident = p.tc ? 1 : rows > 8 ? (D == 128 ? 3 : 4) : D == 64 ? 5 : c->k_bits == 8 && c->v_bits == 8 ? 3 : 4;       // CTAs per SM
-    const long long base = (long long)b->n_seqs * c->n_heads * (p.tc ? (rows + 255) / 256 : (rows + 15) / 16), room = (long long)sm_count() * resident;
+    const int resident = p.tc ? 1 : p.rows > 16 ? (D == 128 ? 2 : 3) : p.rows > 8 ? (D == 128 ? 3 : 4) : D == 64 ? 5 : c->k_bits == 8 && c->v_bits == 8 ? 3 : 4;       // CTAs per SM
+    const long long base = (long long)b->n_seqs * c->n_heads * (p.tc ? (rows + 255) / 256 : (rows + p.rows - 1) / p.rows), room = (long long)sm_count() * resident;
     // the number of parts that makes the waves of CTAs shortest, a CTA costing its tiles and a fixed part, parts in the workspace those, the second launch, too
     const long long fixed = p.tc ? 4 : 16, least = p.tc ? 2 : 4, merge = p.tc ? 4 : 24;
     long long best = 0;
@@ -470,6 +476,6 @@ extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch
         return fail(VARQ_ERR_WORKSPACE, "varq_paged_attn: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
     float *ws_o = reinterpret_cast<float*>(workspace), *ws_ml = ws_o + (size_t)p.splits * a.T * a.Hq * a.c.D;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (int rc = p.tc ? paged_attn_tc_run(a, p.splits, ws_o, ws_ml, st) : paged_attn_decode_run(a, p.splits, p.cluster, p.tiles_per_split, ws_o, ws_ml, st)) return rc;
+    if (int rc = p.tc ? paged_attn_tc_run(a, p.splits, ws_o, ws_ml, st) : paged_attn_decode_run(a, p.rows, p.splits, p.cluster, p.tiles_per_split, ws_o, ws_ml, st)) return rc;
     return need ? paged_attn_merge_run(a, p.splits, ws_o, ws_ml, st) : VARQ_OK;
 }

@@ -71,7 +71,8 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, int p, i
 constexpr int PAGED_CLUSTER = 8;       // up to so many parts of the decode kernel can meet in a cluster, without a workspace
 // Parts of the key range (splits) leave numerators ws_o [split][query row][D] and (reference, sum) ws_ml [split][query row][2]; a second launch merges them
 int paged_attn_tc_run(const PagedAttnArgs& a, int splits, float* ws_o, float* ws_ml, cudaStream_t st);
-int paged_attn_decode_run(const PagedAttnArgs& a, int splits, bool in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st);
+// rows: query rows of a CTA, 8, 16 or 24
+int paged_attn_decode_run(const PagedAttnArgs& a, int rows, int splits, bool in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st);
 int paged_attn_merge_run(const PagedAttnArgs& a, int splits, const float* ws_o, const float* ws_ml, cudaStream_t st);
 int paged_attn_tc_status(int* out);
 int forced_attn_path();                // varq_attn_force_path

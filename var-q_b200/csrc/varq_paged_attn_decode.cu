@@ -1,4 +1,4 @@
-// Attention of a few query rows (eight or sixteen per CTA) over a paged cache: warp-level tensor-core instructions fed straight from the pages.
+// Attention of a few query rows (8, 16 or 24 per CTA) over a paged cache: warp-level tensor-core instructions fed straight from the pages.
 //
 // The work is to stream the codes once, so the kernel is built around instructions per key and bytes in flight.  A warp takes 16 keys at a time, which lie
 // in one page, 16 rows one behind the other: its lanes copy them (cp.async, 16 bytes each) to a ring of its own in shared memory, several tiles ahead.  The
@@ -15,8 +15,8 @@
 //
 // What bounds it (B200): the issue of its instructions, 365 per 16 keys and warp at 128 columns and 4 bits, about half of them the conversion of the codes.
 // 64 sequences of 2000 to 10520 keys, 16 heads x 128, 4 bits: 239 us, 3.9 TB/s, DRAM 47 % busy (its bytes alone take 142 us).  One sequence of 1000 keys, 8 heads: 8 us, a chain
-// of latencies (launch, lengths, pages, rows, two products, the cluster's merge).  Four tokens over a window of 1024 (20 rows, two row tiles) on 24 sequences:
-// 32 us; the row tiles read the keys twice, the second time from L2.  With rows straight from the pages into registers, a tile ahead, instead of the ring: 290 us.
+// of latencies (launch, lengths, pages, rows, two products, the cluster's merge).  Four tokens over a window of 1024 (20 rows of a head) on 24
+// sequences: 29 us.  With rows straight from the pages into registers, a tile ahead, instead of the ring: 290 us.
 #include <cooperative_groups.h>
 
 #include <cfloat>
@@ -101,7 +101,7 @@ template <int BITS, int NW> __device__ __forceinline__ void pd_join(const uint32
 }
 
 template <int KB, int VB, int D, int NT>
-__global__ void __launch_bounds__(PD_WARPS * 32, NT > 1 ? (D == 128 ? 3 : 4) : D == 128 ? (KB == 8 && VB == 8 ? 3 : 4) : 5)
+__global__ void __launch_bounds__(PD_WARPS * 32, NT > 2 ? (D == 128 ? 2 : 3) : NT > 1 ? (D == 128 ? 3 : 4) : D == 128 ? (KB == 8 && VB == 8 ? 3 : 4) : 5)
 paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, int* status) {
     using P = PdPlan<KB, VB, D>;
     constexpr int KBYTES = D / 4 * KB / 8, VBYTES = D / 8 * VB / 8;       // of a row and thread
@@ -466,15 +466,19 @@ int launch_nt(const PagedAttnArgs& a, int splits, bool in_cluster, int tiles_per
     return VARQ_OK;
 }
 template <int KB, int VB, int D>
-int launch(const PagedAttnArgs& a, int splits, bool in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st) {
-    return (long long)a.max_q * a.G <= 8 ? launch_nt<KB, VB, D, 1>(a, splits, in_cluster, tiles_per_split, ws_o, ws_ml, st) : launch_nt<KB, VB, D, 2>(a, splits, in_cluster, tiles_per_split, ws_o, ws_ml, st);
+int launch(const PagedAttnArgs& a, int rows, int splits, bool in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st) {
+    switch (rows) {
+        case 8: return launch_nt<KB, VB, D, 1>(a, splits, in_cluster, tiles_per_split, ws_o, ws_ml, st);
+        case 16: return launch_nt<KB, VB, D, 2>(a, splits, in_cluster, tiles_per_split, ws_o, ws_ml, st);
+        default: return launch_nt<KB, VB, D, 3>(a, splits, in_cluster, tiles_per_split, ws_o, ws_ml, st);
+    }
 }
 
 }  // namespace
 
-int paged_attn_decode_run(const PagedAttnArgs& a, int splits, bool in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st) {
+int paged_attn_decode_run(const PagedAttnArgs& a, int rows, int splits, bool in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st) {
 #define GO(K_, V_) \
-    if (a.c.kb == K_ && a.c.vb == V_) return a.c.D == 64 ? launch<K_, V_, 64>(a, splits, in_cluster, tiles_per_split, ws_o, ws_ml, st) : launch<K_, V_, 128>(a, splits, in_cluster, tiles_per_split, ws_o, ws_ml, st);
+    if (a.c.kb == K_ && a.c.vb == V_) return a.c.D == 64 ? launch<K_, V_, 64>(a, rows, splits, in_cluster, tiles_per_split, ws_o, ws_ml, st) : launch<K_, V_, 128>(a, rows, splits, in_cluster, tiles_per_split, ws_o, ws_ml, st);
     GO(8, 8) GO(8, 4) GO(8, 2) GO(4, 8) GO(4, 4) GO(4, 2) GO(2, 8) GO(2, 4) GO(2, 2)
 #undef GO
     return fail(VARQ_ERR_ARG, "varq_paged_attn: bits must be 2, 4 or 8");

@@ -1,0 +1,70 @@
+"""Scales of a paged cache that nobody wrote, that nobody sees, or that are at the ends of fp32.
+
+Unseen: bit for bit what comes out over clean pools.  Seen: against the formula, tolerances as in test_gpu_paged_attention.py, where they are derived."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_paged_attention import DEV, Batch, queries
+from VAR_Q import _cabi
+
+pytestmark = pytest.mark.gpu
+# subnormals (what small integers look like), zeros, negative numbers, the ends of the range, infinities, NaN
+PATTERNS = [1, 5, 0x1fffff, 0x400000, 0x7fffff, 0x800000, 0, 0x80000000, 0x80000001, 0xbf800000, 0x7f7fffff, 0xff7fffff, 0x7f800000, 0xff800000, 0x7fc00000]
+
+
+@pytest.fixture(params=["tc", "decode"], autouse=True)
+def path(request):
+    _cabi.force_attn_path(request.param)
+    yield request.param
+    _cabi.force_attn_path(None)
+
+
+def bits_of(pattern):
+    return pattern - (1 << 32) if pattern >= 1 << 31 else pattern
+
+
+def put(cache, slots, pattern, names=("k_scale", "v_scale")):
+    for name in names:
+        flat = getattr(cache, name).view(torch.int32)
+        flat[slots.to(DEV) // cache.page_size, :, slots.to(DEV) % cache.page_size] = bits_of(pattern)
+
+
+def everything_but(cache, kept):
+    rest = torch.ones(cache.num_pages * cache.page_size, dtype=torch.bool)
+    rest[torch.cat(kept)] = False
+    return rest.nonzero().flatten()
+
+
+@pytest.mark.parametrize("D,kb,vb", [(64, 8, 8), (128, 4, 4), (64, 2, 2)])
+@pytest.mark.parametrize("counts", [[1, 1, 1, 1], [3, 40, 1, 130]])
+def test_what_is_not_written_does_not_matter(D, kb, vb, counts):
+    """lengths that end inside a tile, a page, or a copy of 16 rows"""
+    b = Batch([3, 50, 333, 201], 2, D, kb, vb, page=32, seed=D)
+    q = queries(sum(counts), 4, D)
+    rest = everything_but(b.cache, b.slots)
+    put(b.cache, rest, 0x3f800000)
+    clean = b.check(q, counts)
+    whole = b.check(q, counts, causal=False)
+    for pattern in PATTERNS:
+        put(b.cache, rest, pattern)
+        for ref, kw in ((clean, {}), (whole, {"causal": False})):
+            out, lse = b.attend(q, counts, 1.0 / math.sqrt(D), **kw)
+            assert torch.equal(out, ref[0]) and torch.equal(lse, ref[1]), hex(pattern)
+
+
+@pytest.mark.parametrize("window,sinks", [(50, 3), (7, 0), (130, 65)])
+@pytest.mark.parametrize("c", [1, 5, 70])
+def test_what_lies_in_front_of_the_window_does_not_matter(window, sinks, c):
+    """tokens that every query has left behind: never written, or in pages that are zero or others' now"""
+    n = 500
+    b = Batch([n, n - 77], 2, 64, page=16, seed=window)
+    q = queries(2 * c, 4, 64)
+    hidden = torch.cat([s[sinks:max(sinks, len(s) - c - window + 1)] for s in b.slots])
+    put(b.cache, hidden, 0x3f800000)
+    clean = b.check(q, [c, c], window=window, sinks=sinks)
+    for pattern in PATTERNS:
+        put(b.cache, hidden, pattern)
+        out, lse = b.attend(q, [c, c], 0.125, window=window, sinks=sinks)
+        assert torch.equal(out, clean[0]) and torch.equal(lse, clean[1]), hex(pattern)

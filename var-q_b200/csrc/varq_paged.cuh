@@ -68,6 +68,10 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, int p, i
     return s;
 }
 
+// 1 / V scale of a key, by which its weight times V scale enters the sum.  Finite whatever lies there, NaN and infinity too, so that 0 times it is 0: a key that is not
+// seen has weight 0, and its scale may be anything.
+__device__ __forceinline__ float paged_inverse(float scale) { return __fdividef(1.f, fmaxf(scale, 0x1p-100f)); }
+
 constexpr int PAGED_CLUSTER = 8;       // up to so many parts of the decode kernel can meet in a cluster, without a workspace
 // Parts of the key range (splits) leave numerators ws_o [split][query row][D] and (reference, sum) ws_ml [split][query row][2]; a second launch merges them
 int paged_attn_tc_run(const PagedAttnArgs& a, int splits, float* ws_o, float* ws_ml, cudaStream_t st);

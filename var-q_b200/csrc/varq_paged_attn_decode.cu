@@ -160,7 +160,7 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
             const int r2 = row0 + t * 8 + 2 * c + e;
             qfac[t][e] = __shfl_sync(0xffffffffu, fi, (2 * c + e) * 4) * a.scale_log2;
             const PagedSpan s = paged_span(a, p_first + r2 / a.G, seq.kv);
-            col_hi[t][e] = r2 < rows ? s.hi : seq.kv; col_lo[t][e] = r2 < rows ? s.lo : 0;
+            col_hi[t][e] = r2 < rows ? s.hi : 0; col_lo[t][e] = s.lo;      // a column without a row sees nothing: what it saw would move the references
         }
     }
 
@@ -248,8 +248,7 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             lv[r] = __log2f(cur.vs[r]);
-            rv[r] = __fdividef(1.f, cur.vs[r]);
-            if (MASKED && !(cur.vs[r] <= FLT_MAX && cur.vs[r] > 0.f)) rv[r] = 1.f;      // what is not seen has weight 0, and 0 times its inverse has to be 0
+            rv[r] = paged_inverse(cur.vs[r]);
         }
         bool over = false;
 #pragma unroll

@@ -265,7 +265,9 @@ int varq_attn_fwd_qnorm(const varq_tensor_t* q, const varq_tensor_t* k_codes, co
  * reference, whose caches hold one batch of equally long samples (VAR_Q/quant.py:180-205); quantization is its
  * symmetric per-token-per-head mode (VAR_Q/quant.py:92-95, 112-121) with each token's own scale.
  *   k_codes / v_codes : int32 [n_pages][n_heads][page_size][head_dim * bits / 32], packed as everywhere in this library
- *   k_scale / v_scale : fp32  [n_pages][n_heads][page_size]; value = code * scale
+ *   k_scale / v_scale : fp32  [n_pages][n_heads][page_size]; value = code * scale.  Attention takes a V scale below 2^-100, 0
+ *                       among them, for 2^-100 (such a value is as good as zero), and a V scale that is no size (NaN, infinite, negative)
+ *                       makes the rows that see it NaN
  * all contiguous and 16-byte aligned.  page_size: a power of two from 16 to 1024; head_dim 64 or 128; bits 2, 4 or 8 for K and V each.
  * A slot is page * page_size + offset.  What is not written may hold anything: nothing reads it. */
 typedef struct {

@@ -68,3 +68,39 @@ def test_what_lies_in_front_of_the_window_does_not_matter(window, sinks, c):
         put(b.cache, hidden, pattern)
         out, lse = b.attend(q, [c, c], 0.125, window=window, sinks=sinks)
         assert torch.equal(out, clean[0]) and torch.equal(lse, clean[1]), hex(pattern)
+
+
+@pytest.mark.parametrize("pattern", [0, 1, 5, 0x1fffff, 0x400000, 0x7fffff, 0x800000])
+@pytest.mark.parametrize("c", [1, 40])
+@pytest.mark.parametrize("every", [1, 3, 1000])
+def test_seen_values_that_are_zero_keep_their_weight(pattern, c, every):
+    """V scales of 0 or next to it, in tiles with and without masks: the key's value is (as good as) zero, its weight counts"""
+    b = Batch([300, 75], 2, 64, page=16, seed=every)
+    put(b.cache, torch.cat([s[::every] for s in b.slots]), pattern, ("v_scale",))
+    put(b.cache, b.slots[0][17:20], pattern, ("v_scale",))
+    q = queries(2 * c, 4, 64)
+    b.check(q, [c, c])
+    b.check(q, [c, c], causal=False)
+    b.check(q, [c, c], window=60, sinks=19)
+
+
+def test_keys_that_are_zero_answer_nothing():
+    """K scales of 0: a score of 0, in V's weight as any other"""
+    b = Batch([300, 75], 2, 64, page=16, seed=1)
+    put(b.cache, torch.cat([s[::3] for s in b.slots]), 0, ("k_scale",))
+    for c in (1, 40):
+        b.check(queries(2 * c, 4, 64), [c, c])
+
+
+@pytest.mark.parametrize("pattern", [0x7f800000, 0x7fc00000, 0xbf800000])
+@pytest.mark.parametrize("at", [0, 20, 290])
+@pytest.mark.parametrize("c", [1, 40])
+def test_scales_that_are_no_sizes_spoil_the_rows_that_see_them(pattern, at, c):
+    b = Batch([300], 2, 64, page=16, seed=at)
+    q = queries(c, 4, 64)
+    clean = b.check(q, [c])
+    put(b.cache, b.slots[0][at:at + 1], pattern, ("v_scale",))
+    out, lse = b.attend(q, [c], 0.125)
+    first = max(0, at - (300 - c))                                     # queries from here on see the key
+    assert torch.isnan(out[first:]).all() and torch.isnan(lse[first:]).all()
+    assert torch.equal(out[:first], clean[0][:first]) and torch.equal(lse[:first], clean[1][:first])

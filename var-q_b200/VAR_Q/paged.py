@@ -45,7 +45,7 @@ class PagedCache:
 
     @classmethod
     def over(cls, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, head_dim: int) -> "PagedCache":
-        """A cache over pools that are there already."""
+        """A cache over pools that are there already.  Scales may be 0 (``attend`` takes V scales below 2^-100 for 2^-100); they are not negative."""
         cache = cls.__new__(cls)
         cache._set(k_codes, v_codes, k_scale, v_scale, head_dim)
         return cache

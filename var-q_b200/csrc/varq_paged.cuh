@@ -68,9 +68,12 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, int p, i
     return s;
 }
 
-// 1 / V scale of a key, by which its weight times V scale enters the sum.  Finite whatever lies there, NaN and infinity too, so that 0 times it is 0: a key that is not
-// seen has weight 0, and its scale may be anything.
-__device__ __forceinline__ float paged_inverse(float scale) { return __fdividef(1.f, fmaxf(scale, 0x1p-100f)); }
+// What the V scale of a key puts into the exponent, and the factor that takes it out of the sum again: log2 of it, 1 / it.  A scale below 2^-100, 0 among them,
+// counts as 2^-100: the key keeps its weight, its value is as good as zero.  One that is no size of values (NaN, infinite, negative) spoils the rows that see
+// it and no other: the inverse is finite whatever lies there, and a key that is not seen has weight 0, which times its inverse has to be 0.
+constexpr float PAGED_LEAST_SCALE = 0x1p-100f;
+__device__ __forceinline__ float paged_exponent(float scale) { return scale >= 0.f ? __log2f(fmaxf(scale, PAGED_LEAST_SCALE)) : __uint_as_float(0x7fffffffu); }
+__device__ __forceinline__ float paged_inverse(float scale) { return __fdividef(1.f, fmaxf(scale, PAGED_LEAST_SCALE)); }
 
 constexpr int PAGED_CLUSTER = 8;       // up to so many parts of the decode kernel can meet in a cluster, without a workspace
 // Parts of the key range (splits) leave numerators ws_o [split][query row][D] and (reference, sum) ws_ml [split][query row][2]; a second launch merges them

@@ -247,7 +247,7 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
         float lv[2], rv[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            lv[r] = __log2f(cur.vs[r]);
+            lv[r] = paged_exponent(cur.vs[r]);
             rv[r] = paged_inverse(cur.vs[r]);
         }
         bool over = false;

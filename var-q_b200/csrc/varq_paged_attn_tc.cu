@@ -500,8 +500,8 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                     float* tab_a = tab + (k >> 1) * 4 + (k & 1);
                     const bool there = tiles.key(tile0 + j) + k < seq.kv;
                     if (is_k) tab_a[0] = there ? sc * a.scale_log2 : 0.f;
-                    else {                                  // a scale that is no number spoils the rows that see it, and no other
-                        tab_a[2] = there ? (sc <= FLT_MAX ? __log2f(sc) : sc - sc) : -INFINITY;
+                    else {
+                        tab_a[2] = there ? paged_exponent(sc) : -INFINITY;
                         tab[2 * PT_N + k] = there ? paged_inverse(sc) : 0.f;
                     }
                 }

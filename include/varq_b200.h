@@ -306,7 +306,8 @@ typedef struct {
 
 /* out = softmax(q k^T * softmax_scale) v over the pages; q and out (1, n_queries, q_heads, head_dim), fp16 or bf16 (one type).  lse (or
  * NULL): fp32 [n_queries][q_heads], log of the sum of exponentials.  A query that sees no key gets zeros and -inf.
- * What a query does not see does not reach its result, whatever it holds. */
+ * What a query does not see does not reach its result, whatever it holds.  Weight times V scale of a key that is 2^-126 of the row's largest, or less, is
+ * taken for 0, and the weight with it. */
 size_t varq_paged_attn_workspace_bytes(const varq_paged_t* cache, const varq_paged_batch_t* batch);
 int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch_t* batch, const varq_tensor_t* q, const varq_tensor_t* out, float* lse,
                     void* workspace, size_t workspace_bytes, void* stream);

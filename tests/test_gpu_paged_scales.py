@@ -104,3 +104,19 @@ def test_scales_that_are_no_sizes_spoil_the_rows_that_see_them(pattern, at, c):
     first = max(0, at - (300 - c))                                     # queries from here on see the key
     assert torch.isnan(out[first:]).all() and torch.isnan(lse[first:]).all()
     assert torch.equal(out[:first], clean[0][:first]) and torch.equal(lse[:first], clean[1][:first])
+
+
+@pytest.mark.parametrize("c", [1, 40])
+@pytest.mark.parametrize("vb,size", [(2, 1.2), (2, 1.9), (4, 1.9), (8, 1.9)])
+def test_values_next_to_the_end_of_fp32(c, vb, size):
+    """V up to size * 2^127: with 2 and 4 bits its scales are above 2^125, whose inverses are next to or below the smallest normal number.
+    The other rows are 2^27 times smaller: weights times V scale of one row have to lie within 2^126 of one another."""
+    n, D = 90, 64
+    b = Batch([n], 1, D, 8, vb, page=16, seed=vb, v_gain=lambda j: torch.full_like(j, 2.0 ** 100, dtype=torch.float32))
+    g = torch.Generator().manual_seed(7)
+    slots = b.slots[0][1::3].to(DEV)
+    v = (torch.rand((len(slots), 1, D), generator=g) * 2 - 1) * size * 2.0 ** 127
+    v[:, 0, 5] = size * 2.0 ** 127
+    b.cache.append(torch.randn((len(slots), 1, D), generator=g).to(DEV), v.to(DEV), slots)
+    b.check(queries(c, 2, D, torch.bfloat16), [c])
+    b.check(queries(c, 2, D, torch.bfloat16), [c], causal=False)

@@ -73,7 +73,11 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, int p, i
 // it and no other: the inverse is finite whatever lies there, and a key that is not seen has weight 0, which times its inverse has to be 0.
 constexpr float PAGED_LEAST_SCALE = 0x1p-100f;
 __device__ __forceinline__ float paged_exponent(float scale) { return scale >= 0.f ? __log2f(fmaxf(scale, PAGED_LEAST_SCALE)) : __uint_as_float(0x7fffffffu); }
-__device__ __forceinline__ float paged_inverse(float scale) { return __fdividef(1.f, fmaxf(scale, PAGED_LEAST_SCALE)); }
+__device__ __forceinline__ float paged_inverse(float scale) {      // (__fdividef gives 0 above 2^126)
+    float r;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(fmaxf(scale, PAGED_LEAST_SCALE)));
+    return r;
+}
 
 constexpr int PAGED_CLUSTER = 8;       // up to so many parts of the decode kernel can meet in a cluster, without a workspace
 // Parts of the key range (splits) leave numerators ws_o [split][query row][D] and (reference, sum) ws_ml [split][query row][2]; a second launch merges them

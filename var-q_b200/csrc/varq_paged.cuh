@@ -71,12 +71,15 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, int p, i
 // What the V scale of a key puts into the exponent, and the factor that takes it out of the sum again: log2 of it, 1 / it.  A scale below 2^-100, 0 among them,
 // counts as 2^-100: the key keeps its weight, its value is as good as zero.  One that is no size of values (NaN, infinite, negative) spoils the rows that see
 // it and no other: the inverse is finite whatever lies there, and a key that is not seen has weight 0, which times its inverse has to be 0.
-constexpr float PAGED_LEAST_SCALE = 0x1p-100f;
-__device__ __forceinline__ float paged_exponent(float scale) { return scale >= 0.f ? __log2f(fmaxf(scale, PAGED_LEAST_SCALE)) : __uint_as_float(0x7fffffffu); }
-__device__ __forceinline__ float paged_inverse(float scale) {      // (__fdividef gives 0 above 2^126)
+__device__ __forceinline__ float paged_exponent(float scale) {
+    float y;
+    asm("{\n\t.reg .f32 t;\n\tlg2.approx.ftz.f32 t, %1;\n\tmax.NaN.f32 %0, t, %2;\n\t}" : "=f"(y) : "f"(scale), "f"(-100.f));
+    return y;
+}
+__device__ __forceinline__ float paged_inverse(float scale) {      // above 2^126 it is subnormal, which the reciprocal alone (and __fdividef) would flush
     float r;
-    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(fmaxf(scale, PAGED_LEAST_SCALE)));
-    return r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaxf(scale, 0x1p-100f) * 0.25f));
+    return r * 0.25f;
 }
 
 constexpr int PAGED_CLUSTER = 8;       // up to so many parts of the decode kernel can meet in a cluster, without a workspace

@@ -293,6 +293,7 @@ int varq_paged_read(const varq_paged_t* cache, const int64_t* slots, int64_t n_t
  * entries), and they are the sequence's last tokens: query i of n stands at position kv_lens[b] - n + i.
  *   causal = 0 : every query sees the whole sequence
  *   causal = 1 : a query at position p sees the keys 0 .. p; with window w > 0 the keys p - w + 1 .. p and the first `sinks` keys
+ * Entries of block_table for pages behind the last token, or for pages in which no query of the sequence sees a key, may hold anything.
  * Query head i uses head i / (q_heads / n_heads) of the cache.  max_q bounds the queries of a sequence, max_kv is the longest kv_lens (a
  * hint: it decides how the work is split).
  * The device checks what the host cannot see: starts, lengths and page numbers outside their bounds are clamped into them and leave a

@@ -1,0 +1,37 @@
+"""Attention over a paged cache where its numbers are large or its pages are gone: pages that no query sees any more, windows and first tokens up to the
+largest int, lengths next to it.  Both kernels; tolerances as in test_gpu_paged_attention.py, where they are derived."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_paged_attention import DEV, Batch, queries
+from VAR_Q import _cabi
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["tc", "decode"], autouse=True)
+def path(request):
+    _cabi.force_attn_path(request.param)
+    yield request.param
+    _cabi.force_attn_path(None)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("window,sinks", [(50, 3), (7, 0), (130, 40)])
+@pytest.mark.parametrize("c", [1, 5, 70, 200])
+def test_pages_that_no_query_sees_need_not_be_there(page, window, sinks, c):
+    """a server gives the pages in front of the window back and leaves -1 in the table"""
+    b = Batch([600, 523], 2, 64, page=page, seed=page)
+    q = queries(2 * c, 4, 64)
+    clean = b.check(q, [c, c], window=window, sinks=sinks)
+    gone = 0
+    for i, n in enumerate(b.kv):
+        first = n - c - window + 1
+        for p in range(-(-sinks // page), first // page):
+            b.table[i, p], gone = -1, gone + 1
+    assert gone > 0
+    out, lse = b.attend(q, [c, c], 0.125, window=window, sinks=sinks)
+    assert torch.equal(out, clean[0]) and torch.equal(lse, clean[1])
+    assert _cabi.device_status() == 0

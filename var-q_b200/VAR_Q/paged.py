@@ -80,7 +80,8 @@ class PagedCache:
         ``q`` ``[tokens, query heads, head_dim]`` (float16 or bfloat16) holds the queries of all sequences one after another, those of sequence
         b in rows ``q_starts[b]`` .. ``q_starts[b + 1] - 1`` (int32, one entry more than sequences).  They are its last tokens: with n queries and
         ``kv_lens[b]`` tokens in the cache (int32, the chunk's own tokens included) query i stands at position ``kv_lens[b] - n + i``.
-        ``block_table`` (int32 ``[sequences, pages]``): the pages of a sequence in order; entries behind its last token are not read.
+        ``block_table`` (int32 ``[sequences, pages]``): the pages of a sequence in order; what stands for pages behind its last token, or for pages in
+        which no query sees a key any more, does not matter.
         ``max_q`` / ``max_kv``: bounds of a sequence's queries and tokens, so that nothing has to come back from the device.
 
         ``causal=False``: every query sees the whole sequence.  ``causal=True``: a query at position p sees the keys up to p, with ``window`` only

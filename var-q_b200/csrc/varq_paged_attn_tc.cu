@@ -119,9 +119,9 @@ template <int BITS> __host__ __device__ constexpr uint32_t pt_neg_base(int cls) 
                                                : (cls == 0 ? 0xE402E402u : cls == 1 ? 0xDC08DC08u : cls == 2 ? 0xD420D420u : 0xCC80CC80u);
 }
 
-// The key tiles of a CTA: `ns` tiles of first tokens, then those from `lo` on
+// The key tiles of a CTA: `ns` tiles of first tokens, then those from `lo` on; `first`: the first key of its windows, in the tile at `lo`
 struct PtTiles {
-    int ns, lo, n;
+    int ns, lo, n, first;
     __device__ __forceinline__ int key(int i) const { return i < ns ? i * PT_N : lo + (i - ns) * PT_N; }
 };
 
@@ -190,7 +190,8 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
     {
         const int t0 = row0 / a.G, t1 = (min(row0 + 2 * PT_M, rows) - 1) / a.G, t_mid = (min(row0 + PT_M, rows) - 1) / a.G;
         const int hi = max(a.causal ? min(seq.kv, p_first + t1 + 1) : seq.kv, 0), hi0 = max(a.causal ? min(seq.kv, p_first + t_mid + 1) : seq.kv, 0);
-        tiles.lo = a.window ? max(p_first + t0 - a.window + 1, 0) & ~(PT_N - 1) : 0;
+        tiles.first = a.window ? max(p_first + t0 - a.window + 1, 0) : 0;
+        tiles.lo = tiles.first & ~(PT_N - 1);
         tiles.ns = min((a.sinks + PT_N - 1) / PT_N, tiles.lo / PT_N);
         const int n = hi > 0 ? tiles.ns + (max(hi - tiles.lo, 0) + PT_N - 1) / PT_N : 0, n0 = hi0 > 0 ? tiles.ns + (max(hi0 - tiles.lo, 0) + PT_N - 1) / PT_N : 0;
         tile0 = (int)((long long)n * split / splits);
@@ -479,7 +480,7 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                 const int k = kq + 32 * it;
                 if (!mbar_wait_warp(&raw_full[rst], rst_ph, abort_flag, is_k ? 211 : 212)) break;
                 const unsigned char* raw = raw_stages + rst * P::RAW_BYTES;
-                uint32_t w[2][NB][NW];                 // rows behind a sequence's end: whatever lay there (any codes are finite; the tables hide them)
+                uint32_t w[2][NB][NW];                 // rows that were not fetched: whatever lay there (any codes are finite; the tables hide them)
 #pragma unroll
                 for (int p = 0; p < 2; ++p)
 #pragma unroll
@@ -498,7 +499,8 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                 float* tab = reinterpret_cast<float*>(smem + P::OFF_TAB) + ts * P::TAB_FLOATS;
                 if (it < 2) {
                     float* tab_a = tab + (k >> 1) * 4 + (k & 1);
-                    const bool there = tiles.key(tile0 + j) + k < seq.kv;
+                    const int key = tiles.key(tile0 + j) + k;
+                    const bool there = key < seq.kv && (key >= tiles.first || key < a.sinks);      // a run that no row sees is not fetched
                     if (is_k) tab_a[0] = there ? sc * a.scale_log2 : 0.f;
                     else {
                         tab_a[2] = there ? paged_exponent(sc) : -INFINITY;
@@ -573,7 +575,8 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
             tc_commit(&bars[P::B_END + t]);
             for (uint32_t i = 0; i < TC_SPIN_LIMIT && !__all_sync(0xffffffffu, mbar_try(&bars[P::B_END + t], 0)); ++i) {}
         } else {
-            // =============================================================== packed rows and scales of K (V): a bulk copy for every run of keys in one page
+            // =============================================================== packed rows and scales of K (V): a bulk copy for every run of keys in one page of which
+            // some row of the CTA sees a key (pages in front of the window may be gone)
             const bool is_k = warp == P::LOAD_WARP;
             const int bits = is_k ? a.c.kb : a.c.vb, row = D / 8 * bits, run = min(PT_N, page_mask + 1), last_key = max(seq.kv - 1, 0);
             const unsigned char* pool = reinterpret_cast<const unsigned char*>(is_k ? a.c.kc : a.c.vc);
@@ -587,7 +590,7 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                 const int st = j % P::RST, key = tiles.key(tile0 + j) + lane * run;
                 const int next = page_of(j + 1);
                 if (j >= P::RST && !mbar_wait_warp(&raw_freed[st], (j / P::RST - 1) & 1, abort_flag, is_k ? 213 : 214)) break;
-                const bool there = lane * run < PT_N && key < seq.kv;
+                const bool there = lane * run < PT_N && key < seq.kv && (key + run > tiles.first || key < a.sinks);
                 const int runs = __popc(__ballot_sync(0xffffffffu, there));
                 if (lane == 0) mbar_expect_tx(&raw_full[st], (uint32_t)(runs * run * (row + 4)));
                 __syncwarp();

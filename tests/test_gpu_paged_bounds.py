@@ -35,3 +35,15 @@ def test_pages_that_no_query_sees_need_not_be_there(page, window, sinks, c):
     out, lse = b.attend(q, [c, c], 0.125, window=window, sinks=sinks)
     assert torch.equal(out, clean[0]) and torch.equal(lse, clean[1])
     assert _cabi.device_status() == 0
+
+
+INT_MAX = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("sinks", [1 << 30, INT_MAX - 1024, INT_MAX - 62, INT_MAX - 14, INT_MAX])
+@pytest.mark.parametrize("c", [1, 100])
+def test_all_tokens_as_first_tokens(sinks, c):
+    b = Batch([500, 111], 2, 64, page=16, seed=3)
+    q = queries(2 * c, 4, 64)
+    out = b.check(q, [c, c], window=5, sinks=sinks)
+    b.check(q, [c, c], out=out)                                        # nothing is hidden

@@ -469,7 +469,8 @@ extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch
     a.B = batch->n_seqs; a.T = (int)batch->n_queries; a.Hq = batch->q_heads; a.G = a.Hq / a.c.H;
     a.max_q = (int)(batch->max_q < batch->n_queries ? batch->max_q : batch->n_queries); a.max_kv = batch->max_kv;
     a.scale_log2 = batch->softmax_scale * 1.4426950408889634f;
-    a.causal = batch->causal != 0; a.window = batch->window; a.sinks = batch->sinks;
+    a.causal = batch->causal != 0; a.window = batch->window;
+    a.sinks = batch->sinks < PAGED_MOST_KEYS ? batch->sinks : PAGED_MOST_KEYS;      // more tokens than there are: all of them
     const AttnPlan p = plan_attn(cache, batch);
     const size_t need = part_floats(p, cache, batch) * sizeof(float);
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))

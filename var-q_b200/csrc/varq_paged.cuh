@@ -35,6 +35,8 @@ struct PagedAttnArgs {
     int causal, window, sinks;         // window 0: none
 };
 
+constexpr int PAGED_MOST_KEYS = 0x7fffffff - 1023;      // a position, and the end of a tile of keys behind it, stay below 2^31
+
 // First thing that was wrong with numbers that only the device sees (lengths, starts, page numbers): the access is clamped into the
 // tensors' bounds and the code is kept for varq_device_status.
 enum PagedStatus : int { PAGED_BAD_STARTS = 64, PAGED_BAD_LENGTH = 65, PAGED_BAD_PAGE = 66 };

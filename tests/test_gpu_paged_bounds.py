@@ -47,3 +47,14 @@ def test_all_tokens_as_first_tokens(sinks, c):
     q = queries(2 * c, 4, 64)
     out = b.check(q, [c, c], window=5, sinks=sinks)
     b.check(q, [c, c], out=out)                                        # nothing is hidden
+
+
+@pytest.mark.parametrize("window", [1 << 30, INT_MAX - 600, INT_MAX - 1, INT_MAX])
+@pytest.mark.parametrize("sinks", [0, 200, INT_MAX])
+@pytest.mark.parametrize("counts", [[1, 1, 2], [5, 9, 700], [3, 90, 130]])
+def test_windows_that_hold_everything(window, sinks, counts):
+    """with more queries than tokens: the first ones stand in front of the sequence"""
+    b = Batch([3, 60, 120], 2, 64, page=16, seed=4)
+    q = queries(sum(counts), 4, 64)
+    out = b.check(q, counts, window=window, sinks=sinks)
+    b.check(q, counts, out=out)

@@ -61,12 +61,14 @@ __device__ __forceinline__ int paged_page(const PagedAttnArgs& a, int p, int* st
     return 0;
 }
 
+// First key of the window of a query at position p, max(p - window + 1, 0), with no number outside an int on the way (p may be negative)
+__device__ __forceinline__ int paged_window(const PagedAttnArgs& a, int p) { return a.window ? max(p, a.window - 1) - (a.window - 1) : 0; }
 // Keys that a query at position p sees: [0, min(sinks, hi)) and [lo, hi); none where hi <= 0
 struct PagedSpan { int lo, hi; };
 __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, int p, int kv) {
     PagedSpan s;
     s.hi = a.causal ? min(p + 1, kv) : kv;
-    s.lo = a.window ? max(p - a.window + 1, 0) : 0;
+    s.lo = paged_window(a, p);
     return s;
 }
 

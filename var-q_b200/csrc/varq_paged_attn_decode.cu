@@ -122,10 +122,10 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
 
     // ---- the 16-key tiles: first tokens, then the window (or everything)
     const int t0 = row0 / a.G, t1 = (min(row0 + ROWS, rows) - 1) / a.G;
-    const int hi = max(a.causal ? min(seq.kv, p_first + t1 + 1) : seq.kv, 0), lo = a.window ? max(p_first + t0 - a.window + 1, 0) & ~(PD_KEYS - 1) : 0;
+    const int hi = max(a.causal ? min(seq.kv, p_first + t1 + 1) : seq.kv, 0), lo = paged_window(a, p_first + t0) & ~(PD_KEYS - 1);
     const int ns = min((a.sinks + PD_KEYS - 1) / PD_KEYS, lo / PD_KEYS), n_tiles = hi > 0 ? ns + (max(hi - lo, 0) + PD_KEYS - 1) / PD_KEYS : 0;
     const int begin = (int)min((long long)split * tiles_per_split, (long long)n_tiles), end = split == splits - 1 ? n_tiles : min(begin + tiles_per_split, n_tiles);
-    const int all_hi = a.causal ? min(p_first + t0 + 1, seq.kv) : seq.kv, all_lo = a.window ? p_first + t1 - a.window + 1 : 0;      // what every row sees
+    const int all_hi = a.causal ? min(p_first + t0 + 1, seq.kv) : seq.kv, all_lo = paged_window(a, p_first + t1);      // what every row sees
     auto key_of = [&](int i) { return i < ns ? i * PD_KEYS : lo + (i - ns) * PD_KEYS; };
 
     // ---- Q fragments: column g is row t * 8 + g, scaled by a power of two to use fp16's range

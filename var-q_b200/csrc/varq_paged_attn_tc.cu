@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
     {
         const int t0 = row0 / a.G, t1 = (min(row0 + 2 * PT_M, rows) - 1) / a.G, t_mid = (min(row0 + PT_M, rows) - 1) / a.G;
         const int hi = max(a.causal ? min(seq.kv, p_first + t1 + 1) : seq.kv, 0), hi0 = max(a.causal ? min(seq.kv, p_first + t_mid + 1) : seq.kv, 0);
-        tiles.first = a.window ? max(p_first + t0 - a.window + 1, 0) : 0;
+        tiles.first = paged_window(a, p_first + t0);
         tiles.lo = tiles.first & ~(PT_N - 1);
         tiles.ns = min((a.sinks + PT_N - 1) / PT_N, tiles.lo / PT_N);
         const int n = hi > 0 ? tiles.ns + (max(hi - tiles.lo, 0) + PT_N - 1) / PT_N : 0, n0 = hi0 > 0 ? tiles.ns + (max(hi0 - tiles.lo, 0) + PT_N - 1) / PT_N : 0;
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
             __syncwarp();
             // keys between which every row of the query tile sees everything
             const int tl = min(row0 + t * PT_M + PT_M, rows) - 1, all_hi = a.causal ? p_first + (row0 + t * PT_M) / a.G + 1 : 0x7fffffff,
-                      all_lo = a.window ? p_first + tl / a.G - a.window + 1 : 0;
+                      all_lo = paged_window(a, p_first + tl / a.G);
             // A thread holds, of every eight columns of S, two of the rows g, g + 8, g + 16, g + 24 of its warp's 32 (g = lane / 4): it needs a quarter of
             // the keys' tables and uses an entry for four rows
             const int g = lane >> 2, cq = lane & 3;

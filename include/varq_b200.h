@@ -296,7 +296,7 @@ int varq_paged_read(const varq_paged_t* cache, const int64_t* slots, int64_t n_t
  * Entries of block_table for pages behind the last token, or for pages in which no query of the sequence sees a key, may hold anything.
  * Query head i uses head i / (q_heads / n_heads) of the cache.  max_q bounds the queries of a sequence, max_kv is the longest kv_lens (a
  * hint: it decides how the work is split).
- * The device checks what the host cannot see: starts, lengths and page numbers outside their bounds are clamped into them and leave a
+ * A sequence has 2^31 - 4096 tokens at most.  The device checks what the host cannot see: starts, lengths and page numbers outside their bounds are clamped into them and leave a
  * code (64, 65, 66) for varq_device_status. */
 typedef struct {
     const int32_t *q_starts, *kv_lens, *block_table;

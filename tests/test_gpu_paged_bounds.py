@@ -58,3 +58,21 @@ def test_windows_that_hold_everything(window, sinks, counts):
     q = queries(sum(counts), 4, 64)
     out = b.check(q, counts, window=window, sinks=sinks)
     b.check(q, counts, out=out)
+
+
+def test_the_longest_sequences(path):
+    """2^31 - 4096 tokens, all in one page; more are clamped and reported.  Sums of up to 2^18 fp32 terms, each addition off by 2^-22 of the sum at most (the tensor
+    core's additions truncate): 2^-4 relative, 2^-4 absolute for the log of the sum"""
+    D, page, most = 64, 1024, 2 ** 31 - 4096
+    b = Batch([page], 1, D, 2, 2, page=page, seed=5)
+    q = queries(1, 1, D)
+    ref, ref_lse, bound, _ = b.reference(q, [1], 0.125)
+    table = torch.full((1, 2 ** 31 // page), int(b.table[0, 0]), dtype=torch.int32, device=DEV)
+    table[0, most // page:] = -1
+    starts = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    for kv, status in ((most, 0), (most + 1, 65), (INT_MAX, 65)):
+        lens = torch.tensor([kv], dtype=torch.int32, device=DEV)
+        out, lse = b.cache.attend(q, table, lens, starts, 1, kv, 0.125, return_lse=True)
+        assert _cabi.device_status() == status
+        assert ((out.double() - ref).abs() <= 2.0 ** -4 * bound + 1e-3).all()
+        assert (lse - (ref_lse + math.log(most // page))).abs().item() <= 2.0 ** -4

@@ -35,7 +35,7 @@ struct PagedAttnArgs {
     int causal, window, sinks;         // window 0: none
 };
 
-constexpr int PAGED_MOST_KEYS = 0x7fffffff - 1023;      // a position, and the end of a tile of keys behind it, stay below 2^31
+constexpr int PAGED_MOST_KEYS = 0x7fffffff - 4095;      // tokens of a sequence: the numbers of the keys that a warp asks for next, 32 x 64 of them, stay below 2^31
 
 // First thing that was wrong with numbers that only the device sees (lengths, starts, page numbers): the access is clamped into the
 // tensors' bounds and the code is kept for varq_device_status.
@@ -50,7 +50,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnArgs& a, int b, int
     PagedSeq s;
     s.q0 = min(max(s0, 0), a.T);
     s.nq = min(min(max(s1, s.q0), a.T) - s.q0, a.max_q);
-    s.kv = (int)min((long long)max(kv, 0), (long long)a.table_pages << a.c.page_shift);
+    s.kv = (int)min((long long)min(max(kv, 0), PAGED_MOST_KEYS), (long long)a.table_pages << a.c.page_shift);
     if (s.q0 != s0 || s.nq != s1 - s0) atomicCAS(status, 0, PAGED_BAD_STARTS);
     if (s.kv != kv) atomicCAS(status, 0, PAGED_BAD_LENGTH);
     return s;

@@ -289,10 +289,13 @@ int varq_paged_read(const varq_paged_t* cache, const int64_t* slots, int64_t n_t
                     void* stream);
 
 /* The queries of a batch and where their sequences lie.  Sequence b has kv_lens[b] tokens in the cache, token i of them in page
- * block_table[b * table_stride + i / page_size]; its queries are rows q_starts[b] .. q_starts[b + 1] - 1 (q_starts[0] = 0, n_seqs + 1
+ * block_table[b * table_stride + i / page_size]; its queries are rows q_starts[b] .. q_starts[b + 1] - 1 (n_seqs + 1
  * entries), and they are the sequence's last tokens: query i of n stands at position kv_lens[b] - n + i.
  *   causal = 0 : every query sees the whole sequence
  *   causal = 1 : a query at position p sees the keys 0 .. p; with window w > 0 the keys p - w + 1 .. p and the first `sinks` keys
+ * Rows of q in front of q_starts[0] (which need not be 0) and behind q_starts[n_seqs] belong to no sequence: zeros and -inf, as for a query that
+ * sees nothing.  With n_queries, n_seqs or max_q 0 a call writes nothing.  Starts fall nowhere; where they do, or where a sequence has more than max_q
+ * queries, code 64 is left and rows in between are not defined.
  * Entries of block_table for pages behind the last token, or for pages in which no query of the sequence sees a key, may hold anything.
  * Query head i uses head i / (q_heads / n_heads) of the cache.  max_q bounds the queries of a sequence, max_kv is the longest kv_lens (a
  * hint: it decides how the work is split).

@@ -84,6 +84,8 @@ class PagedCache:
         which no query sees a key any more, does not matter.
         ``max_q`` / ``max_kv``: bounds of a sequence's queries and tokens, so that nothing has to come back from the device.
 
+        Rows of ``q`` in front of ``q_starts[0]`` and behind ``q_starts[-1]`` belong to no sequence (a batch padded to a fixed size): zeros, and -inf.
+
         ``causal=False``: every query sees the whole sequence.  ``causal=True``: a query at position p sees the keys up to p, with ``window`` only
         the last ``window`` of them and the first ``sinks`` keys of the sequence.  A query that sees nothing gets zeros.
         Returns the output in q's type and shape (contiguous); with ``return_lse`` also the float32 log of the sum of exponentials ``[tokens, query heads]``

@@ -43,13 +43,14 @@ enum PagedStatus : int { PAGED_BAD_STARTS = 64, PAGED_BAD_LENGTH = 65, PAGED_BAD
 int* paged_status_word();              // its device address; null if it cannot be had
 int paged_status(int* out);            // its value where *out is 0; clears it
 
-// Sequence b: its first query token, number of queries, tokens in the cache
-struct PagedSeq { int q0, nq, kv; };
+// Sequence b: its first query token, number of queries, tokens in the cache, query token behind its last one
+struct PagedSeq { int q0, nq, kv, end; };
 __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnArgs& a, int b, int* status) {
     const int s0 = __ldg(a.q_starts + b), s1 = __ldg(a.q_starts + b + 1), kv = __ldg(a.kv_lens + b);
     PagedSeq s;
     s.q0 = min(max(s0, 0), a.T);
-    s.nq = min(min(max(s1, s.q0), a.T) - s.q0, a.max_q);
+    s.end = min(max(s1, s.q0), a.T);
+    s.nq = min(s.end - s.q0, a.max_q);
     s.kv = (int)min((long long)min(max(kv, 0), PAGED_MOST_KEYS), (long long)a.table_pages << a.c.page_shift);
     if (s.q0 != s0 || s.nq != s1 - s0) atomicCAS(status, 0, PAGED_BAD_STARTS);
     if (s.kv != kv) atomicCAS(status, 0, PAGED_BAD_LENGTH);
@@ -70,6 +71,26 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, int p, i
     s.hi = a.causal ? min(p + 1, kv) : kv;
     s.lo = paged_window(a, p);
     return s;
+}
+
+// Query rows in front of the first sequence's and behind the last one's belong to no sequence.  They get zeros and -inf, as rows that see nothing: from the CTAs of
+// those two sequences, each thread (number `i` of `step`) a share of the rows of its head of the cache.
+struct PagedPad { unsigned short* out; long long os_t, os_h; float* lse; int D, G, Hq, h, front, behind, T; };
+__device__ __forceinline__ bool paged_pad_any(const PagedAttnArgs& a, const PagedSeq& seq, int b) { return (b == 0 && seq.q0 > 0) || (b == a.B - 1 && seq.end < a.T); }
+__device__ __forceinline__ PagedPad paged_pad_rows(const PagedAttnArgs& a, const PagedSeq& seq, int b, int h) {
+    return {reinterpret_cast<unsigned short*>(a.out), a.os_t, a.os_h, a.lse, a.c.D, a.G, a.Hq, h, b == 0 ? seq.q0 : 0, b == a.B - 1 ? seq.end : a.T, a.T};
+}
+__device__ __forceinline__ void paged_pad(const PagedPad p, long long i, long long step) {
+    const int chunks = p.D / 8;
+    for (const long long n = (long long)(p.front + p.T - p.behind) * p.G * chunks; i < n; i += step) {
+        const long long row = i / chunks, at = row / p.G, token = at < p.front ? at : at - p.front + p.behind;
+        const int c = (int)(i - row * chunks), head = p.h * p.G + (int)(row % p.G);
+        unsigned short* o = p.out + token * p.os_t + head * p.os_h + 8 * c;
+        if ((reinterpret_cast<uintptr_t>(o) & 15u) == 0) *reinterpret_cast<uint4*>(o) = make_uint4(0, 0, 0, 0);
+        else
+            for (int e = 0; e < 8; ++e) o[e] = 0;
+        if (c == 0 && p.lse) p.lse[token * p.Hq + head] = -INFINITY;
+    }
 }
 
 // What the V scale of a key puts into the exponent, and the factor that takes it out of the sum again: log2 of it, 1 / it.  A scale below 2^-100, 0 among them,

@@ -578,6 +578,7 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
             // =============================================================== packed rows and scales of K (V): a bulk copy for every run of keys in one page of which
             // some row of the CTA sees a key (pages in front of the window may be gone)
             const bool is_k = warp == P::LOAD_WARP;
+            if (paged_pad_any(a, seq, b)) paged_pad(paged_pad_rows(a, seq, b, h), (long long)(qb * splits + split) * 64 + (tid & 63), (long long)n_qblocks * splits * 64);
             const int bits = is_k ? a.c.kb : a.c.vb, row = D / 8 * bits, run = min(PT_N, page_mask + 1), last_key = max(seq.kv - 1, 0);
             const unsigned char* pool = reinterpret_cast<const unsigned char*>(is_k ? a.c.kc : a.c.vc);
             const float* scales = is_k ? a.c.ks : a.c.vs;

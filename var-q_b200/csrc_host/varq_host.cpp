@@ -527,6 +527,12 @@ PyObject* py_paged_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor out = empty({q.size(0), q.size(1), q.size(2)}, q.scalar_type(), dev);
     at::Tensor lse;
     if (with_lse) lse = empty({q.size(0), q.size(1)}, at::kFloat, dev);
+    if (b.n_seqs == 0) {                               // nothing to launch: every row belongs to no sequence
+        out.zero_();
+        if (with_lse) lse.fill_(-INFINITY);
+        return with_lse ? make_pair(out, lse) : THPVariable_Wrap(out);
+    }
+    if (b.max_q == 0) b.max_q = 1;                     // the rows' zeros are written on the device, where the starts are checked
     const varq_tensor_t qd = rows_desc(q), od = rows_desc(out);
     const size_t ws = varq_paged_attn_workspace_bytes(&c, &b);
     const at::Tensor buf = scratch(ws, dev);

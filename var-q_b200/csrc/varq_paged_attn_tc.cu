@@ -342,14 +342,14 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                             up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 1));
                             up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 2));
                             const bool first = (unset >> i & 1u) && up > -INFINITY;
-                            up = first || (up > PT_LAZY && !(unset >> i & 1u)) ? up : 0.f;
+                            // by a whole number: the factor is a power of two, which rounds nothing but weights that become subnormal
+                            up = first ? up : up > PT_LAZY && !(unset >> i & 1u) ? ceilf(up) : 0.f;
                             alpha[i] = first ? 1.f : ex2(-up);           // (nothing is accumulated where the reference is the first)
                             if (first) unset &= ~(1u << i);
                             nm[i] = add2(nm[i], pair_of(-up, -up));
                             l[i] = mul2(l[i], pair_of(alpha[i], alpha[i]));
                         }
                         const float al = by_lane(alpha);
-                        const __half2 ah = __float2half2_rn(al);
                         tmem_wait_st();
 #pragma unroll 1
                         for (int z = 0; z < c; ++z) {                    // P of the tile's chunks before this one
@@ -357,7 +357,10 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                             tmem_ld16(col_s + 16 * z, o);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = h2_mul(o[i], *reinterpret_cast<const uint32_t*>(&ah));
+                            for (int i = 0; i < 16; ++i) {                // (the factor may be too small for fp16)
+                                const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&o[i]));
+                                o[i] = pack_half2(p.x * al, p.y * al);
+                            }
                             tmem_st16(col_s + 16 * z, o);
                         }
                         if (j > 0) {                                     // behind the products of the tile before

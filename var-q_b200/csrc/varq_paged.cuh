@@ -107,6 +107,12 @@ __device__ __forceinline__ float paged_inverse(float scale) {      // above 2^12
     return r * 0.25f;
 }
 
+// Where a row's reference lies: its largest weight times V scale is held as 2^PAGED_SET when the reference is set or raised, and the reference is raised when one
+// passes 2^PAGED_TOP.  fp16 ends at 2^16, its normal numbers at 2^-14: what is 2^-21 of the largest or more is rounded by itself, what is less by 2^-32 of the largest.
+// (With the largest held as 1 to 2^8, one V row 2^13 times the others', at 2^13 times their weight, took the others out of all columns in which its codes are zero.)
+// 8 between the two: raising costs the chunk kernel a tile, and with less of it happens more than once or twice in a long row.
+constexpr float PAGED_SET = 7.f, PAGED_TOP = 15.f;
+
 constexpr int PAGED_CLUSTER = 8;       // up to so many parts of the decode kernel can meet in a cluster, without a workspace
 // Parts of the key range (splits) leave numerators ws_o [split][query row][D] and (reference, sum) ws_ml [split][query row][2]; a second launch merges them
 int paged_attn_tc_run(const PagedAttnArgs& a, int splits, float* ws_o, float* ws_ml, cudaStream_t st);

@@ -9,9 +9,11 @@
 //   O^T = V^T P^T   thread (g, c) holds an eighth of the head_dim of keys 2c, 2c + 1, 2c + 8, 2c + 9; pairs of keys are joined by byte
 //                   permutes, and P^T is the transpose of S^T's fragment (movmatrix).
 // As in the chunk kernel the V scale goes into the exponent: x = S * (K scale * factor of the row) + log2(V scale), P = 2^(x - m) in fp16,
-// l += P / V scale in fp32; the reference m is raised only when an x passes it by more than 8.  Queries are fp16 times a power of two per row, exact
-// but for elements 2^-22 times smaller than the row's largest.  Warps and CTAs (key ranges) are merged by the log-sum-exp rule: where all CTAs are resident
-// at once, up to eight of a row tile are a cluster and read one another's shared memory; else they leave parts in the workspace for a second launch.
+// l += P / V scale in fp32; the reference m is set 7 below the largest x and raised only when an x passes it by more than 15.  What is held in fewer than 32 bits:
+// P, the operand of a 16-bit product (weight times V scale of 2^-21 of the row's largest or more is rounded by itself, 2^-12 of it, a smaller one by 2^-32 of the
+// largest), and the queries, fp16 times a power of two per row: exact but for elements below 2^-22 of the row's largest, which are off by 2^-33 of it at most.
+// Warps and CTAs (key ranges) are merged by the log-sum-exp rule: where all CTAs are resident at once, up to eight of a row tile are a cluster and read one
+// another's shared memory; else they leave parts in the workspace for a second launch.
 //
 // What bounds it (B200): the issue of its instructions, 365 per 16 keys and warp at 128 columns and 4 bits, about half of them the conversion of the codes.
 // 64 sequences of 2000 to 10520 keys, 16 heads x 128, 4 bits: 239 us, 3.9 TB/s, DRAM 47 % busy (its bytes alone take 142 us).  One sequence of 1000 keys, 8 heads: 8 us, a chain
@@ -30,7 +32,6 @@ namespace varq {
 namespace {
 
 constexpr int PD_WARPS = 4, PD_KEYS = 16;
-constexpr float PD_LAZY = 8.f;
 
 __device__ __forceinline__ void pd_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -266,7 +267,7 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
                         if (!(key < col_hi[t][e] && (key >= col_lo[t][e] || key < a.sinks))) x = -INFINITY;
                     }
                     s[t][2 * r + e] = x;
-                    over = over | (x > m[t][e] + PD_LAZY);
+                    over = over | (x > m[t][e] + PAGED_TOP);
                 }
         if (__any_sync(0xffffffffu, over)) {
             // rare after the first tile: new references, the same in every lane of a row, and everything accumulated is rescaled
@@ -277,7 +278,7 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
                     float x = fmaxf(s[t][e], s[t][2 + e]);
 #pragma unroll
                     for (int z = 4; z < 32; z <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, z));
-                    const float mn = fmaxf(m[t][e], x), alpha = pd_ex2(m[t][e] - mn);
+                    const float mn = fmaxf(m[t][e], x - PAGED_SET), alpha = pd_ex2(m[t][e] - mn);
                     m[t][e] = mn;
                     l[t][e] *= alpha;
 #pragma unroll

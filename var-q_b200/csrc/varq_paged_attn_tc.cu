@@ -7,11 +7,14 @@
 //   x = S a_j + b_j with a_j = K scale * softmax_scale * log2 e and b_j = log2 of the V scale
 //   P = 2^(x - m)   fp16, written over S in tensor memory, = weight * V scale relative to the row's reference m
 //   l += P / V scale in fp32, from the unrounded P;      O += P V, V integer codes as exact fp16, O fp32 in tensor memory
-// and at the end out = O / l, log-sum-exp = (m + log2 l) ln 2.  P is the operand of a 16-bit product: its rounding (2^-11 relative, of each weight by itself) is
-// the only one to fewer than 32 bits; the codes are exact in fp16.  The reference m is that of weight times V scale, which is what bounds O.  It is raised only
-// when an x passes it by more than 8 (P then stays below 2^8, far from fp16's end): the tile's scores are then taken again against the new one, O and l
-// rescaled.  fp16 queries are exact, and so are bf16 queries of usual size; a row whose largest element lies outside [2^-4, 2^15) is scaled by a power of two
-// (then S a_j takes a factor).
+// and at the end out = O / l, log-sum-exp = (m + log2 l) ln 2.  The reference m is that of weight times V scale, which is what bounds O: it is set 7 below a row's first
+// largest x, rounded up, and raised, again to 6 or 7 below, only when an x passes it by more than 15 (P then stays below 2^15, fp16 ends at 2^16).  The tile's scores are
+// then taken again against the new one, O, l and the weights of the tile's first half rescaled by a power of two, in fp32.
+// What is held in fewer than 32 bits: P, because it is the operand of a 16-bit product.  A weight times V scale of 2^-20 of the row's largest or more is rounded by
+// itself, 2^-12 of it; a smaller one by 2^-31 of the largest.  (Where one V row is far larger than the others, the others' part in the columns in which its codes are
+// zero is off by as much of *its* size.)  A weight that raising makes subnormal is rounded a second time.  Codes are exact in fp16, and so are fp16 queries; bf16 queries
+// too, but for elements below 2^-13 of their row's largest, which are off by 2^-21 of it at most: a row whose largest element lies outside [2^-4, 2^15) is scaled by a
+// power of two (then S a_j takes a factor).
 //
 // Warps: 0-3 and 4-7 softmax of the two query tiles; 8-11 and 12-15 convert K and V: packed rows from shared memory to 128B-swizzled fp16 tiles, scales to the
 // tables a, b, 1 / V scale; 16 and 17 issue the products of the two query tiles; 18 and 19 fetch packed rows and scales of K and V with a bulk copy for every
@@ -36,7 +39,6 @@ namespace varq {
 namespace {
 
 constexpr int PT_M = 128, PT_N = 64;
-constexpr float PT_LAZY = 8.f;                      // a weight relative to its row's reference stays below 2^PT_LAZY
 
 template <int D> struct PtPlan {
     static constexpr int SB = D == 64 ? 3 : 2;                     // score tiles per query tile
@@ -328,7 +330,7 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                         for (int i = 0; i < 16; ++i) top[i & 3] = fmaxf(top[i & 3], fmaxf(pair_x(x[i]), pair_y(x[i])));
-                        return __any_sync(0xffffffffu, unset != 0u || fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > PT_LAZY) != 0;
+                        return __any_sync(0xffffffffu, unset != 0u || fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > PAGED_TOP) != 0;
                     };
                     // new references from the scores of chunk c, whose predecessors are done; the chunk's scores are then computed once more (changed in place they
                     // would be copied on the way that is always taken)
@@ -343,7 +345,7 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                             up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 2));
                             const bool first = (unset >> i & 1u) && up > -INFINITY;
                             // by a whole number: the factor is a power of two, which rounds nothing but weights that become subnormal
-                            up = first ? up : up > PT_LAZY && !(unset >> i & 1u) ? ceilf(up) : 0.f;
+                            up = first || (up > PAGED_TOP && !(unset >> i & 1u)) ? ceilf(up - PAGED_SET) : 0.f;
                             alpha[i] = first ? 1.f : ex2(-up);           // (nothing is accumulated where the reference is the first)
                             if (first) unset &= ~(1u << i);
                             nm[i] = add2(nm[i], pair_of(-up, -up));

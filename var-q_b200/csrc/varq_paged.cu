@@ -309,15 +309,16 @@ __device__ int g_paged_status = 0;
 
 }  // namespace
 
-int* paged_status_word() {
+int paged_status_word(int** out) {
     static int* known[64] = {nullptr};                       // per device; the address of a variable of the module does not change
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
-    if (dev >= 0 && dev < 64 && known[dev]) return known[dev];
+    VARQ_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev >= 0 && dev < 64 && known[dev]) { *out = known[dev]; return VARQ_OK; }
     void* p = nullptr;
-    if (cudaGetSymbolAddress(&p, g_paged_status) != cudaSuccess) return nullptr;
-    if (dev >= 0 && dev < 64) known[dev] = reinterpret_cast<int*>(p);
-    return reinterpret_cast<int*>(p);
+    VARQ_CUDA_TRY(cudaGetSymbolAddress(&p, g_paged_status));
+    *out = reinterpret_cast<int*>(p);
+    if (dev >= 0 && dev < 64) known[dev] = *out;
+    return VARQ_OK;
 }
 int paged_status(int* out) {
     if (int rc = paged_attn_tc_status(out)) return rc;
@@ -477,6 +478,8 @@ extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch
         return fail(VARQ_ERR_WORKSPACE, "varq_paged_attn: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
     float *ws_o = reinterpret_cast<float*>(workspace), *ws_ml = ws_o + (size_t)p.splits * a.T * a.Hq * a.c.D;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (int rc = p.tc ? paged_attn_tc_run(a, p.splits, ws_o, ws_ml, st) : paged_attn_decode_run(a, p.rows, p.splits, p.cluster, p.tiles_per_split, ws_o, ws_ml, st)) return rc;
+    int* status = nullptr;
+    if (int rc = paged_status_word(&status)) return rc;      // the kernels write to it: no launch without it
+    if (int rc = p.tc ? paged_attn_tc_run(a, p.splits, ws_o, ws_ml, status, st) : paged_attn_decode_run(a, p.rows, p.splits, p.cluster, p.tiles_per_split, ws_o, ws_ml, status, st)) return rc;
     return need ? paged_attn_merge_run(a, p.splits, ws_o, ws_ml, st) : VARQ_OK;
 }

@@ -40,7 +40,7 @@ constexpr int PAGED_MOST_KEYS = 0x7fffffff - 4095;      // tokens of a sequence:
 // First thing that was wrong with numbers that only the device sees (lengths, starts, page numbers): the access is clamped into the
 // tensors' bounds and the code is kept for varq_device_status.
 enum PagedStatus : int { PAGED_BAD_STARTS = 64, PAGED_BAD_LENGTH = 65, PAGED_BAD_PAGE = 66 };
-int* paged_status_word();              // its device address; null if it cannot be had
+int paged_status_word(int** out);      // its device address
 int paged_status(int* out);            // its value where *out is 0; clears it
 
 // Sequence b: its first query token, number of queries, tokens in the cache, query token behind its last one
@@ -115,9 +115,9 @@ constexpr float PAGED_SET = 7.f, PAGED_TOP = 15.f;
 
 constexpr int PAGED_CLUSTER = 8;       // up to so many parts of the decode kernel can meet in a cluster, without a workspace
 // Parts of the key range (splits) leave numerators ws_o [split][query row][D] and (reference, sum) ws_ml [split][query row][2]; a second launch merges them
-int paged_attn_tc_run(const PagedAttnArgs& a, int splits, float* ws_o, float* ws_ml, cudaStream_t st);
+int paged_attn_tc_run(const PagedAttnArgs& a, int splits, float* ws_o, float* ws_ml, int* status, cudaStream_t st);
 // rows: query rows of a CTA, 8, 16 or 24
-int paged_attn_decode_run(const PagedAttnArgs& a, int rows, int splits, bool in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st);
+int paged_attn_decode_run(const PagedAttnArgs& a, int rows, int splits, bool in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, int* status, cudaStream_t st);
 int paged_attn_merge_run(const PagedAttnArgs& a, int splits, const float* ws_o, const float* ws_ml, cudaStream_t st);
 int paged_attn_tc_status(int* out);
 int forced_attn_path();                // varq_attn_force_path

@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(128) paged_attn_merge_kernel(PagedAttnArgs a, 
 }
 
 template <int KB, int VB, int D, int NT>
-int launch_nt(const PagedAttnArgs& a, int splits, bool in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st) {
+int launch_nt(const PagedAttnArgs& a, int splits, bool in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, int* status, cudaStream_t st) {
     constexpr int PART = (PD_WARPS + 1) * 8 * NT * (D + 2) * 4, SMEM = PdPlan<KB, VB, D>::SMEM > PART ? PdPlan<KB, VB, D>::SMEM : PART;
     const long long rows = (long long)a.max_q * a.G;
     const int n_rowtiles = (int)((rows + 8 * NT - 1) / (8 * NT));
@@ -465,24 +465,24 @@ int launch_nt(const PagedAttnArgs& a, int splits, bool in_cluster, int tiles_per
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
     VARQ_CUDA_TRY(launch_pdl(paged_attn_decode_kernel<KB, VB, D, NT>, (unsigned)blocks, PD_WARPS * 32, SMEM, st, in_cluster ? splits : 1, a, n_rowtiles, splits, in_cluster, tiles_per_split, ws_o, ws_ml,
-                             paged_status_word()));
+                             status));
     count_launches(1);
     return VARQ_OK;
 }
 template <int KB, int VB, int D>
-int launch(const PagedAttnArgs& a, int rows, int splits, bool in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st) {
+int launch(const PagedAttnArgs& a, int rows, int splits, bool in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, int* status, cudaStream_t st) {
     switch (rows) {
-        case 8: return launch_nt<KB, VB, D, 1>(a, splits, in_cluster, tiles_per_split, ws_o, ws_ml, st);
-        case 16: return launch_nt<KB, VB, D, 2>(a, splits, in_cluster, tiles_per_split, ws_o, ws_ml, st);
-        default: return launch_nt<KB, VB, D, 3>(a, splits, in_cluster, tiles_per_split, ws_o, ws_ml, st);
+        case 8: return launch_nt<KB, VB, D, 1>(a, splits, in_cluster, tiles_per_split, ws_o, ws_ml, status, st);
+        case 16: return launch_nt<KB, VB, D, 2>(a, splits, in_cluster, tiles_per_split, ws_o, ws_ml, status, st);
+        default: return launch_nt<KB, VB, D, 3>(a, splits, in_cluster, tiles_per_split, ws_o, ws_ml, status, st);
     }
 }
 
 }  // namespace
 
-int paged_attn_decode_run(const PagedAttnArgs& a, int rows, int splits, bool in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, cudaStream_t st) {
+int paged_attn_decode_run(const PagedAttnArgs& a, int rows, int splits, bool in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, int* status, cudaStream_t st) {
 #define GO(K_, V_) \
-    if (a.c.kb == K_ && a.c.vb == V_) return a.c.D == 64 ? launch<K_, V_, 64>(a, rows, splits, in_cluster, tiles_per_split, ws_o, ws_ml, st) : launch<K_, V_, 128>(a, rows, splits, in_cluster, tiles_per_split, ws_o, ws_ml, st);
+    if (a.c.kb == K_ && a.c.vb == V_) return a.c.D == 64 ? launch<K_, V_, 64>(a, rows, splits, in_cluster, tiles_per_split, ws_o, ws_ml, status, st) : launch<K_, V_, 128>(a, rows, splits, in_cluster, tiles_per_split, ws_o, ws_ml, status, st);
     GO(8, 8) GO(8, 4) GO(8, 2) GO(4, 8) GO(4, 4) GO(4, 2) GO(2, 8) GO(2, 4) GO(2, 2)
 #undef GO
     return fail(VARQ_ERR_ARG, "varq_paged_attn: bits must be 2, 4 or 8");

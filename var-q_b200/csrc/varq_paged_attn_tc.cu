@@ -620,7 +620,7 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
     }
 }
 
-template <int D> int launch_tc(const PagedAttnArgs& a, int n_qblocks, int splits, float* ws_o, float* ws_ml, cudaStream_t st) {
+template <int D> int launch_tc(const PagedAttnArgs& a, int n_qblocks, int splits, float* ws_o, float* ws_ml, int* status, cudaStream_t st) {
     using P = PtPlan<D>;
     static bool configured[64] = {false};
     int dev = 0;
@@ -631,16 +631,16 @@ template <int D> int launch_tc(const PagedAttnArgs& a, int n_qblocks, int splits
     }
     const long long blocks = (long long)a.B * a.c.H * n_qblocks * splits;
     if (blocks > 0x7fffffffLL) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_attn: more than 2^31 thread blocks");
-    VARQ_CUDA_TRY(launch_pdl(paged_attn_tc_kernel<D>, (unsigned)blocks, P::THREADS, P::SMEM, st, 1, a, n_qblocks, splits, ws_o, ws_ml, paged_status_word()));
+    VARQ_CUDA_TRY(launch_pdl(paged_attn_tc_kernel<D>, (unsigned)blocks, P::THREADS, P::SMEM, st, 1, a, n_qblocks, splits, ws_o, ws_ml, status));
     count_launches(1);
     return VARQ_OK;
 }
 
 }  // namespace
 
-int paged_attn_tc_run(const PagedAttnArgs& a, int splits, float* ws_o, float* ws_ml, cudaStream_t st) {
+int paged_attn_tc_run(const PagedAttnArgs& a, int splits, float* ws_o, float* ws_ml, int* status, cudaStream_t st) {
     const int n_qblocks = (int)(((long long)a.max_q * a.G + 2 * PT_M - 1) / (2 * PT_M));
-    return a.c.D == 64 ? launch_tc<64>(a, n_qblocks, splits, ws_o, ws_ml, st) : launch_tc<128>(a, n_qblocks, splits, ws_o, ws_ml, st);
+    return a.c.D == 64 ? launch_tc<64>(a, n_qblocks, splits, ws_o, ws_ml, status, st) : launch_tc<128>(a, n_qblocks, splits, ws_o, ws_ml, status, st);
 }
 int paged_attn_tc_status(int* out) { return tc_file_status(out); }
 

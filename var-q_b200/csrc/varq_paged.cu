@@ -458,6 +458,8 @@ extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch
     if (!(batch->softmax_scale > 0.f && batch->softmax_scale < 1e30f)) return fail(VARQ_ERR_ARG, "varq_paged_attn: softmax_scale must be positive and finite");
     if (batch->n_seqs > 65535) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_attn: %d sequences (65535 at most)", batch->n_seqs);
     if (batch->n_queries >= (1ll << 31)) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_attn: 2^31 query tokens or more");
+    if ((batch->max_q < batch->n_queries ? batch->max_q : batch->n_queries) * (batch->q_heads / a.c.H) >= 0x7fffffffLL - 511)
+        return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_attn: %d queries of a sequence, %d query heads over %d: 2^31 - 512 query rows of a head or more", batch->max_q, batch->q_heads, a.c.H);
     if (batch->n_queries == 0 || batch->n_seqs == 0 || batch->max_q == 0) return VARQ_OK;
     if (!q->ptr || !out->ptr || !batch->q_starts || !batch->kv_lens || (batch->table_pages && !batch->block_table)) return fail(VARQ_ERR_ARG, "varq_paged_attn: null pointer");
     if (((uintptr_t)q->ptr | (uintptr_t)out->ptr) % 2 || ((uintptr_t)batch->q_starts | (uintptr_t)batch->kv_lens | (uintptr_t)batch->block_table | (uintptr_t)lse) % 4)

@@ -124,11 +124,15 @@ class StandInDecoder(torch.nn.Module):
     @torch.inference_mode()
     def step(self, seqs: Sequence, xs: Sequence[torch.Tensor]) -> Sequence[torch.Tensor]:
         """``xs[i]`` ``[n_i, width]``: the next inputs of ``seqs[i]`` (new sequences are taken in).  Returns their hidden states."""
-        for s in seqs:
-            if s not in self.table:
-                self.table.add(s)
-        counts = [x.size(0) for x in xs]
-        slots = self.table.extend(seqs, counts, self.device_)
+        new, counts = [s for s in dict.fromkeys(seqs) if s not in self.table], [x.size(0) for x in xs]
+        for s in new:
+            self.table.add(s)
+        try:
+            slots = self.table.extend(seqs, counts, self.device_)
+        except Exception:
+            for s in new:
+                self.table.remove(s)
+            raise
         batch = self.table.batch(seqs, counts, self.device_)
         x = torch.cat(list(xs))
         for b in self.blocks:

@@ -74,3 +74,19 @@ def test_one_loud_key_over_a_long_context(at, D, vb, n, dtype):
     score, gain = torch.rand(n, generator=g) * 2 - 1, torch.full((n,), 1.0)
     score[at], gain[at] = 13 * ln2, 2.0 ** 13
     check(case(score, gain, D, vb, seed=at), 2, dtype, D, max_kv=1)
+
+
+@pytest.mark.parametrize("at", [0, 5, 31, 32, 63, 64, 100, 199])
+@pytest.mark.parametrize("D,vb", [(64, 8), (128, 8), (64, 4)])
+def test_a_key_that_is_nearly_everything_comes_out_as_it_is(at, D, vb):
+    """its weight is held exactly, so that only the output's own rounding is left (and e^-25 of the others, 2^-18 for the reciprocals and the exponential in fp32)"""
+    n = 200
+    score, gain = torch.zeros(n), torch.ones(n)
+    score[at] = 25.0
+    b = case(score, gain, D, vb, seed=at)
+    v = torch.rand((1, 1, D), generator=torch.Generator().manual_seed(at + 1)) - 0.5
+    b.cache.append(torch.full((1, 1, D), 25.0, device=DEV), v.to(DEV), b.slots[0][at:at + 1].to(DEV))
+    q = torch.ones((3, 1, D), dtype=torch.float16, device=DEV)
+    out, _ = b.attend(q, [3], 1.0 / D, causal=False)
+    ref = b.cache.read(b.slots[0][at:at + 1].to(DEV))[1].double()
+    assert ((out.double() - ref).abs() <= 2.0 ** -11 * ref.abs() + 2.0 ** -18 * ref.abs() + n * 2.0 ** -36 + 2.0 ** -25).all()

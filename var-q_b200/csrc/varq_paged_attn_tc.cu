@@ -8,11 +8,12 @@
 //   P = 2^(x - m)   fp16, written over S in tensor memory, = weight * V scale relative to the row's reference m
 //   l += P / V scale in fp32, from the unrounded P;      O += P V, V integer codes as exact fp16, O fp32 in tensor memory
 // and at the end out = O / l, log-sum-exp = (m + log2 l) ln 2.  The reference m is that of weight times V scale, which is what bounds O: it is set 7 below a row's first
-// largest x, rounded up, and raised, again to 6 or 7 below, only when an x passes it by more than 15 (P then stays below 2^15, fp16 ends at 2^16).  The tile's scores are
-// then taken again against the new one, O, l and the weights of the tile's first half rescaled by a power of two, in fp32.
-// What is held in fewer than 32 bits: P, because it is the operand of a 16-bit product.  A weight times V scale of 2^-20 of the row's largest or more is rounded by
-// itself, 2^-12 of it; a smaller one by 2^-31 of the largest.  (Where one V row is far larger than the others, the others' part in the columns in which its codes are
-// zero is off by as much of *its* size.)  A weight that raising makes subnormal is rounded a second time.  Codes are exact in fp16, and so are fp16 queries; bf16 queries
+// largest x, and raised, again to 7 below, only when an x passes it by more than 15 (P then stays below 2^15, fp16 ends at 2^16).  The tile's scores are then taken
+// again against the new one, O, l and the weights of the tile's first half rescaled in fp32.
+// What is held in fewer than 32 bits: P, because it is the operand of a 16-bit product.  A weight times V scale of 2^-21 of the row's largest or more is rounded by
+// itself, 2^-12 of it; a smaller one by 2^-32 of the largest.  (Where one V row is far larger than the others, the others' part in the columns in which its codes are
+// zero is off by as much of *its* size.)  Weights of the first half of a tile whose second half raises the
+// reference are rounded twice.  Codes are exact in fp16, and so are fp16 queries; bf16 queries
 // too, but for elements below 2^-13 of their row's largest, which are off by 2^-21 of it at most: a row whose largest element lies outside [2^-4, 2^15) is scaled by a
 // power of two (then S a_j takes a factor).
 //
@@ -344,8 +345,8 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                             up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 1));
                             up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 2));
                             const bool first = (unset >> i & 1u) && up > -INFINITY;
-                            // by a whole number: the factor is a power of two, which rounds nothing but weights that become subnormal
-                            up = first || (up > PAGED_TOP && !(unset >> i & 1u)) ? ceilf(up - PAGED_SET) : 0.f;
+                            // to the largest x itself, which is then a power of two in fp16: where it is most of the sum, so is its exactness
+                            up = first || (up > PAGED_TOP && !(unset >> i & 1u)) ? up - PAGED_SET : 0.f;
                             alpha[i] = first ? 1.f : ex2(-up);           // (nothing is accumulated where the reference is the first)
                             if (first) unset &= ~(1u << i);
                             nm[i] = add2(nm[i], pair_of(-up, -up));

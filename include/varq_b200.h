@@ -294,7 +294,7 @@ int varq_paged_read(const varq_paged_t* cache, const int64_t* slots, int64_t n_t
  *   causal = 0 : every query sees the whole sequence
  *   causal = 1 : a query at position p sees the keys 0 .. p; with window w > 0 the keys p - w + 1 .. p and the first `sinks` keys
  * Rows of q in front of q_starts[0] (which need not be 0) and behind q_starts[n_seqs] belong to no sequence: zeros and -inf, as for a query that
- * sees nothing.  With n_queries, n_seqs or max_q 0 a call writes nothing.  Starts fall nowhere; where they do, or where a sequence has more than max_q
+ * sees nothing.  With n_queries, n_seqs or max_q 0 a call writes nothing.  Starts must not decrease; where they do, or where a sequence has more than max_q
  * queries, code 64 is left and rows in between are not defined.
  * Entries of block_table for pages behind the last token, or for pages in which no query of the sequence sees a key, may hold anything.
  * Query head i uses head i / (q_heads / n_heads) of the cache.  max_q bounds the queries of a sequence, max_kv is the longest kv_lens (a
@@ -310,8 +310,8 @@ typedef struct {
 
 /* out = softmax(q k^T * softmax_scale) v over the pages; q and out (1, n_queries, q_heads, head_dim), fp16 or bf16 (one type).  lse (or
  * NULL): fp32 [n_queries][q_heads], log of the sum of exponentials.  A query that sees no key gets zeros and -inf.
- * What a query does not see does not reach its result, whatever it holds.  Weight times V scale of a key that is 2^-126 of the row's largest, or less, is
- * taken for 0, and the weight with it. */
+ * What a query does not see does not reach its result, whatever it holds.  Weight times V scale of a key that is less than 2^-126 of the row's largest may be
+ * taken for 0, and the weight with it.  Query tokens of a sequence times q_heads / n_heads: below 2^31 - 512. */
 size_t varq_paged_attn_workspace_bytes(const varq_paged_t* cache, const varq_paged_batch_t* batch);
 int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch_t* batch, const varq_tensor_t* q, const varq_tensor_t* out, float* lse,
                     void* workspace, size_t workspace_bytes, void* stream);

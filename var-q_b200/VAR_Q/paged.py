@@ -11,6 +11,8 @@ keeps fixed-size pages, a block table that says which pages hold a sequence, and
 The quantization is the reference's symmetric per-token-per-head mode (VAR_Q/quant.py:92-95, 112-121) with a scale of its own for every
 token and head; 2, 4 or 8 bits, for K and V separately.  ``PageTable`` is the bookkeeping on the host: which pages are free, which
 belong to whom, and the slots of a sequence's next tokens.
+
+Inference only: outputs have no gradient, whether or not the inputs require one.
 """
 from typing import List, Optional, Sequence, Tuple
 

@@ -10,11 +10,11 @@
 // not see it loses nothing.
 // Read: code * scale, converted to the output's type once.
 //
-// What bounds them (B200): a read its bytes, 32768 tokens of 8 heads x 128 from 8-bit codes to 16-bit values 37 us = 5.5 TB/s (the copy rate is 6.5); an append
-// of the same size the issue of its instructions, 48 us.  Both together: 135 us with eight values a lane and a division and its rounding for each, 93 with sixteen
+// What bounds them (B200): a read its bytes, 32768 tokens of 8 heads x 128 from 8-bit codes to 16-bit values 37 us = 5.5 TB/s (the copy rate is 6.5).  An append
+// of the same size takes 48 us, 31 by its bytes, and fills no unit: issue 66 %, logic pipe 62 %, DRAM 43 %, and waiting for a row's loads is its largest stall.  Both together: 135 us with eight values a lane and a division and its rounding for each, 93 with sixteen
 // and the bracket, 85 with Markstein's scale and narrow codes merged by the byte (their bytes alone take 52).  On random values at most one lane in five hundred
 // finds its bracket open and divides (16 values, each within 127 * 2^-20 of a tie).  Short calls are a launch's latency: 8 or 999 tokens, written and read
-// back, 7.9 us for both launches.
+// back, 8.1 us for both launches.
 #include "varq_attn.cuh"
 #include "varq_codes.cuh"
 #include "varq_paged.cuh"

@@ -15,10 +15,11 @@
 // Warps and CTAs (key ranges) are merged by the log-sum-exp rule: where all CTAs are resident at once, up to eight of a row tile are a cluster and read one
 // another's shared memory; else they leave parts in the workspace for a second launch.
 //
-// What bounds it (B200): the issue of its instructions, 365 per 16 keys and warp at 128 columns and 4 bits, about half of them the conversion of the codes.
-// 64 sequences of 2000 to 10520 keys, 16 heads x 128, 4 bits: 239 us, 3.9 TB/s, DRAM 47 % busy (its bytes alone take 142 us).  One sequence of 1000 keys, 8 heads: 8 us, a chain
-// of latencies (launch, lengths, pages, rows, two products, the cluster's merge).  Four tokens over a window of 1024 (20 rows of a head) on 24
-// sequences: 29 us.  With rows straight from the pages into registers, a tile ahead, instead of the ring: 290 us.
+// What bounds it (B200): no unit is full.  64 sequences of 2000 to 10520 keys, 16 heads x 128, 4 bits: 239 us, 3.9 TB/s, DRAM 47 % busy (its bytes alone take 142 us).  Its
+// instructions, 365 per 16 keys and warp, about half of them the conversion of the codes, would fill a scheduler for some 140 us; it issues in 65 % of the cycles
+// in which it has warps: four of them, each a chain of products, exponentials and unpacking.  Lengths that differ and parts cut by the longest leave an SM without warps for
+// another 6 % of the time.  One sequence of 1000 keys, 8 heads: 7.4 us, a chain of latencies (launch, lengths, pages, rows, two products, the cluster's merge).  Four tokens
+// over a window of 1024 (20 rows of a head) on 24 sequences: 31 us.  With rows straight from the pages into registers, a tile ahead, instead of the ring: 290 us.
 #include <cooperative_groups.h>
 
 #include <cfloat>

@@ -25,10 +25,12 @@
 //
 // What bounds it (B200, 1965 MHz): the softmax warps.  At 128 columns and 8-bit codes a tile of 64 keys takes ~2470 cycles of a CTA, of which the exponentials
 // alone are 1024 (8 cycles a warp instruction on each of the four schedulers); the products by themselves take 440 us of the first case, 240 of the second.  Measured:
-//   2048 queries behind 16384 keys, 32 query / 8 cache heads, 128 columns, 8 bits   740 us   790 TFLOP/s (359 us at the dense rate)
-//   16 sequences, 1024 queries on 2240 keys each, 30 heads, 64 columns, 4 bits       638 us   442 TFLOP/s (half the columns: the same exponentials feed half the products)
-//   4096 queries, window 2048, 128 columns                                          120 us   578 TFLOP/s
-// Tiles tried: 128 keys with one score tile each 784 / 721 / 137 us (the softmax waits for its scores); 64 keys, packed rows straight from the pages into the
+//   2048 queries behind 16384 keys, 32 query / 8 cache heads, 128 columns, 8 bits   736 us   794 TFLOP/s (359 us at the dense rate)
+//   16 sequences, 1024 queries on 2240 keys each, 30 heads, 64 columns, 4 bits       640 us   440 TFLOP/s (173 us at the dense rate; the exponentials alone would take 245)
+//   4096 queries, window 2048, 128 columns                                          121 us   573 TFLOP/s
+// No unit is full (first case: issue 49 %, exponentials' unit 42 %, tensor pipe 35 % of 86 that 256 CTAs on 148 SMs can reach): two softmax warps on a scheduler run load,
+// maximum, vote, exponentials and store as a chain.
+// Measured on the way, one step after another, so that the last figure of a line is that of its day.  Tiles tried: 128 keys with one score tile each 784 / 721 / 137 us (the softmax waits for its scores); 64 keys, packed rows straight from the pages into the
 // converters' registers 770 / 680 / 125 us (a converter waits out its loads at the proxy fence, which lets no load pass); bulk copies 740 / 638 / 120 us.
 // Turned down: the first scores of the next tile under the last exponentials of this one, 876 / 687 / 137 us (P comes later, and the products with it); weights
 // first and one vote on them for the whole tile, 716 / 646 / 119 us, but 1 to 2 us more on a call of 14 to 24 us.

@@ -297,6 +297,9 @@ int varq_paged_read(const varq_paged_t* cache, const int64_t* slots, int64_t n_t
  * sees nothing.  With n_queries, n_seqs or max_q 0 a call writes nothing.  Starts must not decrease; where they do, or where a sequence has more than max_q
  * queries, code 64 is left and rows in between are not defined.
  * Entries of block_table for pages behind the last token, or for pages in which no query of the sequence sees a key, may hold anything.
+ *   tree != NULL (causal = 1) : the queries of a sequence are drafted tokens, no chain.  tree is int32 [n_queries][tree_words], 32 * tree_words >= max_q;
+ *                bit i % 32 of word i / 32 of a query's row says whether it sees drafted token i of its sequence (its own bit, too).  It sees the tokens before the
+ *                drafted ones, with a window (>= max_q) as at position kv_lens[b] - n + (bits of its row) - 1.  Zero-initialised: no tree
  * Query head i uses head i / (q_heads / n_heads) of the cache.  max_q bounds the queries of a sequence, max_kv is the longest kv_lens (a
  * hint: it decides how the work is split).
  * A sequence has 2^31 - 4096 tokens at most.  The device checks what the host cannot see: starts, lengths and page numbers outside their bounds are clamped into them and leave a
@@ -306,6 +309,8 @@ typedef struct {
     int64_t table_stride, n_queries;
     int32_t table_pages, n_seqs, q_heads, max_q, max_kv, causal, window, sinks;
     float softmax_scale;
+    int32_t tree_words;
+    const int32_t* tree;
 } varq_paged_batch_t;
 
 /* out = softmax(q k^T * softmax_scale) v over the pages; q and out (1, n_queries, q_heads, head_dim), fp16 or bf16 (one type).  lse (or
@@ -315,6 +320,59 @@ typedef struct {
 size_t varq_paged_attn_workspace_bytes(const varq_paged_t* cache, const varq_paged_batch_t* batch);
 int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch_t* batch, const varq_tensor_t* q, const varq_tensor_t* out, float* lse,
                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- norms and rotary positions
+ * What happens to queries and keys in front of a cache: a norm per head and the rotation by position, in one pass.
+ *   x <- x / max(|x|_2, eps) (L2), x / sqrt(mean x^2 + eps) (RMS) or x;  x <- x * weight[h][d];
+ *   (a, b) <- (a cos t - b sin t, b cos t + a sin t), t = 2 pi * positions[axis of the pair] * turns of the pair
+ * in fp32.  Pair i of rotary_dim / 2 is the elements (2i, 2i + 1) (interleaved) or (i, i + rotary_dim / 2); elements from rotary_dim on are not turned.
+ *   turns : round(2^64 * frequency / (2 pi)), the frequency in radians per position; angles are exact to 2^-32 turns up to positions of 2^33, to position * 2^-65 turns behind
+ *   axis  : which of the n_axes positions a pair goes by; positions[axis * pos_stride_axis + b * pos_stride_b + l * pos_stride_l], int32 or int64
+ *   weights : fp32 at [h * stride_h + d * stride_d] (a stride of 0 shares them), or NULL
+ * (Infinity/infinity/models/basic.py:316-326: cosine attention and two-axis positions in front of the quantizer.) */
+#define VARQ_NORM_NONE 0
+#define VARQ_NORM_L2   1
+#define VARQ_NORM_RMS  2
+typedef struct {
+    const uint64_t* turns;
+    const int32_t* axis;
+    const void* positions;
+    int64_t pos_stride_axis, pos_stride_b, pos_stride_l;
+    const float *q_weight, *k_weight;
+    int64_t q_weight_stride_h, q_weight_stride_d, k_weight_stride_h, k_weight_stride_d;
+    int32_t pos_bytes, n_axes, rotary_dim, interleaved, norm;
+    float eps;
+} varq_rotary_t;
+
+/* q (B, L, q_heads, head_dim) and k (B, L, k_heads, head_dim) of one type -> q_out, k_out of the same type or fp32; outputs do not overlap the
+ * inputs.  head_dim 64 or 128, rotary_dim a multiple of 16. */
+int varq_rotate(const varq_rotary_t* r, const varq_tensor_t* q, const varq_tensor_t* k, int32_t B, int32_t L, int32_t q_heads, int32_t k_heads,
+                int32_t head_dim, const varq_tensor_t* q_out, const varq_tensor_t* k_out, void* stream);
+
+/* The same in front of a paged cache: q (1, n_tokens, q_heads, head_dim) -> q_out of its type; k, after norm and rotation in fp32, and v as it is are
+ * quantized into their slots as by varq_paged_append (slots, eps: there). */
+int varq_paged_append_rotated(const varq_paged_t* cache, const varq_rotary_t* r, const varq_tensor_t* q, const varq_tensor_t* k, const varq_tensor_t* v,
+                              const int64_t* slots, int64_t n_tokens, int32_t q_heads, float eps, const varq_tensor_t* q_out, void* stream);
+
+/* Masks and positions of drafted tokens from their parents, for the tree of a varq_paged_batch_t: token i of the n drafted tokens of sequence b is row
+ * q_starts[b] + i; parents (int32 [n_tokens]) gives the number of its parent in its sequence, smaller than i, or -1 for a child of the context.
+ *   masks     int32 [n_tokens][words], 32 * words >= max_q : bits of the token's ancestors among the drafted tokens and its own
+ *   positions int32 [n_tokens] : kv_lens[b] - n + number of ancestors
+ * Rows that belong to no sequence get zeros.  A parent out of its range counts as -1 and leaves code 67, starts that decrease and more than max_q tokens code 64
+ * for varq_device_status. */
+int varq_paged_tree(const int32_t* parents, const int32_t* kv_lens, const int32_t* q_starts, int32_t n_seqs, int64_t n_tokens, int32_t max_q, int32_t words,
+                    int32_t* masks, int32_t* positions, void* stream);
+
+/* dst_pages[i] of every cache becomes a copy of its src_pages[i] (int64 [n_pages]), codes and scales; a pair with a number outside a cache's pool copies
+ * nothing there.  The dst_pages are all different, and none of them is a src_page. */
+int varq_paged_copy_pages(const varq_paged_t* caches, int32_t n_caches, const int64_t* src_pages, const int64_t* dst_pages, int64_t n_pages, void* stream);
+
+/* The tokens in slots src[i] of every cache go to slots dst[i] (int64 [n_moves]), codes and scales.  Moves starts[g] .. starts[g + 1] - 1 (int32,
+ * n_groups + 1 entries) are a group: one sequence's.  Within a group a dst may be the src of an earlier move, not of a later one (tokens move towards the
+ * front in order); across groups slots differ, and the dst are all different.  A move with a slot outside a cache's pool does nothing there.
+ * max_moves: the longest group (a hint: it decides how the work is split).  Starts that decrease or pass n_moves are clamped and leave code 64 for varq_device_status. */
+int varq_paged_move_tokens(const varq_paged_t* caches, int32_t n_caches, const int64_t* src, const int64_t* dst, int64_t n_moves, const int32_t* starts,
+                           int32_t n_groups, int32_t max_moves, void* stream);
 
 #ifdef __cplusplus
 }

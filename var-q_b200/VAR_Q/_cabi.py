@@ -24,6 +24,7 @@ SYMBOLS = (
     "varq_attn_workspace_bytes", "varq_attn_fwd", "varq_attn_force_path",
     "varq_qk_norm_stats", "varq_quant_pack_prestats", "varq_attn_fwd_qnorm", "varq_append", "varq_append_workspace_bytes",
     "varq_paged_append", "varq_paged_read", "varq_paged_attn", "varq_paged_attn_workspace_bytes",
+    "varq_rotate", "varq_paged_append_rotated", "varq_paged_tree", "varq_paged_copy_pages", "varq_paged_move_tokens",
 )
 
 
@@ -58,7 +59,17 @@ class PagedBatch(ctypes.Structure):
                 ("table_stride", ctypes.c_int64), ("n_queries", ctypes.c_int64),
                 ("table_pages", ctypes.c_int32), ("n_seqs", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("max_q", ctypes.c_int32),
                 ("max_kv", ctypes.c_int32), ("causal", ctypes.c_int32), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32),
-                ("softmax_scale", ctypes.c_float)]
+                ("softmax_scale", ctypes.c_float), ("tree_words", ctypes.c_int32), ("tree", ctypes.c_void_p)]
+
+
+class Rotary(ctypes.Structure):
+    _fields_ = [("turns", ctypes.c_void_p), ("axis", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+                ("pos_stride_axis", ctypes.c_int64), ("pos_stride_b", ctypes.c_int64), ("pos_stride_l", ctypes.c_int64),
+                ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p),
+                ("q_weight_stride_h", ctypes.c_int64), ("q_weight_stride_d", ctypes.c_int64), ("k_weight_stride_h", ctypes.c_int64),
+                ("k_weight_stride_d", ctypes.c_int64),
+                ("pos_bytes", ctypes.c_int32), ("n_axes", ctypes.c_int32), ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("norm", ctypes.c_int32),
+                ("eps", ctypes.c_float)]
 
 
 _lib = None
@@ -115,6 +126,17 @@ def _declare(lib):
     lib.varq_paged_attn_workspace_bytes.argtypes = [P, B]
     lib.varq_paged_attn.restype = i32
     lib.varq_paged_attn.argtypes = [P, B, T, T, vp, vp, sz, vp]
+    R = ctypes.POINTER(Rotary)
+    lib.varq_rotate.restype = i32
+    lib.varq_rotate.argtypes = [R, T, T, i32, i32, i32, i32, i32, T, T, vp]
+    lib.varq_paged_append_rotated.restype = i32
+    lib.varq_paged_append_rotated.argtypes = [P, R, T, T, T, vp, i64, i32, f32, T, vp]
+    lib.varq_paged_tree.restype = i32
+    lib.varq_paged_tree.argtypes = [vp, vp, vp, i32, i64, i32, i32, vp, vp, vp]
+    lib.varq_paged_copy_pages.restype = i32
+    lib.varq_paged_copy_pages.argtypes = [P, i32, vp, vp, i64, vp]
+    lib.varq_paged_move_tokens.restype = i32
+    lib.varq_paged_move_tokens.argtypes = [P, i32, vp, vp, i64, vp, i32, i32, vp]
     return lib
 
 

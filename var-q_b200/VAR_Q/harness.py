@@ -10,7 +10,7 @@ embedding.  It exists to time the hot path where it runs in practice -- between 
 replayed as one CUDA graph -- not to generate images.
 
 ``StandInDecoder`` is the same for serving: a causal decoder skeleton over paged caches, whose sequences come, are prefilled chunk by chunk next to
-others that decode token by token, and go.
+others that decode token by token, have drafted tokens checked, are forked, and go.
 """
 import math
 from typing import Optional, Sequence
@@ -18,7 +18,8 @@ from typing import Optional, Sequence
 import torch
 
 from .hooks import install
-from .paged import PagedCache, PageTable
+from .paged import PagedCache, PageTable, copy_pages, draft_tree, move_tokens
+from .rotary import Rotary
 
 
 class StandInSelfAttention(torch.nn.Module):
@@ -93,37 +94,48 @@ class StandInVAR(torch.nn.Module):
 
 
 class StandInDecoderBlock(torch.nn.Module):
-    def __init__(self, width: int, heads: int, kv_heads: int, head_dim: int, cache: PagedCache, window: Optional[int], sinks: int):
+    def __init__(self, width: int, heads: int, kv_heads: int, head_dim: int, cache: PagedCache, window: Optional[int], sinks: int, rotary: Optional[Rotary],
+                 qk_norm: Optional[str]):
         super().__init__()
         self.heads, self.kv_heads, self.head_dim, self.cache, self.window, self.sinks = heads, kv_heads, head_dim, cache, window, sinks
+        self.rotary, self.qk_norm = rotary, qk_norm
         self.ln1, self.ln2 = torch.nn.LayerNorm(width), torch.nn.LayerNorm(width)
         self.qkv = torch.nn.Linear(width, (heads + 2 * kv_heads) * head_dim, bias=False)
         self.proj = torch.nn.Linear(heads * head_dim, width, bias=False)
         self.fc1, self.fc2 = torch.nn.Linear(width, 4 * width), torch.nn.Linear(4 * width, width)
 
-    def forward(self, x, slots, batch):
+    def forward(self, x, slots, batch, positions=None, tree=None):
         # q, k and v stay views of the fused activation: the operators read them with their strides
         q, k, v = self.qkv(self.ln1(x)).unflatten(-1, (-1, self.head_dim)).split((self.heads, self.kv_heads, self.kv_heads), 1)
-        self.cache.append(k, v, slots)
-        out = self.cache.attend(q, *batch, 1.0 / math.sqrt(self.head_dim), window=self.window, sinks=self.sinks)
+        if self.rotary is None:
+            self.cache.append(k, v, slots)
+        else:
+            q = self.cache.append_rotated(q, k, v, slots, self.rotary, positions, norm=self.qk_norm)
+        out = self.cache.attend(q, *batch, 1.0 / math.sqrt(self.head_dim), window=self.window, sinks=self.sinks, tree=tree)
         x = x + self.proj(out.flatten(1))
         return x + self.fc2(torch.nn.functional.gelu(self.fc1(self.ln2(x)), approximate='tanh'))
 
 
 class StandInDecoder(torch.nn.Module):
-    """``step`` advances any mix of sequences by any number of tokens each; one ``PageTable`` serves all layers, each of which has a cache of its own."""
+    """``step`` advances any mix of sequences by any number of tokens each; one ``PageTable`` serves all layers, each of which has a cache of its own.
+    ``verify`` and ``accept`` are a round of speculative decoding, ``fork`` one of a search over beams or samples.  ``rotary`` (one axis) gives queries and keys
+    positions, behind ``qk_norm`` (None, "l2" or "rms")."""
 
     def __init__(self, depth: int = 4, width: int = 1024, heads: int = 16, kv_heads: int = 4, head_dim: int = 64, num_pages: int = 256, page_size: int = 64,
-                 k_bits: int = 8, v_bits: int = 8, window: Optional[int] = None, sinks: int = 0, device="cuda"):
+                 k_bits: int = 8, v_bits: int = 8, window: Optional[int] = None, sinks: int = 0, device="cuda", rotary: Optional[Rotary] = None,
+                 qk_norm: Optional[str] = None):
         super().__init__()
+        if qk_norm is not None and rotary is None:
+            raise ValueError("[VAR-Q]: qk_norm goes with rotary")
+        if rotary is not None and rotary.n_axes != 1:
+            raise ValueError(f"[VAR-Q]: the decoder's tokens have one axis of positions, not {rotary.n_axes}")
         self.table, self.device_ = PageTable(num_pages, page_size), device
-        caches = [PagedCache(num_pages, page_size, kv_heads, head_dim, k_bits, v_bits, device) for _ in range(depth)]
-        self.blocks = torch.nn.ModuleList(StandInDecoderBlock(width, heads, kv_heads, head_dim, c, window, sinks) for c in caches)
+        self.caches = [PagedCache(num_pages, page_size, kv_heads, head_dim, k_bits, v_bits, device) for _ in range(depth)]
+        self.rotary = rotary
+        self.blocks = torch.nn.ModuleList(StandInDecoderBlock(width, heads, kv_heads, head_dim, c, window, sinks, rotary, qk_norm) for c in self.caches)
         self.to(device)
 
-    @torch.inference_mode()
-    def step(self, seqs: Sequence, xs: Sequence[torch.Tensor]) -> Sequence[torch.Tensor]:
-        """``xs[i]`` ``[n_i, width]``: the next inputs of ``seqs[i]`` (new sequences are taken in).  Returns their hidden states."""
+    def _run(self, seqs, xs, parents):
         new, counts = [s for s in dict.fromkeys(seqs) if s not in self.table], [x.size(0) for x in xs]
         for s in new:
             self.table.add(s)
@@ -134,10 +146,44 @@ class StandInDecoder(torch.nn.Module):
                 self.table.remove(s)
             raise
         batch = self.table.batch(seqs, counts, self.device_)
+        tree = positions = None
+        if parents is not None:
+            _, kv_lens, q_starts, max_q, _ = batch
+            tree, positions = draft_tree(parents, kv_lens, q_starts, max_q)
+        elif self.rotary is not None:
+            positions = self.table.positions(seqs, counts, self.device_)
         x = torch.cat(list(xs))
         for b in self.blocks:
-            x = b(x, slots, batch)
+            x = b(x, slots, batch, positions, tree)
         return x.split(counts)
+
+    @torch.inference_mode()
+    def step(self, seqs: Sequence, xs: Sequence[torch.Tensor]) -> Sequence[torch.Tensor]:
+        """``xs[i]`` ``[n_i, width]``: the next inputs of ``seqs[i]`` (new sequences are taken in).  Returns their hidden states."""
+        return self._run(seqs, xs, None)
+
+    @torch.inference_mode()
+    def verify(self, seqs: Sequence, xs: Sequence[torch.Tensor], parents: Sequence[Sequence[int]]) -> Sequence[torch.Tensor]:
+        """``step`` on drafted tokens: ``xs[i]`` are the inputs of a tree behind ``seqs[i]``, ``parents[i]`` the numbers of their parents in it (-1: the sequence's
+        last token).  They stay in the cache until ``accept`` says which of them are the sequence's next ones."""
+        if len(parents) != len(xs) or any(len(p) != x.size(0) or any(not -1 <= a < i for i, a in enumerate(p)) for p, x in zip(parents, xs)):
+            raise ValueError("[VAR-Q]: a parent per drafted token, -1 or the number of an earlier one")
+        return self._run(seqs, xs, torch.tensor([a for p in parents for a in p], dtype=torch.int32, device=self.device_))
+
+    @torch.inference_mode()
+    def accept(self, seqs: Sequence, counts: Sequence[int], kept: Sequence[Sequence[int]]) -> None:
+        """Of the ``counts[i]`` drafted tokens of ``seqs[i]`` those with the numbers ``kept[i]`` (a path of the tree) stay."""
+        move_tokens(self.caches, *self.table.accept(seqs, counts, kept, self.device_))
+
+    @torch.inference_mode()
+    def fork(self, seqs: Sequence, children: Sequence) -> None:
+        """Sequences ``children[i]`` that go on from where ``seqs[i]`` is now."""
+        copy_pages(self.caches, *self.table.fork(seqs, children, self.device_))
+
+    @torch.inference_mode()
+    def compact(self) -> None:
+        """All sequences into the first pages of the pools."""
+        copy_pages(self.caches, *self.table.compact(self.device_))
 
     def finish(self, seq) -> None:
         self.table.remove(seq)

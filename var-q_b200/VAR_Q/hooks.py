@@ -23,6 +23,7 @@ import torch
 from . import _cabi
 from .attention import attend, attend_cached
 from .quant import VAR_Q, _host
+from .rotary import Rotary
 
 
 class LayerKV:
@@ -152,6 +153,22 @@ def _step_normalised(self, q, k, v, scale_mul, softmax_scale, out_dtype=None):
 
 
 LayerKV.step_normalised = _step_normalised
+
+
+def _step_rotated(self, q, k, v, rotary: Rotary, positions, softmax_scale, out_dtype=None, norm='l2', q_weight=None, k_weight=None, eps=None):
+    """``LayerKV.step`` behind the norms and the rotation by position of q and k, as Infinity has them (cosine attention and two-axis positions,
+    Infinity/infinity/models/basic.py:316-326): one kernel for both, which leaves them in fp32 as the reference does, in front of quantize, append and attention.
+    ``positions``, ``norm`` and the weights as in ``Rotary.rotate``; ``q_weight`` ``[heads, 1]`` holds the learnt factor of each head."""
+    bhlc = self.k_quant.qkv_format != 'BLHc'
+    if bhlc:
+        q, k = q.transpose(1, 2), k.transpose(1, 2)
+    q, k = rotary.rotate(q, k, positions, norm=norm, q_weight=q_weight, k_weight=k_weight, eps=eps, dtype=torch.float32)
+    if bhlc:
+        q, k = q.transpose(1, 2), k.transpose(1, 2)
+    return self.step(q, k, v, softmax_scale, out_dtype)
+
+
+LayerKV.step_rotated = _step_rotated
 
 
 def install(attn: torch.nn.Module, max_tokens: Optional[int] = None, k_kwargs=None, v_kwargs=None) -> torch.nn.Module:

@@ -18,7 +18,7 @@
 #include "varq_attn.cuh"
 #include "varq_codes.cuh"
 #include "varq_paged.cuh"
-#include "varq_quant.cuh"
+#include "varq_paged_rows.cuh"
 
 namespace varq {
 namespace {
@@ -43,24 +43,6 @@ struct ReadArgs {
 
 constexpr int ROW_THREADS = 256;
 
-// codes of eight values (fp32 with the code in the low mantissa bits) as piece `ch` of a row: 64, 32 or 16 bits
-__device__ __forceinline__ void store_codes(int32_t* row, int ch, int bits, const uint32_t (&q)[8]) {
-    uint32_t w[2];                     // a byte each
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-        w[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040), 0x5410);
-    if (bits == 8) {
-        reinterpret_cast<uint2*>(row)[ch] = make_uint2(w[0], w[1]);
-    } else if (bits == 4) {            // two in a byte: in bytes 0 and 2
-#pragma unroll
-        for (int i = 0; i < 2; ++i) { w[i] &= 0x0f0f0f0fu; w[i] |= w[i] >> 4; }
-        row[ch] = (int32_t)__byte_perm(w[0], w[1], 0x6420);
-    } else {                           // four in a byte: in byte 0
-#pragma unroll
-        for (int i = 0; i < 2; ++i) { w[i] &= 0x03030303u; w[i] |= w[i] >> 6; w[i] |= w[i] >> 12; }
-        reinterpret_cast<unsigned short*>(row)[ch] = (unsigned short)__byte_perm(w[0], w[1], 0x0040);
-    }
-}
 __device__ __forceinline__ void load_codes(const int32_t* row, int ch, int bits, uint32_t (&w)[2]) {
     if (bits == 8) {
         const uint2 x = __ldg(reinterpret_cast<const uint2*>(row) + ch);
@@ -92,47 +74,6 @@ __device__ __forceinline__ void codes_to_float(const uint32_t (&w)[2], int bits,
     }
 }
 
-// eight consecutive values of a row, packed as they come, and their largest absolute value as bits (order of the absolute values, NaN above infinity)
-template <typename T, bool VEC> struct Piece {
-    Vec8<T> r;
-    __device__ __forceinline__ void load(const T* p) {
-        if constexpr (VEC) r.load(p);
-        else {
-            T e[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = p[i];
-            if constexpr (sizeof(T) == 4) { r.a = make_float4(e[0], e[1], e[2], e[3]); r.b = make_float4(e[4], e[5], e[6], e[7]); }
-            else r.r = *reinterpret_cast<const uint4*>(e);
-        }
-    }
-    __device__ __forceinline__ uint32_t top() const {       // 16-bit types: of the even and the odd values, side by side
-        if constexpr (sizeof(T) == 4) {
-            float v[8];
-            r.get(v);
-            uint32_t m = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-            return m;
-        } else {
-            return __vmaxu2(__vmaxu2(r.r.x & 0x7fff7fffu, r.r.y & 0x7fff7fffu), __vmaxu2(r.r.z & 0x7fff7fffu, r.r.w & 0x7fff7fffu));
-        }
-    }
-};
-template <typename T> __device__ __forceinline__ uint32_t merge_top(uint32_t a, uint32_t b) { return sizeof(T) == 4 ? max(a, b) : __vmaxu2(a, b); }
-template <typename T> __device__ __forceinline__ float top_value(uint32_t m) {                 // the value itself
-    if constexpr (sizeof(T) == 4) return __uint_as_float(m);
-    else {
-        const unsigned short b = (unsigned short)max(m & 0xffffu, m >> 16);
-        return to_f32<T>(*reinterpret_cast<const T*>(&b));
-    }
-}
-__device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-
 template <typename T, int D, int U, bool VEC>
 __global__ void __launch_bounds__(ROW_THREADS) paged_append_kernel(AppendArgs a) {
     constexpr int LPR = D / 16, RPB = ROW_THREADS / LPR;
@@ -146,7 +87,7 @@ __global__ void __launch_bounds__(ROW_THREADS) paged_append_kernel(AppendArgs a)
     int32_t* pool = is_v ? a.c.vc : a.c.kc;
     float* scales = is_v ? a.c.vs : a.c.ks;
     const long long n_slots = (long long)a.c.n_pages << a.c.page_shift;
-    const float most = (float)((1 << (bits - 1)) - 1), inv = bits == 8 ? 1.f / 127.f : bits == 4 ? 1.f / 7.f : 1.f;
+    const float most = paged_most(bits), inv = paged_most_inv(bits);
     const uint32_t row0 = blockIdx.x * (RPB * U) + threadIdx.x / LPR;
     Piece<T, VEC> f[U][2];
     uint32_t at[U];                    // row of the pools
@@ -174,35 +115,17 @@ __global__ void __launch_bounds__(ROW_THREADS) paged_append_kernel(AppendArgs a)
         for (int z = LPR / 2; z; z >>= 1) m = merge_top<T>(m, __shfl_xor_sync(0xffffffffu, m, z));
         if (!there[u]) continue;
         const float top = top_value<T>(m);
-        const bool fine = top <= 3.402823466e38f;
-        const float quot = top * inv, scale = fine ? fmaxf(fmaf(fmaf(-quot, most, top), inv, quot), a.eps) : __uint_as_float(0x7fffffffu);
-        float r;                                             // within 2^-23, as long as it is a normal number
-        asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(scale));
-        const float lo = r * (1.f - 0x1p-21f), hi = r * (1.f + 0x1p-21f);
-        const uint32_t small = scale > 0x1p125f ? 1u : 0u;
+        const PagedRow row(top, most, inv, a.eps);
         int32_t* out = pool + (size_t)at[u] * words;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             float v[8];
-            uint32_t q[8], differ = small;
+            uint32_t q[8];
             f[u][e].r.get(v);
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                const float2 x2 = make_float2(v[i], v[i + 1]), magic = make_float2(Q_MAGIC, Q_MAGIC);
-                const float2 y = fma_pair(x2, make_float2(lo, lo), magic), z = fma_pair(x2, make_float2(hi, hi), magic);
-                q[i] = __float_as_uint(y.x); q[i + 1] = __float_as_uint(y.y);
-                differ |= (q[i] ^ __float_as_uint(z.x)) | (q[i + 1] ^ __float_as_uint(z.y));
-            }
-            if (!fine) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) q[i] = 0u;
-            } else if (differ) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(rintf(__fdiv_rn(v[i], scale)) + Q_MAGIC);
-            }
+            row.codes(v, q);
             store_codes(out, lane + e * LPR, bits, q);
         }
-        if (lane == 0) scales[at[u]] = scale;
+        if (lane == 0) scales[at[u]] = row.scale;
     }
 }
 
@@ -253,11 +176,9 @@ __global__ void __launch_bounds__(ROW_THREADS) paged_read_kernel(ReadArgs a) {
     }
 }
 
-bool rows_aligned16(const void* p, long long st, long long sh, int es) {
-    return aligned16(p) && (st * es) % 16 == 0 && (sh * es) % 16 == 0;
-}
+}  // namespace
 
-int check_cache(const char* who, const varq_paged_t* c, PagedView& v) {
+int paged_check_cache(const char* who, const varq_paged_t* c, PagedView& v) {
     if (!c) return fail(VARQ_ERR_ARG, "%s: null cache", who);
     if (c->n_pages < 1 || c->n_heads < 1) return fail(VARQ_ERR_ARG, "%s: %d pages, %d heads", who, c->n_pages, c->n_heads);
     if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)))
@@ -275,11 +196,13 @@ int check_cache(const char* who, const varq_paged_t* c, PagedView& v) {
     v.H = c->n_heads; v.D = c->head_dim; v.kb = c->k_bits; v.vb = c->v_bits;
     return VARQ_OK;
 }
-int check_rows(const char* who, const PagedView& c, long long n) {
+int paged_check_rows(const char* who, const PagedView& c, long long n) {
     if (n < 0) return fail(VARQ_ERR_ARG, "%s: %lld tokens", who, n);
     if (n * c.H >= 0x7fffffffLL) return fail(VARQ_ERR_UNSUPPORTED, "%s: %lld tokens of %d heads are 2^31 rows or more", who, n, c.H);
     return VARQ_OK;
 }
+
+namespace {
 
 // Rows per thread: two keep more bytes in flight once the call fills every SM four times over, one spreads a shorter call over the SMs.
 // One / two / four rows, 32768 tokens of 8 heads x 128, 8 bits: append of 16-bit values 56.4 / 50.1 / 59.6 us, of fp32 (half the tokens) 32.0 / 33.5 / 48; read
@@ -339,8 +262,8 @@ using namespace varq;
 extern "C" int varq_paged_append(const varq_paged_t* cache, const varq_tensor_t* k, const varq_tensor_t* v, const int64_t* slots, int64_t n_tokens,
                                  float eps, void* stream) {
     AppendArgs a;
-    if (int rc = check_cache("varq_paged_append", cache, a.c)) return rc;
-    if (int rc = check_rows("varq_paged_append", a.c, n_tokens)) return rc;
+    if (int rc = paged_check_cache("varq_paged_append", cache, a.c)) return rc;
+    if (int rc = paged_check_rows("varq_paged_append", a.c, n_tokens)) return rc;
     if (!k || !v) return fail(VARQ_ERR_ARG, "varq_paged_append: null descriptor");
     if (!dtype_ok(k->dtype) || k->dtype != v->dtype) return fail(VARQ_ERR_ARG, "varq_paged_append: K and V must have one type, fp32, fp16 or bf16");
     if (!(eps >= 1e-30f && eps < 1e30f)) return fail(VARQ_ERR_ARG, "varq_paged_append: eps must lie in [1e-30, 1e30)");
@@ -362,8 +285,8 @@ extern "C" int varq_paged_append(const varq_paged_t* cache, const varq_tensor_t*
 extern "C" int varq_paged_read(const varq_paged_t* cache, const int64_t* slots, int64_t n_tokens, const varq_tensor_t* k_out,
                                const varq_tensor_t* v_out, void* stream) {
     ReadArgs a;
-    if (int rc = check_cache("varq_paged_read", cache, a.c)) return rc;
-    if (int rc = check_rows("varq_paged_read", a.c, n_tokens)) return rc;
+    if (int rc = paged_check_cache("varq_paged_read", cache, a.c)) return rc;
+    if (int rc = paged_check_rows("varq_paged_read", a.c, n_tokens)) return rc;
     if (!k_out || !v_out) return fail(VARQ_ERR_ARG, "varq_paged_read: null descriptor");
     if (!dtype_ok(k_out->dtype) || k_out->dtype != v_out->dtype) return fail(VARQ_ERR_ARG, "varq_paged_read: K and V must have one type, fp32, fp16 or bf16");
     if (n_tokens == 0) return VARQ_OK;
@@ -445,7 +368,7 @@ extern "C" size_t varq_paged_attn_workspace_bytes(const varq_paged_t* cache, con
 extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch_t* batch, const varq_tensor_t* q, const varq_tensor_t* out, float* lse,
                                void* workspace, size_t workspace_bytes, void* stream) {
     PagedAttnArgs a;
-    if (int rc = check_cache("varq_paged_attn", cache, a.c)) return rc;
+    if (int rc = paged_check_cache("varq_paged_attn", cache, a.c)) return rc;
     if (!batch || !q || !out) return fail(VARQ_ERR_ARG, "varq_paged_attn: null descriptor");
     if (batch->n_seqs < 0 || batch->n_queries < 0 || batch->max_q < 0 || batch->max_kv < 0 || batch->table_pages < 0)
         return fail(VARQ_ERR_ARG, "varq_paged_attn: negative size");
@@ -455,6 +378,13 @@ extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch
     if (batch->window < 0 || batch->sinks < 0) return fail(VARQ_ERR_ARG, "varq_paged_attn: window %d, sinks %d", batch->window, batch->sinks);
     if (batch->window && !batch->causal) return fail(VARQ_ERR_ARG, "varq_paged_attn: a window needs causal attention");
     if (batch->sinks && !batch->window) return fail(VARQ_ERR_ARG, "varq_paged_attn: sinks need a window");
+    if (batch->tree) {
+        if (!batch->causal) return fail(VARQ_ERR_ARG, "varq_paged_attn: a tree needs causal attention");
+        if (batch->tree_words < 0 || batch->tree_words > (1 << 26) || 32ll * batch->tree_words < batch->max_q)
+            return fail(VARQ_ERR_ARG, "varq_paged_attn: %d words of a tree's mask for %d tokens of a sequence", batch->tree_words, batch->max_q);
+        if (batch->window && batch->window < batch->max_q) return fail(VARQ_ERR_ARG, "varq_paged_attn: a window of %d is shorter than trees of %d tokens", batch->window, batch->max_q);
+        if ((uintptr_t)batch->tree % 4) return fail(VARQ_ERR_ARG, "varq_paged_attn: misaligned pointer");
+    }
     if (!(batch->softmax_scale > 0.f && batch->softmax_scale < 1e30f)) return fail(VARQ_ERR_ARG, "varq_paged_attn: softmax_scale must be positive and finite");
     if (batch->n_seqs > 65535) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_attn: %d sequences (65535 at most)", batch->n_seqs);
     if (batch->n_queries >= (1ll << 31)) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_attn: 2^31 query tokens or more");
@@ -474,6 +404,7 @@ extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch
     a.scale_log2 = batch->softmax_scale * 1.4426950408889634f;
     a.causal = batch->causal != 0; a.window = batch->window;
     a.sinks = batch->sinks < PAGED_MOST_KEYS ? batch->sinks : PAGED_MOST_KEYS;      // more tokens than there are: all of them
+    a.tree = batch->tree; a.tree_words = batch->tree ? batch->tree_words : 0;
     const AttnPlan p = plan_attn(cache, batch);
     const size_t need = part_floats(p, cache, batch) * sizeof(float);
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))

@@ -22,6 +22,10 @@ struct PagedView {
     int n_pages, page_shift, H, D, kb, vb;
 };
 
+// host checks that the entry points share: a cache and its view, a number of tokens
+int paged_check_cache(const char* who, const varq_paged_t* c, PagedView& v);
+int paged_check_rows(const char* who, const PagedView& c, long long n);
+
 struct PagedAttnArgs {
     PagedView c;
     const void* q; int dtype; long long qs_t, qs_h;
@@ -33,13 +37,14 @@ struct PagedAttnArgs {
     int max_q, max_kv;
     float scale_log2;                  // softmax_scale * log2(e)
     int causal, window, sinks;         // window 0: none
+    const int32_t* tree; int tree_words;      // [T][tree_words] or null: which drafted tokens a query sees
 };
 
 constexpr int PAGED_MOST_KEYS = 0x7fffffff - 4095;      // tokens of a sequence: the numbers of the keys that a warp asks for next, 32 x 64 of them, stay below 2^31
 
 // First thing that was wrong with numbers that only the device sees (lengths, starts, page numbers): the access is clamped into the
 // tensors' bounds and the code is kept for varq_device_status.
-enum PagedStatus : int { PAGED_BAD_STARTS = 64, PAGED_BAD_LENGTH = 65, PAGED_BAD_PAGE = 66 };
+enum PagedStatus : int { PAGED_BAD_STARTS = 64, PAGED_BAD_LENGTH = 65, PAGED_BAD_PAGE = 66, PAGED_BAD_PARENT = 67 };
 int paged_status_word(int** out);      // its device address
 int paged_status(int* out);            // its value where *out is 0; clears it
 
@@ -71,6 +76,24 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, int p, i
     s.hi = a.causal ? min(p + 1, kv) : kv;
     s.lo = paged_window(a, p);
     return s;
+}
+
+// Drafted tokens.  They are the sequence's queries and its last tokens, positions p_first on in the cache; a query sees those of its row of bits, and the tokens in
+// front of them as at the position behind its other ancestors.
+__device__ __forceinline__ int paged_tree_position(const PagedAttnArgs& a, int token, int p_first, int nq) {
+    const int32_t* row = a.tree + (long long)token * a.tree_words;
+    int n = 0;
+    for (int w = 0; w < a.tree_words; ++w) n += __popc(__ldg(row + w));
+    return p_first + min(n, nq) - 1;
+}
+// bit k: key p_first + rel + k is seen as far as the tree goes; keys in front of p_first are
+__device__ __forceinline__ uint32_t paged_tree_bits(const PagedAttnArgs& a, int token, int rel) {
+    const int32_t* row = a.tree + (long long)token * a.tree_words;
+    auto word = [&](int w) { return w < 0 ? ~0u : w < a.tree_words ? (uint32_t)__ldg(row + w) : 0u; };
+    return __funnelshift_r(word(rel >> 5), word((rel >> 5) + 1), rel & 31);
+}
+__device__ __forceinline__ bool paged_tree_bit(const PagedAttnArgs& a, int token, int rel) {
+    return rel < 0 || (rel < 32 * a.tree_words && (__ldg(a.tree + (long long)token * a.tree_words + (rel >> 5)) >> (rel & 31) & 1));
 }
 
 // Query rows in front of the first sequence's and behind the last one's belong to no sequence.  They get zeros and -inf, as rows that see nothing: from the CTAs of

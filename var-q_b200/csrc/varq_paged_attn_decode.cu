@@ -127,10 +127,11 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
 
     // ---- the 16-key tiles: first tokens, then the window (or everything)
     const int t0 = row0 / a.G, t1 = (min(row0 + ROWS, rows) - 1) / a.G;
-    const int hi = max(a.causal ? min(seq.kv, p_first + t1 + 1) : seq.kv, 0), lo = paged_window(a, p_first + t0) & ~(PD_KEYS - 1);
+    const int hi = max(a.causal && !a.tree ? min(seq.kv, p_first + t1 + 1) : seq.kv, 0), lo = paged_window(a, a.tree ? p_first - 1 : p_first + t0) & ~(PD_KEYS - 1);
     const int ns = min((a.sinks + PD_KEYS - 1) / PD_KEYS, lo / PD_KEYS), n_tiles = hi > 0 && row0 < rows ? ns + (max(hi - lo, 0) + PD_KEYS - 1) / PD_KEYS : 0;
     const int begin = (int)min((long long)split * tiles_per_split, (long long)n_tiles), end = split == splits - 1 ? n_tiles : min(begin + tiles_per_split, n_tiles);
-    const int all_hi = a.causal ? min(p_first + t0 + 1, seq.kv) : seq.kv, all_lo = paged_window(a, p_first + t1);      // what every row sees
+    // what every row sees
+    const int all_hi = a.tree ? p_first : a.causal ? min(p_first + t0 + 1, seq.kv) : seq.kv, all_lo = paged_window(a, p_first + (a.tree ? seq.nq - 1 : t1));
     auto key_of = [&](int i) { return i < ns ? i * PD_KEYS : lo + (i - ns) * PD_KEYS; };
 
     // ---- Q fragments: column g is row t * 8 + g, scaled by a power of two to use fp16's range
@@ -164,7 +165,11 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
         for (int e = 0; e < 2; ++e) {
             const int r2 = row0 + t * 8 + 2 * c + e;
             qfac[t][e] = __shfl_sync(0xffffffffu, fi, (2 * c + e) * 4) * a.scale_log2;
-            const PagedSpan s = paged_span(a, p_first + r2 / a.G, seq.kv);
+            PagedSpan s = paged_span(a, p_first + r2 / a.G, seq.kv);
+            if (a.tree) {
+                s.hi = seq.kv;
+                if (a.window && r2 < rows) s.lo = paged_window(a, paged_tree_position(a, seq.q0 + r2 / a.G, p_first, seq.nq));
+            }
             col_hi[t][e] = r2 < rows ? s.hi : 0; col_lo[t][e] = s.lo;      // a column without a row sees nothing: what it saw would move the references
         }
     }
@@ -266,6 +271,7 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
                     if (MASKED) {
                         const int key = k0 + g + 8 * r;
                         if (!(key < col_hi[t][e] && (key >= col_lo[t][e] || key < a.sinks))) x = -INFINITY;
+                        else if (a.tree && key >= p_first && !paged_tree_bit(a, seq.q0 + (row0 + t * 8 + 2 * c + e) / a.G, key - p_first)) x = -INFINITY;
                     }
                     s[t][2 * r + e] = x;
                     over = over | (x > m[t][e] + PAGED_TOP);

@@ -194,8 +194,9 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
     int n_t[2], tile0 = 0;                                                   // key tiles of the two query tiles
     {
         const int t0 = row0 / a.G, t1 = (min(row0 + 2 * PT_M, rows) - 1) / a.G, t_mid = (min(row0 + PT_M, rows) - 1) / a.G;
-        const int hi = max(a.causal ? min(seq.kv, p_first + t1 + 1) : seq.kv, 0), hi0 = max(a.causal ? min(seq.kv, p_first + t_mid + 1) : seq.kv, 0);
-        tiles.first = paged_window(a, p_first + t0);
+        const bool chain = a.causal && !a.tree;
+        const int hi = max(chain ? min(seq.kv, p_first + t1 + 1) : seq.kv, 0), hi0 = max(chain ? min(seq.kv, p_first + t_mid + 1) : seq.kv, 0);
+        tiles.first = paged_window(a, a.tree ? p_first - 1 : p_first + t0);
         tiles.lo = tiles.first & ~(PT_N - 1);
         tiles.ns = min((a.sinks + PT_N - 1) / PT_N, tiles.lo / PT_N);
         const int n = hi > 0 ? tiles.ns + (max(hi - tiles.lo, 0) + PT_N - 1) / PT_N : 0, n0 = hi0 > 0 ? tiles.ns + (max(hi0 - tiles.lo, 0) + PT_N - 1) / PT_N : 0;
@@ -258,14 +259,17 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
             if (scaled) reinterpret_cast<float*>(smem + P::OFF_QF)[t * PT_M + r] = q_factor;
             __syncwarp();
             // keys between which every row of the query tile sees everything
-            const int tl = min(row0 + t * PT_M + PT_M, rows) - 1, all_hi = a.causal ? p_first + (row0 + t * PT_M) / a.G + 1 : 0x7fffffff,
-                      all_lo = paged_window(a, p_first + tl / a.G);
+            const int tl = min(row0 + t * PT_M + PT_M, rows) - 1, all_hi = a.tree ? p_first : a.causal ? p_first + (row0 + t * PT_M) / a.G + 1 : 0x7fffffff,
+                      all_lo = paged_window(a, p_first + (a.tree ? seq.nq - 1 : tl / a.G));
             // A thread holds, of every eight columns of S, two of the rows g, g + 8, g + 16, g + 24 of its warp's 32 (g = lane / 4): it needs a quarter of
             // the keys' tables and uses an entry for four rows
             const int g = lane >> 2, cq = lane & 3;
             int pos[4];                                                     // positions of the four rows' tokens
 #pragma unroll
-            for (int i = 0; i < 4; ++i) pos[i] = p_first + min(row0 + t * PT_M + quarter * 32 + g + 8 * i, rows - 1) / a.G;
+            for (int i = 0; i < 4; ++i) {
+                const int at = min(row0 + t * PT_M + quarter * 32 + g + 8 * i, rows - 1) / a.G;
+                pos[i] = a.tree ? at : p_first + at;                        // (of a drafted token: which one it is)
+            }
             pair nm[4] = {0ull, 0ull, 0ull, 0ull};                          // minus the reference, twice
             pair l[4] = {0ull, 0ull, 0ull, 0ull};
             unsigned unset = 15u;                                           // rows that have no reference yet: they have seen no key
@@ -318,11 +322,18 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                         if (SPECIAL) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                const PagedSpan sp = paged_span(a, pos[i], seq.kv);
+                                PagedSpan sp = paged_span(a, pos[i], seq.kv);
                                 // bit k: this thread's column 2c + k of the 32 is seen
                                 auto below = [](int k) { return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1u; };
                                 const int c0 = key0 + 32 * c + 2 * cq;
-                                const uint32_t sees = below(sp.hi - c0) & (~below(sp.lo - c0) | below(a.sinks - c0));
+                                uint32_t tree = ~0u;
+                                if (a.tree) {
+                                    const int token = seq.q0 + pos[i];
+                                    sp.hi = seq.kv;
+                                    sp.lo = a.window ? paged_window(a, paged_tree_position(a, token, p_first, seq.nq)) : 0;
+                                    tree = paged_tree_bits(a, token, c0 - p_first);
+                                }
+                                const uint32_t sees = below(sp.hi - c0) & (~below(sp.lo - c0) | below(a.sinks - c0)) & tree;
 #pragma unroll
                                 for (int v = 0; v < 4; ++v) {
                                     pair& y = x[(i >> 1) * 8 + v * 2 + (i & 1)];

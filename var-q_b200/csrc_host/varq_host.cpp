@@ -492,10 +492,10 @@ PyObject* py_paged_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     GUARD_PAGED_END
 }
 // paged_attend(k_codes, v_codes, k_scale, v_scale, head_dim, q, block_table, kv_lens, q_starts, max_q, max_kv, softmax_scale, causal, window or None, sinks,
-//              return_lse) -> out or (out, lse)
+//              return_lse, tree or None) -> out or (out, lse)
 PyObject* py_paged_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     GUARD_BEGIN
-    if (!want(n, 16)) return nullptr;
+    if (!want(n, 17)) return nullptr;
     const at::Tensor* kc;
     const varq_paged_t c = paged_desc(a, kc);
     const at::Tensor &q = on_device(tensor_arg(a[5], "q"), *kc, "q"), &table = on_device(tensor_arg(a[6], "block_table"), *kc, "block_table"),
@@ -508,7 +508,7 @@ PyObject* py_paged_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
          "q_starts must be a contiguous int32 vector with one entry more than kv_lens");
     need(table.dim() == 2 && table.scalar_type() == at::kInt && table.size(0) == lens.size(0) && (table.stride(1) == 1 || table.size(1) < 2) && table.size(1) <= INT32_MAX,
          "block_table must be int32 [sequences, pages] with contiguous rows");
-    varq_paged_batch_t b;
+    varq_paged_batch_t b{};
     b.q_starts = starts.data_ptr<int32_t>(); b.kv_lens = lens.data_ptr<int32_t>(); b.block_table = table.data_ptr<int32_t>();
     b.table_stride = table.stride(0); b.n_queries = q.size(0); b.table_pages = (int)table.size(1);
     need(lens.size(0) <= INT32_MAX, "too many sequences");
@@ -522,6 +522,15 @@ PyObject* py_paged_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     b.causal = causal;
     b.window = a[13] == Py_None ? 0 : (int)int_arg(a[13], 1, INT32_MAX, "window");
     b.sinks = (int)int_arg(a[14], 0, INT32_MAX, "sinks");
+    if (a[16] != Py_None) {
+        const at::Tensor& tree = on_device(tensor_arg(a[16], "tree"), *kc, "tree");
+        need(tree.dim() == 2 && tree.scalar_type() == at::kInt && tree.size(0) == q.size(0) && tree.is_contiguous() && tree.size(1) <= (1 << 26),
+             "tree must be contiguous int32 [tokens, words]");
+        need(tree.size(1) * 32 >= std::min<long long>(b.max_q, q.size(0)), "tree has fewer bits a row than max_q");
+        need(causal, "a tree needs causal attention");
+        if (tree.size(1) == 0) b.max_q = 0;
+        else { b.tree = tree.data_ptr<int32_t>(); b.tree_words = (int)tree.size(1); b.max_q = (int)std::min<long long>(b.max_q, std::max<long long>(q.size(0), 1)); }
+    }
     const c10::DeviceIndex dev = kc->device().index();
     const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, dev));
     const at::Tensor out = empty({q.size(0), q.size(1), q.size(2)}, q.scalar_type(), dev);
@@ -539,6 +548,188 @@ PyObject* py_paged_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int rc = varq_paged_attn(&c, &b, &qd, &od, with_lse ? lse.data_ptr<float>() : nullptr, scratch_ptr(buf), ws, c10::cuda::getCurrentCUDAStream(dev).stream());
     if (rc != VARQ_OK) return raise(rc);
     return with_lse ? make_pair(out, lse) : THPVariable_Wrap(out);
+    GUARD_PAGED_END
+}
+
+// paged_tree(parents, kv_lens, q_starts, max_q) -> (masks, positions)
+PyObject* py_paged_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    GUARD_BEGIN
+    if (!want(n, 4)) return nullptr;
+    const at::Tensor& parents = tensor_arg(a[0], "parents");
+    const at::Tensor &lens = tensor_arg(a[1], "kv_lens"), &starts = tensor_arg(a[2], "q_starts");
+    need(lens.device() == parents.device() && starts.device() == parents.device(), "kv_lens and q_starts must be on the device of parents");
+    for (const at::Tensor* t : {&parents, &lens, &starts}) need(t->dim() == 1 && t->scalar_type() == at::kInt && t->is_contiguous(), "parents, kv_lens and q_starts must be contiguous int32 vectors");
+    need(starts.size(0) == lens.size(0) + 1, "q_starts must have one entry more than kv_lens");
+    need(lens.size(0) < INT32_MAX, "too many sequences");
+    const long long T = parents.size(0), max_q = std::min(int_arg(a[3], 0, INT32_MAX, "max_q"), T), words = (max_q + 31) / 32;
+    const c10::DeviceIndex dev = parents.device().index();
+    const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, dev));
+    const at::Tensor masks = empty({T, words}, at::kInt, dev), positions = empty({T}, at::kInt, dev);
+    const int rc = varq_paged_tree(parents.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), starts.data_ptr<int32_t>(), (int)lens.size(0), T, (int)max_q, (int)words,
+                                   masks.data_ptr<int32_t>(), positions.data_ptr<int32_t>(), c10::cuda::getCurrentCUDAStream(dev).stream());
+    return rc == VARQ_OK ? make_pair(masks, positions) : raise(rc);
+    GUARD_PAGED_END
+}
+// a sequence of (k_codes, v_codes, k_scale, v_scale, head_dim)
+std::vector<varq_paged_t> caches_arg(PyObject* o, const at::Tensor*& first) {
+    if (!PyList_Check(o)) throw Refuse(PyExc_TypeError, "caches must be a list");
+    std::vector<varq_paged_t> c;
+    first = nullptr;
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(o); ++i) {
+        PyObject* p = PyList_GET_ITEM(o, i);
+        if (!PyTuple_Check(p) || PyTuple_GET_SIZE(p) != 5) throw Refuse(PyExc_TypeError, "a cache is its four pools and head_dim");
+        PyObject* a[5];
+        for (int j = 0; j < 5; ++j) a[j] = PyTuple_GET_ITEM(p, j);
+        const at::Tensor* kc;
+        c.push_back(paged_desc(a, kc));
+        if (first) need(kc->device() == first->device(), "the caches are on different devices");
+        else first = kc;
+    }
+    return c;
+}
+const int64_t* longs_arg(PyObject* o, const at::Tensor& like, const char* name, long long& n) {
+    const at::Tensor& s = on_device(tensor_arg(o, name), like, name);
+    if (!(s.dim() == 1 && s.scalar_type() == at::kLong && (s.is_contiguous() || s.numel() == 0))) throw Refuse(PyExc_ValueError, std::string(name) + " must be a contiguous int64 vector");
+    n = s.size(0);
+    return s.data_ptr<int64_t>();
+}
+// paged_copy_pages(caches, src, dst)
+PyObject* py_paged_copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    GUARD_BEGIN
+    if (!want(n, 3)) return nullptr;
+    const at::Tensor* kc;
+    const std::vector<varq_paged_t> c = caches_arg(a[0], kc);
+    if (!kc) Py_RETURN_NONE;
+    long long ns, nd;
+    const int64_t *src = longs_arg(a[1], *kc, "src", ns), *dst = longs_arg(a[2], *kc, "dst", nd);
+    need(ns == nd, "src and dst must have one length");
+    const c10::DeviceIndex dev = kc->device().index();
+    const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, dev));
+    const int rc = varq_paged_copy_pages(c.data(), (int)c.size(), src, dst, ns, c10::cuda::getCurrentCUDAStream(dev).stream());
+    if (rc != VARQ_OK) return raise(rc);
+    Py_RETURN_NONE;
+    GUARD_PAGED_END
+}
+// paged_move_tokens(caches, src, dst, starts, most)
+PyObject* py_paged_move_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    GUARD_BEGIN
+    if (!want(n, 5)) return nullptr;
+    const at::Tensor* kc;
+    const std::vector<varq_paged_t> c = caches_arg(a[0], kc);
+    if (!kc) Py_RETURN_NONE;
+    long long ns, nd;
+    const int64_t *src = longs_arg(a[1], *kc, "src", ns), *dst = longs_arg(a[2], *kc, "dst", nd);
+    need(ns == nd, "src and dst must have one length");
+    const at::Tensor& starts = on_device(tensor_arg(a[3], "starts"), *kc, "starts");
+    need(starts.dim() == 1 && starts.scalar_type() == at::kInt && starts.is_contiguous() && starts.size(0) >= 1 && starts.size(0) <= INT32_MAX,
+         "starts must be a contiguous int32 vector with one entry more than groups");
+    const int most = (int)int_arg(a[4], 0, INT32_MAX, "most");
+    const c10::DeviceIndex dev = kc->device().index();
+    const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, dev));
+    const int rc = varq_paged_move_tokens(c.data(), (int)c.size(), src, dst, ns, starts.data_ptr<int32_t>(), (int)starts.size(0) - 1, most,
+                                          c10::cuda::getCurrentCUDAStream(dev).stream());
+    if (rc != VARQ_OK) return raise(rc);
+    Py_RETURN_NONE;
+    GUARD_PAGED_END
+}
+
+// ---------------------------------------------------------------- norms and rotary positions
+// a[0..5]: turns, axis, n_axes, rotary_dim, interleaved, head_dim; at norm[0..3]: norm, eps, q_weight or None, k_weight or None
+void weight_arg(PyObject* o, const at::Tensor& like, const char* name, long long heads, long long D, const float*& p, int64_t& sh, int64_t& sd) {
+    p = nullptr; sh = sd = 0;
+    if (o == Py_None) return;
+    const at::Tensor& w = on_device(tensor_arg(o, name), like, name);
+    const long long n = w.dim();
+    const bool fits = w.scalar_type() == at::kFloat && (n == 1 ? w.size(0) == D : n == 2 && (w.size(0) == 1 || w.size(0) == heads) && (w.size(1) == 1 || w.size(1) == D));
+    if (!fits) throw Refuse(PyExc_ValueError, std::string(name) + " must be float32 [head_dim], or [heads, head_dim] with 1 in either place");
+    p = w.data_ptr<float>();
+    sh = n == 2 && w.size(0) > 1 ? w.stride(0) : 0;
+    sd = w.size(n - 1) > 1 ? w.stride(n - 1) : 0;
+}
+varq_rotary_t rotary_desc(PyObject* const* a, PyObject* const* norm, const at::Tensor& q, const at::Tensor& k, PyObject* positions) {
+    varq_rotary_t r{};
+    const at::Tensor &turns = on_device(tensor_arg(a[0], "the rotary table"), q, "the rotary table"), &axis = on_device(tensor_arg(a[1], "the rotary table"), q, "the rotary table");
+    r.n_axes = (int)int_arg(a[2], 1, INT32_MAX, "n_axes");
+    r.rotary_dim = (int)int_arg(a[3], 0, INT32_MAX, "rotary_dim");
+    r.interleaved = PyObject_IsTrue(a[4]);
+    const long long D = int_arg(a[5], 1, 4096, "head_dim");
+    need(turns.scalar_type() == at::kLong && axis.scalar_type() == at::kInt && turns.dim() == 1 && axis.dim() == 1 && turns.is_contiguous() && axis.is_contiguous() &&
+             turns.size(0) * 2 == r.rotary_dim && axis.size(0) == turns.size(0), "the rotary table is int64 turns and int32 axes, one for every pair");
+    need(q.size(q.dim() - 1) == D, "q and k do not have the head_dim of the rotary positions");
+    r.turns = reinterpret_cast<const uint64_t*>(turns.data_ptr<int64_t>()); r.axis = axis.data_ptr<int32_t>();
+    const at::Tensor& pos = on_device(tensor_arg(positions, "positions"), q, "positions");
+    need(pos.scalar_type() == at::kInt || pos.scalar_type() == at::kLong, "positions must be int32 or int64");
+    const bool batched = q.dim() == 4;
+    const long long B = batched ? q.size(0) : 1, L = q.size(batched ? 1 : 0), n = pos.dim();
+    need(n >= 1 && n <= (batched ? 3 : 2) && pos.size(n - 1) == L && (n == 1 ? r.n_axes == 1 : pos.size(0) == r.n_axes) && (n < 3 || pos.size(1) == B),
+         "positions must be [axes, tokens], [axes, batch, tokens], or [tokens] for one axis");
+    r.positions = pos.data_ptr(); r.pos_bytes = pos.scalar_type() == at::kInt ? 4 : 8;
+    r.pos_stride_l = pos.stride(n - 1); r.pos_stride_axis = n > 1 ? pos.stride(0) : 0; r.pos_stride_b = n == 3 ? pos.stride(1) : 0;
+    r.norm = (int)int_arg(norm[0], 0, 2, "norm");
+    const double eps = PyFloat_AsDouble(norm[1]);
+    if (PyErr_Occurred()) throw std::runtime_error("");
+    r.eps = (float)eps;
+    weight_arg(norm[2], q, "q_weight", q.size(q.dim() - 2), D, r.q_weight, r.q_weight_stride_h, r.q_weight_stride_d);
+    weight_arg(norm[3], q, "k_weight", k.size(k.dim() - 2), D, r.k_weight, r.k_weight_stride_h, r.k_weight_stride_d);
+    return r;
+}
+// rotate(turns, axis, n_axes, rotary_dim, interleaved, head_dim, q, k, positions, norm, eps, q_weight, k_weight, dtype or None) -> (q, k)
+PyObject* py_rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    GUARD_BEGIN
+    if (!want(n, 14)) return nullptr;
+    const at::Tensor& q = tensor_arg(a[6], "q");
+    const at::Tensor& k = tensor_arg(a[7], "k");
+    need(k.device() == q.device(), "q and k are on different devices");
+    const long long d = q.dim();
+    need((d == 3 || d == 4) && k.dim() == d && k.size(d - 1) == q.size(d - 1) && k.size(0) == q.size(0) && k.size(d - 3) == q.size(d - 3),
+         "q and k must be [tokens, heads, head_dim] or [batch, tokens, heads, head_dim] of the same tokens");
+    need((q.stride(d - 1) == 1 || q.numel() == 0) && (k.stride(d - 1) == 1 || k.numel() == 0), "the last dimension of q and k must be contiguous");
+    need(dtype_code(q.scalar_type()) >= 0 && k.scalar_type() == q.scalar_type(), "q and k must have one type: float32, float16 or bfloat16");
+    for (int i = 0; i < d; ++i) need(q.size(i) <= INT32_MAX && k.size(i) <= INT32_MAX, "q or k is too large");
+    at::ScalarType s = q.scalar_type();
+    if (a[13] != Py_None) {
+        if (!THPDtype_Check(a[13])) throw Refuse(PyExc_TypeError, "dtype must be a torch.dtype");
+        s = reinterpret_cast<THPDtype*>(a[13])->scalar_type;
+        need(s == q.scalar_type() || s == at::kFloat, "dtype must be the type of q and k or float32");
+    }
+    const varq_rotary_t r = rotary_desc(a, a + 9, q, k, a[8]);
+    const c10::DeviceIndex dev = q.device().index();
+    const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, dev));
+    const at::Tensor qo = empty(q.sizes(), s, dev), ko = empty(k.sizes(), s, dev);
+    auto desc = [d](const at::Tensor& t) -> varq_tensor_t { return {t.data_ptr(), dtype_code(t.scalar_type()), 0, d == 4 ? t.stride(0) : 0, t.stride(d - 3), t.stride(d - 2)}; };
+    const varq_tensor_t qd = desc(q), kd = desc(k), qod = desc(qo), kod = desc(ko);
+    const int rc = varq_rotate(&r, &qd, &kd, d == 4 ? (int)q.size(0) : 1, (int)q.size(d - 3), (int)q.size(d - 2), (int)k.size(d - 2), (int)q.size(d - 1), &qod, &kod,
+                               c10::cuda::getCurrentCUDAStream(dev).stream());
+    return rc == VARQ_OK ? make_pair(qo, ko) : raise(rc);
+    GUARD_PAGED_END
+}
+// paged_append_rotated(k_codes, v_codes, k_scale, v_scale, head_dim, turns, axis, n_axes, rotary_dim, interleaved, head_dim, q, k, v, slots, positions, norm, norm_eps,
+//                      q_weight, k_weight, eps) -> q
+PyObject* py_paged_append_rotated(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    GUARD_BEGIN
+    if (!want(n, 21)) return nullptr;
+    const at::Tensor* kc;
+    const varq_paged_t c = paged_desc(a, kc);
+    const at::Tensor *x[3] = {&on_device(tensor_arg(a[11], "q"), *kc, "q"), &on_device(tensor_arg(a[12], "k"), *kc, "k"), &on_device(tensor_arg(a[13], "v"), *kc, "v")};
+    long long tokens;
+    const int64_t* slots = slots_arg(a[14], *kc, tokens);
+    for (int i = 0; i < 3; ++i) {
+        const at::Tensor* t = x[i];
+        need(t->dim() == 3 && t->size(0) == tokens && (i == 0 || t->size(1) == c.n_heads) && t->size(2) == c.head_dim,
+             "q, k and v must be [tokens, heads, head_dim], k and v with the heads of the cache, a slot per token");
+        need(t->stride(2) == 1 || t->numel() == 0, "the last dimension of q, k and v must be contiguous");
+        need(dtype_code(t->scalar_type()) >= 0 && t->scalar_type() == x[0]->scalar_type(), "q, k and v must have one type: float32, float16 or bfloat16");
+    }
+    need(x[0]->size(1) <= INT32_MAX, "q is too large");
+    const varq_rotary_t r = rotary_desc(a + 5, a + 16, *x[0], *x[1], a[15]);
+    const double eps = PyFloat_AsDouble(a[20]);
+    if (PyErr_Occurred()) return nullptr;
+    const c10::DeviceIndex dev = kc->device().index();
+    const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, dev));
+    const at::Tensor out = empty(x[0]->sizes(), x[0]->scalar_type(), dev);
+    const varq_tensor_t qd = rows_desc(*x[0]), kd = rows_desc(*x[1]), vd = rows_desc(*x[2]), od = rows_desc(out);
+    const int rc = varq_paged_append_rotated(&c, &r, &qd, &kd, &vd, slots, tokens, (int)x[0]->size(1), (float)eps, &od, c10::cuda::getCurrentCUDAStream(dev).stream());
+    return rc == VARQ_OK ? THPVariable_Wrap(out) : raise(rc);
     GUARD_PAGED_END
 }
 
@@ -655,7 +846,13 @@ PyMethodDef methods[] = {
     FAST("paged_append", py_paged_append, "paged_append(k_codes, v_codes, k_scale, v_scale, head_dim, k, v, slots, eps)"),
     FAST("paged_read", py_paged_read, "paged_read(k_codes, v_codes, k_scale, v_scale, head_dim, slots, dtype) -> (k, v)"),
     FAST("paged_attend", py_paged_attend, "paged_attend(k_codes, v_codes, k_scale, v_scale, head_dim, q, block_table, kv_lens, q_starts, max_q, max_kv, "
-         "softmax_scale, causal, window, sinks, return_lse) -> out or (out, lse)"),
+         "softmax_scale, causal, window, sinks, return_lse, tree) -> out or (out, lse)"),
+    FAST("paged_append_rotated", py_paged_append_rotated, "paged_append_rotated(k_codes, v_codes, k_scale, v_scale, head_dim, turns, axis, n_axes, rotary_dim, interleaved, "
+         "head_dim, q, k, v, slots, positions, norm, norm_eps, q_weight, k_weight, eps) -> q"),
+    FAST("paged_tree", py_paged_tree, "paged_tree(parents, kv_lens, q_starts, max_q) -> (masks, positions)"),
+    FAST("paged_copy_pages", py_paged_copy_pages, "paged_copy_pages(caches, src, dst)"),
+    FAST("paged_move_tokens", py_paged_move_tokens, "paged_move_tokens(caches, src, dst, starts, most)"),
+    FAST("rotate", py_rotate, "rotate(turns, axis, n_axes, rotary_dim, interleaved, head_dim, q, k, positions, norm, eps, q_weight, k_weight, dtype) -> (q, k)"),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Host path of the VAR_Q package.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -245,6 +245,7 @@ int paged_status_word(int** out) {
 }
 int paged_status(int* out) {
     if (int rc = paged_attn_tc_status(out)) return rc;
+    if (int rc = paged_attn_tree_status(out)) return rc;
     int v = 0;
     VARQ_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_paged_status, sizeof(int)));
     if (v != 0) {
@@ -329,12 +330,16 @@ struct AttnPlan {
     int rows;                          // query rows of a CTA (decode kernel)
     int splits, tiles_per_split;       // tiles of 16 keys (decode kernel)
 };
+int paged_max_q(const varq_paged_batch_t* b) { return (int)(b->max_q < b->n_queries ? b->max_q : b->n_queries); }
+constexpr long long TREE_BLOCKS = 8000;
 AttnPlan plan_attn(const varq_paged_t* c, const varq_paged_batch_t* b) {
-    AttnPlan p;
-    const int max_q = (int)(b->max_q < b->n_queries ? b->max_q : b->n_queries), D = c->head_dim;
+    AttnPlan p{};
+    const int max_q = paged_max_q(b), D = c->head_dim;
     const long long rows = (long long)max_q * (b->q_heads / c->n_heads);
     const long long seen = (long long)b->window + max_q + b->sinks, span = b->window && seen < b->max_kv ? seen : b->max_kv;      // keys of a CTA, about
-    p.tc = forced_attn_path() == VARQ_ATTN_PATH_TC || (forced_attn_path() != VARQ_ATTN_PATH_DECODE && rows > (D == 64 ? 80 : 32));
+    const long long blocks16 = (long long)b->n_seqs * c->n_heads * ((rows + 15) / 16) * ((span + 15) / 16);      // products of 16 rows and 16 keys
+    const bool many = b->tree ? rows > 32 && blocks16 > TREE_BLOCKS : rows > (D == 64 ? 80 : 32);
+    p.tc = forced_attn_path() == VARQ_ATTN_PATH_TC || (forced_attn_path() != VARQ_ATTN_PATH_DECODE && many);
     p.rows = rows <= 8 ? 8 : rows > 16 && rows <= 24 && 4ll * b->n_seqs * c->n_heads >= sm_count() ? 24 : 16;
     const long long unit = p.tc ? 128 : 16, tiles = span > unit ? (span + unit - 1) / unit : 1;
     const int resident = p.tc ? 1 : p.rows > 16 ? (D == 128 ? 2 : 3) : p.rows > 8 ? (D == 128 ? 3 : 4) : D == 64 ? 5 : c->k_bits == 8 && c->v_bits == 8 ? 3 : 4;       // CTAs per SM
@@ -345,7 +350,11 @@ AttnPlan plan_attn(const varq_paged_t* c, const varq_paged_batch_t* b) {
     p.splits = 1; p.cluster = false;
     for (long long s = 1; s == 1 || (s <= tiles / least && s <= 256); ++s) {
         const bool near = !p.tc && s <= PAGED_CLUSTER && base * s <= room;
-        const long long cost = (base * s + room - 1) / room * ((tiles + s - 1) / s + fixed + (s > 1 && p.tc ? fixed : 0)) + (s > 1 && !near ? merge : 0);
+        long long cost = (base * s + room - 1) / room * ((tiles + s - 1) / s + fixed + (s > 1 && p.tc ? fixed : 0)) + (s > 1 && !near ? merge : 0);
+        if (b->tree && !p.tc) {                              // contexts differ: the longest part, or what all of them come to at three fifths of the longest
+            const long long longest = (tiles + s - 1) / s + fixed, all = base * (tiles * 3 / 5 + s * fixed) / room;
+            cost = (longest > all ? longest : all) + (s > 1 && !near ? merge : 0);
+        }
         if (best == 0 || cost < best) { best = cost; p.splits = (int)s; p.cluster = s > 1 && near; }
         if (base * s > 8 * room) break;
     }
@@ -400,7 +409,7 @@ extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch
     a.q_starts = batch->q_starts; a.kv_lens = batch->kv_lens; a.table = batch->block_table;
     a.table_stride = batch->table_stride; a.table_pages = batch->table_pages;
     a.B = batch->n_seqs; a.T = (int)batch->n_queries; a.Hq = batch->q_heads; a.G = a.Hq / a.c.H;
-    a.max_q = (int)(batch->max_q < batch->n_queries ? batch->max_q : batch->n_queries); a.max_kv = batch->max_kv;
+    a.max_q = paged_max_q(batch); a.max_kv = batch->max_kv;
     a.scale_log2 = batch->softmax_scale * 1.4426950408889634f;
     a.causal = batch->causal != 0; a.window = batch->window;
     a.sinks = batch->sinks < PAGED_MOST_KEYS ? batch->sinks : PAGED_MOST_KEYS;      // more tokens than there are: all of them
@@ -413,6 +422,6 @@ extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch
     const cudaStream_t st = (cudaStream_t)stream;
     int* status = nullptr;
     if (int rc = paged_status_word(&status)) return rc;      // the kernels write to it: no launch without it
-    if (int rc = p.tc ? paged_attn_tc_run(a, p.splits, ws_o, ws_ml, status, st) : paged_attn_decode_run(a, p.rows, p.splits, p.cluster, p.tiles_per_split, ws_o, ws_ml, status, st)) return rc;
+    if (int rc = p.tc ? (a.tree ? paged_attn_tree_run : paged_attn_tc_run)(a, p.splits, ws_o, ws_ml, status, st) : (a.tree ? paged_attn_decode_tree_run : paged_attn_decode_run)(a, p.rows, p.splits, p.cluster, p.tiles_per_split, ws_o, ws_ml, status, st)) return rc;
     return need ? paged_attn_merge_run(a, p.splits, ws_o, ws_ml, st) : VARQ_OK;
 }

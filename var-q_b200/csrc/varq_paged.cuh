@@ -141,8 +141,11 @@ constexpr int PAGED_CLUSTER = 8;       // up to so many parts of the decode kern
 int paged_attn_tc_run(const PagedAttnArgs& a, int splits, float* ws_o, float* ws_ml, int* status, cudaStream_t st);
 // rows: query rows of a CTA, 8, 16 or 24
 int paged_attn_decode_run(const PagedAttnArgs& a, int rows, int splits, bool in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, int* status, cudaStream_t st);
+int paged_attn_decode_tree_run(const PagedAttnArgs& a, int rows, int splits, bool in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, int* status, cudaStream_t st);
 int paged_attn_merge_run(const PagedAttnArgs& a, int splits, const float* ws_o, const float* ws_ml, cudaStream_t st);
 int paged_attn_tc_status(int* out);
+int paged_attn_tree_run(const PagedAttnArgs& a, int splits, float* ws_o, float* ws_ml, int* status, cudaStream_t st);      // drafted tokens; parts as of the others
+int paged_attn_tree_status(int* out);
 int forced_attn_path();                // varq_attn_force_path
 
 }  // namespace varq

@@ -35,13 +35,10 @@
 // Turned down: the first scores of the next tile under the last exponentials of this one, 876 / 687 / 137 us (P comes later, and the products with it); weights
 // first and one vote on them for the whole tile, 716 / 646 / 119 us, but 1 to 2 us more on a call of 14 to 24 us.
 // Register shares 152 / 64 (softmax / converters) 768 / 638, 144 / 72 740 / 638, 160 / 56 756 / 638 us.
-#include "varq_attn_tc.cuh"
-#include "varq_paged.cuh"
+#include "varq_paged_attn_tc.cuh"
 
 namespace varq {
 namespace {
-
-constexpr int PT_M = 128, PT_N = 64;
 
 template <int D> struct PtPlan {
     static constexpr int SB = D == 64 ? 3 : 2;                     // score tiles per query tile
@@ -64,91 +61,6 @@ template <int D> struct PtPlan {
     static constexpr int REGS = 96, REGS_SOFT = 144, REGS_CONV = 72, REGS_MISC = 48;
     static_assert(SOFT * 32 * REGS_SOFT + 256 * REGS_CONV + 128 * REGS_MISC <= THREADS * REGS, "register plan");
 };
-
-// 16-byte chunk `ch` (eight head_dim values) of row `r` in a 128B-swizzled tile of ROWS rows: blocks of 64 columns
-template <int ROWS> __device__ __forceinline__ uint32_t pt_chunk(int r, int ch) {
-    return (uint32_t)((ch >> 3) * (ROWS * 128) + (r >> 3) * 1024 + (r & 7) * 128 + (((ch & 7) ^ (r & 7)) << 4));
-}
-// D[tmem] (+)= A[smem] B[smem]
-__device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, e;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
-}
-// pairs of fp32 in one 64-bit register
-using pair = unsigned long long;
-__device__ __forceinline__ pair pair_of(float x, float y) { pair d; asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y)); return d; }
-__device__ __forceinline__ float pair_x(pair p) { float x; [[maybe_unused]] float y; asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); return x; }
-__device__ __forceinline__ float pair_y(pair p) { [[maybe_unused]] float x; float y; asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); return y; }
-__device__ __forceinline__ pair fma2(pair a, pair b, pair c) { pair d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c)); return d; }
-__device__ __forceinline__ pair add2(pair a, pair b) { pair d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
-__device__ __forceinline__ pair mul2(pair a, pair b) { pair d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
-// 16 rows x 32 columns: thread (g, c) = (lane / 4, lane % 4) gets columns 2c, 2c + 1 of every eight, of row g (r[4n], r[4n + 1]) and row g + 8
-__device__ __forceinline__ void tmem_ld_16x256(uint32_t taddr, uint32_t* r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr) : "memory");
-}
-// 16 rows x 16 columns: column c of every four, of row g (r[2n]) and row g + 8 (r[2n + 1])
-__device__ __forceinline__ void tmem_st_16x128(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
-}
-// waits for the loads from tensor memory in flight, and keeps the use of what they left in `r` behind that
-__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
-                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
-                   "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]),
-                   "+r"(r[31])
-                 :: "memory");
-}
-__device__ __forceinline__ pair pair_of_bits(uint32_t x, uint32_t y) { pair d; asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(x), "r"(y)); return d; }
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-// one arrival for a warp, behind what all its lanes did
-__device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
-    __syncwarp();
-    if (lane == 0) mbar_arrive(bar);
-}
-template <int BITS> __host__ __device__ constexpr uint32_t pt_neg_base(int cls) {      // fp16 pairs of -(1024 / 2^p + bias), by class of bit position
-    return BITS == 8 ? 0xE480E480u : BITS == 4 ? (cls == 0 ? 0xE408E408u : 0xD480D480u)
-                                               : (cls == 0 ? 0xE402E402u : cls == 1 ? 0xDC08DC08u : cls == 2 ? 0xD420D420u : 0xCC80CC80u);
-}
-
-// The key tiles of a CTA: `ns` tiles of first tokens, then those from `lo` on; `first`: the first key of its windows, in the tile at `lo`
-struct PtTiles {
-    int ns, lo, n, first;
-    __device__ __forceinline__ int key(int i) const { return i < ns ? i * PT_N : lo + (i - ns) * PT_N; }
-};
-
-// one of the two 16-element halves of a query row's 32, packed fp16 in element order -> operand order of codes of `kb` bits
-__device__ __forceinline__ void q_operand_order(uint32_t (&w)[8], int kb) {
-    if (kb == 8) return;
-    uint32_t o[8];
-    if (kb == 4) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                o[4 * i + 2 * j] = __byte_perm(w[4 * i + j], w[4 * i + 2 + j], 0x5410);
-                o[4 * i + 2 * j + 1] = __byte_perm(w[4 * i + j], w[4 * i + 2 + j], 0x7632);
-            }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { o[2 * j] = __byte_perm(w[j], w[4 + j], 0x5410); o[2 * j + 1] = __byte_perm(w[j], w[4 + j], 0x7632); }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = o[i];
-}
 
 template <int D>
 __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(PagedAttnArgs a, int n_qblocks, int splits, float* ws_o, float* ws_ml, int* status) {
@@ -194,9 +106,8 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
     int n_t[2], tile0 = 0;                                                   // key tiles of the two query tiles
     {
         const int t0 = row0 / a.G, t1 = (min(row0 + 2 * PT_M, rows) - 1) / a.G, t_mid = (min(row0 + PT_M, rows) - 1) / a.G;
-        const bool chain = a.causal && !a.tree;
-        const int hi = max(chain ? min(seq.kv, p_first + t1 + 1) : seq.kv, 0), hi0 = max(chain ? min(seq.kv, p_first + t_mid + 1) : seq.kv, 0);
-        tiles.first = paged_window(a, a.tree ? p_first - 1 : p_first + t0);
+        const int hi = max(a.causal ? min(seq.kv, p_first + t1 + 1) : seq.kv, 0), hi0 = max(a.causal ? min(seq.kv, p_first + t_mid + 1) : seq.kv, 0);
+        tiles.first = paged_window(a, p_first + t0);
         tiles.lo = tiles.first & ~(PT_N - 1);
         tiles.ns = min((a.sinks + PT_N - 1) / PT_N, tiles.lo / PT_N);
         const int n = hi > 0 ? tiles.ns + (max(hi - tiles.lo, 0) + PT_N - 1) / PT_N : 0, n0 = hi0 > 0 ? tiles.ns + (max(hi0 - tiles.lo, 0) + PT_N - 1) / PT_N : 0;
@@ -259,17 +170,14 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
             if (scaled) reinterpret_cast<float*>(smem + P::OFF_QF)[t * PT_M + r] = q_factor;
             __syncwarp();
             // keys between which every row of the query tile sees everything
-            const int tl = min(row0 + t * PT_M + PT_M, rows) - 1, all_hi = a.tree ? p_first : a.causal ? p_first + (row0 + t * PT_M) / a.G + 1 : 0x7fffffff,
-                      all_lo = paged_window(a, p_first + (a.tree ? seq.nq - 1 : tl / a.G));
+            const int tl = min(row0 + t * PT_M + PT_M, rows) - 1, all_hi = a.causal ? p_first + (row0 + t * PT_M) / a.G + 1 : 0x7fffffff,
+                      all_lo = paged_window(a, p_first + tl / a.G);
             // A thread holds, of every eight columns of S, two of the rows g, g + 8, g + 16, g + 24 of its warp's 32 (g = lane / 4): it needs a quarter of
             // the keys' tables and uses an entry for four rows
             const int g = lane >> 2, cq = lane & 3;
             int pos[4];                                                     // positions of the four rows' tokens
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int at = min(row0 + t * PT_M + quarter * 32 + g + 8 * i, rows - 1) / a.G;
-                pos[i] = a.tree ? at : p_first + at;                        // (of a drafted token: which one it is)
-            }
+            for (int i = 0; i < 4; ++i) pos[i] = p_first + min(row0 + t * PT_M + quarter * 32 + g + 8 * i, rows - 1) / a.G;
             pair nm[4] = {0ull, 0ull, 0ull, 0ull};                          // minus the reference, twice
             pair l[4] = {0ull, 0ull, 0ull, 0ull};
             unsigned unset = 15u;                                           // rows that have no reference yet: they have seen no key
@@ -322,18 +230,11 @@ __global__ void __launch_bounds__(PtPlan<D>::THREADS, 1) paged_attn_tc_kernel(Pa
                         if (SPECIAL) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                PagedSpan sp = paged_span(a, pos[i], seq.kv);
+                                const PagedSpan sp = paged_span(a, pos[i], seq.kv);
                                 // bit k: this thread's column 2c + k of the 32 is seen
                                 auto below = [](int k) { return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1u; };
                                 const int c0 = key0 + 32 * c + 2 * cq;
-                                uint32_t tree = ~0u;
-                                if (a.tree) {
-                                    const int token = seq.q0 + pos[i];
-                                    sp.hi = seq.kv;
-                                    sp.lo = a.window ? paged_window(a, paged_tree_position(a, token, p_first, seq.nq)) : 0;
-                                    tree = paged_tree_bits(a, token, c0 - p_first);
-                                }
-                                const uint32_t sees = below(sp.hi - c0) & (~below(sp.lo - c0) | below(a.sinks - c0)) & tree;
+                                const uint32_t sees = below(sp.hi - c0) & (~below(sp.lo - c0) | below(a.sinks - c0));
 #pragma unroll
                                 for (int v = 0; v < 4; ++v) {
                                     pair& y = x[(i >> 1) * 8 + v * 2 + (i & 1)];

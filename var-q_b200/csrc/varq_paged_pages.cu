@@ -56,58 +56,84 @@ __global__ void __launch_bounds__(COPY_THREADS) paged_copy_pages_kernel(const __
     }
 }
 
-constexpr int MOVE_THREADS = 256, MOVE_ROWS = 64;      // moves of a chunk
+constexpr int MOVE_THREADS = 256, MOVE_UNITS = 4, MOVE_ROWS = 64;      // 16-byte units of a thread, moves of a chunk at most
 
-__global__ void __launch_bounds__(MOVE_THREADS) paged_move_kernel(const __grid_constant__ CopyArgs a, int* status) {
-    __shared__ long long s_at[2][MOVE_ROWS];           // rows of the pools, source and destination, -1: nothing moves
+// A block: one group, `heads` heads of one cache, K or V of it or both (parts).  A unit is 16 bytes of codes of a (move, head); a chunk is as many moves as fill the
+// threads' units.  The next chunk is read before this one is written, which is allowed for the same reason.
+__global__ void __launch_bounds__(MOVE_THREADS) paged_move_kernel(const __grid_constant__ CopyArgs a, int heads, int parts, int* status) {
+    __shared__ uint2 s_at[2][MOVE_ROWS];               // rows of the pools at head 0, source and destination; equal: nothing moves
     pdl_trigger();
     pdl_wait();
     const CopyCache& c = a.c[blockIdx.z];
-    const int g = blockIdx.x, h = blockIdx.y;
-    if (h >= c.H) return;
+    const int g = blockIdx.x, h0 = ((int)blockIdx.y / parts) * heads, hn = min(heads, c.H - h0), part = (int)blockIdx.y % parts;
+    if (hn <= 0) return;
     const int s0 = __ldg(a.starts + g), s1 = __ldg(a.starts + g + 1);
     const int begin = (int)min((long long)max(s0, 0), a.n), end = (int)min((long long)max(s1, begin), a.n);
     if ((s0 != begin || s1 != end) && threadIdx.x == 0) atomicCAS(status, 0, PAGED_BAD_STARTS);
+    if (begin == end) return;
     const long long n_slots = (long long)c.n_pages << a.page_shift;
     const int page_mask = (1 << a.page_shift) - 1;
-    const int kp = c.krow / 16, vp = c.vrow / 16, pieces = kp + vp;                  // 16-byte pieces of a token's codes
-    constexpr int U = MOVE_ROWS * 16 / MOVE_THREADS;   // of a thread, at most: 8 pieces of K and of V
-    for (int m0 = begin; m0 < end; m0 += MOVE_ROWS) {
-        const int n = min(MOVE_ROWS, end - m0);
-        __syncthreads();
-        if (threadIdx.x < MOVE_ROWS) {
-            long long r[2] = {-1, -1};
-            if (threadIdx.x < n) {
-                const long long s = __ldg(a.src + m0 + threadIdx.x), d = __ldg(a.dst + m0 + threadIdx.x);
-                if ((unsigned long long)s < (unsigned long long)n_slots && (unsigned long long)d < (unsigned long long)n_slots && s != d) {
-                    r[0] = (((s >> a.page_shift) * c.H + h) << a.page_shift) + (s & page_mask);
-                    r[1] = (((d >> a.page_shift) * c.H + h) << a.page_shift) + (d & page_mask);
-                }
+    const int kp = part == 1 ? 0 : c.krow / 16, vp = parts == 2 && part == 0 ? 0 : c.vrow / 16;      // units of a row
+    const int per = (kp + vp) * hn, kinds = (kp > 0) + (vp > 0), rows = max(min(MOVE_ROWS, min(MOVE_UNITS * MOVE_THREADS / per, MOVE_THREADS / (kinds * hn))), 1);
+    // where this thread's units lie: (move of the chunk, offset in bytes behind the row at head 0), the same for every chunk; its scale likewise
+    int row[MOVE_UNITS], head[MOVE_UNITS], piece[MOVE_UNITS];
+#pragma unroll
+    for (int i = 0; i < MOVE_UNITS; ++i) {
+        const int u = threadIdx.x + i * MOVE_THREADS, in = u % per;
+        row[i] = u / per < rows ? u / per : MOVE_ROWS;
+        head[i] = h0 + in / (kp + vp);
+        piece[i] = in % (kp + vp);
+    }
+    const int s_in = threadIdx.x % (kinds * hn), s_row = threadIdx.x / (kinds * hn) < rows ? (int)threadIdx.x / (kinds * hn) : MOVE_ROWS, s_head = h0 + s_in / kinds;
+    float* const scales = kinds == 2 ? (s_in & 1 ? c.vs : c.ks) : kp > 0 ? c.ks : c.vs;
+    auto unit = [&](int i, uint32_t at) -> uint4* {
+        const size_t r = (size_t)(at + ((uint32_t)head[i] << a.page_shift));
+        return piece[i] < kp ? reinterpret_cast<uint4*>(c.kc + r * c.krow) + piece[i] : reinterpret_cast<uint4*>(c.vc + r * c.vrow) + (piece[i] - kp);
+    };
+    auto slots = [&](int m) -> uint2 {                 // of move m + this thread's number
+        uint2 r = make_uint2(0u, 0u);
+        if (threadIdx.x < rows && m + (int)threadIdx.x < end) {
+            const long long s = __ldg(a.src + m + threadIdx.x), d = __ldg(a.dst + m + threadIdx.x);
+            if ((unsigned long long)s < (unsigned long long)n_slots && (unsigned long long)d < (unsigned long long)n_slots) {
+                r.x = ((uint32_t)(s >> a.page_shift) * c.H << a.page_shift) + ((uint32_t)s & page_mask);
+                r.y = ((uint32_t)(d >> a.page_shift) * c.H << a.page_shift) + ((uint32_t)d & page_mask);
             }
-            s_at[0][threadIdx.x] = r[0]; s_at[1][threadIdx.x] = r[1];
         }
-        __syncthreads();
-        uint4 x[U];
-        float sc = 0.f;
-        const int srow = threadIdx.x >> 1;             // scale of K (even threads) or V
-        auto at = [&](int u, int which) -> uint4* {    // unit u of the chunk, in its source (0) or destination (1)
-            const int row = u / pieces, p = u - row * pieces;
-            const long long r = s_at[which][row];
-            return p < kp ? reinterpret_cast<uint4*>(c.kc + r * c.krow) + p : reinterpret_cast<uint4*>(c.vc + r * c.vrow) + (p - kp);
-        };
+        return r;
+    };
+    uint4 x[MOVE_UNITS];
+    uint2 at[MOVE_UNITS], s_slot = make_uint2(0u, 0u);
+    float sc = 0.f;
+    auto read = [&](int buffer, uint4 (&v)[MOVE_UNITS], uint2 (&w)[MOVE_UNITS], float& f, uint2& fw) {
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int u = threadIdx.x + i * MOVE_THREADS;
-            if (u < n * pieces && s_at[0][u / pieces] >= 0) x[i] = *at(u, 0);
+        for (int i = 0; i < MOVE_UNITS; ++i) {
+            w[i] = row[i] < MOVE_ROWS ? s_at[buffer][row[i]] : make_uint2(0u, 0u);
+            if (w[i].x != w[i].y) v[i] = *unit(i, w[i].x);
         }
-        if (srow < n && s_at[0][srow] >= 0) sc = (threadIdx.x & 1 ? c.vs : c.ks)[s_at[0][srow]];
-        __syncthreads();
+        fw = s_row < MOVE_ROWS ? s_at[buffer][s_row] : make_uint2(0u, 0u);
+        if (fw.x != fw.y) f = scales[fw.x + ((uint32_t)s_head << a.page_shift)];
+    };
+    uint2 next = slots(begin);
+    if (threadIdx.x < rows) s_at[0][threadIdx.x] = next;
+    next = slots(begin + rows);
+    __syncthreads();
+    read(0, x, at, sc, s_slot);
+    for (int m0 = begin, buffer = 1; m0 < end; m0 += rows, buffer ^= 1) {
+        uint4 y[MOVE_UNITS];
+        uint2 bt[MOVE_UNITS], t_slot;
+        float tc = 0.f;
+        if (threadIdx.x < rows) s_at[buffer][threadIdx.x] = next;
+        next = slots(m0 + 2 * rows);
+        __syncthreads();                               // the slots of the next chunk are there, and this one is read by everybody
+        read(buffer, y, bt, tc, t_slot);
+        // (a later chunk's reads may pass this one's writes: they never meet)
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int u = threadIdx.x + i * MOVE_THREADS;
-            if (u < n * pieces && s_at[0][u / pieces] >= 0) *at(u, 1) = x[i];
-        }
-        if (srow < n && s_at[0][srow] >= 0) (threadIdx.x & 1 ? c.vs : c.ks)[s_at[1][srow]] = sc;
+        for (int i = 0; i < MOVE_UNITS; ++i)
+            if (at[i].x != at[i].y) *unit(i, at[i].y) = x[i];
+        if (s_slot.x != s_slot.y) scales[s_slot.y + ((uint32_t)s_head << a.page_shift)] = sc;
+#pragma unroll
+        for (int i = 0; i < MOVE_UNITS; ++i) { x[i] = y[i]; at[i] = bt[i]; }
+        sc = tc; s_slot = t_slot;
     }
 }
 
@@ -217,8 +243,12 @@ extern "C" int varq_paged_move_tokens(const varq_paged_t* caches, int32_t n_cach
         const int n = n_caches - from < MOST_CACHES ? n_caches - from : MOST_CACHES;
         int heads = 0;
         for (int i = 0; i < n; ++i) heads = a.c[i].H > heads ? a.c[i].H : heads;
-        if (heads > 65535) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_move_tokens: %d heads (65535 at most)", heads);
-        VARQ_CUDA_TRY(launch_pdl(paged_move_kernel, dim3((unsigned)n_groups, (unsigned)heads, (unsigned)n), MOVE_THREADS, 0, (cudaStream_t)stream, 1, a, status));
+        if (heads > 32767) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_move_tokens: %d heads (32767 at most)", heads);
+        // short groups: all heads in a block, up to 64 units of a thread's kind; long ones: a block per head, K and V apart
+        int each = 1;
+        while (each < heads && each < 64 && 2ll * each * max_moves <= 64) each *= 2;
+        const int parts = each > 1 ? 1 : 2;
+        VARQ_CUDA_TRY(launch_pdl(paged_move_kernel, dim3((unsigned)n_groups, (unsigned)((heads + each - 1) / each * parts), (unsigned)n), MOVE_THREADS, 0, (cudaStream_t)stream, 1, a, each, parts, status));
         count_launches(1);
     }
     return VARQ_OK;

@@ -82,8 +82,17 @@ struct PagedRow {
         lo = r * (1.f - 0x1p-21f); hi = r * (1.f + 0x1p-21f);
         small = scale > 0x1p125f ? 1u : 0u;
     }
-    // the codes, in the low mantissa bits of `q`
+    // the codes of a piece or two, in the low mantissa bits of `q`
     __device__ __forceinline__ void codes(const float (&v)[8], uint32_t (&q)[8]) const {
+        fix(v, q, bracket(v, q));
+    }
+    __device__ __forceinline__ void codes(const float (&v)[2][8], uint32_t (&q)[2][8]) const {
+        const uint32_t differ = bracket(v[0], q[0]) | bracket(v[1], q[1]);
+        if (!fine || differ) { fix(v[0], q[0], differ); fix(v[1], q[1], differ); }
+    }
+private:
+    // one end of the bracket; nonzero where the other end may be another integer
+    __device__ __forceinline__ uint32_t bracket(const float (&v)[8], uint32_t (&q)[8]) const {
         uint32_t differ = small;
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
@@ -92,6 +101,9 @@ struct PagedRow {
             q[i] = __float_as_uint(y.x); q[i + 1] = __float_as_uint(y.y);
             differ |= (q[i] ^ __float_as_uint(z.x)) | (q[i + 1] ^ __float_as_uint(z.y));
         }
+        return differ;
+    }
+    __device__ __forceinline__ void fix(const float (&v)[8], uint32_t (&q)[8], uint32_t differ) const {
         if (!fine) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) q[i] = 0u;

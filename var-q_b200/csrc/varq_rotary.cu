@@ -21,20 +21,67 @@ struct RotArgs {
     const unsigned long long* turns; const int32_t* axis; const void* pos;
     int pos_bytes, n_axes, R, inter;
     long long ps_a, ps_b, ps_l;
-    int norm; float eps;
-    const float *qw, *kw; long long qw_h, qw_d, kw_h, kw_d;
+    int norm; float inv_eps, least, sum_mul, sum_add;      // 1 / sqrt(sum * sum_mul + sum_add), or inv_eps where that sum is less than `least`
+    const float *qw, *kw; long long qw_h, qw_d, kw_h, kw_d; int qw_vec, kw_vec;
     const void *q, *k, *v; long long qs_b, qs_l, qs_h, ks_b, ks_l, ks_h, vs_l, vs_h;
     void *qo, *ko; long long qo_b, qo_l, qo_h, ko_b, ko_l, ko_h;
     int Hq, Hk, Hv;
-    uint32_t tokens; FastDiv L;
+    uint32_t tokens; FastDiv L, half;
     int lanes_log2, parts;            // rows of a token that a block works on side by side (log2), parts of a token's rows
     PagedView c; const long long* slots; float qeps;
 };
 
-template <typename T, typename O, int D, bool VEC, bool PAGED, int U>
-__global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(RotArgs a) {
+// pairs of fp32 in one 64-bit register
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pack2(float x, float y) { f32x2 d; asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y)); return d; }
+__device__ __forceinline__ float2 unpack2(f32x2 p) { float2 v; asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(p)); return v; }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) { f32x2 d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { f32x2 d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c)); return d; }
+
+// A lane's sixteen values as eight pairs (x[j], y[j]) that turn together, two of them in a register: the pieces themselves where pairs are half the rotary
+// dimension apart, even and odd elements where they are neighbours.  Element i of piece e is value `at` of x (or y).
+template <bool INTER> struct Pairs {
+    f32x2 x[4], y[4];
+    __device__ __forceinline__ Pairs(const float (&v)[2][8]) {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            if constexpr (INTER) {
+                const float* p = v[m >> 1] + 4 * (m & 1);
+                x[m] = pack2(p[0], p[2]); y[m] = pack2(p[1], p[3]);
+            } else {
+                x[m] = pack2(v[0][2 * m], v[0][2 * m + 1]); y[m] = pack2(v[1][2 * m], v[1][2 * m + 1]);
+            }
+        }
+    }
+    __device__ __forceinline__ void values(float (&v)[2][8]) const {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            const float2 a = unpack2(x[m]), b = unpack2(y[m]);
+            if constexpr (INTER) {
+                float* p = v[m >> 1] + 4 * (m & 1);
+                p[0] = a.x; p[1] = b.x; p[2] = a.y; p[3] = b.y;
+            } else {
+                v[0][2 * m] = a.x; v[0][2 * m + 1] = a.y; v[1][2 * m] = b.x; v[1][2 * m + 1] = b.y;
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ float max_abs(float m, float x) {      // a NaN stays one
+    float d;
+    asm("{\n\t.reg .f32 t;\n\tabs.f32 t, %2;\n\tmax.NaN.f32 %0, %1, t;\n\t}" : "=f"(d) : "f"(m), "f"(x));
+    return d;
+}
+
+constexpr int ROT_AHEAD = 4;           // places of a thread's ring
+enum Role : int { ROLE_Q, ROLE_K, ROLE_V };
+template <int V> struct IsRole { static constexpr int value = V; };
+
+template <typename T, typename O, int D, bool VEC, bool PAGED, bool INTER>
+__global__ void __launch_bounds__(ROT_THREADS, PAGED || sizeof(T) == 4 ? 2 : 3) rotary_kernel(RotArgs a) {
     constexpr int LPR = D / 16, GROUPS = ROT_THREADS / LPR;
-    extern __shared__ float2 s_cs[];                         // [token][pair]: cos, sin
+    constexpr bool RING = VEC && sizeof(T) == 2;
+    extern __shared__ __align__(16) float2 s_cs[];           // [token][pair]: cos, sin
     pdl_trigger();
     pdl_wait();
     const int lane = threadIdx.x & (LPR - 1), group = threadIdx.x / LPR, side = 1 << a.lanes_log2;
@@ -43,30 +90,56 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(RotArgs a) {
     const uint32_t t0 = block * tb, t = t0 + (uint32_t)(group >> a.lanes_log2);
     const bool token_there = t < a.tokens;
     const uint32_t b = token_there ? a.L.div(t) : 0, l = token_there ? t - b * a.L.d : 0;
-    const int rows = a.Hq + a.Hk + a.Hv, first = (int)part * side + (group & (side - 1)), step = side * a.parts;
+    const int step = side * a.parts, k_row = a.Hq, v_row = a.Hq + a.Hk, end = token_there ? v_row + a.Hv : 0;
     // pieces of a lane: 8 values each, from c0 * 8 and c1 * 8 on
     const int r16 = a.R >> 4;
-    const int c0 = a.inter ? lane : lane < r16 ? lane : 2 * lane, c1 = a.inter ? lane + LPR : lane < r16 ? lane + r16 : 2 * lane + 1;
+    const int c0 = INTER || lane < r16 ? lane : 2 * lane, c1 = INTER ? lane + LPR : lane < r16 ? lane + r16 : 2 * lane + 1, apart = (c1 - c0) * 8;
+    // the rows of a lane group, one after another: h = first, first + step, ...; where a row is, by steps while it stays one of q, k or v
+    auto row_at = [&](int h) -> const T* {
+        if (h < k_row) return reinterpret_cast<const T*>(a.q) + b * a.qs_b + l * a.qs_l + h * a.qs_h + c0 * 8;
+        if (h < v_row) return reinterpret_cast<const T*>(a.k) + b * a.ks_b + l * a.ks_l + (h - k_row) * a.ks_h + c0 * 8;
+        return reinterpret_cast<const T*>(a.v) + l * a.vs_l + (h - v_row) * a.vs_h + c0 * 8;
+    };
+    int h = (int)part * side + (group & (side - 1)), ahead = h, ahead_end = 0, stage = 0, ahead_stage = 0;
+    const T* next = nullptr;
+    long long next_step = 0;
+    // A thread's pieces of its next rows wait in shared memory, in places that only this thread writes and reads: several rows in flight without their registers.
+    // (fp32 rows, of whose pieces such a copy takes half sectors, and rows that are not 16-byte aligned are held in registers, one ahead.)
+    unsigned char* const ring = reinterpret_cast<unsigned char*>(s_cs + tb * half) + threadIdx.x * 16;
+    constexpr int STAGE = 2 * ROT_THREADS * 16;
+    Piece<T, VEC> held[2];
+    auto advance = [&]() {                                   // `next`: row `ahead`
+        next += next_step;
+        if (ahead < ahead_end || ahead >= end) return;
+        next = row_at(ahead);
+        next_step = step * (ahead < k_row ? a.qs_h : ahead < v_row ? a.ks_h : a.vs_h);
+        ahead_end = ahead < k_row ? k_row : ahead < v_row ? v_row : end;
+    };
+    auto request = [&]() {
+        advance();
+        if constexpr (RING) {
+            if (ahead < end) {
+                const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring + ahead_stage);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(next) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + ROT_THREADS * 16), "l"(next + apart) : "memory");
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            ahead_stage = ahead_stage == (ROT_AHEAD - 1) * STAGE ? 0 : ahead_stage + STAGE;
+        } else if (ahead < end) {
+            held[0].load(next);
+            held[1].load(next + apart);
+        }
+        ahead += step;
+    };
+#pragma unroll
+    for (int i = 0; i < (RING ? ROT_AHEAD - 1 : 1); ++i) request();
     long long slot = -1;
     if (PAGED && token_there) slot = __ldg(a.slots + t);
     const bool kept = PAGED && (unsigned long long)slot < ((unsigned long long)a.c.n_pages << a.c.page_shift);
 
-    Piece<T, VEC> f[U][2];
-    auto fetch = [&](int h, Piece<T, VEC> (&p)[2]) {
-        if (!token_there || h >= rows) return;
-        const T* x;
-        if (h < a.Hq) x = reinterpret_cast<const T*>(a.q) + b * a.qs_b + l * a.qs_l + h * a.qs_h;
-        else if (h < a.Hq + a.Hk) x = reinterpret_cast<const T*>(a.k) + b * a.ks_b + l * a.ks_l + (h - a.Hq) * a.ks_h;
-        else x = reinterpret_cast<const T*>(a.v) + l * a.vs_l + (h - a.Hq - a.Hk) * a.vs_h;
-        p[0].load(x + c0 * 8);
-        p[1].load(x + c1 * 8);
-    };
-#pragma unroll
-    for (int u = 0; u < U; ++u) fetch(first + u * step, f[u]);
-
     // ---- angles of the block's tokens
     for (int i = threadIdx.x; i < tb * half; i += ROT_THREADS) {
-        const int tk = i / half, p = i - tk * half;
+        const int tk = (int)a.half.div((uint32_t)i), p = i - tk * half;
         const uint32_t tt = t0 + tk;
         float s = 0.f, c = 1.f;
         if (tt < a.tokens) {
@@ -80,121 +153,150 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(RotArgs a) {
         s_cs[i] = make_float2(c, s);
     }
     __syncthreads();
-    // (cos, sin) of the lane's eight pairs
-    float cs[8], sn[8];
-    const float2* mine = s_cs + (group >> a.lanes_log2) * half;
-    const bool turn0 = a.inter ? c0 * 8 < a.R : lane < r16, turn1 = a.inter ? c1 * 8 < a.R : false;
+    // (cos, sin) of the lane's eight pairs; elements that do not turn are left alone (not multiplied by 1 and 0: an infinity would become NaN)
+    f32x2 cs[4], sn[4];
+    const bool turn0 = INTER ? c0 * 8 < a.R : lane < r16, turn1 = INTER ? c1 * 8 < a.R : turn0;
+    {
+        const float2* mine = s_cs + (group >> a.lanes_log2) * half;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float2 x = make_float2(1.f, 0.f);
-        if (a.inter) { if (i < 4 ? turn0 : turn1) x = mine[(i < 4 ? c0 * 4 : c1 * 4 - 4) + i]; }
-        else if (turn0) x = mine[lane * 8 + i];
-        cs[i] = x.x; sn[i] = x.y;
-    }
-    const int page_mask = (1 << a.c.page_shift) - 1;
-
-    auto work = [&](int h, const Piece<T, VEC> (&p)[2]) {
-        const bool there = token_there && h < rows, is_q = h < a.Hq, is_k = !is_q && h < a.Hq + a.Hk;
-        float v[2][8];
-        p[0].r.get(v[0]);
-        p[1].r.get(v[1]);
-        const float* w = is_q ? a.qw : a.kw;
-        const long long wh = is_q ? a.qw_h : a.kw_h, wd = is_q ? a.qw_d : a.kw_d;
-        const int head = is_q ? h : is_k ? h - a.Hq : h - a.Hq - a.Hk;
-        float factor = 1.f;
-        if (a.norm) {
-            float sum = 0.f;
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sum = fmaf(v[e][i], v[e][i], sum);
-#pragma unroll
-            for (int z = LPR / 2; z; z >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, z);
-            if (a.norm == VARQ_NORM_L2) {
-                const float length = sqrtf(sum);
-                factor = 1.f / (length < a.eps ? a.eps : length);      // (a NaN stays one)
-            } else factor = 1.f / sqrtf(sum * (1.f / D) + a.eps);
+        for (int m = 0; m < 4; ++m) {
+            float2 u = make_float2(1.f, 0.f), w = u;
+            if (m < 2 ? turn0 : turn1) {
+                const int p = INTER ? (m < 2 ? c0 * 4 + 2 * m : c1 * 4 + 2 * m - 4) : lane * 8 + 2 * m;
+                u = mine[p]; w = mine[p + 1];
+            }
+            cs[m] = pack2(u.x, w.x); sn[m] = pack2(u.y, w.y);
         }
-        if (is_q || is_k) {
-            if (w && there) {
-                if (wd == 0) {
-                    const float m = __ldg(w + head * wh);
+    }
+    const unsigned mask = ((1u << LPR) - 1u) << (threadIdx.x & 31 & ~(LPR - 1));      // the lanes of a row: they go the same way
+
+    auto rows_of = [&](auto role_) {
+        constexpr int ROLE = decltype(role_)::value;
+        constexpr bool CODES = PAGED && ROLE != ROLE_Q;
+        const int row0 = ROLE == ROLE_Q ? 0 : ROLE == ROLE_K ? k_row : v_row, behind = min(end, ROLE == ROLE_Q ? k_row : ROLE == ROLE_K ? v_row : end);
+        if (h >= behind) return;
+        const int head0 = h - row0;
+        // factors: one for a row, or one for every element, the same for all heads (held) or not (loaded with each row)
+        const float* w = ROLE == ROLE_Q ? a.qw : ROLE == ROLE_K ? a.kw : nullptr;
+        const long long wh = ROLE == ROLE_Q ? a.qw_h : a.kw_h, wd = ROLE == ROLE_Q ? a.qw_d : a.kw_d;
+        f32x2 wx[4], wy[4];
+        auto load_weights = [&](int head) {
+            float g[2][8];
+            const float* p = w + head * wh;
+            if (ROLE == ROLE_Q ? a.qw_vec : a.kw_vec) {
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
+                for (int e = 0; e < 2; ++e)
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[e][i] = v[e][i] * factor * m;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) v[e][i] = v[e][i] * factor * __ldg(w + head * wh + ((e ? c1 : c0) * 8 + i) * wd);
-                }
+                    for (int j = 0; j < 2; ++j) *reinterpret_cast<float4*>(&g[e][4 * j]) = __ldg(reinterpret_cast<const float4*>(p) + (e ? c1 : c0) * 2 + j);
             } else {
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[e][i] *= factor;
+                    for (int j = 0; j < 8; ++j) g[e][j] = __ldg(p + ((e ? c1 : c0) * 8 + j) * wd);
             }
-            if (a.inter) {
+            const Pairs<INTER> z(g);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    if (!(e ? turn1 : turn0)) continue;
+            for (int m = 0; m < 4; ++m) { wx[m] = z.x[m]; wy[m] = z.y[m]; }
+        };
+        const int weights = !w ? 0 : wd && !wh ? 1 : 2;        // none; held; of each head
+        if (weights == 1) load_weights(head0);
+        // where the rows go
+        O* out = nullptr;
+        long long out_step = 0;
+        size_t at = 0;
+        const int bits = ROLE == ROLE_V ? a.c.vb : a.c.kb;
+        if constexpr (CODES) {
+            const int page_mask = (1 << a.c.page_shift) - 1;
+            at = kept ? (((size_t)(slot >> a.c.page_shift) * a.c.H + head0) << a.c.page_shift) + ((uint32_t)slot & page_mask) : 0;
+            out_step = (long long)step << a.c.page_shift;
+        } else {
+            out = ROLE == ROLE_Q ? reinterpret_cast<O*>(a.qo) + b * a.qo_b + l * a.qo_l + head0 * a.qo_h : reinterpret_cast<O*>(a.ko) + b * a.ko_b + l * a.ko_l + head0 * a.ko_h;
+            out += c0 * 8;
+            out_step = step * (ROLE == ROLE_Q ? a.qo_h : a.ko_h);
+        }
+        const float most = paged_most(bits), most_inv = paged_most_inv(bits);
+#pragma unroll 1
+        for (; h < behind; h += step) {
+            Piece<T, VEC> f[2];
+            if constexpr (RING) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(ROT_AHEAD - 2) : "memory");
+                const uint4* from = reinterpret_cast<const uint4*>(ring + stage);
+                f[0].r.r = from[0];
+                f[1].r.r = from[ROT_THREADS];
+                stage = stage == (ROT_AHEAD - 1) * STAGE ? 0 : stage + STAGE;
+            } else { f[0] = held[0]; f[1] = held[1]; }
+            float v[2][8];
+            f[0].r.get(v[0]);
+            f[1].r.get(v[1]);
+            request();
+            if constexpr (ROLE != ROLE_V) {
+                Pairs<INTER> z(v);
+                float factor = 1.f;
+                if (a.norm) {
+                    f32x2 s0 = mul2(z.x[0], z.x[0]), s1 = mul2(z.y[0], z.y[0]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float x = v[e][2 * i], y = v[e][2 * i + 1], c = cs[4 * e + i], s = sn[4 * e + i];
-                        v[e][2 * i] = fmaf(x, c, -(y * s));
-                        v[e][2 * i + 1] = fmaf(y, c, x * s);
+                    for (int m = 1; m < 4; ++m) { s0 = fma2(z.x[m], z.x[m], s0); s1 = fma2(z.y[m], z.y[m], s1); }
+                    const float2 u = unpack2(s0), y = unpack2(s1);
+                    float sum = (u.x + u.y) + (y.x + y.y);
+#pragma unroll
+                    for (int n = LPR / 2; n; n >>= 1) sum += __shfl_xor_sync(mask, sum, n);
+                    sum = fmaf(sum, a.sum_mul, a.sum_add);     // a NaN stays one; 0 becomes 0 / eps
+                    factor = sum < a.least ? a.inv_eps : rsqrtf(sum);
+                }
+                if (weights) {
+                    if (weights == 2) {
+                        if (wd) load_weights(h - row0);
+                        else {
+                            const float g = __ldg(w + (h - row0) * wh);
+#pragma unroll
+                            for (int m = 0; m < 4; ++m) wx[m] = wy[m] = pack2(g, g);
+                        }
                     }
-                }
-            } else if (turn0) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float x = v[0][i], y = v[1][i], c = cs[i], s = sn[i];
-                    v[0][i] = fmaf(x, c, -(y * s));
-                    v[1][i] = fmaf(y, c, x * s);
+                    for (int m = 0; m < 4; ++m) { z.x[m] = mul2(z.x[m], wx[m]); z.y[m] = mul2(z.y[m], wy[m]); }
                 }
+                const f32x2 ff = pack2(factor, factor);
+#pragma unroll
+                for (int m = 0; m < 4; ++m) { z.x[m] = mul2(z.x[m], ff); z.y[m] = mul2(z.y[m], ff); }
+                auto turn = [&](int m) {
+                    const float2 xc = unpack2(mul2(z.x[m], cs[m])), u = unpack2(z.y[m]), s = unpack2(sn[m]);
+                    z.y[m] = fma2(z.y[m], cs[m], mul2(z.x[m], sn[m]));
+                    z.x[m] = pack2(fmaf(-u.x, s.x, xc.x), fmaf(-u.y, s.y, xc.y));
+                };
+                if constexpr (INTER) {
+                    if (turn0) { turn(0); turn(1); }
+                    if (turn1) { turn(2); turn(3); }
+                } else if (turn0) { turn(0); turn(1); turn(2); turn(3); }
+                z.values(v);
+            }
+            if constexpr (CODES) {
+                float top = 0.f;
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) top = max_abs(top, v[e][j]);
+#pragma unroll
+                for (int n = LPR / 2; n; n >>= 1) top = max_abs(top, __shfl_xor_sync(mask, top, n));
+                if (kept) {
+                    const PagedRow row(top, most, most_inv, a.qeps);
+                    int32_t* to = (ROLE == ROLE_V ? a.c.vc : a.c.kc) + at * (D * bits / 32);
+                    uint32_t q[2][8];
+                    row.codes(v, q);
+                    store_codes(to, c0, bits, q[0]);
+                    store_codes(to, c1, bits, q[1]);
+                    if (lane == 0) (ROLE == ROLE_V ? a.c.vs : a.c.ks)[at] = row.scale;
+                }
+                at += out_step;
+            } else {
+                store_vals<O, 8, VEC>(out, v[0], 8);
+                store_vals<O, 8, VEC>(out + apart, v[1], 8);
+                out += out_step;
             }
         }
-        if (PAGED) {
-            uint32_t m = 0;
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[e][i]) & 0x7fffffffu);
-#pragma unroll
-            for (int z = LPR / 2; z; z >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, z));
-            if (!is_q) {
-                if (!there || !kept) return;
-                const int bits = is_k ? a.c.kb : a.c.vb;
-                const uint32_t at = (((uint32_t)(slot >> a.c.page_shift) * a.c.H + head) << a.c.page_shift) + ((uint32_t)slot & page_mask);
-                const PagedRow row(__uint_as_float(m), paged_most(bits), paged_most_inv(bits), a.qeps);
-                int32_t* out = (is_k ? a.c.kc : a.c.vc) + (size_t)at * (D * bits / 32);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    uint32_t q[8];
-                    row.codes(v[e], q);
-                    store_codes(out, e ? c1 : c0, bits, q);
-                }
-                if (lane == 0) (is_k ? a.c.ks : a.c.vs)[at] = row.scale;
-                return;
-            }
-        }
-        if (!there) return;
-        O* o = is_q ? reinterpret_cast<O*>(a.qo) + b * a.qo_b + l * a.qo_l + head * a.qo_h : reinterpret_cast<O*>(a.ko) + b * a.ko_b + l * a.ko_l + head * a.ko_h;
-        store_vals<O, 8, VEC>(o + c0 * 8, v[0], 8);
-        store_vals<O, 8, VEC>(o + c1 * 8, v[1], 8);
     };
-    // every warp takes every turn: lanes without a row keep its shuffles company
-    for (int i = (int)part * side; i < rows; i += U * step) {
-        const int h = first + (i - (int)part * side);
-        Piece<T, VEC> g[U][2];
-#pragma unroll
-        for (int u = 0; u < U; ++u) fetch(h + (U + u) * step, g[u]);
-#pragma unroll
-        for (int u = 0; u < U; ++u) work(h + u * step, f[u]);
-#pragma unroll
-        for (int u = 0; u < U; ++u) { f[u][0] = g[u][0]; f[u][1] = g[u][1]; }
-    }
+    rows_of(IsRole<ROLE_Q>());
+    rows_of(IsRole<ROLE_K>());
+    if constexpr (PAGED) rows_of(IsRole<ROLE_V>());
 }
 
 int rotary_args(const char* who, RotArgs& a, const varq_rotary_t* r, int q_heads, int k_heads, int D) {
@@ -203,14 +305,18 @@ int rotary_args(const char* who, RotArgs& a, const varq_rotary_t* r, int q_heads
     if (r->n_axes < 1) return fail(VARQ_ERR_ARG, "%s: %d axes", who, r->n_axes);
     if (r->pos_bytes != 4 && r->pos_bytes != 8) return fail(VARQ_ERR_ARG, "%s: positions have 4 or 8 bytes (got %d)", who, r->pos_bytes);
     if (r->norm != VARQ_NORM_NONE && r->norm != VARQ_NORM_L2 && r->norm != VARQ_NORM_RMS) return fail(VARQ_ERR_ARG, "%s: norm %d", who, r->norm);
-    if (r->norm != VARQ_NORM_NONE && !(r->eps >= 1e-30f && r->eps < 1e30f)) return fail(VARQ_ERR_ARG, "%s: eps of the norm must lie in [1e-30, 1e30)", who);
+    if (r->norm != VARQ_NORM_NONE && !(r->eps >= 1e-18f && r->eps < 1e18f)) return fail(VARQ_ERR_ARG, "%s: eps of the norm must lie in [1e-18, 1e18)", who);
     if (q_heads < 0 || k_heads < 0) return fail(VARQ_ERR_ARG, "%s: %d query heads, %d key heads", who, q_heads, k_heads);
     a.turns = reinterpret_cast<const unsigned long long*>(r->turns); a.axis = r->axis; a.pos = r->positions;
     a.pos_bytes = r->pos_bytes; a.n_axes = r->n_axes; a.R = r->rotary_dim; a.inter = r->interleaved != 0;
     a.ps_a = r->pos_stride_axis; a.ps_b = r->pos_stride_b; a.ps_l = r->pos_stride_l;
-    a.norm = r->norm; a.eps = r->eps;
+    a.norm = r->norm;
+    a.inv_eps = 1.f / r->eps; a.least = r->norm == VARQ_NORM_L2 ? r->eps * r->eps : -1.f;
+    a.sum_mul = r->norm == VARQ_NORM_L2 ? 1.f : 1.f / (float)D; a.sum_add = r->norm == VARQ_NORM_L2 ? 0.f : r->eps;
+    a.half = FastDiv((uint32_t)r->rotary_dim / 2);
     a.qw = r->q_weight; a.qw_h = r->q_weight_stride_h; a.qw_d = r->q_weight_stride_d;
     a.kw = r->k_weight; a.kw_h = r->k_weight_stride_h; a.kw_d = r->k_weight_stride_d;
+    a.qw_vec = aligned16(a.qw) && a.qw_d == 1 && a.qw_h % 4 == 0; a.kw_vec = aligned16(a.kw) && a.kw_d == 1 && a.kw_h % 4 == 0;
     return VARQ_OK;
 }
 int rotary_pointers(const char* who, const RotArgs& a) {
@@ -231,7 +337,10 @@ template <typename T, typename O, int D, bool VEC, bool PAGED> int run_rotary(Ro
     const int tb = GROUPS >> a.lanes_log2;
     const unsigned long long blocks = ((unsigned long long)a.tokens + tb - 1) / tb * a.parts;
     if (blocks > 0x7fffffffull) return fail(VARQ_ERR_UNSUPPORTED, "varq_rotate: more than 2^31 thread blocks");
-    VARQ_CUDA_TRY(launch_pdl(rotary_kernel<T, O, D, VEC, PAGED, 2>, (unsigned)blocks, ROT_THREADS, (size_t)tb * (a.R / 2) * sizeof(float2), st, 1, a));
+    const size_t smem = (size_t)tb * (a.R / 2) * sizeof(float2) + (VEC && sizeof(T) == 2 ? ROT_AHEAD * 2 * ROT_THREADS * 16 : 0);
+    const auto kernel = a.inter ? rotary_kernel<T, O, D, VEC, PAGED, true> : rotary_kernel<T, O, D, VEC, PAGED, false>;
+    if (smem > 48 * 1024) VARQ_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    VARQ_CUDA_TRY(launch_pdl(kernel, (unsigned)blocks, ROT_THREADS, smem, st, 1, a));
     count_launches(1);
     return VARQ_OK;
 }

@@ -323,7 +323,7 @@ int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch_t* batch, 
 
 /* ---------------------------------------------------------------- norms and rotary positions
  * What happens to queries and keys in front of a cache: a norm per head and the rotation by position, in one pass.
- *   x <- x / max(|x|_2, eps) (L2), x / sqrt(mean x^2 + eps) (RMS) or x;  x <- x * weight[h][d];
+ *   x <- x / max(|x|_2, eps) (L2), x / sqrt(mean x^2 + eps) (RMS) or x (eps: 1e-18 to 1e18);  x <- x * weight[h][d];
  *   (a, b) <- (a cos t - b sin t, b cos t + a sin t), t = 2 pi * positions[axis of the pair] * turns of the pair
  * in fp32.  Pair i of rotary_dim / 2 is the elements (2i, 2i + 1) (interleaved) or (i, i + rotary_dim / 2); elements from rotary_dim on are not turned.
  *   turns : round(2^64 * frequency / (2 pi)), the frequency in radians per position; angles are exact to 2^-32 turns up to positions of 2^33, to position * 2^-65 turns behind

@@ -331,13 +331,16 @@ struct AttnPlan {
     int splits, tiles_per_split;       // tiles of 16 keys (decode kernel)
 };
 int paged_max_q(const varq_paged_batch_t* b) { return (int)(b->max_q < b->n_queries ? b->max_q : b->n_queries); }
-constexpr long long TREE_BLOCKS = 8000;
+// Trees: up to 32 rows of a head, and calls of little work in all (products of 16 rows and 16 keys), go to the decode kernel, the others to the tree kernel, us: 32 rows, 16
+// sequences of 1000 to 4000 keys, 8 heads x 128 66 / 58; 1 of 1000 13.0 / 15.5; 24 of up to 3000, 12 heads x 64 41 / 55; 64 rows, 1 sequence of 1000 (2000 products) 14.4 / 16.1, 1 of
+// 4000 with 104 rows (14000) 26 / 20; 40 rows, 8 of 300 (4200) 19.3 / 14.6, 4 of 1000 at 64 columns (2100 x 2) 19.9 / 15.5; 256 rows, 1 of 1000 (8700) 23 / 27.
+constexpr double TREE_BLOCKS = 4000;
 AttnPlan plan_attn(const varq_paged_t* c, const varq_paged_batch_t* b) {
     AttnPlan p{};
     const int max_q = paged_max_q(b), D = c->head_dim;
     const long long rows = (long long)max_q * (b->q_heads / c->n_heads);
     const long long seen = (long long)b->window + max_q + b->sinks, span = b->window && seen < b->max_kv ? seen : b->max_kv;      // keys of a CTA, about
-    const long long blocks16 = (long long)b->n_seqs * c->n_heads * ((rows + 15) / 16) * ((span + 15) / 16);      // products of 16 rows and 16 keys
+    const double blocks16 = (double)b->n_seqs * c->n_heads * ((rows + 15) / 16) * ((span + 15) / 16);      // products of 16 rows and 16 keys
     const bool many = b->tree ? rows > 32 && blocks16 > TREE_BLOCKS : rows > (D == 64 ? 80 : 32);
     p.tc = forced_attn_path() == VARQ_ATTN_PATH_TC || (forced_attn_path() != VARQ_ATTN_PATH_DECODE && many);
     p.rows = rows <= 8 ? 8 : rows > 16 && rows <= 24 && 4ll * b->n_seqs * c->n_heads >= sm_count() ? 24 : 16;
@@ -345,12 +348,13 @@ AttnPlan plan_attn(const varq_paged_t* c, const varq_paged_batch_t* b) {
     const int resident = p.tc ? 1 : p.rows > 16 ? (D == 128 ? 2 : 3) : p.rows > 8 ? (D == 128 ? 3 : 4) : D == 64 ? 5 : c->k_bits == 8 && c->v_bits == 8 ? 3 : 4;       // CTAs per SM
     const long long base = (long long)b->n_seqs * c->n_heads * (p.tc ? (rows + 255) / 256 : (rows + p.rows - 1) / p.rows), room = (long long)sm_count() * resident;
     // the number of parts that makes the waves of CTAs shortest, a CTA costing its tiles and a fixed part, parts in the workspace those, the second launch, too
-    const long long fixed = p.tc ? 4 : 16, least = p.tc ? 2 : 4, merge = p.tc ? 4 : 24;
+    const bool trees = b->tree && p.tc;
+    const long long fixed = trees ? 3 : p.tc ? 4 : 16, least = p.tc ? 2 : 4, merge = trees ? 2 : p.tc ? 4 : 24;
     long long best = 0;
     p.splits = 1; p.cluster = false;
     for (long long s = 1; s == 1 || (s <= tiles / least && s <= 256); ++s) {
         const bool near = !p.tc && s <= PAGED_CLUSTER && base * s <= room;
-        long long cost = (base * s + room - 1) / room * ((tiles + s - 1) / s + fixed + (s > 1 && p.tc ? fixed : 0)) + (s > 1 && !near ? merge : 0);
+        long long cost = (base * s + room - 1) / room * ((tiles + s - 1) / s + fixed + (s > 1 && p.tc && !trees ? fixed : 0)) + (s > 1 && !near ? merge : 0);
         if (b->tree && !p.tc) {                              // contexts differ: the longest part, or what all of them come to at three fifths of the longest
             const long long longest = (tiles + s - 1) / s + fixed, all = base * (tiles * 3 / 5 + s * fixed) / room;
             cost = (longest > all ? longest : all) + (s > 1 && !near ? merge : 0);

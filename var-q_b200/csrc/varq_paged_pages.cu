@@ -4,6 +4,11 @@
 // A page of a cache is four contiguous pieces (codes and scales of K and V, multiples of 64 bytes each); blocks take spans of a page's 16-byte units.
 // Tokens: a block takes one group (sequence) of moves of one head of one cache, chunk by chunk: all reads of a chunk, a barrier, all its writes.  What a later chunk reads
 // no earlier one writes, because no destination is the source of a later move.
+//
+// What bounds them (B200): their bytes, read and written.  301 pages of 64 tokens, 8 heads x 128, 8 and 4 bits, 16 caches: 986 MB in 148 us, 6.7 TB/s, the copy rate.
+// 16000 tokens of 8 sequences to other pages, 8 caches: 551 MB in 111 us, 5.0 TB/s; its blocks are chains of chunks (in registers, one after the other, 216 us).
+// Accepted paths of 64 sequences, one to six tokens, 32 caches: 15 us for 32 MB, 2048 blocks of three dependent loads each (a block per head 31 us).  Pages of
+// four sequences, 32 caches: 5.1 us, by bytes 5.3 (part of it stays in L2).
 #include "varq_paged.cuh"
 
 namespace varq {
@@ -27,12 +32,12 @@ struct CopyArgs {
 
 constexpr int COPY_THREADS = 256, COPY_UNITS = 8;      // 16-byte units of a thread
 
-__global__ void __launch_bounds__(COPY_THREADS) paged_copy_pages_kernel(const __grid_constant__ CopyArgs a) {
+// Block (x, y, cache): span y of page x, or, where pages are smaller than a block's units (MANY), `each` pages
+template <bool MANY>
+__global__ void __launch_bounds__(COPY_THREADS) paged_copy_pages_kernel(const __grid_constant__ CopyArgs a, int each) {
     pdl_trigger();
     pdl_wait();
     const CopyCache& c = a.c[blockIdx.z];
-    const long long src = __ldg(a.src + blockIdx.x), dst = __ldg(a.dst + blockIdx.x);
-    if ((unsigned long long)src >= (unsigned long long)c.n_pages || (unsigned long long)dst >= (unsigned long long)c.n_pages) return;
     const uint32_t tokens = (uint32_t)c.H << a.page_shift, ku = tokens * (c.krow / 16), vu = tokens * (c.vrow / 16), su = tokens / 4, all = ku + vu + 2 * su;
     const uint32_t u0 = blockIdx.y * (COPY_THREADS * COPY_UNITS) + threadIdx.x;
     uint4 x[COPY_UNITS];
@@ -44,97 +49,134 @@ __global__ void __launch_bounds__(COPY_THREADS) paged_copy_pages_kernel(const __
         if (u < su) return reinterpret_cast<uint4*>(c.ks) + (size_t)page * su + u;
         return reinterpret_cast<uint4*>(c.vs) + (size_t)page * su + (u - su);
     };
+    auto there = [&](long long src, long long dst) { return (unsigned long long)src < (unsigned long long)c.n_pages && (unsigned long long)dst < (unsigned long long)c.n_pages; };
+    if constexpr (MANY) {
+        const long long first = (long long)blockIdx.x * each;
+        const uint32_t here = (uint32_t)min((long long)each, a.n - first);
+        uint4* to[COPY_UNITS];                         // null: nothing to copy
 #pragma unroll
-    for (int i = 0; i < COPY_UNITS; ++i) {
-        const uint32_t u = u0 + i * COPY_THREADS;
-        if (u < all) x[i] = *at(u, src);
-    }
+        for (int i = 0; i < COPY_UNITS; ++i) {
+            const uint32_t v = u0 + i * COPY_THREADS, p = v / all, u = v - p * all;
+            to[i] = nullptr;
+            if (p < here) {
+                const long long src = __ldg(a.src + first + p), dst = __ldg(a.dst + first + p);
+                if (there(src, dst)) { x[i] = *at(u, src); to[i] = at(u, dst); }
+            }
+        }
 #pragma unroll
-    for (int i = 0; i < COPY_UNITS; ++i) {
-        const uint32_t u = u0 + i * COPY_THREADS;
-        if (u < all) *at(u, dst) = x[i];
+        for (int i = 0; i < COPY_UNITS; ++i)
+            if (to[i]) *to[i] = x[i];
+    } else {
+        const long long src = __ldg(a.src + blockIdx.x), dst = __ldg(a.dst + blockIdx.x);
+        if (!there(src, dst)) return;
+#pragma unroll
+        for (int i = 0; i < COPY_UNITS; ++i) {
+            const uint32_t u = u0 + i * COPY_THREADS;
+            if (u < all) x[i] = *at(u, src);
+        }
+#pragma unroll
+        for (int i = 0; i < COPY_UNITS; ++i) {
+            const uint32_t u = u0 + i * COPY_THREADS;
+            if (u < all) *at(u, dst) = x[i];
+        }
     }
 }
 
-constexpr int MOVE_THREADS = 256, MOVE_UNITS = 4, MOVE_ROWS = 64;      // 16-byte units of a thread, moves of a chunk at most
+constexpr int MOVE_THREADS = 256, MOVE_UNITS = 4;       // 16-byte units of a thread in a chunk
+struct MoveStage {
+    uint4 units[MOVE_UNITS * MOVE_THREADS];
+    float scales[MOVE_THREADS];
+    uint2 at[MOVE_THREADS];            // rows of the pools at head 0, source and destination; equal: nothing moves
+};
 
 // A block: one group, `heads` heads of one cache, K or V of it or both (parts).  A unit is 16 bytes of codes of a (move, head); a chunk is as many moves as fill the
-// threads' units.  The next chunk is read before this one is written, which is allowed for the same reason.
-__global__ void __launch_bounds__(MOVE_THREADS) paged_move_kernel(const __grid_constant__ CopyArgs a, int heads, int parts, int* status) {
-    __shared__ uint2 s_at[2][MOVE_ROWS];               // rows of the pools at head 0, source and destination; equal: nothing moves
+// threads' units, in shared memory on its way.  AHEAD 3: two chunks are being read while one is written; 1: groups of one chunk, more blocks on an SM.
+template <int AHEAD>
+__global__ void __launch_bounds__(MOVE_THREADS, AHEAD == 1 ? 6 : 4) paged_move_kernel(const __grid_constant__ CopyArgs a, int heads, int parts, int* status) {
+    extern __shared__ __align__(16) unsigned char move_smem[];
+    MoveStage* const stages = reinterpret_cast<MoveStage*>(move_smem);
     pdl_trigger();
     pdl_wait();
     const CopyCache& c = a.c[blockIdx.z];
-    const int g = blockIdx.x, h0 = ((int)blockIdx.y / parts) * heads, hn = min(heads, c.H - h0), part = (int)blockIdx.y % parts;
+    const int tid = threadIdx.x, g = blockIdx.x, h0 = ((int)blockIdx.y / parts) * heads, hn = min(heads, c.H - h0), part = (int)blockIdx.y % parts;
     if (hn <= 0) return;
     const int s0 = __ldg(a.starts + g), s1 = __ldg(a.starts + g + 1);
     const int begin = (int)min((long long)max(s0, 0), a.n), end = (int)min((long long)max(s1, begin), a.n);
-    if ((s0 != begin || s1 != end) && threadIdx.x == 0) atomicCAS(status, 0, PAGED_BAD_STARTS);
+    if ((s0 != begin || s1 != end) && tid == 0) atomicCAS(status, 0, PAGED_BAD_STARTS);
     if (begin == end) return;
     const long long n_slots = (long long)c.n_pages << a.page_shift;
-    const int page_mask = (1 << a.page_shift) - 1;
+    const int page_mask = (1 << a.page_shift) - 1, shift = a.page_shift;
     const int kp = part == 1 ? 0 : c.krow / 16, vp = parts == 2 && part == 0 ? 0 : c.vrow / 16;      // units of a row
-    const int per = (kp + vp) * hn, kinds = (kp > 0) + (vp > 0), rows = max(min(MOVE_ROWS, min(MOVE_UNITS * MOVE_THREADS / per, MOVE_THREADS / (kinds * hn))), 1);
-    // where this thread's units lie: (move of the chunk, offset in bytes behind the row at head 0), the same for every chunk; its scale likewise
-    int row[MOVE_UNITS], head[MOVE_UNITS], piece[MOVE_UNITS];
+    const int per = (kp + vp) * hn, kinds = (kp > 0) + (vp > 0), rows = max(min(MOVE_UNITS * MOVE_THREADS / per, MOVE_THREADS / (kinds * hn)), 1);
+    // this thread's units and its scale: move of the chunk (-1: none), head, piece
+    int row[MOVE_UNITS], piece[MOVE_UNITS];
+    uint32_t head[MOVE_UNITS];
 #pragma unroll
     for (int i = 0; i < MOVE_UNITS; ++i) {
-        const int u = threadIdx.x + i * MOVE_THREADS, in = u % per;
-        row[i] = u / per < rows ? u / per : MOVE_ROWS;
-        head[i] = h0 + in / (kp + vp);
-        piece[i] = in % (kp + vp);
+        const int u = tid + i * MOVE_THREADS, r = u / per, in = u - r * per, h = in / (kp + vp);
+        row[i] = r < rows ? r : -1;
+        head[i] = (uint32_t)(h0 + h) << shift;
+        piece[i] = in - h * (kp + vp);
     }
-    const int s_in = threadIdx.x % (kinds * hn), s_row = threadIdx.x / (kinds * hn) < rows ? (int)threadIdx.x / (kinds * hn) : MOVE_ROWS, s_head = h0 + s_in / kinds;
-    float* const scales = kinds == 2 ? (s_in & 1 ? c.vs : c.ks) : kp > 0 ? c.ks : c.vs;
+    const int s_r = tid / (kinds * hn), s_in = tid - s_r * (kinds * hn), s_row = s_r < rows ? s_r : -1;
+    const uint32_t s_head = (uint32_t)(h0 + s_in / kinds) << shift;
+    float* const scales = (kinds == 2 ? (s_in & 1) != 0 : kp == 0) ? c.vs : c.ks;
     auto unit = [&](int i, uint32_t at) -> uint4* {
-        const size_t r = (size_t)(at + ((uint32_t)head[i] << a.page_shift));
+        const size_t r = (size_t)(at + head[i]);
         return piece[i] < kp ? reinterpret_cast<uint4*>(c.kc + r * c.krow) + piece[i] : reinterpret_cast<uint4*>(c.vc + r * c.vrow) + (piece[i] - kp);
     };
     auto slots = [&](int m) -> uint2 {                 // of move m + this thread's number
-        uint2 r = make_uint2(0u, 0u);
-        if (threadIdx.x < rows && m + (int)threadIdx.x < end) {
-            const long long s = __ldg(a.src + m + threadIdx.x), d = __ldg(a.dst + m + threadIdx.x);
-            if ((unsigned long long)s < (unsigned long long)n_slots && (unsigned long long)d < (unsigned long long)n_slots) {
-                r.x = ((uint32_t)(s >> a.page_shift) * c.H << a.page_shift) + ((uint32_t)s & page_mask);
-                r.y = ((uint32_t)(d >> a.page_shift) * c.H << a.page_shift) + ((uint32_t)d & page_mask);
-            }
+        if (tid < rows && m < end - tid) {
+            const long long s = __ldg(a.src + m + tid), d = __ldg(a.dst + m + tid);
+            if ((unsigned long long)s < (unsigned long long)n_slots && (unsigned long long)d < (unsigned long long)n_slots)
+                return make_uint2(((uint32_t)(s >> shift) * c.H << shift) + ((uint32_t)s & page_mask), ((uint32_t)(d >> shift) * c.H << shift) + ((uint32_t)d & page_mask));
         }
-        return r;
+        return make_uint2(0u, 0u);
     };
-    uint4 x[MOVE_UNITS];
-    uint2 at[MOVE_UNITS], s_slot = make_uint2(0u, 0u);
-    float sc = 0.f;
-    auto read = [&](int buffer, uint4 (&v)[MOVE_UNITS], uint2 (&w)[MOVE_UNITS], float& f, uint2& fw) {
+    auto copy = [&](MoveStage& t) {
 #pragma unroll
         for (int i = 0; i < MOVE_UNITS; ++i) {
-            w[i] = row[i] < MOVE_ROWS ? s_at[buffer][row[i]] : make_uint2(0u, 0u);
-            if (w[i].x != w[i].y) v[i] = *unit(i, w[i].x);
+            const uint2 at = row[i] < 0 ? make_uint2(0u, 0u) : t.at[row[i]];
+            if (at.x != at.y)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(&t.units[tid + i * MOVE_THREADS])), "l"(unit(i, at.x)) : "memory");
         }
-        fw = s_row < MOVE_ROWS ? s_at[buffer][s_row] : make_uint2(0u, 0u);
-        if (fw.x != fw.y) f = scales[fw.x + ((uint32_t)s_head << a.page_shift)];
+        const uint2 at = s_row < 0 ? make_uint2(0u, 0u) : t.at[s_row];
+        if (at.x != at.y) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(&t.scales[tid])), "l"(scales + (at.x + s_head)) : "memory");
     };
     uint2 next = slots(begin);
-    if (threadIdx.x < rows) s_at[0][threadIdx.x] = next;
-    next = slots(begin + rows);
-    __syncthreads();
-    read(0, x, at, sc, s_slot);
-    for (int m0 = begin, buffer = 1; m0 < end; m0 += rows, buffer ^= 1) {
-        uint4 y[MOVE_UNITS];
-        uint2 bt[MOVE_UNITS], t_slot;
-        float tc = 0.f;
-        if (threadIdx.x < rows) s_at[buffer][threadIdx.x] = next;
-        next = slots(m0 + 2 * rows);
-        __syncthreads();                               // the slots of the next chunk are there, and this one is read by everybody
-        read(buffer, y, bt, tc, t_slot);
-        // (a later chunk's reads may pass this one's writes: they never meet)
-#pragma unroll
-        for (int i = 0; i < MOVE_UNITS; ++i)
-            if (at[i].x != at[i].y) *unit(i, at[i].y) = x[i];
-        if (s_slot.x != s_slot.y) scales[s_slot.y + ((uint32_t)s_head << a.page_shift)] = sc;
-#pragma unroll
-        for (int i = 0; i < MOVE_UNITS; ++i) { x[i] = y[i]; at[i] = bt[i]; }
-        sc = tc; s_slot = t_slot;
+#pragma unroll 1
+    for (int i = 0; i < AHEAD - 1; ++i) {
+        if (tid < rows) stages[i].at[tid] = next;
+        next = begin + (long long)(i + 1) * rows < end ? slots(begin + (i + 1) * rows) : make_uint2(0u, 0u);
+        __syncthreads();
+        copy(stages[i]);
+        asm volatile("cp.async.commit_group;" ::: "memory");
     }
+    int stage = 0;
+#pragma unroll 1
+    for (long long m0 = begin; m0 < end; m0 += rows) {
+        MoveStage &t = stages[stage], &ahead = stages[stage == 0 ? AHEAD - 1 : stage - 1];
+        if constexpr (AHEAD > 1) asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 2) : "memory");
+        __syncthreads();                               // (this chunk is read by everybody, and) the one before it written
+        if (tid < rows) ahead.at[tid] = next;
+        next = m0 + (long long)AHEAD * rows < end ? slots((int)m0 + AHEAD * rows) : make_uint2(0u, 0u);
+        __syncthreads();
+        copy(ahead);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if constexpr (AHEAD == 1) {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            __syncthreads();
+        }
+#pragma unroll
+        for (int i = 0; i < MOVE_UNITS; ++i) {
+            const uint2 at = row[i] < 0 ? make_uint2(0u, 0u) : t.at[row[i]];
+            if (at.x != at.y) *unit(i, at.y) = t.units[tid + i * MOVE_THREADS];
+        }
+        const uint2 at = s_row < 0 ? make_uint2(0u, 0u) : t.at[s_row];
+        if (at.x != at.y) scales[at.y + s_head] = t.scales[tid];
+        stage = stage == AHEAD - 1 ? 0 : stage + 1;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 int copy_caches(const char* who, const varq_paged_t* caches, int n_caches, CopyArgs& a, int from) {
@@ -148,10 +190,11 @@ int copy_caches(const char* who, const varq_paged_t* caches, int n_caches, CopyA
     }
     return VARQ_OK;
 }
+// all of them checked, and the first ones in `a`
 int check_caches(const char* who, const varq_paged_t* caches, int n_caches, CopyArgs& a) {
     if (n_caches < 0) return fail(VARQ_ERR_ARG, "%s: %d caches", who, n_caches);
     if (n_caches && !caches) return fail(VARQ_ERR_ARG, "%s: null caches", who);
-    for (int from = 0; from < n_caches; from += MOST_CACHES)
+    for (int from = n_caches > 0 ? (n_caches - 1) / MOST_CACHES * MOST_CACHES : 0; from >= 0; from -= MOST_CACHES)
         if (int rc = copy_caches(who, caches, n_caches, a, from)) return rc;
     return VARQ_OK;
 }
@@ -204,7 +247,7 @@ __global__ void __launch_bounds__(TREE_THREADS) paged_tree_kernel(TreeArgs a, in
 using namespace varq;
 
 extern "C" int varq_paged_copy_pages(const varq_paged_t* caches, int32_t n_caches, const int64_t* src_pages, const int64_t* dst_pages, int64_t n_pages, void* stream) {
-    CopyArgs a{};
+    CopyArgs a;
     if (int rc = check_caches("varq_paged_copy_pages", caches, n_caches, a)) return rc;
     if (n_pages < 0 || n_pages > 0x7fffffffLL) return fail(VARQ_ERR_ARG, "varq_paged_copy_pages: %lld pages", (long long)n_pages);
     if (n_pages == 0 || n_caches == 0) return VARQ_OK;
@@ -212,7 +255,8 @@ extern "C" int varq_paged_copy_pages(const varq_paged_t* caches, int32_t n_cache
     if (((uintptr_t)src_pages | (uintptr_t)dst_pages) % 8) return fail(VARQ_ERR_ARG, "varq_paged_copy_pages: misaligned pointer");
     a.src = reinterpret_cast<const long long*>(src_pages); a.dst = reinterpret_cast<const long long*>(dst_pages); a.n = n_pages;
     for (int from = 0; from < n_caches; from += MOST_CACHES) {
-        if (int rc = copy_caches("varq_paged_copy_pages", caches, n_caches, a, from)) return rc;
+        if (from)
+            if (int rc = copy_caches("varq_paged_copy_pages", caches, n_caches, a, from)) return rc;
         const int n = n_caches - from < MOST_CACHES ? n_caches - from : MOST_CACHES;
         unsigned long long units = 0;
         for (int i = 0; i < n; ++i) {
@@ -221,7 +265,9 @@ extern "C" int varq_paged_copy_pages(const varq_paged_t* caches, int32_t n_cache
         }
         const unsigned long long blocks = (units + COPY_THREADS * COPY_UNITS - 1) / (COPY_THREADS * COPY_UNITS);
         if (blocks > 65535) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_copy_pages: pages of 2 GB or more");
-        VARQ_CUDA_TRY(launch_pdl(paged_copy_pages_kernel, dim3((unsigned)n_pages, (unsigned)blocks, (unsigned)n), COPY_THREADS, 0, (cudaStream_t)stream, 1, a));
+        const int each = (int)(COPY_THREADS * COPY_UNITS / units > 1 ? COPY_THREADS * COPY_UNITS / units : 1);
+        VARQ_CUDA_TRY(launch_pdl(each > 1 ? paged_copy_pages_kernel<true> : paged_copy_pages_kernel<false>, dim3((unsigned)((n_pages + each - 1) / each), (unsigned)blocks, (unsigned)n),
+                                 COPY_THREADS, 0, (cudaStream_t)stream, 1, a, each));
         count_launches(1);
     }
     return VARQ_OK;
@@ -229,7 +275,7 @@ extern "C" int varq_paged_copy_pages(const varq_paged_t* caches, int32_t n_cache
 
 extern "C" int varq_paged_move_tokens(const varq_paged_t* caches, int32_t n_caches, const int64_t* src, const int64_t* dst, int64_t n_moves, const int32_t* starts,
                                       int32_t n_groups, int32_t max_moves, void* stream) {
-    CopyArgs a{};
+    CopyArgs a;
     if (int rc = check_caches("varq_paged_move_tokens", caches, n_caches, a)) return rc;
     if (n_moves < 0 || n_moves > 0x7fffffffLL || n_groups < 0 || max_moves < 0) return fail(VARQ_ERR_ARG, "varq_paged_move_tokens: %lld moves, %d groups, %d at most", (long long)n_moves, n_groups, max_moves);
     if (n_moves == 0 || n_caches == 0 || n_groups == 0) return VARQ_OK;
@@ -239,16 +285,29 @@ extern "C" int varq_paged_move_tokens(const varq_paged_t* caches, int32_t n_cach
     int* status = nullptr;
     if (int rc = paged_status_word(&status)) return rc;
     for (int from = 0; from < n_caches; from += MOST_CACHES) {
-        if (int rc = copy_caches("varq_paged_move_tokens", caches, n_caches, a, from)) return rc;
+        if (from)
+            if (int rc = copy_caches("varq_paged_move_tokens", caches, n_caches, a, from)) return rc;
         const int n = n_caches - from < MOST_CACHES ? n_caches - from : MOST_CACHES;
         int heads = 0;
         for (int i = 0; i < n; ++i) heads = a.c[i].H > heads ? a.c[i].H : heads;
         if (heads > 32767) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_move_tokens: %d heads (32767 at most)", heads);
-        // short groups: all heads in a block, up to 64 units of a thread's kind; long ones: a block per head, K and V apart
+        // short groups: as many heads in a block as its units hold; long ones: a block per head, K and V apart
         int each = 1;
-        while (each < heads && each < 64 && 2ll * each * max_moves <= 64) each *= 2;
+        while (each < heads && each < 64 && 2ll * each * max_moves <= MOVE_UNITS * MOVE_THREADS / 16) each *= 2;
         const int parts = each > 1 ? 1 : 2;
-        VARQ_CUDA_TRY(launch_pdl(paged_move_kernel, dim3((unsigned)n_groups, (unsigned)((heads + each - 1) / each * parts), (unsigned)n), MOVE_THREADS, 0, (cudaStream_t)stream, 1, a, each, parts, status));
+        const dim3 grid((unsigned)n_groups, (unsigned)((heads + each - 1) / each * parts), (unsigned)n);
+        if (each > 1 && 2ll * each * max_moves <= MOVE_UNITS * MOVE_THREADS / 8) {
+            VARQ_CUDA_TRY(launch_pdl(paged_move_kernel<1>, grid, MOVE_THREADS, sizeof(MoveStage), (cudaStream_t)stream, 1, a, each, parts, status));
+        } else {
+            static bool configured[64] = {false};
+            int dev = 0;
+            VARQ_CUDA_TRY(cudaGetDevice(&dev));
+            if (dev < 0 || dev >= 64 || !configured[dev]) {
+                VARQ_CUDA_TRY(cudaFuncSetAttribute(paged_move_kernel<3>, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * (int)sizeof(MoveStage)));
+                if (dev >= 0 && dev < 64) configured[dev] = true;
+            }
+            VARQ_CUDA_TRY(launch_pdl(paged_move_kernel<3>, grid, MOVE_THREADS, 3 * sizeof(MoveStage), (cudaStream_t)stream, 1, a, each, parts, status));
+        }
         count_launches(1);
     }
     return VARQ_OK;

@@ -9,7 +9,17 @@
 // behind is fp32, rounded once to the output's type, or to the code of the cache.
 //
 // D / 16 neighbouring lanes hold a row with two pieces of eight values each, chosen so that both values of a pair are in one lane.  The lanes of a
-// token share its angles, which the block computes once for all heads.
+// token share its angles, which the block computes once for all heads.  The next rows' pieces are on their way to shared memory (cp.async), three ahead, which keeps enough
+// bytes in flight without registers for them.
+//
+// What bounds it (B200): its bytes, as long as it only turns.  16384 tokens of 16 + 16 heads x 128, bf16, L2 norm: 268 MB in 46 us, 5.8 TB/s (41 us at the copy rate).  In front
+// of a cache issue: 16384 tokens of 32 + 8 + 8 heads, K in 8 bits, V in 4: 82 us, 55 by its bytes; some 310 instructions for a row and warp, where the quantized rows
+// take twice those of a query's.  A few tokens: a launch, 3.5 us for 16.  On the way (first case / last one): values one by one in registers, one row ahead 72 / 111 us;
+// pairs of fp32 in one instruction 53 / 111; rows copied ahead 46 / 109; a loop for each of q, k and v, with addresses by steps 46 / 89; registers for two blocks
+// on an SM instead of three where rows are quantized 46 / 82.  fp32 rows, whose pieces such copies would take half a sector at a time, are held one ahead: 36.9
+// us for 8192 tokens of 16 + 4 heads, 44 with copies.
+#include <type_traits>
+
 #include "varq_paged_rows.cuh"
 
 namespace varq {
@@ -74,6 +84,25 @@ __device__ __forceinline__ float max_abs(float m, float x) {      // a NaN stays
 }
 
 constexpr int ROT_AHEAD = 4;           // places of a thread's ring
+__device__ __forceinline__ float rsqrt_normal(float x) {          // of a normal number, an infinity or a NaN
+    float y;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// eight values, rounded once; two conversions in an instruction
+template <typename O, bool VEC> __device__ __forceinline__ void store_piece(O* p, const float (&v)[8]) {
+    if constexpr (sizeof(O) == 4 || !VEC) store_vals<O, 8, VEC>(p, v, 8);
+    else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same<O, __half>::value) { const __half2 x = __floats2half2_rn(v[2 * i], v[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t*>(&x); }
+            else { const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t*>(&x); }
+        }
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
 enum Role : int { ROLE_Q, ROLE_K, ROLE_V };
 template <int V> struct IsRole { static constexpr int value = V; };
 
@@ -198,8 +227,8 @@ __global__ void __launch_bounds__(ROT_THREADS, PAGED || sizeof(T) == 4 ? 2 : 3) 
 #pragma unroll
             for (int m = 0; m < 4; ++m) { wx[m] = z.x[m]; wy[m] = z.y[m]; }
         };
-        const int weights = !w ? 0 : wd && !wh ? 1 : 2;        // none; held; of each head
-        if (weights == 1) load_weights(head0);
+        const int weights = !w ? 0 : !wd ? 1 : !wh ? 2 : 3;    // none; one for a row; held; of each head
+        if (weights == 2) load_weights(head0);
         // where the rows go
         O* out = nullptr;
         long long out_step = 0;
@@ -241,17 +270,11 @@ __global__ void __launch_bounds__(ROT_THREADS, PAGED || sizeof(T) == 4 ? 2 : 3) 
 #pragma unroll
                     for (int n = LPR / 2; n; n >>= 1) sum += __shfl_xor_sync(mask, sum, n);
                     sum = fmaf(sum, a.sum_mul, a.sum_add);     // a NaN stays one; 0 becomes 0 / eps
-                    factor = sum < a.least ? a.inv_eps : rsqrtf(sum);
+                    factor = sum < a.least ? a.inv_eps : rsqrt_normal(sum);
                 }
-                if (weights) {
-                    if (weights == 2) {
-                        if (wd) load_weights(h - row0);
-                        else {
-                            const float g = __ldg(w + (h - row0) * wh);
-#pragma unroll
-                            for (int m = 0; m < 4; ++m) wx[m] = wy[m] = pack2(g, g);
-                        }
-                    }
+                if (weights == 1) factor *= __ldg(w + (h - row0) * wh);
+                else if (weights) {
+                    if (weights == 3) load_weights(h - row0);
 #pragma unroll
                     for (int m = 0; m < 4; ++m) { z.x[m] = mul2(z.x[m], wx[m]); z.y[m] = mul2(z.y[m], wy[m]); }
                 }
@@ -288,8 +311,8 @@ __global__ void __launch_bounds__(ROT_THREADS, PAGED || sizeof(T) == 4 ? 2 : 3) 
                 }
                 at += out_step;
             } else {
-                store_vals<O, 8, VEC>(out, v[0], 8);
-                store_vals<O, 8, VEC>(out + apart, v[1], 8);
+                store_piece<O, VEC>(out, v[0]);
+                store_piece<O, VEC>(out + apart, v[1]);
                 out += out_step;
             }
         }
@@ -325,12 +348,14 @@ int rotary_pointers(const char* who, const RotArgs& a) {
     return VARQ_OK;
 }
 
-// Rows of a token side by side: four (neighbours in memory, one warp's worth at 128 columns) where the tokens alone fill the chip, more where they are few.
+// Rows of a token side by side: four (neighbours in memory, one warp's worth at 128 columns) where the tokens alone give every SM some warps, more where they are few: a row
+// more on a group of lanes spreads its angles and addresses over more rows, a group more keeps more rows in flight.  Threads per SM from which on it is four, us for
+// 300 / 1000 tokens of 32 + 4 and of 48 rows: rotate 256: 4.0 / 6.3, 512: 3.9 / 6.5, 1024: 4.1 / 8.2 (1777 tokens 9.3 / 8.1 / 9.3); append 256: 5.8 / 8.7, 512: 8.2 / 10.6.
 template <typename T, typename O, int D, bool VEC, bool PAGED> int run_rotary(RotArgs& a, cudaStream_t st) {
     constexpr int LPR = D / 16, GROUPS = ROT_THREADS / LPR;
     const int rows = a.Hq + a.Hk + a.Hv;
     int lanes = 4;
-    while (lanes < rows && (unsigned long long)a.tokens * lanes * LPR < 1024ull * sm_count()) lanes *= 2;
+    while (lanes < rows && (unsigned long long)a.tokens * lanes * LPR < (PAGED ? 256ull : 512ull) * sm_count()) lanes *= 2;
     a.lanes_log2 = 0;
     while ((1 << a.lanes_log2) < lanes && (1 << a.lanes_log2) < GROUPS) ++a.lanes_log2;
     a.parts = lanes > GROUPS ? lanes / GROUPS : 1;
@@ -339,7 +364,6 @@ template <typename T, typename O, int D, bool VEC, bool PAGED> int run_rotary(Ro
     if (blocks > 0x7fffffffull) return fail(VARQ_ERR_UNSUPPORTED, "varq_rotate: more than 2^31 thread blocks");
     const size_t smem = (size_t)tb * (a.R / 2) * sizeof(float2) + (VEC && sizeof(T) == 2 ? ROT_AHEAD * 2 * ROT_THREADS * 16 : 0);
     const auto kernel = a.inter ? rotary_kernel<T, O, D, VEC, PAGED, true> : rotary_kernel<T, O, D, VEC, PAGED, false>;
-    if (smem > 48 * 1024) VARQ_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     VARQ_CUDA_TRY(launch_pdl(kernel, (unsigned)blocks, ROT_THREADS, smem, st, 1, a));
     count_launches(1);
     return VARQ_OK;
@@ -360,7 +384,7 @@ using namespace varq;
 
 extern "C" int varq_rotate(const varq_rotary_t* r, const varq_tensor_t* q, const varq_tensor_t* k, int32_t B, int32_t L, int32_t q_heads, int32_t k_heads,
                            int32_t head_dim, const varq_tensor_t* q_out, const varq_tensor_t* k_out, void* stream) {
-    RotArgs a{};
+    RotArgs a = RotArgs();
     if (head_dim != 64 && head_dim != 128) return fail(VARQ_ERR_UNSUPPORTED, "varq_rotate: head_dim %d is not 64 or 128", head_dim);
     if (int rc = rotary_args("varq_rotate", a, r, q_heads, k_heads, head_dim)) return rc;
     if (!q || !k || !q_out || !k_out) return fail(VARQ_ERR_ARG, "varq_rotate: null descriptor");
@@ -388,7 +412,7 @@ extern "C" int varq_rotate(const varq_rotary_t* r, const varq_tensor_t* q, const
 
 extern "C" int varq_paged_append_rotated(const varq_paged_t* cache, const varq_rotary_t* r, const varq_tensor_t* q, const varq_tensor_t* k, const varq_tensor_t* v,
                                          const int64_t* slots, int64_t n_tokens, int32_t q_heads, float eps, const varq_tensor_t* q_out, void* stream) {
-    RotArgs a{};
+    RotArgs a = RotArgs();
     if (int rc = paged_check_cache("varq_paged_append_rotated", cache, a.c)) return rc;
     if (int rc = rotary_args("varq_paged_append_rotated", a, r, q_heads, a.c.H, a.c.D)) return rc;
     if (n_tokens < 0) return fail(VARQ_ERR_ARG, "varq_paged_append_rotated: %lld tokens", (long long)n_tokens);

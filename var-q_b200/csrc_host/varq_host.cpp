@@ -417,18 +417,21 @@ long long int_arg(PyObject* o, long long lo, long long hi, const char* name) {
 varq_paged_t paged_desc(PyObject* const* a, const at::Tensor*& kc) {
     static const char* const names[4] = {"k_codes", "v_codes", "k_scale", "v_scale"};
     const at::Tensor* t[4];
+    c10::IntArrayRef first;
     for (int i = 0; i < 4; ++i) {
         t[i] = &tensor_arg(a[i], names[i]);
-        need(t[i]->is_contiguous() && t[i]->dim() == (i < 2 ? 4 : 3) && t[i]->scalar_type() == (i < 2 ? at::kInt : at::kFloat),
+        const c10::IntArrayRef size = t[i]->sizes();
+        need(t[i]->is_contiguous() && size.size() == (i < 2 ? 4u : 3u) && t[i]->scalar_type() == (i < 2 ? at::kInt : at::kFloat),
              "the pools are contiguous int32 codes [pages, heads, page_size, words] and fp32 scales [pages, heads, page_size]");
-        on_device(*t[i], *t[0], names[i]);
-        for (int d = 0; d < 3; ++d) need(t[i]->size(d) == t[0]->size(d) && t[i]->size(d) <= INT32_MAX, "the pools differ in pages, heads or page size");
+        if (i == 0) first = size;
+        else on_device(*t[i], *t[0], names[i]);
+        for (int d = 0; d < 3; ++d) need(size[d] == first[d] && size[d] <= INT32_MAX, "the pools differ in pages, heads or page size");
     }
     const long long D = int_arg(a[4], 1, 4096, "head_dim");
     varq_paged_t c;
     c.k_codes = t[0]->data_ptr<int32_t>(); c.v_codes = t[1]->data_ptr<int32_t>();
     c.k_scale = t[2]->data_ptr<float>(); c.v_scale = t[3]->data_ptr<float>();
-    c.n_pages = (int)t[0]->size(0); c.n_heads = (int)t[0]->size(1); c.page_size = (int)t[0]->size(2); c.head_dim = (int)D;
+    c.n_pages = (int)first[0]; c.n_heads = (int)first[1]; c.page_size = (int)first[2]; c.head_dim = (int)D;
     c.k_bits = (int)(t[0]->size(3) * 32 / D); c.v_bits = (int)(t[1]->size(3) * 32 / D);
     need(c.k_bits * D == t[0]->size(3) * 32 && c.v_bits * D == t[1]->size(3) * 32, "words per row do not match head_dim");
     kc = t[0];
@@ -574,6 +577,7 @@ PyObject* py_paged_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
 std::vector<varq_paged_t> caches_arg(PyObject* o, const at::Tensor*& first) {
     if (!PyList_Check(o)) throw Refuse(PyExc_TypeError, "caches must be a list");
     std::vector<varq_paged_t> c;
+    c.reserve(PyList_GET_SIZE(o));
     first = nullptr;
     for (Py_ssize_t i = 0; i < PyList_GET_SIZE(o); ++i) {
         PyObject* p = PyList_GET_ITEM(o, i);

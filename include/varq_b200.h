@@ -297,9 +297,6 @@ int varq_paged_read(const varq_paged_t* cache, const int64_t* slots, int64_t n_t
  * sees nothing.  With n_queries, n_seqs or max_q 0 a call writes nothing.  Starts must not decrease; where they do, or where a sequence has more than max_q
  * queries, code 64 is left and rows in between are not defined.
  * Entries of block_table for pages behind the last token, or for pages in which no query of the sequence sees a key, may hold anything.
- *   tree != NULL (causal = 1) : the queries of a sequence are drafted tokens, no chain.  tree is int32 [n_queries][tree_words], 32 * tree_words >= max_q;
- *                bit i % 32 of word i / 32 of a query's row says whether it sees drafted token i of its sequence (its own bit, too).  It sees the tokens before the
- *                drafted ones, with a window (>= max_q) as at position kv_lens[b] - n + (bits of its row) - 1.  Zero-initialised: no tree
  * Query head i uses head i / (q_heads / n_heads) of the cache.  max_q bounds the queries of a sequence, max_kv is the longest kv_lens (a
  * hint: it decides how the work is split).
  * A sequence has 2^31 - 4096 tokens at most.  The device checks what the host cannot see: starts, lengths and page numbers outside their bounds are clamped into them and leave a
@@ -309,8 +306,6 @@ typedef struct {
     int64_t table_stride, n_queries;
     int32_t table_pages, n_seqs, q_heads, max_q, max_kv, causal, window, sinks;
     float softmax_scale;
-    int32_t tree_words;
-    const int32_t* tree;
 } varq_paged_batch_t;
 
 /* out = softmax(q k^T * softmax_scale) v over the pages; q and out (1, n_queries, q_heads, head_dim), fp16 or bf16 (one type).  lse (or
@@ -320,6 +315,13 @@ typedef struct {
 size_t varq_paged_attn_workspace_bytes(const varq_paged_t* cache, const varq_paged_batch_t* batch);
 int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch_t* batch, const varq_tensor_t* q, const varq_tensor_t* out, float* lse,
                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same where the queries of a sequence are drafted tokens, no chain (causal = 1).  tree: int32 [n_queries][tree_words], 32 * tree_words >= max_q; bit i % 32 of
+ * word i / 32 of a query's row says whether it sees drafted token i of its sequence (its own bit, too).  It sees the tokens before the drafted ones, with a window
+ * (>= max_q) as at position kv_lens[b] - n + (bits of its row) - 1. */
+size_t varq_paged_attn_tree_workspace_bytes(const varq_paged_t* cache, const varq_paged_batch_t* batch);
+int varq_paged_attn_tree(const varq_paged_t* cache, const varq_paged_batch_t* batch, const int32_t* tree, int32_t tree_words, const varq_tensor_t* q,
+                         const varq_tensor_t* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------- norms and rotary positions
  * What happens to queries and keys in front of a cache: a norm per head and the rotation by position, in one pass.
@@ -354,7 +356,7 @@ int varq_rotate(const varq_rotary_t* r, const varq_tensor_t* q, const varq_tenso
 int varq_paged_append_rotated(const varq_paged_t* cache, const varq_rotary_t* r, const varq_tensor_t* q, const varq_tensor_t* k, const varq_tensor_t* v,
                               const int64_t* slots, int64_t n_tokens, int32_t q_heads, float eps, const varq_tensor_t* q_out, void* stream);
 
-/* Masks and positions of drafted tokens from their parents, for the tree of a varq_paged_batch_t: token i of the n drafted tokens of sequence b is row
+/* Masks and positions of drafted tokens from their parents, for varq_paged_attn_tree: token i of the n drafted tokens of sequence b is row
  * q_starts[b] + i; parents (int32 [n_tokens]) gives the number of its parent in its sequence, smaller than i, or -1 for a child of the context.
  *   masks     int32 [n_tokens][words], 32 * words >= max_q : bits of the token's ancestors among the drafted tokens and its own
  *   positions int32 [n_tokens] : kv_lens[b] - n + number of ancestors

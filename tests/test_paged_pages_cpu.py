@@ -1,4 +1,5 @@
 """Forked, cut and compacted sequences, rotary tables, refusals of the C entries: what needs no GPU."""
+import ctypes
 import math
 
 import pytest
@@ -215,9 +216,11 @@ def test_refusals_and_empty_calls_of_copies_and_trees():
     assert lib.varq_paged_tree(256, 256, 256, 1, 4, 33, 1, 256, 256, None) == -1 and b"words" in lib.varq_last_error()
     assert lib.varq_paged_tree(None, 256, 256, 1, 4, 4, 1, 256, 256, None) == -1 and lib.varq_paged_tree(256, None, 256, 1, 4, 4, 1, 256, 256, None) == -1
     assert lib.varq_paged_tree(256, 256, 256, -1, 4, 4, 1, 256, 256, None) == -1 and lib.varq_paged_tree(256, 256, 258, 1, 4, 4, 1, 256, 256, None) == -1
-    batch = _cabi.PagedBatch(256, 256, 256, 4, 6, 4, 2, 4, 3, 64, 1, 0, 0, 0.125, 1, 256)
     cache, _, t = descriptors()
-    for field, value, word in (("causal", 0, b"causal"), ("tree_words", 0, b"words"), ("window", 2, b"window"), ("tree", 258, b"misaligned")):
-        batch = _cabi.PagedBatch(256, 256, 256, 4, 6, 4, 2, 4, 3, 64, 1, 0, 0, 0.125, 1, 256)
+    for tree, words, field, value, word in ((256, 1, "causal", 0, b"causal"), (256, 0, "window", 0, b"words"), (256, 1, "window", 2, b"window"),
+                                            (258, 1, "window", 0, b"misaligned"), (None, 1, "window", 0, b"null")):
+        batch = _cabi.PagedBatch(256, 256, 256, 4, 6, 4, 2, 4, 3, 64, 1, 0, 0, 0.125)
         setattr(batch, field, value)
-        assert lib.varq_paged_attn(cache, batch, t, t, None, None, 0, None) == -1 and word in lib.varq_last_error()
+        assert lib.varq_paged_attn_tree(cache, batch, tree, words, t, t, None, None, 0, None) == -1 and word in lib.varq_last_error()
+    # the descriptor of a batch is what it was: who calls varq_paged_attn with it needs no new one
+    assert ctypes.sizeof(_cabi.PagedBatch) == 80

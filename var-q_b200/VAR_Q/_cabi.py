@@ -23,7 +23,7 @@ SYMBOLS = (
     "varq_quant_static_scratch_bytes", "varq_unpack_dequant",
     "varq_attn_workspace_bytes", "varq_attn_fwd", "varq_attn_force_path",
     "varq_qk_norm_stats", "varq_quant_pack_prestats", "varq_attn_fwd_qnorm", "varq_append", "varq_append_workspace_bytes",
-    "varq_paged_append", "varq_paged_read", "varq_paged_attn", "varq_paged_attn_workspace_bytes",
+    "varq_paged_append", "varq_paged_read", "varq_paged_attn", "varq_paged_attn_workspace_bytes", "varq_paged_attn_tree", "varq_paged_attn_tree_workspace_bytes",
     "varq_rotate", "varq_paged_append_rotated", "varq_paged_tree", "varq_paged_copy_pages", "varq_paged_move_tokens",
 )
 
@@ -59,7 +59,7 @@ class PagedBatch(ctypes.Structure):
                 ("table_stride", ctypes.c_int64), ("n_queries", ctypes.c_int64),
                 ("table_pages", ctypes.c_int32), ("n_seqs", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("max_q", ctypes.c_int32),
                 ("max_kv", ctypes.c_int32), ("causal", ctypes.c_int32), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32),
-                ("softmax_scale", ctypes.c_float), ("tree_words", ctypes.c_int32), ("tree", ctypes.c_void_p)]
+                ("softmax_scale", ctypes.c_float)]
 
 
 class Rotary(ctypes.Structure):
@@ -126,6 +126,10 @@ def _declare(lib):
     lib.varq_paged_attn_workspace_bytes.argtypes = [P, B]
     lib.varq_paged_attn.restype = i32
     lib.varq_paged_attn.argtypes = [P, B, T, T, vp, vp, sz, vp]
+    lib.varq_paged_attn_tree_workspace_bytes.restype = sz
+    lib.varq_paged_attn_tree_workspace_bytes.argtypes = [P, B]
+    lib.varq_paged_attn_tree.restype = i32
+    lib.varq_paged_attn_tree.argtypes = [P, B, vp, i32, T, T, vp, vp, sz, vp]
     R = ctypes.POINTER(Rotary)
     lib.varq_rotate.restype = i32
     lib.varq_rotate.argtypes = [R, T, T, i32, i32, i32, i32, i32, T, T, vp]

@@ -335,27 +335,27 @@ int paged_max_q(const varq_paged_batch_t* b) { return (int)(b->max_q < b->n_quer
 // sequences of 1000 to 4000 keys, 8 heads x 128 66 / 58; 1 of 1000 13.0 / 15.5; 24 of up to 3000, 12 heads x 64 41 / 55; 64 rows, 1 sequence of 1000 (2000 products) 14.4 / 16.1, 1 of
 // 4000 with 104 rows (14000) 26 / 20; 40 rows, 8 of 300 (4200) 19.3 / 14.6, 4 of 1000 at 64 columns (2100 x 2) 19.9 / 15.5; 256 rows, 1 of 1000 (8700) 23 / 27.
 constexpr double TREE_BLOCKS = 4000;
-AttnPlan plan_attn(const varq_paged_t* c, const varq_paged_batch_t* b) {
+AttnPlan plan_attn(const varq_paged_t* c, const varq_paged_batch_t* b, bool tree) {
     AttnPlan p{};
     const int max_q = paged_max_q(b), D = c->head_dim;
     const long long rows = (long long)max_q * (b->q_heads / c->n_heads);
     const long long seen = (long long)b->window + max_q + b->sinks, span = b->window && seen < b->max_kv ? seen : b->max_kv;      // keys of a CTA, about
     const double blocks16 = (double)b->n_seqs * c->n_heads * ((rows + 15) / 16) * ((span + 15) / 16);      // products of 16 rows and 16 keys
-    const bool many = b->tree ? rows > 32 && blocks16 > TREE_BLOCKS : rows > (D == 64 ? 80 : 32);
+    const bool many = tree ? rows > 32 && blocks16 > TREE_BLOCKS : rows > (D == 64 ? 80 : 32);
     p.tc = forced_attn_path() == VARQ_ATTN_PATH_TC || (forced_attn_path() != VARQ_ATTN_PATH_DECODE && many);
     p.rows = rows <= 8 ? 8 : rows > 16 && rows <= 24 && 4ll * b->n_seqs * c->n_heads >= sm_count() ? 24 : 16;
     const long long unit = p.tc ? 128 : 16, tiles = span > unit ? (span + unit - 1) / unit : 1;
     const int resident = p.tc ? 1 : p.rows > 16 ? (D == 128 ? 2 : 3) : p.rows > 8 ? (D == 128 ? 3 : 4) : D == 64 ? 5 : c->k_bits == 8 && c->v_bits == 8 ? 3 : 4;       // CTAs per SM
     const long long base = (long long)b->n_seqs * c->n_heads * (p.tc ? (rows + 255) / 256 : (rows + p.rows - 1) / p.rows), room = (long long)sm_count() * resident;
     // the number of parts that makes the waves of CTAs shortest, a CTA costing its tiles and a fixed part, parts in the workspace those, the second launch, too
-    const bool trees = b->tree && p.tc;
+    const bool trees = tree && p.tc;
     const long long fixed = trees ? 3 : p.tc ? 4 : 16, least = p.tc ? 2 : 4, merge = trees ? 2 : p.tc ? 4 : 24;
     long long best = 0;
     p.splits = 1; p.cluster = false;
     for (long long s = 1; s == 1 || (s <= tiles / least && s <= 256); ++s) {
         const bool near = !p.tc && s <= PAGED_CLUSTER && base * s <= room;
         long long cost = (base * s + room - 1) / room * ((tiles + s - 1) / s + fixed + (s > 1 && p.tc && !trees ? fixed : 0)) + (s > 1 && !near ? merge : 0);
-        if (b->tree && !p.tc) {                              // contexts differ: the longest part, or what all of them come to at three fifths of the longest
+        if (tree && !p.tc) {                              // contexts differ: the longest part, or what all of them come to at three fifths of the longest
             const long long longest = (tiles + s - 1) / s + fixed, all = base * (tiles * 3 / 5 + s * fixed) / room;
             cost = (longest > all ? longest : all) + (s > 1 && !near ? merge : 0);
         }
@@ -369,17 +369,16 @@ size_t part_floats(const AttnPlan& p, const varq_paged_t* c, const varq_paged_ba
     return p.splits > 1 && !p.cluster ? (size_t)p.splits * b->n_queries * b->q_heads * (c->head_dim + 2) : 0;
 }
 
-}  // namespace
-
-extern "C" size_t varq_paged_attn_workspace_bytes(const varq_paged_t* cache, const varq_paged_batch_t* batch) {
+size_t attn_workspace(const varq_paged_t* cache, const varq_paged_batch_t* batch, bool tree) {
     if (!cache || !batch || cache->n_heads < 1 || batch->q_heads < cache->n_heads || batch->n_seqs < 1 || batch->n_queries < 1 || batch->max_q < 1 || batch->max_kv < 0 ||
         batch->window < 0 || batch->sinks < 0 || cache->head_dim < 1)
         return 0;
-    return part_floats(plan_attn(cache, batch), cache, batch) * sizeof(float);
+    return part_floats(plan_attn(cache, batch, tree), cache, batch) * sizeof(float);
 }
 
-extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch_t* batch, const varq_tensor_t* q, const varq_tensor_t* out, float* lse,
-                               void* workspace, size_t workspace_bytes, void* stream) {
+// tree null: the queries of a sequence are a chain
+int attn(const varq_paged_t* cache, const varq_paged_batch_t* batch, const int32_t* tree, int tree_words, const varq_tensor_t* q, const varq_tensor_t* out, float* lse,
+         void* workspace, size_t workspace_bytes, void* stream) {
     PagedAttnArgs a;
     if (int rc = paged_check_cache("varq_paged_attn", cache, a.c)) return rc;
     if (!batch || !q || !out) return fail(VARQ_ERR_ARG, "varq_paged_attn: null descriptor");
@@ -391,12 +390,12 @@ extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch
     if (batch->window < 0 || batch->sinks < 0) return fail(VARQ_ERR_ARG, "varq_paged_attn: window %d, sinks %d", batch->window, batch->sinks);
     if (batch->window && !batch->causal) return fail(VARQ_ERR_ARG, "varq_paged_attn: a window needs causal attention");
     if (batch->sinks && !batch->window) return fail(VARQ_ERR_ARG, "varq_paged_attn: sinks need a window");
-    if (batch->tree) {
+    if (tree) {
         if (!batch->causal) return fail(VARQ_ERR_ARG, "varq_paged_attn: a tree needs causal attention");
-        if (batch->tree_words < 0 || batch->tree_words > (1 << 26) || 32ll * batch->tree_words < batch->max_q)
-            return fail(VARQ_ERR_ARG, "varq_paged_attn: %d words of a tree's mask for %d tokens of a sequence", batch->tree_words, batch->max_q);
+        if (tree_words < 0 || tree_words > (1 << 26) || 32ll * tree_words < batch->max_q)
+            return fail(VARQ_ERR_ARG, "varq_paged_attn: %d words of a tree's mask for %d tokens of a sequence", tree_words, batch->max_q);
         if (batch->window && batch->window < batch->max_q) return fail(VARQ_ERR_ARG, "varq_paged_attn: a window of %d is shorter than trees of %d tokens", batch->window, batch->max_q);
-        if ((uintptr_t)batch->tree % 4) return fail(VARQ_ERR_ARG, "varq_paged_attn: misaligned pointer");
+        if ((uintptr_t)tree % 4) return fail(VARQ_ERR_ARG, "varq_paged_attn: misaligned pointer");
     }
     if (!(batch->softmax_scale > 0.f && batch->softmax_scale < 1e30f)) return fail(VARQ_ERR_ARG, "varq_paged_attn: softmax_scale must be positive and finite");
     if (batch->n_seqs > 65535) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_attn: %d sequences (65535 at most)", batch->n_seqs);
@@ -417,8 +416,8 @@ extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch
     a.scale_log2 = batch->softmax_scale * 1.4426950408889634f;
     a.causal = batch->causal != 0; a.window = batch->window;
     a.sinks = batch->sinks < PAGED_MOST_KEYS ? batch->sinks : PAGED_MOST_KEYS;      // more tokens than there are: all of them
-    a.tree = batch->tree; a.tree_words = batch->tree ? batch->tree_words : 0;
-    const AttnPlan p = plan_attn(cache, batch);
+    a.tree = tree; a.tree_words = tree ? tree_words : 0;
+    const AttnPlan p = plan_attn(cache, batch, tree != nullptr);
     const size_t need = part_floats(p, cache, batch) * sizeof(float);
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
         return fail(VARQ_ERR_WORKSPACE, "varq_paged_attn: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
@@ -428,4 +427,18 @@ extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch
     if (int rc = paged_status_word(&status)) return rc;      // the kernels write to it: no launch without it
     if (int rc = p.tc ? (a.tree ? paged_attn_tree_run : paged_attn_tc_run)(a, p.splits, ws_o, ws_ml, status, st) : (a.tree ? paged_attn_decode_tree_run : paged_attn_decode_run)(a, p.rows, p.splits, p.cluster, p.tiles_per_split, ws_o, ws_ml, status, st)) return rc;
     return need ? paged_attn_merge_run(a, p.splits, ws_o, ws_ml, st) : VARQ_OK;
+}
+
+}  // namespace
+
+extern "C" size_t varq_paged_attn_workspace_bytes(const varq_paged_t* cache, const varq_paged_batch_t* batch) { return attn_workspace(cache, batch, false); }
+extern "C" int varq_paged_attn(const varq_paged_t* cache, const varq_paged_batch_t* batch, const varq_tensor_t* q, const varq_tensor_t* out, float* lse,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+    return attn(cache, batch, nullptr, 0, q, out, lse, workspace, workspace_bytes, stream);
+}
+extern "C" size_t varq_paged_attn_tree_workspace_bytes(const varq_paged_t* cache, const varq_paged_batch_t* batch) { return attn_workspace(cache, batch, true); }
+extern "C" int varq_paged_attn_tree(const varq_paged_t* cache, const varq_paged_batch_t* batch, const int32_t* tree, int32_t tree_words, const varq_tensor_t* q,
+                                    const varq_tensor_t* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!tree) return fail(VARQ_ERR_ARG, "varq_paged_attn_tree: null tree");
+    return attn(cache, batch, tree, tree_words, q, out, lse, workspace, workspace_bytes, stream);
 }

@@ -511,7 +511,7 @@ PyObject* py_paged_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
          "q_starts must be a contiguous int32 vector with one entry more than kv_lens");
     need(table.dim() == 2 && table.scalar_type() == at::kInt && table.size(0) == lens.size(0) && (table.stride(1) == 1 || table.size(1) < 2) && table.size(1) <= INT32_MAX,
          "block_table must be int32 [sequences, pages] with contiguous rows");
-    varq_paged_batch_t b{};
+    varq_paged_batch_t b;
     b.q_starts = starts.data_ptr<int32_t>(); b.kv_lens = lens.data_ptr<int32_t>(); b.block_table = table.data_ptr<int32_t>();
     b.table_stride = table.stride(0); b.n_queries = q.size(0); b.table_pages = (int)table.size(1);
     need(lens.size(0) <= INT32_MAX, "too many sequences");
@@ -525,6 +525,8 @@ PyObject* py_paged_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     b.causal = causal;
     b.window = a[13] == Py_None ? 0 : (int)int_arg(a[13], 1, INT32_MAX, "window");
     b.sinks = (int)int_arg(a[14], 0, INT32_MAX, "sinks");
+    const int32_t* masks = nullptr;
+    int words = 0;
     if (a[16] != Py_None) {
         const at::Tensor& tree = on_device(tensor_arg(a[16], "tree"), *kc, "tree");
         need(tree.dim() == 2 && tree.scalar_type() == at::kInt && tree.size(0) == q.size(0) && tree.is_contiguous() && tree.size(1) <= (1 << 26),
@@ -532,7 +534,7 @@ PyObject* py_paged_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
         need(tree.size(1) * 32 >= std::min<long long>(b.max_q, q.size(0)), "tree has fewer bits a row than max_q");
         need(causal, "a tree needs causal attention");
         if (tree.size(1) == 0) b.max_q = 0;
-        else { b.tree = tree.data_ptr<int32_t>(); b.tree_words = (int)tree.size(1); b.max_q = (int)std::min<long long>(b.max_q, std::max<long long>(q.size(0), 1)); }
+        else { masks = tree.data_ptr<int32_t>(); words = (int)tree.size(1); b.max_q = (int)std::min<long long>(b.max_q, std::max<long long>(q.size(0), 1)); }
     }
     const c10::DeviceIndex dev = kc->device().index();
     const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, dev));
@@ -546,9 +548,12 @@ PyObject* py_paged_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     if (b.max_q == 0) b.max_q = 1;                     // the rows' zeros are written on the device, where the starts are checked
     const varq_tensor_t qd = rows_desc(q), od = rows_desc(out);
-    const size_t ws = varq_paged_attn_workspace_bytes(&c, &b);
+    const size_t ws = (masks ? varq_paged_attn_tree_workspace_bytes : varq_paged_attn_workspace_bytes)(&c, &b);
     const at::Tensor buf = scratch(ws, dev);
-    const int rc = varq_paged_attn(&c, &b, &qd, &od, with_lse ? lse.data_ptr<float>() : nullptr, scratch_ptr(buf), ws, c10::cuda::getCurrentCUDAStream(dev).stream());
+    float* const lse_ptr = with_lse ? lse.data_ptr<float>() : nullptr;
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev).stream();
+    const int rc = masks ? varq_paged_attn_tree(&c, &b, masks, words, &qd, &od, lse_ptr, scratch_ptr(buf), ws, stream)
+                         : varq_paged_attn(&c, &b, &qd, &od, lse_ptr, scratch_ptr(buf), ws, stream);
     if (rc != VARQ_OK) return raise(rc);
     return with_lse ? make_pair(out, lse) : THPVariable_Wrap(out);
     GUARD_PAGED_END

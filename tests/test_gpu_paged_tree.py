@@ -274,6 +274,113 @@ def test_captured_and_replayed(path):
     assert _cabi.device_status() == 0
 
 
+@pytest.mark.parametrize("seqs,heads,counts,lens", [
+    (24, 8, [0, 36, 1, 20], [0, 300, 300, 77, 1, 640]),                      # more blocks than multiprocessors, sequences ranked by length: equal ones, empty ones
+    (32, 5, [5, 33], [64, 65, 400]), (33, 5, [5, 33], [64, 65, 400]),        # as many as are ranked, and more
+])
+def test_many_sequences_of_different_lengths(seqs, heads, counts, lens, path):
+    """also as a padded batch, whose rows in front and behind are the first and the last sequence's"""
+    D, counts = 64, [counts[i % len(counts)] for i in range(seqs)]
+    kv = [lens[i % len(lens)] if counts[i] == 0 else lens[i % len(lens)] + counts[i] for i in range(seqs)]
+    b = Trees(kv, heads, D, 4, 8, page=16, seed=seqs)
+    see = [ancestors(some_tree(c, c + i)) for i, c in enumerate(counts)]
+    n, front, behind = sum(counts), 3, 70
+    tree = torch.cat([torch.full((front, 2), -1, dtype=torch.int32), *(pack(s, 2) for s in see), torch.full((behind, 2), -1, dtype=torch.int32)]).to(DEV)
+    q = queries(front + n + behind, heads, D)
+    got = b.check(q[front:front + n], counts, tree=tree[front:front + n], see=see)
+    starts = torch.tensor([front + sum(counts[:i]) for i in range(seqs + 1)], dtype=torch.int32, device=DEV)
+    out, lse = b.cache.attend(q, b.table.to(DEV), b.kv_dev, starts, max(counts), max(kv), D ** -0.5, return_lse=True, tree=tree)
+    assert torch.equal(out[front:front + n], got[0]) and torch.equal(lse[front:front + n], got[1])
+    for rows in (slice(0, front), slice(front + n, None)):
+        assert (out[rows] == 0).all() and (lse[rows] == -math.inf).all()
+    assert _cabi.device_status() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kb", [8, 4, 2])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("pad,at", [(1, 1), (8, 0), (8, 3)])
+def test_queries_at_any_address(D, kb, dtype, pad, at, path):
+    counts = [26, 4]
+    b = Trees([130, 40], 2, D, kb, 8, page=16, seed=kb)
+    see = [ancestors(some_tree(c, c)) for c in counts]
+    q = queries(30, 10, D + pad, dtype)[:, :, at:at + D]
+    b.check(q, counts, out=b.attend(q, counts, D ** -0.5, tree=torch.cat([pack(s, 1) for s in see]).to(DEV)), see=see)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kb", [8, 4, 2])
+@pytest.mark.parametrize("gain", [2.0 ** -40, 2.0 ** -8, 2.0 ** 9, 2.0 ** 30])
+def test_queries_of_any_size(D, kb, gain, path):
+    """bf16 queries beyond fp16's range, next to rows of zeros and ordinary ones, at scores of ordinary size"""
+    counts = [40, 26]
+    b = Trees([300, 90], 2, D, kb, 4, page=16, seed=kb)
+    see = [ancestors(some_tree(c, c)) for c in counts]
+    q = queries(66, 8, D, torch.bfloat16, gain=gain)
+    q[3::7] = 0
+    q[5::7] *= 2.0 ** (-3 if gain > 1 else 3)
+    b.check(q, counts, D ** -0.5 / gain, tree=torch.cat([pack(s, 2) for s in see]).to(DEV), see=see)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_queries_that_are_no_numbers(dtype, value, path):
+    """spoil their own row"""
+    counts, D = [40, 26], 128
+    b = Trees([300, 90], 2, D, page=16, seed=1)
+    tree = torch.cat([pack(ancestors(some_tree(c, c)), 2) for c in counts]).to(DEV)
+    q = queries(66, 8, D, dtype)
+    ref, ref_lse = b.attend(q, counts, D ** -0.5, tree=tree)
+    bad = torch.zeros((66, 8), dtype=torch.bool, device=DEV)
+    bad[7, 3] = bad[41, 0] = bad[65, 7] = True
+    q[7, 3, 5] = q[41, 0, 0] = q[65, 7, 127] = value
+    out, lse = b.attend(q, counts, D ** -0.5, tree=tree)
+    assert torch.equal(out[~bad], ref[~bad]) and torch.equal(lse[~bad], ref_lse[~bad])
+    assert not torch.isfinite(lse[bad]).any() if math.isnan(value) else True
+    assert torch.isnan(out[bad]).all() if math.isnan(value) else not (out[bad] == ref[bad]).all()
+    assert _cabi.device_status() == 0
+
+
+@pytest.mark.parametrize("kv,counts", [([4, 30, 0], [9, 30, 6]), ([70, 3], [90, 60])])
+def test_fewer_tokens_than_queries(kv, counts, path):
+    """the first drafted tokens are not in the cache"""
+    b = Trees(kv, 2, 64, page=16, seed=1)
+    b.run(counts, 2, 64)
+
+
+def test_two_streams_and_two_graphs(path):
+    """calls in parts, whose partial results lie in workspaces, next to each other"""
+    D, counts = 128, [16, 64]
+    b = Trees([6000, 3000], 1, D, 8, 4, page=64, seed=1)
+    tree = torch.cat([pack(ancestors(some_tree(c, c)), 2) for c in counts]).to(DEV)
+    qs = [queries(80, 4, D, seed=s) for s in (1, 2)]
+    refs = [b.attend(q, counts, D ** -0.5, tree=tree) for q in qs]
+    table, starts = b.table.to(DEV), torch.tensor([0, 16, 80], dtype=torch.int32, device=DEV)
+    call = lambda q: b.cache.attend(q, table, b.kv_dev, starts, 64, 6000, D ** -0.5, return_lse=True, tree=tree)
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(call(qs[i]))
+    graphs = []
+    torch.cuda.synchronize()
+    for q in qs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call(q)
+        graphs.append((graph, out))
+    for _ in range(20):
+        for s, (graph, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for ref, mine, (_, out) in zip(refs, got, graphs):
+        assert all(torch.equal(x, y) for r in mine + [out] for x, y in zip(ref, r))
+    assert _cabi.device_status() == 0
+
+
 def test_refusals():
     b = Trees([40], 2, 64)
     q = queries(10, 2, 64)

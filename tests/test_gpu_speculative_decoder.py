@@ -86,6 +86,11 @@ def test_refusals():
         with pytest.raises(ValueError, match="parent"):
             model.verify(["x"], [inputs(1, 1)], parents)
     assert model.table.length("x") == 5
+    model = make(window=8)
+    model.step(["x"], [inputs(5, 1)])
+    with pytest.raises(ValueError, match="window"):                        # before its tokens have taken any room
+        model.verify(["x"], [inputs(9, 1)], [[-1] * 9])
+    assert model.table.length("x") == 5
     with pytest.raises(ValueError, match="rotary"):
         StandInDecoder(depth=1, width=64, heads=1, kv_heads=1, qk_norm="l2")
     with pytest.raises(ValueError, match="axis"):

@@ -131,7 +131,7 @@ class StandInDecoder(torch.nn.Module):
             raise ValueError(f"[VAR-Q]: the decoder's tokens have one axis of positions, not {rotary.n_axes}")
         self.table, self.device_ = PageTable(num_pages, page_size), device
         self.caches = [PagedCache(num_pages, page_size, kv_heads, head_dim, k_bits, v_bits, device) for _ in range(depth)]
-        self.rotary = rotary
+        self.rotary, self.window = rotary, window
         self.blocks = torch.nn.ModuleList(StandInDecoderBlock(width, heads, kv_heads, head_dim, c, window, sinks, rotary, qk_norm) for c in self.caches)
         self.to(device)
 
@@ -168,6 +168,8 @@ class StandInDecoder(torch.nn.Module):
         last token).  They stay in the cache until ``accept`` says which of them are the sequence's next ones."""
         if len(parents) != len(xs) or any(len(p) != x.size(0) or any(not -1 <= a < i for i, a in enumerate(p)) for p, x in zip(parents, xs)):
             raise ValueError("[VAR-Q]: a parent per drafted token, -1 or the number of an earlier one")
+        if self.window and any(x.size(0) > self.window for x in xs):
+            raise ValueError(f"[VAR-Q]: drafts of more tokens than the window of {self.window}")
         return self._run(seqs, xs, torch.tensor([a for p in parents for a in p], dtype=torch.int32, device=self.device_))
 
     @torch.inference_mode()

@@ -165,6 +165,27 @@ def test_streams_and_graphs():
     assert same(cs, expected)
 
 
+def test_pools_of_more_than_two_to_the_31_words():
+    page, H, D = 64, 8, 128
+    pages = 2 ** 31 // (H * page * D // 4) + 3
+    cs = [PagedCache(pages, page, H, D, 8, 8)]
+    for pool in pools(cs[0]):
+        pool.zero_()
+        pool[-2].random_()
+        pool[1].random_()
+    first, last = ([p[i].clone() for p in pools(cs[0])] for i in (1, -2))
+    copy_pages(cs, longs([pages - 2, 1]), longs([0, pages - 1]))
+    for p, a, z in zip(pools(cs[0]), first, last):
+        assert torch.equal(p[0], z) and torch.equal(p[-1], a) and not p[2].any() and not p[-3].any()
+    src, dst = [(pages - 2) * page + i for i in range(3, 64)], [2 * page + i for i in range(61)]
+    for most in (61, 1):
+        move_tokens(cs, longs(src + [page + 5]), longs(dst + [(pages - 3) * page + 63]), torch.tensor([0, 61, 62], dtype=torch.int32, device=DEV), most)
+        for p, a, z in zip(pools(cs[0]), first, last):
+            assert torch.equal(p[2, :, :61], z[:, 3:]) and not p[2, :, 61:].any() and torch.equal(p[-3, :, 63], a[:, 5]) and not p[-3, :, :63].any()
+            p[2] = p[-3] = 0
+    assert _cabi.device_status() == 0
+
+
 def test_refusals():
     a, b = caches(1, 4, 16)[0], caches(1, 4, 32)[0]
     one = longs([1])

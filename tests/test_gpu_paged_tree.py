@@ -8,7 +8,7 @@ import torch
 
 from test_gpu_paged_attention import BITS, DEV, Batch, queries
 from VAR_Q import _cabi
-from VAR_Q.paged import draft_tree
+from VAR_Q.paged import PagedCache, draft_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -378,6 +378,24 @@ def test_two_streams_and_two_graphs(path):
     torch.cuda.synchronize()
     for ref, mine, (_, out) in zip(refs, got, graphs):
         assert all(torch.equal(x, y) for r in mine + [out] for x, y in zip(ref, r))
+    assert _cabi.device_status() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_pools_of_more_than_two_to_the_31_words(D, path):
+    counts = [40, 3]
+    b = Trees([300, 70], 8, D, page=64, seed=1)
+    tree = torch.cat([pack(ancestors(some_tree(c, c)), 2) for c in counts]).to(DEV)
+    q = queries(43, 16, D)
+    ref = b.attend(q, counts, D ** -0.5, tree=tree)
+    small, pages = b.cache, 2 ** 31 // (8 * 64 * D // 4) + 16
+    b.cache = PagedCache(pages, 64, 8, D, 8, 8)
+    assert b.cache.k_codes.numel() > 2 ** 31
+    last = pages - small.k_codes.shape[0]
+    for name in ("k_codes", "v_codes", "k_scale", "v_scale"):
+        getattr(b.cache, name)[last:] = getattr(small, name)
+    b.table = torch.where(b.table >= 0, b.table + last, b.table)
+    assert all(torch.equal(x, y) for x, y in zip(ref, b.attend(q, counts, D ** -0.5, tree=tree)))
     assert _cabi.device_status() == 0
 
 

@@ -276,6 +276,39 @@ def test_streams_and_graphs():
     assert torch.equal(out, rot.rotate(q, k, pos, norm="rms")[0])
 
 
+def test_offsets_behind_two_to_the_31():
+    rot, heads, few = Rotary(128, interleaved=True), 32, 50
+    tokens = 2 ** 31 // (heads * 128) + few
+    last = rows(few, heads + 2, 128, dtype=torch.bfloat16)
+    q, pos = torch.zeros((tokens, heads + 2, 128), dtype=torch.bfloat16, device=DEV), torch.arange(tokens, device=DEV)
+    q[-few:] = last
+    ref = rot.rotate(last[:, :heads], last[:, heads:], pos[-few:], norm="l2")
+    for got, x in zip(rot.rotate(q[:, :heads], q[:, heads:], pos, norm="l2"), ref):
+        assert torch.equal(got[-few:], x) and not got[:few].any()
+    del q, got
+    page = 64
+    pages = 2 ** 31 // (2 * page * 128 // 4) + 3                            # a pool of as many words
+    far, near = PagedCache(pages, page, 2, 128), PagedCache(1, page, 2, 128)
+    slots = torch.arange(few, device=DEV)
+    q, k = last[:, :heads], last[:, heads:]
+    out = [c.append_rotated(q, k, k, slots + at, rot, pos[-few:], norm="l2") for c, at in ((near, 0), (far, (pages - 1) * page))]
+    assert torch.equal(*out) and torch.equal(out[0], ref[0])
+    for a, b in ((near.k_codes, far.k_codes), (near.v_codes, far.v_codes), (near.k_scale, far.k_scale), (near.v_scale, far.v_scale)):
+        assert torch.equal(a[0, :, :few], b[-1, :, :few])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_shared_rows(dtype):
+    """strides of zero: one row for all tokens, or for all heads"""
+    rot = Rotary(64, rotary_dim=48)
+    x, pos = rows(1, 1, 64, dtype=dtype), torch.arange(30, device=DEV) * 1000
+    q, k = x.expand(30, 5, 64), x[0].expand(30, 2, 64)
+    got, ref = rot.rotate(q, k, pos, norm="rms"), rot.rotate(q.contiguous(), k.contiguous(), pos, norm="rms")
+    assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    at = pos[:1].expand(30)
+    assert all(torch.equal(a, b) for a, b in zip(rot.rotate(q, k, at), rot.rotate(q, k, at.contiguous())))
+
+
 # ------------------------------------------------------------------------------------------------ in front of an image schedule
 @pytest.mark.parametrize("fmt", ["BLHc", "BHLc"])
 def test_a_schedule_with_two_axes(fmt):

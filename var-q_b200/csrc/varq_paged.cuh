@@ -92,8 +92,22 @@ __device__ __forceinline__ uint32_t paged_tree_bits(const PagedAttnArgs& a, int 
     auto word = [&](int w) { return w < 0 ? ~0u : w < a.tree_words ? (uint32_t)__ldg(row + w) : 0u; };
     return __funnelshift_r(word(rel >> 5), word((rel >> 5) + 1), rel & 31);
 }
-__device__ __forceinline__ bool paged_tree_bit(const PagedAttnArgs& a, int token, int rel) {
-    return rel < 0 || (rel < 32 * a.tree_words && (__ldg(a.tree + (long long)token * a.tree_words + (rel >> 5)) >> (rel & 31) & 1));
+
+// The CTAs of much work begin first: the sequence with the `rank`-th most of it (the earlier one of equals), of up to PAGED_RANKED, by one warp.  Work: tiles of
+// `rows` query rows times keys.
+constexpr int PAGED_RANKED = 32;
+__device__ __forceinline__ int paged_ranked(const PagedAttnArgs& a, int rank, int rows) {
+    const int lane = threadIdx.x & 31;
+    unsigned long long key = 0;        // all different, 0 behind the last sequence
+    if (lane < a.B) {
+        const long long nq = min(max((long long)__ldg(a.q_starts + lane + 1) - __ldg(a.q_starts + lane), 0ll), (long long)a.max_q), kv = max(__ldg(a.kv_lens + lane), 0);
+        const long long seen = a.window ? min(kv, (long long)a.window + a.sinks + nq) : kv;
+        key = (unsigned long long)(min((nq * a.G + rows - 1) / rows, 1ll << 24) * seen) * 32 + (31 - lane) + 1;
+    }
+    int above = 0;
+#pragma unroll 8
+    for (int j = 0; j < 32; ++j) above += __shfl_sync(0xffffffffu, key, j) > key ? 1 : 0;
+    return __ffs(__ballot_sync(0xffffffffu, lane < a.B && above == rank)) - 1;
 }
 
 // Query rows in front of the first sequence's and behind the last one's belong to no sequence.  They get zeros and -inf, as rows that see nothing: from the CTAs of

@@ -108,9 +108,12 @@ template <int BITS, int NW> __device__ __forceinline__ void pd_join(const uint32
 // A call, and behind the keys' loop: inlined in front of it, it took 1.3 % of a long call
 __device__ __noinline__ void pd_pad(PagedPad p, long long i, long long step) { paged_pad(p, i, step); }
 
+template <int KB, int VB, int D, int NT> constexpr int PD_CTAS = NT > 2 ? (D == 128 ? 2 : 3) : NT > 1 ? (D == 128 ? 3 : 4) : D == 128 ? (KB == 8 && VB == 8 ? 3 : 4) : 5;      // on an SM
+
+// ranked (TREE): the CTAs of the sequences with most work begin first
 template <int KB, int VB, int D, int NT, bool TREE>
-__global__ void __launch_bounds__(PD_WARPS * 32, NT > 2 ? (D == 128 ? 2 : 3) : NT > 1 ? (D == 128 ? 3 : 4) : D == 128 ? (KB == 8 && VB == 8 ? 3 : 4) : 5)
-paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, int* status) {
+__global__ void __launch_bounds__(PD_WARPS * 32, PD_CTAS<KB, VB, D, NT>)
+paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_cluster, int tiles_per_split, float* ws_o, float* ws_ml, int* status, int ranked) {
     using P = PdPlan<KB, VB, D>;
     constexpr int KBYTES = D / 4 * KB / 8, VBYTES = D / 8 * VB / 8;       // of a row and thread
     constexpr int KROW = P::KROW, VROW = P::VROW, ST = P::ST;
@@ -123,7 +126,8 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
     const int split = (int)(blockIdx.x % (unsigned)splits);
     const unsigned item = blockIdx.x / (unsigned)splits;
-    const int rt = (int)(item % (unsigned)n_rowtiles), bh = (int)(item / (unsigned)n_rowtiles), b = bh / a.c.H, h = bh - b * a.c.H;
+    const int rt = (int)(item % (unsigned)n_rowtiles), bh = (int)(item / (unsigned)n_rowtiles), rank = bh / a.c.H, h = bh - rank * a.c.H;
+    const int b = TREE && ranked ? paged_ranked(a, rank, ROWS) : rank;
     const PagedSeq seq = paged_seq(a, b, status);
     const int rows = seq.nq * a.G, row0 = rt * ROWS, p_first = seq.kv - seq.nq;
     if (row0 >= rows && !paged_pad_any(a, seq, b)) return;
@@ -137,20 +141,71 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
     const int all_hi = TREE ? p_first : a.causal ? min(p_first + t0 + 1, seq.kv) : seq.kv, all_lo = paged_window(a, p_first + (TREE ? seq.nq - 1 : t1));
     auto key_of = [&](int i) { return i < ns ? i * PD_KEYS : lo + (i - ns) * PD_KEYS; };
 
+    const int32_t* table = a.table + b * a.table_stride;
+    const int page_mask = (1 << a.c.page_shift) - 1;
+    unsigned char* ring = pd_smem + warp * (ST * P::TILE);
+    // A warp takes the tiles begin + warp, + PD_WARPS, ...: `n` of them.  Lane x keeps the page of tile (x mod 32) of the next 32.
+    const int n = begin + warp < end ? (end - begin - warp + PD_WARPS - 1) / PD_WARPS : 0;
+    int pages = 0;
+    auto request = [&](int i) {                  // tile i of the warp, into its place in the ring; an empty group behind the last
+        if (i < n) {
+            const int key = key_of(begin + warp + i * PD_WARPS);
+            if ((i & 31) == 0) {
+                const int mine = i + lane;
+                pages = mine < n ? __ldg(table + (key_of(begin + warp + mine * PD_WARPS) >> a.c.page_shift)) : 0;
+            }
+            const int page = paged_page(a, __shfl_sync(0xffffffffu, pages, i & 31), status);
+            const uint32_t at = (uint32_t)((page * a.c.H + h) << a.c.page_shift) + (key & page_mask);      // whole tiles: a page's rows behind the sequence's end may be
+            unsigned char* t = ring + (i % ST) * P::TILE;                                                  // copied, not used
+            pd_copy<KROW>(t, reinterpret_cast<const unsigned char*>(a.c.kc) + (size_t)at * KROW, lane);
+            pd_copy<VROW>(t + 16 * KROW, reinterpret_cast<const unsigned char*>(a.c.vc) + (size_t)at * VROW, lane);
+            if (lane < 8) {
+                const float* src = (lane < 4 ? a.c.ks : a.c.vs) + at + (lane & 3) * 4;
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(t + 16 * (KROW + VROW) + lane * 16)), "l"(src) : "memory");
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll 1
+    for (int i = 0; i < ST - 1; ++i) request(i);
+
     // ---- Q fragments: column g is row t * 8 + g, scaled by a power of two to use fp16's range
+    uint4 raw[NT][D / 32];             // a quarter of a row each, all of them asked for before the first is used
+    const unsigned short* const q = reinterpret_cast<const unsigned short*>(a.q);
+    const bool q16 = ((reinterpret_cast<uintptr_t>(a.q) | (unsigned long long)a.qs_t * 2 | (unsigned long long)a.qs_h * 2) & 15u) == 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int row = row0 + t * 8 + g, token = row / a.G, head = h * a.G + row - token * a.G;
+        const unsigned short* const src = q + (long long)(seq.q0 + token) * a.qs_t + head * a.qs_h + c * (D / 4);
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+            raw[t][j] = make_uint4(0u, 0u, 0u, 0u);
+            if (q16 && row < rows) raw[t][j] = __ldg(reinterpret_cast<const uint4*>(src) + j);
+        }
+        if (!q16 && row < rows) {
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+                auto two = [&](int i) { return (uint32_t)__ldg(src + 8 * j + i) | (uint32_t)__ldg(src + 8 * j + i + 1) << 16; };
+                raw[t][j] = make_uint4(two(0), two(2), two(4), two(6));
+            }
+        }
+    }
     uint32_t qf[NT][KSTEPS][2];
     float qfac[NT][2];                 // of this thread's two score columns: softmax scale in the log2 domain / power of two
     int col_hi[NT][2], col_lo[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         float v[D / 4], mx = 0.f;
-        const int row = row0 + t * 8 + g, token = row / a.G, head = h * a.G + row - token * a.G;
 #pragma unroll
-        for (int j = 0; j < D / 4; j += 8) {
-            float e[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (row < rows) load_q8(a.q, a.dtype, (long long)(seq.q0 + token) * a.qs_t + head * a.qs_h + c * (D / 4) + j, e);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { v[j + i] = e[i]; mx = fmaxf(mx, fabsf(e[i])); }
+        for (int j = 0; j < D / 8; ++j) {
+            const uint32_t w = j % 4 == 0 ? raw[t][j / 4].x : j % 4 == 1 ? raw[t][j / 4].y : j % 4 == 2 ? raw[t][j / 4].z : raw[t][j / 4].w;
+            if (a.dtype == VARQ_F16) {
+                const float2 e = __half22float2(*reinterpret_cast<const __half2*>(&w));
+                v[2 * j] = e.x; v[2 * j + 1] = e.y;
+            } else {                         // a bf16 is the upper half of an fp32
+                v[2 * j] = __uint_as_float(w << 16); v[2 * j + 1] = __uint_as_float(w & 0xffff0000u);
+            }
+            mx = fmaxf(mx, fmaxf(fabsf(v[2 * j]), fabsf(v[2 * j + 1])));
         }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1)); mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         // 2^(8 - exponent of the largest element), inside fp32's range
@@ -189,31 +244,6 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
     CodeMagic<VB> vmagic;
     kmagic.init();
     vmagic.init();
-    const int32_t* table = a.table + b * a.table_stride;
-    const int page_mask = (1 << a.c.page_shift) - 1;
-    unsigned char* ring = pd_smem + warp * (ST * P::TILE);
-    // A warp takes the tiles begin + warp, + PD_WARPS, ...: `n` of them.  Lane x keeps the page of tile (x mod 32) of the next 32.
-    const int n = begin + warp < end ? (end - begin - warp + PD_WARPS - 1) / PD_WARPS : 0;
-    int pages = 0;
-    auto request = [&](int i) {                  // tile i of the warp, into its place in the ring; an empty group behind the last
-        if (i < n) {
-            const int key = key_of(begin + warp + i * PD_WARPS);
-            if ((i & 31) == 0) {
-                const int mine = i + lane;
-                pages = mine < n ? __ldg(table + (key_of(begin + warp + mine * PD_WARPS) >> a.c.page_shift)) : 0;
-            }
-            const int page = paged_page(a, __shfl_sync(0xffffffffu, pages, i & 31), status);
-            const uint32_t at = (uint32_t)((page * a.c.H + h) << a.c.page_shift) + (key & page_mask);      // whole tiles: a page's rows behind the sequence's end may be
-            unsigned char* t = ring + (i % ST) * P::TILE;                                                  // copied, not used
-            pd_copy<KROW>(t, reinterpret_cast<const unsigned char*>(a.c.kc) + (size_t)at * KROW, lane);
-            pd_copy<VROW>(t + 16 * KROW, reinterpret_cast<const unsigned char*>(a.c.vc) + (size_t)at * VROW, lane);
-            if (lane < 8) {
-                const float* src = (lane < 4 ? a.c.ks : a.c.vs) + at + (lane & 3) * 4;
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(t + 16 * (KROW + VROW) + lane * 16)), "l"(src) : "memory");
-            }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
     struct Tile {
         PdRaw<KBYTES> k[2];                // keys g, g + 8
         PdRaw<VBYTES> v[4];                // keys 2c, 2c + 1, 2c + 8, 2c + 9
@@ -264,6 +294,13 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
             rv[r] = paged_inverse(cur.vs[r]);
         }
         bool over = false;
+        uint32_t drafts[NT][2];            // bit k: the column sees key k0 + k, as far as the tree goes; all words are asked for at once
+        if constexpr (TREE && MASKED) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) drafts[t][e] = paged_tree_bits(a, seq.q0 + min(row0 + t * 8 + 2 * c + e, rows - 1) / a.G, k0 - p_first) >> g;
+        }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -274,7 +311,7 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
                     if (MASKED) {
                         const int key = k0 + g + 8 * r;
                         if (!(key < col_hi[t][e] && (key >= col_lo[t][e] || key < a.sinks))) x = -INFINITY;
-                        else if (TREE && key >= p_first && !paged_tree_bit(a, seq.q0 + (row0 + t * 8 + 2 * c + e) / a.G, key - p_first)) x = -INFINITY;
+                        if constexpr (TREE) x = drafts[t][e] >> (8 * r) & 1u ? x : -INFINITY;
                     }
                     s[t][2 * r + e] = x;
                     over = over | (x > m[t][e] + PAGED_TOP);
@@ -321,8 +358,6 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
         }
     };
 #pragma unroll 1
-    for (int i = 0; i < ST - 1; ++i) request(i);
-#pragma unroll 1
     for (int i = 0; i < n; ++i) {
         asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
         __syncwarp();                            // all lanes' copies of tile i are there, and all lanes are done with tile i - 1
@@ -345,65 +380,86 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
 #pragma unroll
         for (int j = 0; j < MT; ++j)
 #pragma unroll
-            for (int z = 0; z < 4; ++z)      // row g (z < 2) or g + 8 of row tile j = elements 2 j, 2 j + 1 of this thread's eighth of the head_dim
-                s_part[warp][t * 8 + 2 * c + (z & 1)][g * (D / 8) + 2 * j + (z >> 1)] = o[t][j][z];
+            for (int e = 0; e < 2; ++e)      // rows g and g + 8 of row tile j = elements 2 j, 2 j + 1 of this thread's eighth of the head_dim
+                *reinterpret_cast<float2*>(&s_part[warp][t * 8 + 2 * c + e][g * (D / 8) + 2 * j]) = make_float2(o[t][j][e], o[t][j][2 + e]);
         if (g == 0) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                s_part[warp][t * 8 + 2 * c + e][D] = m[t][e];
-                s_part[warp][t * 8 + 2 * c + e][D + 1] = l[t][e];
-            }
+            for (int e = 0; e < 2; ++e) *reinterpret_cast<float2*>(&s_part[warp][t * 8 + 2 * c + e][D]) = make_float2(m[t][e], l[t][e]);
         }
     }
     __syncthreads();
     // ---- merge the warps, then write the output, meet the cluster, or leave this split's part
     const long long n_rows = (long long)a.T * a.Hq;
-    auto finish = [&](int row, int d, float num, float den, float M) {
+    struct Out { unsigned short* to; float* lse; };
+    auto out_of = [&](int row) -> Out {
         const int token = row / a.G, head = h * a.G + row - token * a.G;
-        store_o_elem(a.out, a.dtype, (long long)(seq.q0 + token) * a.os_t + head * a.os_h + d, den != 0.f ? num / den : 0.f);
-        if (d == 0 && a.lse) a.lse[(long long)(seq.q0 + token) * a.Hq + head] = den != 0.f ? (M + __log2f(den)) * 0.6931471805599453f : -INFINITY;
+        return {reinterpret_cast<unsigned short*>(a.out) + (long long)(seq.q0 + token) * a.os_t + head * a.os_h, a.lse ? a.lse + (long long)(seq.q0 + token) * a.Hq + head : nullptr};
+    };
+    auto finish = [&](const Out& out, int d, float2 num, float den, float M) {
+        const float x = den != 0.f ? num.x / den : 0.f, y = den != 0.f ? num.y / den : 0.f;
+        const __half2 h2 = __floats2half2_rn(x, y);
+        const __nv_bfloat162 b2 = __floats2bfloat162_rn(x, y);
+        const uint32_t w = a.dtype == VARQ_F16 ? *reinterpret_cast<const uint32_t*>(&h2) : *reinterpret_cast<const uint32_t*>(&b2);
+        unsigned short* const to = out.to + d;
+        if ((reinterpret_cast<uintptr_t>(to) & 3u) == 0) *reinterpret_cast<uint32_t*>(to) = w;
+        else { to[0] = (unsigned short)w; to[1] = (unsigned short)(w >> 16); }
+        if (d == 0 && out.lse) *out.lse = den != 0.f ? (M + __log2f(den)) * 0.6931471805599453f : -INFINITY;
     };
     float (*s_cta)[D + 2] = reinterpret_cast<float (*)[D + 2]>(pd_smem + PD_WARPS * ROWS * (D + 2) * 4);
-    for (int j = threadIdx.x; j < ROWS * D; j += PD_WARPS * 32) {
-        const int r = j / D, d = j - r * D, row = row0 + r;
-        if (row >= rows) break;
-        float M = -FLT_MAX;
+    constexpr int SHARE = NT == 1 ? 16 : NT == 2 ? 8 : 4;                  // threads of a row, each with every SHARE-th pair of elements
+    if (const int r = threadIdx.x / SHARE, k = threadIdx.x % SHARE, row = row0 + r; r < ROWS && row < rows) {
+        float M = -FLT_MAX, den = 0.f, wt[PD_WARPS];
 #pragma unroll
         for (int w = 0; w < PD_WARPS; ++w) M = fmaxf(M, s_part[w][r][D]);
-        float num = 0.f, den = 0.f;
 #pragma unroll
         for (int w = 0; w < PD_WARPS; ++w) {
-            const float wt = pd_ex2(s_part[w][r][D] - M);
-            num = fmaf(wt, s_part[w][r][d], num);
-            den = fmaf(wt, s_part[w][r][D + 1], den);
+            wt[w] = pd_ex2(s_part[w][r][D] - M);
+            den = fmaf(wt[w], s_part[w][r][D + 1], den);
         }
-        if (splits == 1) finish(row, d, num, den, M);
-        else if (in_cluster) {
-            s_cta[r][d] = num;
-            if (d == 0) { s_cta[r][D] = M; s_cta[r][D + 1] = den; }
-        } else {
-            const int token = row / a.G, head = h * a.G + row - token * a.G;
-            const long long out_row = (long long)(seq.q0 + token) * a.Hq + head;
-            ws_o[(split * n_rows + out_row) * D + d] = num;
-            if (d == 0) *reinterpret_cast<float2*>(ws_ml + (split * n_rows + out_row) * 2) = make_float2(M, den);
+        const Out out = out_of(row);
+        const long long part = split * n_rows + (long long)(seq.q0 + row / a.G) * a.Hq + h * a.G + row % a.G;
+#pragma unroll 4
+        for (int d = 2 * k; d < D; d += 2 * SHARE) {
+            float2 num = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < PD_WARPS; ++w) {
+                const float2 p = *reinterpret_cast<const float2*>(&s_part[w][r][d]);
+                num.x = fmaf(wt[w], p.x, num.x); num.y = fmaf(wt[w], p.y, num.y);
+            }
+            if (splits == 1) finish(out, d, num, den, M);
+            else if (in_cluster) *reinterpret_cast<float2*>(&s_cta[r][d]) = num;
+            else *reinterpret_cast<float2*>(ws_o + part * D + d) = num;
         }
+        if (k == 0 && splits > 1) *reinterpret_cast<float2*>(in_cluster ? &s_cta[r][D] : ws_ml + part * 2) = make_float2(M, den);
     }
     if (paged_pad_any(a, seq, b)) pd_pad(paged_pad_rows(a, seq, b, h), (long long)(rt * splits + split) * (PD_WARPS * 32) + threadIdx.x, (long long)n_rowtiles * splits * (PD_WARPS * 32));
     if (in_cluster) {
         const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
         cluster.sync();
-        for (int j = threadIdx.x + split * (PD_WARPS * 32); j < ROWS * D; j += splits * (PD_WARPS * 32)) {      // the CTAs share out the elements
-            const int r = j / D, d = j - r * D;
+        for (int j = threadIdx.x + split * (PD_WARPS * 32); j < ROWS * (D / 2); j += splits * (PD_WARPS * 32)) {      // the CTAs share out the pairs of elements
+            const int r = j / (D / 2), d = 2 * (j - r * (D / 2));
             if (row0 + r >= rows) break;
-            float M = -FLT_MAX, num = 0.f, den = 0.f;
-            for (int s = 0; s < splits; ++s) M = fmaxf(M, cluster.map_shared_rank(&s_cta[r][D], s)[0]);
-            for (int s = 0; s < splits; ++s) {
-                const float* p = cluster.map_shared_rank(&s_cta[r][0], s);
-                const float wt = pd_ex2(p[D] - M);
-                num = fmaf(wt, p[d], num);
-                den = fmaf(wt, p[D + 1], den);
-            }
-            finish(row0 + r, d, num, den, M);
+            float2 ml[PAGED_CLUSTER], p[PAGED_CLUSTER];
+#pragma unroll
+            for (int s = 0; s < PAGED_CLUSTER; ++s)
+                if (s < splits) {
+                    const float* from = cluster.map_shared_rank(&s_cta[r][0], s);
+                    ml[s] = *reinterpret_cast<const float2*>(from + D);
+                    p[s] = *reinterpret_cast<const float2*>(from + d);
+                }
+            float M = -FLT_MAX, den = 0.f;
+            float2 num = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int s = 0; s < PAGED_CLUSTER; ++s)
+                if (s < splits) M = fmaxf(M, ml[s].x);
+#pragma unroll
+            for (int s = 0; s < PAGED_CLUSTER; ++s)
+                if (s < splits) {
+                    const float wt = pd_ex2(ml[s].x - M);
+                    num.x = fmaf(wt, p[s].x, num.x); num.y = fmaf(wt, p[s].y, num.y);
+                    den = fmaf(wt, ml[s].y, den);
+                }
+            finish(out_of(row0 + r), d, num, den, M);
         }
         cluster.sync();                          // nobody leaves while its shared memory is read
     }
@@ -416,6 +472,7 @@ int launch_nt(const PagedAttnArgs& a, int splits, bool in_cluster, int tiles_per
     const int n_rowtiles = (int)((rows + 8 * NT - 1) / (8 * NT));
     const long long blocks = (long long)a.B * a.c.H * n_rowtiles * splits;
     if (blocks > 0x7fffffffLL) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_attn: more than 2^31 thread blocks");
+    const int ranked = TREE && a.B > 1 && a.B <= PAGED_RANKED && blocks > (long long)PD_CTAS<KB, VB, D, NT> * sm_count();
     static bool configured[64] = {false};
     int dev = 0;
     VARQ_CUDA_TRY(cudaGetDevice(&dev));
@@ -424,7 +481,7 @@ int launch_nt(const PagedAttnArgs& a, int splits, bool in_cluster, int tiles_per
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
     VARQ_CUDA_TRY(launch_pdl(paged_attn_decode_kernel<KB, VB, D, NT, TREE>, (unsigned)blocks, PD_WARPS * 32, SMEM, st, in_cluster ? splits : 1, a, n_rowtiles, splits, in_cluster, tiles_per_split, ws_o, ws_ml,
-                             status));
+                             status, ranked));
     count_launches(1);
     return VARQ_OK;
 }

@@ -7,7 +7,7 @@
 //   keys, an accumulator each, merged on tensor memory at the end; with more rows each group has a tile of 128 of its own.  Warps without a row skip the exponentials.
 // * A query sees the context by its own position (window, first tokens) and of the drafted tokens those of its row of bits.  Tiles with drafted tokens or an end of a
 //   window take the form with masks; there a lane makes the bits of one row of its warp, and the threads that hold the row's scores get them by shuffles.
-// * Contexts differ, and the CTAs of long ones begin first: sequences are ranked by length where a call has more CTAs than SMs.
+// * Contexts and drafts differ, and the CTAs of the sequences with most work begin first where a call has more CTAs than SMs.
 //
 // What bounds it (B200): the softmax warps' chain, 2500 cycles for a tile of 64 keys (450 instructions; its 64 exponentials take 512 of them), which two warps on a scheduler
 // do not fill, and about 15000 cycles of a CTA around its tiles (lengths, queries, the first tile's copies and conversion, the output).  32 sequences, drafts of 64, 2000 to 8000
@@ -49,17 +49,6 @@ template <int D> struct TrPlan {
     static_assert(SOFT * 32 * REGS_SOFT + 256 * REGS_CONV + 128 * REGS_MISC <= THREADS * REGS, "register plan");
 };
 
-// The sequence with the `rank`-th longest context (the earlier one of equals) of up to 32, by one warp
-constexpr int TREE_RANKED = 32;
-__device__ __forceinline__ int tree_ranked(const PagedAttnArgs& a, int rank) {
-    const int lane = threadIdx.x & 31, n = lane < a.B ? max(__ldg(a.kv_lens + lane), 0) : -1;
-    const unsigned long long key = lane < a.B ? (unsigned long long)(unsigned)n * 32 + (31 - lane) + 1 : 0;      // all different, 0 behind the last
-    int above = 0;
-#pragma unroll 8
-    for (int j = 0; j < 32; ++j) above += __shfl_sync(0xffffffffu, key, j) > key ? 1 : 0;
-    return __ffs(__ballot_sync(0xffffffffu, lane < a.B && above == rank)) - 1;
-}
-
 __device__ __forceinline__ void pair_sync(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); }      // the two warps that share rows
 
 template <int D>
@@ -95,7 +84,7 @@ __global__ void __launch_bounds__(TrPlan<D>::THREADS, 1) paged_attn_tree_kernel(
     const unsigned item = blockIdx.x / (unsigned)splits, per_seq = (unsigned)(a.c.H * n_qblocks);
     const int rank = (int)(item / per_seq), hq = (int)(item - rank * per_seq), h = hq / n_qblocks, row0 = (hq - h * n_qblocks) * (2 * PT_M);
     if (warp == 0 && ranked) {
-        const int b = tree_ranked(a, rank);
+        const int b = paged_ranked(a, rank, 2 * PT_M);
         if (lane == 0) *my_seq = b;
     }
     tc_fence_before();
@@ -602,7 +591,7 @@ template <int D> int launch_tree(const PagedAttnArgs& a, int n_qblocks, int spli
     }
     const long long blocks = (long long)a.B * a.c.H * n_qblocks * splits;
     if (blocks > 0x7fffffffLL) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_attn: more than 2^31 thread blocks");
-    const int ranked = a.B > 1 && a.B <= TREE_RANKED && blocks > sm_count();
+    const int ranked = a.B > 1 && a.B <= PAGED_RANKED && blocks > sm_count();
     VARQ_CUDA_TRY(launch_pdl(paged_attn_tree_kernel<D>, (unsigned)blocks, P::THREADS, P::SMEM, st, 1, a, n_qblocks, splits, ranked, ws_o, ws_ml, status));
     count_launches(1);
     return VARQ_OK;

@@ -141,6 +141,26 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
     const int all_hi = TREE ? p_first : a.causal ? min(p_first + t0 + 1, seq.kv) : seq.kv, all_lo = paged_window(a, p_first + (TREE ? seq.nq - 1 : t1));
     auto key_of = [&](int i) { return i < ns ? i * PD_KEYS : lo + (i - ns) * PD_KEYS; };
 
+    uint4 raw[NT][D / 32];             // a quarter of a row each, all of them asked for before the first is used
+    const unsigned short* const q = reinterpret_cast<const unsigned short*>(a.q);
+    const bool q16 = ((reinterpret_cast<uintptr_t>(a.q) | (unsigned long long)a.qs_t * 2 | (unsigned long long)a.qs_h * 2) & 15u) == 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int row = row0 + t * 8 + g, token = row / a.G, head = h * a.G + row - token * a.G;
+        const unsigned short* const src = q + (long long)(seq.q0 + token) * a.qs_t + head * a.qs_h + c * (D / 4);
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+            raw[t][j] = make_uint4(0u, 0u, 0u, 0u);
+            if (q16 && row < rows) raw[t][j] = __ldg(reinterpret_cast<const uint4*>(src) + j);
+        }
+        if (!q16 && row < rows) {
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+                auto two = [&](int i) { return (uint32_t)__ldg(src + 8 * j + i) | (uint32_t)__ldg(src + 8 * j + i + 1) << 16; };
+                raw[t][j] = make_uint4(two(0), two(2), two(4), two(6));
+            }
+        }
+    }
     const int32_t* table = a.table + b * a.table_stride;
     const int page_mask = (1 << a.c.page_shift) - 1;
     unsigned char* ring = pd_smem + warp * (ST * P::TILE);
@@ -170,26 +190,6 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
     for (int i = 0; i < ST - 1; ++i) request(i);
 
     // ---- Q fragments: column g is row t * 8 + g, scaled by a power of two to use fp16's range
-    uint4 raw[NT][D / 32];             // a quarter of a row each, all of them asked for before the first is used
-    const unsigned short* const q = reinterpret_cast<const unsigned short*>(a.q);
-    const bool q16 = ((reinterpret_cast<uintptr_t>(a.q) | (unsigned long long)a.qs_t * 2 | (unsigned long long)a.qs_h * 2) & 15u) == 0;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int row = row0 + t * 8 + g, token = row / a.G, head = h * a.G + row - token * a.G;
-        const unsigned short* const src = q + (long long)(seq.q0 + token) * a.qs_t + head * a.qs_h + c * (D / 4);
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-            raw[t][j] = make_uint4(0u, 0u, 0u, 0u);
-            if (q16 && row < rows) raw[t][j] = __ldg(reinterpret_cast<const uint4*>(src) + j);
-        }
-        if (!q16 && row < rows) {
-#pragma unroll
-            for (int j = 0; j < D / 32; ++j) {
-                auto two = [&](int i) { return (uint32_t)__ldg(src + 8 * j + i) | (uint32_t)__ldg(src + 8 * j + i + 1) << 16; };
-                raw[t][j] = make_uint4(two(0), two(2), two(4), two(6));
-            }
-        }
-    }
     uint32_t qf[NT][KSTEPS][2];
     float qfac[NT][2];                 // of this thread's two score columns: softmax scale in the log2 domain / power of two
     int col_hi[NT][2], col_lo[NT][2];

@@ -331,17 +331,21 @@ struct AttnPlan {
     int splits, tiles_per_split;       // tiles of 16 keys (decode kernel)
 };
 int paged_max_q(const varq_paged_batch_t* b) { return (int)(b->max_q < b->n_queries ? b->max_q : b->n_queries); }
-// Trees: up to 32 rows of a head, and calls of little work in all (products of 16 rows and 16 keys), go to the decode kernel, the others to the tree kernel, us: 32 rows, 16
-// sequences of 1000 to 4000 keys, 8 heads x 128 66 / 58; 1 of 1000 13.0 / 15.5; 24 of up to 3000, 12 heads x 64 41 / 55; 64 rows, 1 sequence of 1000 (2000 products) 14.4 / 16.1, 1 of
-// 4000 with 104 rows (14000) 26 / 20; 40 rows, 8 of 300 (4200) 19.3 / 14.6, 4 of 1000 at 64 columns (2100 x 2) 19.9 / 15.5; 256 rows, 1 of 1000 (8700) 23 / 27.
-constexpr double TREE_BLOCKS = 4000;
+// Trees: up to 32 rows of a head, and calls of little work in all (products of 16 rows, 16 keys and 128 columns), go to the decode kernel, the others to the tree kernel, us
+// (decode / tree): 32 rows, 64 sequences of 8000 keys, 8 heads x 128, 8 bits 415 / 413, 16 of 1000 to 4000 59 / 58, 20 of 2000 in 4 bits 49 / 68, 24 of up to 3000, 12 heads x 64
+// 37 / 55 (but 1 of 64000 77 / 61); 64 rows, 1 of 1000 (2000 products) 11.1 / 16.3, 1 of 3000 (6000) 15.8 / 17.9; 256 rows, 1 of 1000 (8600) 17.7 / 27.5; 80 rows, 4 of 1000 at
+// 64 columns (5200) 13.6 / 17.4; 70 rows, 2 heads, 1 of 20000 (12500) 27.7 / 21.1; 104 rows, 1 of 4000 (14000) 20.9 / 19.9.
+// Their parts on the decode kernel: contexts differ, so no waves.  All of the work, at three fifths of the longest context, and half of a CTA for the end; one wave or less takes
+// its longest CTA.  Picks / best of 1 to 8 parts: 24 of up to 3000 at 64 columns 37.1 / 37.1, 64 single tokens over 2000 to 10000 keys 212 / 209, four tokens over a window of 1024
+// on 24 28.2 / 28.2, 8 of up to 4000 27 / 27, 30 of up to 2000 45 / 43, 32 of 4000 120 / 117, at 64 columns 76 / 70.
+constexpr double TREE_BLOCKS = 9000;
 AttnPlan plan_attn(const varq_paged_t* c, const varq_paged_batch_t* b, bool tree) {
     AttnPlan p{};
     const int max_q = paged_max_q(b), D = c->head_dim;
     const long long rows = (long long)max_q * (b->q_heads / c->n_heads);
     const long long seen = (long long)b->window + max_q + b->sinks, span = b->window && seen < b->max_kv ? seen : b->max_kv;      // keys of a CTA, about
     const double blocks16 = (double)b->n_seqs * c->n_heads * ((rows + 15) / 16) * ((span + 15) / 16);      // products of 16 rows and 16 keys
-    const bool many = tree ? rows > 32 && blocks16 > TREE_BLOCKS : rows > (D == 64 ? 80 : 32);
+    const bool many = tree ? rows > 32 && blocks16 * D > 128 * TREE_BLOCKS : rows > (D == 64 ? 80 : 32);
     p.tc = forced_attn_path() == VARQ_ATTN_PATH_TC || (forced_attn_path() != VARQ_ATTN_PATH_DECODE && many);
     p.rows = rows <= 8 ? 8 : rows > 16 && rows <= 24 && 4ll * b->n_seqs * c->n_heads >= sm_count() ? 24 : 16;
     const long long unit = p.tc ? 128 : 16, tiles = span > unit ? (span + unit - 1) / unit : 1;
@@ -355,9 +359,9 @@ AttnPlan plan_attn(const varq_paged_t* c, const varq_paged_batch_t* b, bool tree
     for (long long s = 1; s == 1 || (s <= tiles / least && s <= 256); ++s) {
         const bool near = !p.tc && s <= PAGED_CLUSTER && base * s <= room;
         long long cost = (base * s + room - 1) / room * ((tiles + s - 1) / s + fixed + (s > 1 && p.tc && !trees ? fixed : 0)) + (s > 1 && !near ? merge : 0);
-        if (tree && !p.tc) {                              // contexts differ: the longest part, or what all of them come to at three fifths of the longest
-            const long long longest = (tiles + s - 1) / s + fixed, all = base * (tiles * 3 / 5 + s * fixed) / room;
-            cost = (longest > all ? longest : all) + (s > 1 && !near ? merge : 0);
+        if (tree && !p.tc) {
+            const long long part = (tiles + s - 1) / s + fixed, all = base * ((b->window ? tiles : tiles * 3 / 5) + s * fixed) / room;
+            cost = (base * s <= room ? part * 5 / 4 : all + part / 2) + (s > 1 && !near ? merge : 0);
         }
         if (best == 0 || cost < best) { best = cost; p.splits = (int)s; p.cluster = s > 1 && near; }
         if (base * s > 8 * room) break;

@@ -371,7 +371,7 @@ int varq_paged_copy_pages(const varq_paged_t* caches, int32_t n_caches, const in
 
 /* The tokens in slots src[i] of every cache go to slots dst[i] (int64 [n_moves]), codes and scales.  Moves starts[g] .. starts[g + 1] - 1 (int32,
  * n_groups + 1 entries) are a group: one sequence's.  Within a group a dst may be the src of an earlier move, not of a later one (tokens move towards the
- * front in order); across groups slots differ, and the dst are all different.  A move with a slot outside a cache's pool does nothing there.
+ * front in order); across groups slots differ, and the dst are all different.  A move with a slot outside a cache's pool does nothing there.  No cache is there twice.
  * max_moves: the longest group (a hint: it decides how the work is split).  Starts that decrease or pass n_moves are clamped and leave code 64 for varq_device_status. */
 int varq_paged_move_tokens(const varq_paged_t* caches, int32_t n_caches, const int64_t* src, const int64_t* dst, int64_t n_moves, const int32_t* starts,
                            int32_t n_groups, int32_t max_moves, void* stream);

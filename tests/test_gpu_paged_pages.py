@@ -108,6 +108,34 @@ def test_accepted_drafts(page, layers, draft):
     assert same(cs, expected) and _cabi.device_status() == 0
 
 
+@pytest.mark.parametrize("layers,shape", [(40, (8, 128, 8, 8)), (70, (3, 64, 2, 4)), (9, (37, 128, 8, 4)), (2, (70, 64, 8, 8))])
+@pytest.mark.parametrize("groups,most", [(70, 5), (64, 31), (1, 6), (1, 300)])
+def test_caches_of_one_shape(layers, shape, groups, most):
+    """a block may go through several caches and heads; one cache has fewer pages than the others"""
+    page, span = 16, -(-2 * most // 16) * 16
+    heads, D, kb, vb = shape
+    rng = random.Random(groups + most)
+    cs = [PagedCache(groups * span // page // (2 if i == layers - 1 and groups > 1 else 1), page, heads, D, kb, vb) for i in range(layers)]
+    for c in cs:
+        for pool in pools(c):
+            pool.random_(-2 ** 31, 2 ** 31 - 1)
+    src, dst, starts = [], [], [0]
+    for g in range(groups):
+        kept = sorted(rng.sample(range(2 * most), rng.randint(0 if groups > 1 else most, most)))
+        src += [g * span + i for j, i in enumerate(kept) if i != j]
+        dst += [g * span + j for j, i in enumerate(kept) if i != j]
+        starts.append(len(src))
+    src, dst = longs(src), longs(dst)
+    expected = snapshot(cs)
+    for e, c in zip(expected, cs):
+        there = (src < c.num_pages * page) & (dst < c.num_pages * page)
+        s, d = src[there], dst[there]
+        for p in e:                                                        # no place is written before it is read
+            p[d // page, :, d % page] = p[s // page, :, s % page]
+    move_tokens(cs, src, dst, torch.tensor(starts, dtype=torch.int32, device=DEV), most)
+    assert same(cs, expected) and _cabi.device_status() == 0
+
+
 def test_long_moves_to_fresh_pages_with_any_hint():
     page, n = 32, 1500
     rng = random.Random(4)

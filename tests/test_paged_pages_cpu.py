@@ -200,6 +200,8 @@ def test_more_refusals_and_empty_calls_of_rotations():
 def test_refusals_and_empty_calls_of_copies_and_trees():
     lib = _cabi.lib()
     two = (_cabi.Paged * 2)(descriptors()[0], descriptors()[0])
+    assert lib.varq_paged_move_tokens(two, 2, 256, 256, 3, 256, 1, 0, None) == -1 and b"0 and 1 are one" in lib.varq_last_error()
+    two[1].k_codes = two[0].k_codes + 256
     assert lib.varq_paged_copy_pages(two, 2, 256, 256, 0, None) == 0 and lib.varq_paged_copy_pages(None, 0, 256, 256, 3, None) == 0
     assert lib.varq_paged_copy_pages(two, -1, 256, 256, 3, None) == -1 and lib.varq_paged_copy_pages(None, 2, 256, 256, 3, None) == -1
     assert lib.varq_paged_copy_pages(two, 2, None, 256, 3, None) == -1 and lib.varq_paged_copy_pages(two, 2, 256, 260, 3, None) == -1

@@ -130,7 +130,7 @@ def move_tokens(caches: Sequence[PagedCache], src: torch.Tensor, dst: torch.Tens
 
     Moves ``starts[g]`` .. ``starts[g + 1] - 1`` (int32) are those of one sequence, ``most`` of them at most (a hint).  A sequence's moves go towards its front, in
     order: its ``dst`` may be the ``src`` of an earlier move, never of a later one.  All ``dst`` are different, and no other sequence has them.  A move with a slot
-    that a cache does not have (-1) does nothing."""
+    that a cache does not have (-1) does nothing.  No cache may be there twice."""
     _native().paged_move_tokens([c._pools for c in caches], src, dst, starts, most)
 
 

@@ -2,13 +2,14 @@
 // drafts, kept tokens), for all layers in one launch: one page table serves them all, and a launch per layer would cost more than the copies.
 //
 // A page of a cache is four contiguous pieces (codes and scales of K and V, multiples of 64 bytes each); blocks take spans of a page's 16-byte units.
-// Tokens: a block takes one group (sequence) of moves of one head of one cache, chunk by chunk: all reads of a chunk, a barrier, all its writes.  What a later chunk reads
-// no earlier one writes, because no destination is the source of a later move.
+// Tokens: a block takes one group (sequence) of moves of some heads of some caches, chunk by chunk: all reads of a chunk, a barrier, all its writes.  What a later chunk
+// reads no earlier one writes, because no destination is the source of a later move.
 //
 // What bounds them (B200): their bytes, read and written.  301 pages of 64 tokens, 8 heads x 128, 8 and 4 bits, 16 caches: 986 MB in 148 us, 6.7 TB/s, the copy rate.
-// 16000 tokens of 8 sequences to other pages, 8 caches: 551 MB in 111 us, 5.0 TB/s; its blocks are chains of chunks (in registers, one after the other, 216 us).
-// Accepted paths of 64 sequences, one to six tokens, 32 caches: 15 us for 32 MB, 2048 blocks of three dependent loads each (a block per head 31 us).  Pages of
-// four sequences, 32 caches: 5.1 us, by bytes 5.3 (part of it stays in L2).
+// 16000 tokens of 8 sequences of 1000 to 3000 to other pages, 8 caches: 551 MB in 107 us, 5.1 TB/s; its blocks are chains of chunks, the longest of which the others wait for
+// (8 times 2000 tokens: 98; in registers, one chunk after the other, 216).  Accepted paths of 64 sequences, one to six tokens, 32 caches: 10.6 us for 32 MB, chains of a launch,
+// starts, slots, then three caches after one another (a block per head 31 us; per cache, in two and a half waves, 15).  Pages of four sequences, 32 caches: 5.1 us, by
+// bytes 5.3 (part of it stays in L2).
 #include "varq_paged.cuh"
 
 namespace varq {
@@ -82,101 +83,131 @@ __global__ void __launch_bounds__(COPY_THREADS) paged_copy_pages_kernel(const __
     }
 }
 
-constexpr int MOVE_THREADS = 256, MOVE_UNITS = 4;       // 16-byte units of a thread in a chunk
-struct MoveStage {
-    uint4 units[MOVE_UNITS * MOVE_THREADS];
-    float scales[MOVE_THREADS];
-    uint2 at[MOVE_THREADS];            // rows of the pools at head 0, source and destination; equal: nothing moves
+constexpr int MOVE_UNITS = 4, MOVE_AHEAD = 3;           // 16-byte units of a thread in a chunk; stages
+template <int THREADS> constexpr int MOVE_BLOCKS = THREADS == 128 ? 7 : 3;      // on an SM
+template <int THREADS> struct MoveStage {
+    uint4 units[MOVE_UNITS * THREADS];
+    float scales[THREADS];
+    uint2 at[THREADS];                 // rows of the pools at head 0, source and destination; equal: nothing moves
 };
 
-// A block: one group, `heads` heads of one cache, K or V of it or both (parts).  A unit is 16 bytes of codes of a (move, head); a chunk is as many moves as fill the
-// threads' units, in shared memory on its way.  AHEAD 3: two chunks are being read while one is written; 1: groups of one chunk, more blocks on an SM.
-template <int AHEAD>
-__global__ void __launch_bounds__(MOVE_THREADS, AHEAD == 1 ? 6 : 4) paged_move_kernel(const __grid_constant__ CopyArgs a, int heads, int parts, int* status) {
+// A block: one group, `heads` heads of `each` caches of one shape, K or V of them or both (parts).  A unit is 16 bytes of codes of a (move, head); a chunk is as many moves of a
+// cache as fill the threads' units, in shared memory on its way: two chunks are being read while one is written.
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS, MOVE_BLOCKS<THREADS>) paged_move_kernel(const __grid_constant__ CopyArgs a, int n_caches, int each, int heads, int parts, int* status) {
     extern __shared__ __align__(16) unsigned char move_smem[];
-    MoveStage* const stages = reinterpret_cast<MoveStage*>(move_smem);
+    using Stage = MoveStage<THREADS>;
+    Stage* const stages = reinterpret_cast<Stage*>(move_smem);
     pdl_trigger();
     pdl_wait();
-    const CopyCache& c = a.c[blockIdx.z];
-    const int tid = threadIdx.x, g = blockIdx.x, h0 = ((int)blockIdx.y / parts) * heads, hn = min(heads, c.H - h0), part = (int)blockIdx.y % parts;
+    const int first = (int)blockIdx.z * each, behind = min(first + each, n_caches);
+    const CopyCache& shape = a.c[first];
+    const int tid = threadIdx.x, g = blockIdx.x, h0 = ((int)blockIdx.y / parts) * heads, hn = min(heads, shape.H - h0), part = (int)blockIdx.y % parts;
     if (hn <= 0) return;
     const int s0 = __ldg(a.starts + g), s1 = __ldg(a.starts + g + 1);
     const int begin = (int)min((long long)max(s0, 0), a.n), end = (int)min((long long)max(s1, begin), a.n);
     if ((s0 != begin || s1 != end) && tid == 0) atomicCAS(status, 0, PAGED_BAD_STARTS);
     if (begin == end) return;
-    const long long n_slots = (long long)c.n_pages << a.page_shift;
     const int page_mask = (1 << a.page_shift) - 1, shift = a.page_shift;
-    const int kp = part == 1 ? 0 : c.krow / 16, vp = parts == 2 && part == 0 ? 0 : c.vrow / 16;      // units of a row
-    const int per = (kp + vp) * hn, kinds = (kp > 0) + (vp > 0), rows = max(min(MOVE_UNITS * MOVE_THREADS / per, MOVE_THREADS / (kinds * hn)), 1);
+    const int kp = part == 1 ? 0 : shape.krow / 16, vp = parts == 2 && part == 0 ? 0 : shape.vrow / 16;      // units of a row
+    const int per = (kp + vp) * hn, kinds = (kp > 0) + (vp > 0), rows = max(min(MOVE_UNITS * THREADS / per, THREADS / (kinds * hn)), 1);
     // this thread's units and its scale: move of the chunk (-1: none), head, piece
     int row[MOVE_UNITS], piece[MOVE_UNITS];
     uint32_t head[MOVE_UNITS];
 #pragma unroll
     for (int i = 0; i < MOVE_UNITS; ++i) {
-        const int u = tid + i * MOVE_THREADS, r = u / per, in = u - r * per, h = in / (kp + vp);
+        const int u = tid + i * THREADS, r = u / per, in = u - r * per, h = in / (kp + vp);
         row[i] = r < rows ? r : -1;
         head[i] = (uint32_t)(h0 + h) << shift;
         piece[i] = in - h * (kp + vp);
     }
     const int s_r = tid / (kinds * hn), s_in = tid - s_r * (kinds * hn), s_row = s_r < rows ? s_r : -1;
     const uint32_t s_head = (uint32_t)(h0 + s_in / kinds) << shift;
-    float* const scales = (kinds == 2 ? (s_in & 1) != 0 : kp == 0) ? c.vs : c.ks;
-    auto unit = [&](int i, uint32_t at) -> uint4* {
+    const bool s_v = kinds == 2 ? (s_in & 1) != 0 : kp == 0;
+    auto unit = [&](const CopyCache& c, int i, uint32_t at) -> uint4* {
         const size_t r = (size_t)(at + head[i]);
         return piece[i] < kp ? reinterpret_cast<uint4*>(c.kc + r * c.krow) + piece[i] : reinterpret_cast<uint4*>(c.vc + r * c.vrow) + (piece[i] - kp);
     };
-    auto slots = [&](int m) -> uint2 {                 // of move m + this thread's number
-        if (tid < rows && m < end - tid) {
-            const long long s = __ldg(a.src + m + tid), d = __ldg(a.dst + m + tid);
+    auto scale = [&](const CopyCache& c, uint32_t at) -> float* { return (s_v ? c.vs : c.ks) + (at + s_head); };
+    // chunks: those of a cache, then those of the next one
+    struct Chunk { int cache, m; };
+    auto behind_it = [&](Chunk& x) {
+        if (x.m < end - rows) x.m += rows;
+        else { x.m = begin; ++x.cache; }
+    };
+    auto slots = [&](const Chunk& x) -> uint2 {        // of move x.m + this thread's number
+        if (x.cache < behind && tid < rows && x.m < end - tid) {
+            const CopyCache& c = a.c[x.cache];
+            const long long s = __ldg(a.src + x.m + tid), d = __ldg(a.dst + x.m + tid), n_slots = (long long)c.n_pages << shift;
             if ((unsigned long long)s < (unsigned long long)n_slots && (unsigned long long)d < (unsigned long long)n_slots)
                 return make_uint2(((uint32_t)(s >> shift) * c.H << shift) + ((uint32_t)s & page_mask), ((uint32_t)(d >> shift) * c.H << shift) + ((uint32_t)d & page_mask));
         }
         return make_uint2(0u, 0u);
     };
-    auto copy = [&](MoveStage& t) {
+    Chunk ahead{first, begin};                         // the next one to be read
+    uint2 next = slots(ahead);
+    auto copy = [&](Stage& t) {
+        __syncthreads();                               // (everybody's copies of an earlier chunk are there, and) this place is written out
+        if (tid < rows) t.at[tid] = next;
+        const CopyCache& c = a.c[min(ahead.cache, behind - 1)];
+        behind_it(ahead);
+        next = slots(ahead);
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < MOVE_UNITS; ++i) {
             const uint2 at = row[i] < 0 ? make_uint2(0u, 0u) : t.at[row[i]];
             if (at.x != at.y)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(&t.units[tid + i * MOVE_THREADS])), "l"(unit(i, at.x)) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(&t.units[tid + i * THREADS])), "l"(unit(c, i, at.x)) : "memory");
         }
         const uint2 at = s_row < 0 ? make_uint2(0u, 0u) : t.at[s_row];
-        if (at.x != at.y) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(&t.scales[tid])), "l"(scales + (at.x + s_head)) : "memory");
-    };
-    uint2 next = slots(begin);
-#pragma unroll 1
-    for (int i = 0; i < AHEAD - 1; ++i) {
-        if (tid < rows) stages[i].at[tid] = next;
-        next = begin + (long long)(i + 1) * rows < end ? slots(begin + (i + 1) * rows) : make_uint2(0u, 0u);
-        __syncthreads();
-        copy(stages[i]);
+        if (at.x != at.y) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(&t.scales[tid])), "l"(scale(c, at.x)) : "memory");
         asm volatile("cp.async.commit_group;" ::: "memory");
-    }
+    };
+#pragma unroll 1
+    for (int i = 0; i < MOVE_AHEAD - 1; ++i) copy(stages[i]);
     int stage = 0;
 #pragma unroll 1
-    for (long long m0 = begin; m0 < end; m0 += rows) {
-        MoveStage &t = stages[stage], &ahead = stages[stage == 0 ? AHEAD - 1 : stage - 1];
-        if constexpr (AHEAD > 1) asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 2) : "memory");
-        __syncthreads();                               // (this chunk is read by everybody, and) the one before it written
-        if (tid < rows) ahead.at[tid] = next;
-        next = m0 + (long long)AHEAD * rows < end ? slots((int)m0 + AHEAD * rows) : make_uint2(0u, 0u);
-        __syncthreads();
-        copy(ahead);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if constexpr (AHEAD == 1) {
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            __syncthreads();
-        }
+    for (Chunk x{first, begin}; x.cache < behind; behind_it(x)) {
+        Stage& t = stages[stage];
+        asm volatile("cp.async.wait_group %0;" ::"n"(MOVE_AHEAD - 2) : "memory");
+        copy(stages[stage == 0 ? MOVE_AHEAD - 1 : stage - 1]);
+        const CopyCache& c = a.c[x.cache];
 #pragma unroll
         for (int i = 0; i < MOVE_UNITS; ++i) {
             const uint2 at = row[i] < 0 ? make_uint2(0u, 0u) : t.at[row[i]];
-            if (at.x != at.y) *unit(i, at.y) = t.units[tid + i * MOVE_THREADS];
+            if (at.x != at.y) *unit(c, i, at.y) = t.units[tid + i * THREADS];
         }
         const uint2 at = s_row < 0 ? make_uint2(0u, 0u) : t.at[s_row];
-        if (at.x != at.y) scales[at.y + s_head] = t.scales[tid];
-        stage = stage == AHEAD - 1 ? 0 : stage + 1;
+        if (at.x != at.y) *scale(c, at.y) = t.scales[tid];
+        stage = stage == MOVE_AHEAD - 1 ? 0 : stage + 1;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// How moves are shared out: a block per head, K and V apart, as long as all blocks are resident at once; else, and where a group does not fill a block's units, more heads, then more
+// caches of one shape.  Blocks of 128 threads, 7 on an SM / of 256, 3 on an SM, us: accepted paths as above 10.6 / 11.8, of 200 sequences, 4 heads x 64, 2 bits, 64 caches
+// 18.8 / 36.1; 8 times 2000 tokens, 8 caches 98 / 109; but where few blocks are long chains, 2000 tokens of one sequence, 16 caches 54.7 / 35.7, one cache 38.6 / 22.0.
+template <int THREADS>
+int launch_move(const CopyArgs& a, int n, int heads, int max_moves, int* status, cudaStream_t st) {
+    const long long room = (long long)MOVE_BLOCKS<THREADS> * sm_count();
+    bool alike = true;
+    for (int i = 1; i < n; ++i) alike = alike && a.c[i].H == a.c[0].H && a.c[i].krow == a.c[0].krow && a.c[i].vrow == a.c[0].vrow;
+    int each = 1, parts = 2;
+    auto blocks = [&] { return (long long)a.n_groups * ((heads + each - 1) / each) * parts * n; };
+    while (each < heads && 32 * each <= MOVE_UNITS * THREADS && (blocks() > room || 32ll * each * max_moves <= MOVE_UNITS * THREADS)) { each *= 2; parts = 1; }
+    const int share = !alike || blocks() <= room ? 1 : (int)(blocks() / room < n ? (blocks() + room - 1) / room : n);
+    constexpr int SMEM = MOVE_AHEAD * (int)sizeof(MoveStage<THREADS>);
+    static bool configured[64] = {false};
+    int dev = 0;
+    VARQ_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        VARQ_CUDA_TRY(cudaFuncSetAttribute(paged_move_kernel<THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+        if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
+    const dim3 grid((unsigned)a.n_groups, (unsigned)((heads + each - 1) / each * parts), (unsigned)((n + share - 1) / share));
+    VARQ_CUDA_TRY(launch_pdl(paged_move_kernel<THREADS>, grid, THREADS, SMEM, st, 1, a, n, share, each, parts, status));
+    count_launches(1);
+    return VARQ_OK;
 }
 
 int copy_caches(const char* who, const varq_paged_t* caches, int n_caches, CopyArgs& a, int from) {
@@ -281,6 +312,9 @@ extern "C" int varq_paged_move_tokens(const varq_paged_t* caches, int32_t n_cach
     if (n_moves == 0 || n_caches == 0 || n_groups == 0) return VARQ_OK;
     if (!src || !dst || !starts) return fail(VARQ_ERR_ARG, "varq_paged_move_tokens: null pointer");
     if (((uintptr_t)src | (uintptr_t)dst) % 8 || (uintptr_t)starts % 4) return fail(VARQ_ERR_ARG, "varq_paged_move_tokens: misaligned pointer");
+    for (int i = 0; i < n_caches; ++i)
+        for (int j = 0; j < i; ++j)
+            if (caches[i].k_codes == caches[j].k_codes) return fail(VARQ_ERR_ARG, "varq_paged_move_tokens: caches %d and %d are one", j, i);      // its tokens would move twice
     a.src = reinterpret_cast<const long long*>(src); a.dst = reinterpret_cast<const long long*>(dst); a.n = n_moves; a.starts = starts; a.n_groups = n_groups;
     int* status = nullptr;
     if (int rc = paged_status_word(&status)) return rc;
@@ -291,24 +325,8 @@ extern "C" int varq_paged_move_tokens(const varq_paged_t* caches, int32_t n_cach
         int heads = 0;
         for (int i = 0; i < n; ++i) heads = a.c[i].H > heads ? a.c[i].H : heads;
         if (heads > 32767) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_move_tokens: %d heads (32767 at most)", heads);
-        // short groups: as many heads in a block as its units hold; long ones: a block per head, K and V apart
-        int each = 1;
-        while (each < heads && each < 64 && 2ll * each * max_moves <= MOVE_UNITS * MOVE_THREADS / 16) each *= 2;
-        const int parts = each > 1 ? 1 : 2;
-        const dim3 grid((unsigned)n_groups, (unsigned)((heads + each - 1) / each * parts), (unsigned)n);
-        if (each > 1 && 2ll * each * max_moves <= MOVE_UNITS * MOVE_THREADS / 8) {
-            VARQ_CUDA_TRY(launch_pdl(paged_move_kernel<1>, grid, MOVE_THREADS, sizeof(MoveStage), (cudaStream_t)stream, 1, a, each, parts, status));
-        } else {
-            static bool configured[64] = {false};
-            int dev = 0;
-            VARQ_CUDA_TRY(cudaGetDevice(&dev));
-            if (dev < 0 || dev >= 64 || !configured[dev]) {
-                VARQ_CUDA_TRY(cudaFuncSetAttribute(paged_move_kernel<3>, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * (int)sizeof(MoveStage)));
-                if (dev >= 0 && dev < 64) configured[dev] = true;
-            }
-            VARQ_CUDA_TRY(launch_pdl(paged_move_kernel<3>, grid, MOVE_THREADS, 3 * sizeof(MoveStage), (cudaStream_t)stream, 1, a, each, parts, status));
-        }
-        count_launches(1);
+        const bool few = 2ll * n_groups * heads * n <= (long long)MOVE_BLOCKS<256> * sm_count() && max_moves > 64;
+        if (int rc = (few ? launch_move<256> : launch_move<128>)(a, n, heads, max_moves, status, (cudaStream_t)stream)) return rc;
     }
     return VARQ_OK;
 }

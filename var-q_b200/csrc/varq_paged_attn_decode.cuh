@@ -15,13 +15,16 @@
 // Warps and CTAs (key ranges) are merged by the log-sum-exp rule: where all CTAs are resident at once, up to eight of a row tile are a cluster and read one
 // another's shared memory; else they leave parts in the workspace for a second launch.
 //
-// What bounds it (B200): no unit is full.  64 sequences of 2000 to 10520 keys, 16 heads x 128, 4 bits: 239 us, 3.9 TB/s, DRAM 47 % busy (its bytes alone take 142 us).  Its
+// What bounds it (B200): no unit is full.  64 sequences of 2000 to 10520 keys, 16 heads x 128, 4 bits: 238 us, 3.9 TB/s, DRAM 47 % busy (its bytes alone take 142 us).  Its
 // instructions, 365 per 16 keys and warp, about half of them the conversion of the codes, would fill a scheduler for some 140 us; it issues in 65 % of the cycles
 // in which it has warps: four of them, each a chain of products, exponentials and unpacking.  Lengths that differ and parts cut by the longest leave an SM without warps for
-// another 6 % of the time.  One sequence of 1000 keys, 8 heads: 7.4 us, a chain of latencies (launch, lengths, pages, rows, two products, the cluster's merge).  Four tokens
-// over a window of 1024 (20 rows of a head) on 24 sequences: 31 us.  With rows straight from the pages into registers, a tile ahead, instead of the ring: 290 us.
+// another 6 % of the time.  One sequence of 1000 keys, 8 heads: 6.1 us, a chain of latencies (launch, lengths, pages, rows, two products, the cluster's merge).  Four tokens
+// over a window of 1024 (20 rows of a head) on 24 sequences: 26 us.  (Queries loaded and converted piece by piece in front of the first tile's copies, weights of a row's parts made for
+// every element: 7.4 and 30.)  With rows straight from the pages into registers, a tile ahead, instead of the ring: 290 us.
 //
 // TREE: queries that are drafted tokens see, of one another, what their rows of bits say; in its own instantiations, the other kernels' registers being as full as they can be.
+// A tree of 16 over 1000 keys, 4 query heads to each of 8: 11.1 us; drafts of 1 to 32 on 24 sequences of up to 3000 keys, 12 heads x 64, 4 and 2 bits: 37 us, 29 % of them on SMs that
+// have run out of work, the rest issue (53 %) and chains.  32 rows in a CTA at 64 columns, for drafts of 17 to 32: 52 us; sequences in their order instead of most work first: 38.
 #pragma once
 #include <cooperative_groups.h>
 

@@ -13,10 +13,10 @@
 // bytes in flight without registers for them.
 //
 // What bounds it (B200): its bytes, as long as it only turns.  16384 tokens of 16 + 16 heads x 128, bf16, L2 norm: 268 MB in 45 us, 5.9 TB/s (41 us at the copy rate).  In front
-// of a cache issue: 16384 tokens of 32 + 8 + 8 heads, K in 8 bits, V in 4: 82 us, 55 by its bytes; some 260 instructions for a row and warp, where the quantized rows
+// of a cache issue: 16384 tokens of 32 + 8 + 8 heads, K in 8 bits, V in 4: 80 us, 55 by its bytes; some 260 instructions for a row and warp, where the quantized rows
 // take twice those of a query's.  A few tokens: a launch, 3.5 us for 16.  On the way (first case / last one): values one by one in registers, one row ahead 72 / 111 us;
 // pairs of fp32 in one instruction 53 / 111; rows copied ahead 46 / 109; a loop for each of q, k and v, with addresses by steps 46 / 89; registers for two blocks
-// on an SM instead of three where rows are quantized 46 / 82; two conversions in an instruction, one factor for a row 45 / 82.  fp32 rows, whose pieces such
+// on an SM instead of three where rows are quantized 46 / 82; two conversions in an instruction, one factor for a row 45 / 82; blocks of 128 threads 45 / 80.  fp32 rows, whose pieces such
 // copies would take half a sector at a time, are held one ahead: 36.9 us for 8192 tokens of 16 + 4 heads, 44 with copies.
 #include <type_traits>
 
@@ -25,7 +25,8 @@
 namespace varq {
 namespace {
 
-constexpr int ROT_THREADS = 256;
+// Where rows are quantized, 126 registers are needed and smaller blocks begin and end less at a time: 80.0 us against 82.4 with two of 256
+template <bool PAGED> constexpr int ROT_THREADS = PAGED ? 128 : 256;
 
 struct RotArgs {
     const unsigned long long* turns; const int32_t* axis; const void* pos;
@@ -107,8 +108,8 @@ enum Role : int { ROLE_Q, ROLE_K, ROLE_V };
 template <int V> struct IsRole { static constexpr int value = V; };
 
 template <typename T, typename O, int D, bool VEC, bool PAGED, bool INTER>
-__global__ void __launch_bounds__(ROT_THREADS, PAGED || sizeof(T) == 4 ? 2 : 3) rotary_kernel(RotArgs a) {
-    constexpr int LPR = D / 16, GROUPS = ROT_THREADS / LPR;
+__global__ void __launch_bounds__(ROT_THREADS<PAGED>, PAGED ? 4 : sizeof(T) == 4 ? 2 : 3) rotary_kernel(RotArgs a) {
+    constexpr int LPR = D / 16, GROUPS = ROT_THREADS<PAGED> / LPR;
     constexpr bool RING = VEC && sizeof(T) == 2;
     extern __shared__ __align__(16) float2 s_cs[];           // [token][pair]: cos, sin
     pdl_trigger();
@@ -135,7 +136,7 @@ __global__ void __launch_bounds__(ROT_THREADS, PAGED || sizeof(T) == 4 ? 2 : 3) 
     // A thread's pieces of its next rows wait in shared memory, in places that only this thread writes and reads: several rows in flight without their registers.
     // (fp32 rows, of whose pieces such a copy takes half sectors, and rows that are not 16-byte aligned are held in registers, one ahead.)
     unsigned char* const ring = reinterpret_cast<unsigned char*>(s_cs + tb * half) + threadIdx.x * 16;
-    constexpr int STAGE = 2 * ROT_THREADS * 16;
+    constexpr int STAGE = 2 * ROT_THREADS<PAGED> * 16;
     Piece<T, VEC> held[2];
     auto advance = [&]() {                                   // `next`: row `ahead`
         next += next_step;
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(ROT_THREADS, PAGED || sizeof(T) == 4 ? 2 : 3) 
             if (ahead < end) {
                 const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring + ahead_stage);
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(next) : "memory");
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + ROT_THREADS * 16), "l"(next + apart) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + ROT_THREADS<PAGED> * 16), "l"(next + apart) : "memory");
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
             ahead_stage = ahead_stage == (ROT_AHEAD - 1) * STAGE ? 0 : ahead_stage + STAGE;
@@ -167,7 +168,7 @@ __global__ void __launch_bounds__(ROT_THREADS, PAGED || sizeof(T) == 4 ? 2 : 3) 
     const bool kept = PAGED && (unsigned long long)slot < ((unsigned long long)a.c.n_pages << a.c.page_shift);
 
     // ---- angles of the block's tokens
-    for (int i = threadIdx.x; i < tb * half; i += ROT_THREADS) {
+    for (int i = threadIdx.x; i < tb * half; i += ROT_THREADS<PAGED>) {
         const int tk = (int)a.half.div((uint32_t)i), p = i - tk * half;
         const uint32_t tt = t0 + tk;
         float s = 0.f, c = 1.f;
@@ -251,7 +252,7 @@ __global__ void __launch_bounds__(ROT_THREADS, PAGED || sizeof(T) == 4 ? 2 : 3) 
                 asm volatile("cp.async.wait_group %0;" ::"n"(ROT_AHEAD - 2) : "memory");
                 const uint4* from = reinterpret_cast<const uint4*>(ring + stage);
                 f[0].r.r = from[0];
-                f[1].r.r = from[ROT_THREADS];
+                f[1].r.r = from[ROT_THREADS<PAGED>];
                 stage = stage == (ROT_AHEAD - 1) * STAGE ? 0 : stage + STAGE;
             } else { f[0] = held[0]; f[1] = held[1]; }
             float v[2][8];
@@ -352,7 +353,7 @@ int rotary_pointers(const char* who, const RotArgs& a) {
 // more on a group of lanes spreads its angles and addresses over more rows, a group more keeps more rows in flight.  Threads per SM from which on it is four, us for
 // 300 / 1000 tokens of 32 + 4 and of 48 rows: rotate 256: 4.0 / 6.3, 512: 3.9 / 6.5, 1024: 4.1 / 8.2 (1777 tokens 9.3 / 8.1 / 9.3); append 256: 5.8 / 8.7, 512: 8.2 / 10.6.
 template <typename T, typename O, int D, bool VEC, bool PAGED> int run_rotary(RotArgs& a, cudaStream_t st) {
-    constexpr int LPR = D / 16, GROUPS = ROT_THREADS / LPR;
+    constexpr int LPR = D / 16, GROUPS = ROT_THREADS<PAGED> / LPR;
     const int rows = a.Hq + a.Hk + a.Hv;
     int lanes = 4;
     while (lanes < rows && (unsigned long long)a.tokens * lanes * LPR < (PAGED ? 256ull : 512ull) * sm_count()) lanes *= 2;
@@ -362,9 +363,9 @@ template <typename T, typename O, int D, bool VEC, bool PAGED> int run_rotary(Ro
     const int tb = GROUPS >> a.lanes_log2;
     const unsigned long long blocks = ((unsigned long long)a.tokens + tb - 1) / tb * a.parts;
     if (blocks > 0x7fffffffull) return fail(VARQ_ERR_UNSUPPORTED, "varq_rotate: more than 2^31 thread blocks");
-    const size_t smem = (size_t)tb * (a.R / 2) * sizeof(float2) + (VEC && sizeof(T) == 2 ? ROT_AHEAD * 2 * ROT_THREADS * 16 : 0);
+    const size_t smem = (size_t)tb * (a.R / 2) * sizeof(float2) + (VEC && sizeof(T) == 2 ? ROT_AHEAD * 2 * ROT_THREADS<PAGED> * 16 : 0);
     const auto kernel = a.inter ? rotary_kernel<T, O, D, VEC, PAGED, true> : rotary_kernel<T, O, D, VEC, PAGED, false>;
-    VARQ_CUDA_TRY(launch_pdl(kernel, (unsigned)blocks, ROT_THREADS, smem, st, 1, a));
+    VARQ_CUDA_TRY(launch_pdl(kernel, (unsigned)blocks, ROT_THREADS<PAGED>, smem, st, 1, a));
     count_launches(1);
     return VARQ_OK;
 }

@@ -50,8 +50,10 @@ int paged_status(int* out);            // its value where *out is 0; clears it
 
 // Sequence b: its first query token, number of queries, tokens in the cache, query token behind its last one
 struct PagedSeq { int q0, nq, kv, end; };
-__device__ __forceinline__ PagedSeq paged_seq(const PagedAttnArgs& a, int b, int* status) {
-    const int s0 = __ldg(a.q_starts + b), s1 = __ldg(a.q_starts + b + 1), kv = __ldg(a.kv_lens + b);
+struct PagedGiven { int s0, s1, kv; };          // as the caller's tensors have it
+__device__ __forceinline__ PagedGiven paged_given(const PagedAttnArgs& a, int b) { return {__ldg(a.q_starts + b), __ldg(a.q_starts + b + 1), __ldg(a.kv_lens + b)}; }
+__device__ __forceinline__ PagedSeq paged_seq(const PagedAttnArgs& a, PagedGiven given, int* status) {
+    const int s0 = given.s0, s1 = given.s1, kv = given.kv;
     PagedSeq s;
     s.q0 = min(max(s0, 0), a.T);
     s.end = min(max(s1, s.q0), a.T);
@@ -61,6 +63,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnArgs& a, int b, int
     if (s.kv != kv) atomicCAS(status, 0, PAGED_BAD_LENGTH);
     return s;
 }
+__device__ __forceinline__ PagedSeq paged_seq(const PagedAttnArgs& a, int b, int* status) { return paged_seq(a, paged_given(a, b), status); }
 __device__ __forceinline__ int paged_page(const PagedAttnArgs& a, int p, int* status) {
     if ((unsigned)p < (unsigned)a.c.n_pages) return p;
     atomicCAS(status, 0, PAGED_BAD_PAGE);
@@ -94,20 +97,20 @@ __device__ __forceinline__ uint32_t paged_tree_bits(const PagedAttnArgs& a, int 
 }
 
 // The CTAs of much work begin first: the sequence with the `rank`-th most of it (the earlier one of equals), of up to PAGED_RANKED, by one warp.  Work: tiles of
-// `rows` query rows times keys.
+// `rows` query rows times keys, to 18 bits.
 constexpr int PAGED_RANKED = 32;
-__device__ __forceinline__ int paged_ranked(const PagedAttnArgs& a, int rank, int rows) {
+__device__ __forceinline__ int paged_ranked(const PagedAttnArgs& a, int rank, int rows, PagedGiven& given) {
     const int lane = threadIdx.x & 31;
-    unsigned long long key = 0;        // all different, 0 behind the last sequence
-    if (lane < a.B) {
-        const long long nq = min(max((long long)__ldg(a.q_starts + lane + 1) - __ldg(a.q_starts + lane), 0ll), (long long)a.max_q), kv = max(__ldg(a.kv_lens + lane), 0);
-        const long long seen = a.window ? min(kv, (long long)a.window + a.sinks + nq) : kv;
-        key = (unsigned long long)(min((nq * a.G + rows - 1) / rows, 1ll << 24) * seen) * 32 + (31 - lane) + 1;
-    }
+    const PagedGiven mine = paged_given(a, min(lane, a.B - 1));
+    const float nq = fminf(fmaxf((float)mine.s1 - (float)mine.s0, 0.f), (float)a.max_q), kv = fmaxf((float)mine.kv, 0.f);
+    const float work = ceilf(nq * (float)a.G / (float)rows) * (a.window ? fminf(kv, (float)a.window + (float)a.sinks + nq) : kv);
+    const uint32_t key = lane < a.B ? ((__float_as_uint(work) & ~31u) | (31 - lane)) + 1 : 0u;      // all different, 0 behind the last sequence
     int above = 0;
 #pragma unroll 8
     for (int j = 0; j < 32; ++j) above += __shfl_sync(0xffffffffu, key, j) > key ? 1 : 0;
-    return __ffs(__ballot_sync(0xffffffffu, lane < a.B && above == rank)) - 1;
+    const int b = __ffs(__ballot_sync(0xffffffffu, lane < a.B && above == rank)) - 1;
+    given = {__shfl_sync(0xffffffffu, mine.s0, b), __shfl_sync(0xffffffffu, mine.s1, b), __shfl_sync(0xffffffffu, mine.kv, b)};
+    return b;
 }
 
 // Query rows in front of the first sequence's and behind the last one's belong to no sequence.  They get zeros and -inf, as rows that see nothing: from the CTAs of

@@ -130,8 +130,11 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
     const int split = (int)(blockIdx.x % (unsigned)splits);
     const unsigned item = blockIdx.x / (unsigned)splits;
     const int rt = (int)(item % (unsigned)n_rowtiles), bh = (int)(item / (unsigned)n_rowtiles), rank = bh / a.c.H, h = bh - rank * a.c.H;
-    const int b = TREE && ranked ? paged_ranked(a, rank, ROWS) : rank;
-    const PagedSeq seq = paged_seq(a, b, status);
+    int b = rank;
+    PagedGiven given;
+    if (TREE && ranked) b = paged_ranked(a, rank, ROWS, given);
+    else given = paged_given(a, b);
+    const PagedSeq seq = paged_seq(a, given, status);
     const int rows = seq.nq * a.G, row0 = rt * ROWS, p_first = seq.kv - seq.nq;
     if (row0 >= rows && !paged_pad_any(a, seq, b)) return;
 

@@ -42,7 +42,7 @@ template <int D> struct TrPlan {
     static constexpr int OFF_BAR = OFF_TAB + TS * TAB_FLOATS * 4;
     static constexpr int OFF_QF = (OFF_BAR + N_BARS * 8 + 15) / 16 * 16;              // factors of the queries [2][128]
     static constexpr int OFF_ML = OFF_QF + 2 * PT_M * 4;                              // reference and sum of the two groups' rows [2][128][2]
-    static constexpr int OFF_MISC = OFF_ML + 2 * PT_M * 8, SMEM = OFF_MISC + 16 + 1024;
+    static constexpr int OFF_MISC = OFF_ML + 2 * PT_M * 8, SMEM = OFF_MISC + 32 + 1024;
     static constexpr int COL_O = 0, COL_S = 2 * D, TMEM_COLS = 512;
     static_assert(COL_S + 2 * SB * PT_N <= TMEM_COLS && SMEM <= 227 * 1024 && OFF_RK % 128 == 0, "plan");
     static constexpr int SOFT = 8, K_WARP0 = SOFT, V_WARP0 = K_WARP0 + 4, MMA_WARP = V_WARP0 + 4, LOAD_WARP = MMA_WARP + 2, THREADS = (LOAD_WARP + 2) * 32;
@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(TrPlan<D>::THREADS, 1) paged_attn_tree_kernel(
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + P::OFF_BAR);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + P::OFF_MISC);
-    int* my_seq = reinterpret_cast<int*>(smem + P::OFF_MISC + 4);
+    int* my_seq = reinterpret_cast<int*>(smem + P::OFF_MISC + 16);          // its number; starts and length
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + P::OFF_MISC + 8);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
@@ -85,16 +85,17 @@ __global__ void __launch_bounds__(TrPlan<D>::THREADS, 1) paged_attn_tree_kernel(
     const unsigned item = blockIdx.x / (unsigned)splits, per_seq = (unsigned)(a.c.H * n_qblocks);
     const int rank = (int)(item / per_seq), hq = (int)(item - rank * per_seq), h = hq / n_qblocks, row0 = (hq - h * n_qblocks) * (2 * PT_M);
     if (warp == 0 && ranked) {
-        const int b = paged_ranked(a, rank, 2 * PT_M);
-        if (lane == 0) *my_seq = b;
+        PagedGiven given;
+        const int b = paged_ranked(a, rank, 2 * PT_M, given);
+        if (lane == 0) { my_seq[0] = b; my_seq[1] = given.s0; my_seq[2] = given.s1; my_seq[3] = given.kv; }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     pdl_trigger();       // behind the allocation: a CTA of a next launch must not take tensor memory that one of this launch still asks for
     const uint32_t tmem_base = *tmem_slot;
-    const int b = ranked ? *my_seq : rank, page_mask = (1 << a.c.page_shift) - 1;
-    const PagedSeq seq = paged_seq(a, b, status);
+    const int b = ranked ? my_seq[0] : rank, page_mask = (1 << a.c.page_shift) - 1;
+    const PagedSeq seq = paged_seq(a, ranked ? PagedGiven{my_seq[1], my_seq[2], my_seq[3]} : paged_given(a, b), status);
     const int rows = seq.nq * a.G, p_first = seq.kv - seq.nq;               // rows of the (sequence, head); position of the first drafted token
     const bool both = rows - row0 > PT_M;                                   // each group has rows of its own
     PtTiles tiles;

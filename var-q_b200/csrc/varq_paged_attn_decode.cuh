@@ -142,7 +142,9 @@ paged_attn_decode_kernel(PagedAttnArgs a, int n_rowtiles, int splits, int in_clu
     const int t0 = row0 / a.G, t1 = (min(row0 + ROWS, rows) - 1) / a.G;
     const int hi = max(!TREE && a.causal ? min(seq.kv, p_first + t1 + 1) : seq.kv, 0), lo = paged_window(a, TREE ? p_first - 1 : p_first + t0) & ~(PD_KEYS - 1);
     const int ns = min((a.sinks + PD_KEYS - 1) / PD_KEYS, lo / PD_KEYS), n_tiles = hi > 0 && row0 < rows ? ns + (max(hi - lo, 0) + PD_KEYS - 1) / PD_KEYS : 0;
-    const int begin = (int)min((long long)split * tiles_per_split, (long long)n_tiles), end = split == splits - 1 ? n_tiles : min(begin + tiles_per_split, n_tiles);
+    // a sequence's own tiles in equal parts of whole turns of the warps, or (chains) parts of the longest sequence's
+    const int of_part = TREE ? (int)((unsigned)(n_tiles + PD_WARPS * splits - 1) / (unsigned)(PD_WARPS * splits)) * PD_WARPS : tiles_per_split;
+    const int begin = (int)min((long long)split * of_part, (long long)n_tiles), end = split == splits - 1 ? n_tiles : min(begin + of_part, n_tiles);
     // what every row sees
     const int all_hi = TREE ? p_first : a.causal ? min(p_first + t0 + 1, seq.kv) : seq.kv, all_lo = paged_window(a, p_first + (TREE ? seq.nq - 1 : t1));
     auto key_of = [&](int i) { return i < ns ? i * PD_KEYS : lo + (i - ns) * PD_KEYS; };

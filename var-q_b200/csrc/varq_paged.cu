@@ -332,12 +332,12 @@ struct AttnPlan {
 };
 int paged_max_q(const varq_paged_batch_t* b) { return (int)(b->max_q < b->n_queries ? b->max_q : b->n_queries); }
 // Trees: up to 32 rows of a head, and calls of little work in all (products of 16 rows, 16 keys and 128 columns), go to the decode kernel, the others to the tree kernel, us
-// (decode / tree): 32 rows, 64 sequences of 8000 keys, 8 heads x 128, 8 bits 415 / 413, 16 of 1000 to 4000 59 / 58, 20 of 2000 in 4 bits 49 / 68, 24 of up to 3000, 12 heads x 64
-// 37 / 55 (but 1 of 64000 77 / 61); 64 rows, 1 of 1000 (2000 products) 11.1 / 16.3, 1 of 3000 (6000) 15.8 / 17.9; 256 rows, 1 of 1000 (8600) 17.7 / 27.5; 80 rows, 4 of 1000 at
+// (decode / tree): 32 rows, 64 sequences of 8000 keys, 8 heads x 128, 8 bits 415 / 413, 16 of 1000 to 4000 51 / 58, 20 of 2000 in 4 bits 49 / 68, 24 of up to 3000, 12 heads x 64
+// 34 / 55 (but 1 of 64000 77 / 61); 64 rows, 1 of 1000 (2000 products) 11.1 / 16.3, 1 of 3000 (6000) 15.8 / 17.9; 256 rows, 1 of 1000 (8600) 17.7 / 27.5; 80 rows, 4 of 1000 at
 // 64 columns (5200) 13.6 / 17.4; 70 rows, 2 heads, 1 of 20000 (12500) 27.7 / 21.1; 104 rows, 1 of 4000 (14000) 20.9 / 19.9.
 // Their parts on the decode kernel: contexts differ, so no waves.  All of the work, at three fifths of the longest context, and half of a CTA for the end; one wave or less takes
-// its longest CTA.  Picks / best of 1 to 8 parts: 24 of up to 3000 at 64 columns 37.1 / 37.1, 64 single tokens over 2000 to 10000 keys 212 / 209, four tokens over a window of 1024
-// on 24 28.2 / 28.2, 8 of up to 4000 27 / 27, 30 of up to 2000 45 / 43, 32 of 4000 120 / 117, at 64 columns 76 / 70.
+// its longest CTA.  Picks / best of 1 to 8 parts: 24 of up to 3000 at 64 columns 34.2 / 34.2, 64 single tokens over 2000 to 10000 keys 207 / 205, four tokens over a window of 1024
+// on 24 28.5 / 28.5, 8 of up to 4000 26.6 / 24.5, 16 of 1000 to 4000 50.5 / 47.3, 30 of up to 2000 45 / 41, 32 of 4000 119 / 115, at 64 columns 76 / 69.
 constexpr double TREE_BLOCKS = 9000;
 AttnPlan plan_attn(const varq_paged_t* c, const varq_paged_batch_t* b, bool tree) {
     AttnPlan p{};

@@ -23,8 +23,9 @@
 // every element: 7.4 and 30.)  With rows straight from the pages into registers, a tile ahead, instead of the ring: 290 us.
 //
 // TREE: queries that are drafted tokens see, of one another, what their rows of bits say; in its own instantiations, the other kernels' registers being as full as they can be.
-// A tree of 16 over 1000 keys, 4 query heads to each of 8: 11.1 us; drafts of 1 to 32 on 24 sequences of up to 3000 keys, 12 heads x 64, 4 and 2 bits: 37 us, 29 % of them on SMs that
-// have run out of work, the rest issue (53 %) and chains.  32 rows in a CTA at 64 columns, for drafts of 17 to 32: 52 us; sequences in their order instead of most work first: 38.
+// A tree of 16 over 1000 keys, 4 query heads to each of 8: 11.1 us; drafts of 1 to 32 on 24 sequences of up to 3000 keys, 12 heads x 64, 4 and 2 bits: 34 us: issue in 59 % of the
+// cycles in which an SM has warps, which is 77 % of the time.  On the way (the latter): sequences in their order instead of most work first 38.6, parts cut by the longest sequence
+// 37; 32 rows in a CTA at 64 columns, for drafts of 17 to 32, took 52.
 #pragma once
 #include <cooperative_groups.h>
 

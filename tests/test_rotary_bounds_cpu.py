@@ -1,0 +1,17 @@
+"""Sizes that leave 31 or 63 bits at the C entries in front of and around a paged cache: refused on the host, before a launch."""
+import pytest
+
+from test_paged_pages_cpu import descriptors
+from VAR_Q import _cabi
+
+LAST = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("B,L,q_heads,k_heads", [(LAST, LAST, 2, 2), (LAST, LAST, 0, 1), (1 << 16, 1 << 16, LAST, LAST), (1 << 16, 1 << 16, 1 << 30, 1 << 30), (1, LAST, LAST, LAST),
+                                                 (LAST, 1, 1, 0), (1 << 16, 1 << 15, 1, 0)])
+def test_rows_of_a_rotation_are_counted_without_wrapping(B, L, q_heads, k_heads):
+    """strides of zero make such sizes a call that somebody can write down: the product of them is no small number"""
+    lib = _cabi.lib()
+    _, rot, _ = descriptors()
+    shared = _cabi.Tensor(256, _cabi.F16, 0, 0, 0, 0)
+    assert lib.varq_rotate(rot, shared, shared, B, L, q_heads, k_heads, 64, shared, shared, None) == -2 and b"2^31" in lib.varq_last_error()

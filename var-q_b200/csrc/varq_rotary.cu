@@ -392,7 +392,8 @@ extern "C" int varq_rotate(const varq_rotary_t* r, const varq_tensor_t* q, const
     if (B < 0 || L < 0) return fail(VARQ_ERR_ARG, "varq_rotate: negative size");
     if (!dtype_ok(q->dtype) || k->dtype != q->dtype) return fail(VARQ_ERR_ARG, "varq_rotate: q and k must have one type, fp32, fp16 or bf16");
     if ((q_out->dtype != q->dtype && q_out->dtype != VARQ_F32) || k_out->dtype != q_out->dtype) return fail(VARQ_ERR_ARG, "varq_rotate: outputs have q's type or fp32, both one");
-    if ((long long)B * L * ((long long)q_heads + k_heads) >= 0x7fffffffLL) return fail(VARQ_ERR_UNSUPPORTED, "varq_rotate: 2^31 rows or more");
+    const long long n_tokens = (long long)B * L;              // below 2^31, before it is multiplied by heads of up to 2^32
+    if (n_tokens >= 0x7fffffffLL || n_tokens * ((long long)q_heads + k_heads) >= 0x7fffffffLL) return fail(VARQ_ERR_UNSUPPORTED, "varq_rotate: 2^31 rows or more");
     if (B == 0 || L == 0 || q_heads + k_heads == 0) return VARQ_OK;
     if (int rc = rotary_pointers("varq_rotate", a)) return rc;
     if ((q_heads && (!q->ptr || !q_out->ptr)) || (k_heads && (!k->ptr || !k_out->ptr))) return fail(VARQ_ERR_ARG, "varq_rotate: null pointer");

@@ -15,3 +15,14 @@ def test_rows_of_a_rotation_are_counted_without_wrapping(B, L, q_heads, k_heads)
     _, rot, _ = descriptors()
     shared = _cabi.Tensor(256, _cabi.F16, 0, 0, 0, 0)
     assert lib.varq_rotate(rot, shared, shared, B, L, q_heads, k_heads, 64, shared, shared, None) == -2 and b"2^31" in lib.varq_last_error()
+
+
+@pytest.mark.parametrize("q_heads,k_heads", [(LAST - 1, 0), (0, LAST - 1), (LAST - 3, 2), (LAST - 2 ** 19, 1)])
+def test_rows_of_a_token_end_before_their_number_does(q_heads, k_heads):
+    """the steps from row to row go behind the last one: none of them leaves an int"""
+    lib = _cabi.lib()
+    cache, rot, _ = descriptors()
+    shared = _cabi.Tensor(256, _cabi.F16, 0, 0, 0, 0)
+    assert lib.varq_rotate(rot, shared, shared, 1, 1, q_heads, k_heads, 64, shared, shared, None) == -2 and b"2^31" in lib.varq_last_error()
+    if q_heads:
+        assert lib.varq_paged_append_rotated(cache, rot, shared, shared, shared, 256, 1, q_heads - 4, 1e-12, shared, None) == -2 and b"2^31" in lib.varq_last_error()

@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(ROT_THREADS<PAGED>, PAGED ? 4 : sizeof(T) == 4
     if constexpr (PAGED) rows_of(IsRole<ROLE_V>());
 }
 
-int rotary_args(const char* who, RotArgs& a, const varq_rotary_t* r, int q_heads, int k_heads, int D) {
+int rotary_args(const char* who, RotArgs& a, const varq_rotary_t* r, int q_heads, int k_heads, int v_heads, int D) {
     if (!r) return fail(VARQ_ERR_ARG, "%s: null rotary descriptor", who);
     if (r->rotary_dim < 16 || r->rotary_dim > D || r->rotary_dim % 16) return fail(VARQ_ERR_UNSUPPORTED, "%s: rotary_dim %d is not a multiple of 16 up to head_dim %d", who, r->rotary_dim, D);
     if (r->n_axes < 1) return fail(VARQ_ERR_ARG, "%s: %d axes", who, r->n_axes);
@@ -331,6 +331,9 @@ int rotary_args(const char* who, RotArgs& a, const varq_rotary_t* r, int q_heads
     if (r->norm != VARQ_NORM_NONE && r->norm != VARQ_NORM_L2 && r->norm != VARQ_NORM_RMS) return fail(VARQ_ERR_ARG, "%s: norm %d", who, r->norm);
     if (r->norm != VARQ_NORM_NONE && !(r->eps >= 1e-18f && r->eps < 1e18f)) return fail(VARQ_ERR_ARG, "%s: eps of the norm must lie in [1e-18, 1e18)", who);
     if (q_heads < 0 || k_heads < 0) return fail(VARQ_ERR_ARG, "%s: %d query heads, %d key heads", who, q_heads, k_heads);
+    // a lane group's rows are counted in an int, up to four steps (each below 2^17) behind the last one
+    if ((long long)q_heads + k_heads + v_heads >= (1ll << 31) - (1 << 20))
+        return fail(VARQ_ERR_UNSUPPORTED, "%s: %d query heads, %d key heads: 2^31 - 2^20 rows of a token or more", who, q_heads, k_heads);
     a.turns = reinterpret_cast<const unsigned long long*>(r->turns); a.axis = r->axis; a.pos = r->positions;
     a.pos_bytes = r->pos_bytes; a.n_axes = r->n_axes; a.R = r->rotary_dim; a.inter = r->interleaved != 0;
     a.ps_a = r->pos_stride_axis; a.ps_b = r->pos_stride_b; a.ps_l = r->pos_stride_l;
@@ -387,7 +390,7 @@ extern "C" int varq_rotate(const varq_rotary_t* r, const varq_tensor_t* q, const
                            int32_t head_dim, const varq_tensor_t* q_out, const varq_tensor_t* k_out, void* stream) {
     RotArgs a = RotArgs();
     if (head_dim != 64 && head_dim != 128) return fail(VARQ_ERR_UNSUPPORTED, "varq_rotate: head_dim %d is not 64 or 128", head_dim);
-    if (int rc = rotary_args("varq_rotate", a, r, q_heads, k_heads, head_dim)) return rc;
+    if (int rc = rotary_args("varq_rotate", a, r, q_heads, k_heads, 0, head_dim)) return rc;
     if (!q || !k || !q_out || !k_out) return fail(VARQ_ERR_ARG, "varq_rotate: null descriptor");
     if (B < 0 || L < 0) return fail(VARQ_ERR_ARG, "varq_rotate: negative size");
     if (!dtype_ok(q->dtype) || k->dtype != q->dtype) return fail(VARQ_ERR_ARG, "varq_rotate: q and k must have one type, fp32, fp16 or bf16");
@@ -416,7 +419,7 @@ extern "C" int varq_paged_append_rotated(const varq_paged_t* cache, const varq_r
                                          const int64_t* slots, int64_t n_tokens, int32_t q_heads, float eps, const varq_tensor_t* q_out, void* stream) {
     RotArgs a = RotArgs();
     if (int rc = paged_check_cache("varq_paged_append_rotated", cache, a.c)) return rc;
-    if (int rc = rotary_args("varq_paged_append_rotated", a, r, q_heads, a.c.H, a.c.D)) return rc;
+    if (int rc = rotary_args("varq_paged_append_rotated", a, r, q_heads, a.c.H, a.c.H, a.c.D)) return rc;
     if (n_tokens < 0) return fail(VARQ_ERR_ARG, "varq_paged_append_rotated: %lld tokens", (long long)n_tokens);
     if (n_tokens >= 0x7fffffffLL || n_tokens * (2ll * a.c.H + q_heads) >= 0x7fffffffLL)
         return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_append_rotated: %lld tokens of %d and 2 x %d heads are 2^31 rows or more", (long long)n_tokens, q_heads, a.c.H);

@@ -362,7 +362,7 @@ int varq_paged_append_rotated(const varq_paged_t* cache, const varq_rotary_t* r,
  *   masks     int32 [n_tokens][words], 32 * words >= max_q : bits of the token's ancestors among the drafted tokens and its own
  *   positions int32 [n_tokens] : kv_lens[b] - n + number of ancestors
  * Rows that belong to no sequence get zeros.  A parent out of its range counts as -1 and leaves code 67, starts that decrease and more than max_q tokens code 64
- * for varq_device_status. */
+ * for varq_device_status.  n_tokens: below 2^31 - 512, as the query tokens that the masks are for. */
 int varq_paged_tree(const int32_t* parents, const int32_t* kv_lens, const int32_t* q_starts, int32_t n_seqs, int64_t n_tokens, int32_t max_q, int32_t words,
                     int32_t* masks, int32_t* positions, void* stream);
 

@@ -26,3 +26,10 @@ def test_rows_of_a_token_end_before_their_number_does(q_heads, k_heads):
     assert lib.varq_rotate(rot, shared, shared, 1, 1, q_heads, k_heads, 64, shared, shared, None) == -2 and b"2^31" in lib.varq_last_error()
     if q_heads:
         assert lib.varq_paged_append_rotated(cache, rot, shared, shared, shared, 256, 1, q_heads - 4, 1e-12, shared, None) == -2 and b"2^31" in lib.varq_last_error()
+
+
+@pytest.mark.parametrize("tokens", [LAST, LAST - 1, LAST - 127, 2 ** 31 - 512])
+def test_drafted_tokens_end_before_their_number_does(tokens):
+    """the threads of a block go through a sequence's tokens in steps of an int"""
+    lib = _cabi.lib()
+    assert lib.varq_paged_tree(256, 256, 256, 1, tokens, 32, 1, 256, 256, None) == -2 and b"2^31" in lib.varq_last_error()

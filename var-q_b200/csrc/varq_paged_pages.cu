@@ -334,7 +334,8 @@ extern "C" int varq_paged_move_tokens(const varq_paged_t* caches, int32_t n_cach
 extern "C" int varq_paged_tree(const int32_t* parents, const int32_t* kv_lens, const int32_t* q_starts, int32_t n_seqs, int64_t n_tokens, int32_t max_q, int32_t words,
                                int32_t* masks, int32_t* positions, void* stream) {
     if (n_seqs < 0 || n_tokens < 0 || max_q < 0 || words < 0) return fail(VARQ_ERR_ARG, "varq_paged_tree: negative size");
-    if (n_tokens > 0x7fffffffLL || n_seqs == 0x7fffffff) return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_tree: 2^31 tokens or sequences or more");
+    if (n_tokens >= (1ll << 31) - 512 || n_seqs == 0x7fffffff)          // a block's threads step through a sequence's tokens, and one step behind them, in an int
+        return fail(VARQ_ERR_UNSUPPORTED, "varq_paged_tree: 2^31 - 512 tokens or 2^31 sequences or more");
     if (words > (1 << 26) || (long long)words * 32 < max_q) return fail(VARQ_ERR_ARG, "varq_paged_tree: %d words for %d tokens of a sequence", words, max_q);
     if (n_tokens == 0) return VARQ_OK;
     if (!parents || !q_starts || !positions || (words && !masks) || (n_seqs && !kv_lens)) return fail(VARQ_ERR_ARG, "varq_paged_tree: null pointer");

@@ -274,15 +274,22 @@ __global__ void __launch_bounds__(ROT_THREADS<PAGED>, PAGED ? 4 : sizeof(T) == 4
                         return sum;
                     };
                     float sum = squares();
-                    // Squares of finite fp32 and bf16 rows leave fp32 where the norm passes 2^64 (in all lanes of the row): of the row times 2^-68 they sum up to 2^127 at most,
-                    // and eps is nothing next to them.  The test costs four instructions of a row's two hundred: bf16, first case above 44.9 -> 46.0 us, last one 83.3 -> 85.8
-                    if (!std::is_same<T, __half>::value && sum == INFINITY) {
-                        const f32x2 down = pack2(0x1p-68f, 0x1p-68f);
+                    // Rows whose norm lies outside of 2^-40 .. 2^40 (and rows that are no numbers; in all lanes of a row) are divided by it here, in front of their factors, whose
+                    // products with the elements alone may be subnormal or infinite.  Squares that leave fp32 (norms from 2^64 on): of the row times 2^-68 they sum up to 2^127
+                    // at most, and eps is nothing next to them.  fp16 has no such rows but zeros.  (Every row divided in front of its factors: registers, and up to 17 % of the
+                    // time.  The test costs bf16, first case above, 44.9 -> 45.8 us, last one 83.3 -> 85.9)
+                    if (!std::is_same<T, __half>::value && __float_as_uint(sum) - __float_as_uint(0x1p-80f) > __float_as_uint(0x1p80f) - __float_as_uint(0x1p-80f)) {
+                        const bool far = sum == INFINITY;
+                        auto scale = [&](float f) {
+                            const f32x2 ff = pack2(f, f);
 #pragma unroll
-                        for (int m = 0; m < 4; ++m) { z.x[m] = mul2(z.x[m], down); z.y[m] = mul2(z.y[m], down); }
-                        factor = rsqrt_normal(squares() * a.sum_mul);
+                            for (int m = 0; m < 4; ++m) { z.x[m] = mul2(z.x[m], ff); z.y[m] = mul2(z.y[m], ff); }
+                        };
+                        if (far) { scale(0x1p-68f); sum = squares(); }
+                        sum = fmaf(sum, a.sum_mul, far ? 0.f : a.sum_add);
+                        scale(sum < a.least && !far ? a.inv_eps : rsqrt_normal(sum));
                     } else {
-                        sum = fmaf(sum, a.sum_mul, a.sum_add);     // a NaN stays one; 0 becomes 0 / eps
+                        sum = fmaf(sum, a.sum_mul, a.sum_add);     // 0 becomes 0 / eps
                         factor = sum < a.least ? a.inv_eps : rsqrt_normal(sum);
                     }
                 }

@@ -106,3 +106,21 @@ def test_append(D, kb, dtype, norm):
     step = ref.abs().amax(-1, keepdim=True) / (2 ** (kb - 1) - 1)
     assert ((one.read(slots)[0].double().cpu() - ref).abs() <= step * (0.5 + 1e-3)).all()
     assert _cabi.device_status() == 0
+
+
+@pytest.mark.parametrize("eps", [1e-18, 1e-9, 1e-3, 1.0, 1e6, 1e11, 1e13, 9e17])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("norm", ["l2", "rms"])
+def test_any_eps(eps, dtype, norm):
+    """norms around eps, wherever it lies, with a factor for the row and for its elements"""
+    rot = Rotary(64)
+    g = torch.Generator().manual_seed(4)
+    sizes = torch.logspace(-3, 3, 25, dtype=torch.float64).view(-1, 1, 1) * (eps if norm == "l2" else eps ** 0.5) / 8
+    sizes[7] = 0.0
+    most = 6e4 if dtype == torch.float16 else MOST
+    q = (torch.randn((25, 3, 64), generator=g, dtype=torch.float64) * sizes).clamp(-most, most).to(dtype).to(DEV)
+    pos = torch.arange(25, dtype=torch.int32)
+    per_head, per_dim = torch.rand((3, 1), generator=g) + 0.5, torch.rand(64, generator=g) + 0.5
+    for weight in (None, per_head, per_dim):
+        out, _ = rot.rotate(q, q, pos.to(DEV), norm=norm, eps=eps, q_weight=None if weight is None else weight.to(DEV), dtype=torch.float32)
+        check(rot, q, out, pos.view(1, -1), norm, weight, eps)

@@ -18,6 +18,7 @@
 // pairs of fp32 in one instruction 53 / 111; rows copied ahead 46 / 109; a loop for each of q, k and v, with addresses by steps 46 / 89; registers for two blocks
 // on an SM instead of three where rows are quantized 46 / 82; two conversions in an instruction, one factor for a row 45 / 82; blocks of 128 threads 45 / 80.  fp32 rows, whose pieces such
 // copies would take half a sector at a time, are held one ahead: 36.9 us for 8192 tokens of 16 + 4 heads, 44 with copies.
+#include <cstring>
 #include <type_traits>
 
 #include "varq_paged_rows.cuh"
@@ -33,6 +34,7 @@ struct RotArgs {
     int pos_bytes, n_axes, R, inter;
     long long ps_a, ps_b, ps_l;
     int norm; float inv_eps, least, sum_mul, sum_add;      // 1 / sqrt(sum * sum_mul + sum_add), or inv_eps where that sum is less than `least`
+    uint32_t fair, fair_span;         // sums of squares of ordinary rows: from 2^-80 and `least` to 2^80 (bits of the first, how far to the last)
     const float *qw, *kw; long long qw_h, qw_d, kw_h, kw_d; int qw_vec, kw_vec;
     const void *q, *k, *v; long long qs_b, qs_l, qs_h, ks_b, ks_l, ks_h, vs_l, vs_h;
     void *qo, *ko; long long qo_b, qo_l, qo_h, ko_b, ko_l, ko_h;
@@ -274,11 +276,11 @@ __global__ void __launch_bounds__(ROT_THREADS<PAGED>, PAGED ? 4 : sizeof(T) == 4
                         return sum;
                     };
                     float sum = squares();
-                    // Rows whose norm lies outside of 2^-40 .. 2^40 (and rows that are no numbers; in all lanes of a row) are divided by it here, in front of their factors, whose
-                    // products with the elements alone may be subnormal or infinite.  Squares that leave fp32 (norms from 2^64 on): of the row times 2^-68 they sum up to 2^127
-                    // at most, and eps is nothing next to them.  fp16 has no such rows but zeros.  (Every row divided in front of its factors: registers, and up to 17 % of the
-                    // time.  The test costs bf16, first case above, 44.9 -> 45.8 us, last one 83.3 -> 85.9)
-                    if (!std::is_same<T, __half>::value && __float_as_uint(sum) - __float_as_uint(0x1p-80f) > __float_as_uint(0x1p80f) - __float_as_uint(0x1p-80f)) {
+                    // Rows whose norm lies outside of 2^-40 .. 2^40 or below eps (and rows that are no numbers; in all lanes of a row) are divided by it here, in front of their
+                    // factors, whose products with the elements alone may be subnormal or infinite.  Squares that leave fp32 (norms from 2^64 on): of the row times 2^-68 they
+                    // sum up to 2^127 at most, and eps is nothing next to them.  fp16 has no such rows but zeros.  (Every row divided in front of its factors: registers, and
+                    // up to 17 % of the time.  The test costs bf16, first case above, 45.2 -> 45.7 us, last one 83.5 -> 85.2)
+                    if (!std::is_same<T, __half>::value && __float_as_uint(sum) - a.fair > a.fair_span) {
                         const bool far = sum == INFINITY;
                         auto scale = [&](float f) {
                             const f32x2 ff = pack2(f, f);
@@ -289,8 +291,8 @@ __global__ void __launch_bounds__(ROT_THREADS<PAGED>, PAGED ? 4 : sizeof(T) == 4
                         sum = fmaf(sum, a.sum_mul, far ? 0.f : a.sum_add);
                         scale(sum < a.least && !far ? a.inv_eps : rsqrt_normal(sum));
                     } else {
-                        sum = fmaf(sum, a.sum_mul, a.sum_add);     // 0 becomes 0 / eps
-                        factor = sum < a.least ? a.inv_eps : rsqrt_normal(sum);
+                        sum = fmaf(sum, a.sum_mul, a.sum_add);
+                        factor = std::is_same<T, __half>::value && sum < a.least ? a.inv_eps : rsqrt_normal(sum);      // (fp16: 0 becomes 0 / eps)
                     }
                 }
                 if (weights == 1) factor *= __ldg(w + (h - row0) * wh);
@@ -360,6 +362,10 @@ int rotary_args(const char* who, RotArgs& a, const varq_rotary_t* r, int q_heads
     a.norm = r->norm;
     a.inv_eps = 1.f / r->eps; a.least = r->norm == VARQ_NORM_L2 ? r->eps * r->eps : -1.f;
     a.sum_mul = r->norm == VARQ_NORM_L2 ? 1.f : 1.f / (float)D; a.sum_add = r->norm == VARQ_NORM_L2 ? 0.f : r->eps;
+    const float fair = a.least > 0x1p-80f ? a.least : 0x1p-80f, most = fair > 0x1p80f ? fair : 0x1p80f;
+    memcpy(&a.fair, &fair, 4);
+    memcpy(&a.fair_span, &most, 4);
+    a.fair_span -= a.fair;
     a.half = FastDiv((uint32_t)r->rotary_dim / 2);
     a.qw = r->q_weight; a.qw_h = r->q_weight_stride_h; a.qw_d = r->q_weight_stride_d;
     a.kw = r->k_weight; a.kw_h = r->k_weight_stride_h; a.kw_d = r->k_weight_stride_d;

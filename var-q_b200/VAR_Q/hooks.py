@@ -158,8 +158,14 @@ LayerKV.step_normalised = _step_normalised
 def _step_rotated(self, q, k, v, rotary: Rotary, positions, softmax_scale, out_dtype=None, norm='l2', q_weight=None, k_weight=None, eps=None):
     """``LayerKV.step`` behind the norms and the rotation by position of q and k, as Infinity has them (cosine attention and two-axis positions,
     Infinity/infinity/models/basic.py:316-326): one kernel for both, which leaves them in fp32 as the reference does, in front of quantize, append and attention.
-    ``positions``, ``norm`` and the weights as in ``Rotary.rotate``; ``q_weight`` ``[heads, 1]`` holds the learnt factor of each head."""
+    ``positions``, ``norm`` and the weights as in ``Rotary.rotate``; ``q_weight`` ``[heads, 1]`` holds the learnt factor of each head, or in the module's own
+    shape and type, four dimensions of which the others are 1 (``scale_mul_1H11``)."""
     bhlc = self.k_quant.qkv_format != 'BLHc'
+    if q_weight is not None and q_weight.dim() == 4:
+        heads = q.size(1 if bhlc else 2)
+        if q_weight.numel() != heads or max(q_weight.shape) != heads:
+            raise ValueError(f"[VAR-Q]: q_weight must hold one factor per head ({heads}), got {tuple(q_weight.shape)}")
+        q_weight = q_weight.detach().float().reshape(heads, 1)
     if bhlc:
         q, k = q.transpose(1, 2), k.transpose(1, 2)
     q, k = rotary.rotate(q, k, positions, norm=norm, q_weight=q_weight, k_weight=k_weight, eps=eps, dtype=torch.float32)

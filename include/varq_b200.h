@@ -327,9 +327,9 @@ int varq_paged_attn_tree(const varq_paged_t* cache, const varq_paged_batch_t* ba
  * What happens to queries and keys in front of a cache: a norm per head and the rotation by position, in one pass.
  *   x <- x / max(|x|_2, eps) (L2), x / sqrt(mean x^2 + eps) (RMS) or x (eps: 1e-18 to 1e18);  x <- x * weight[h][d];
  *   (a, b) <- (a cos t - b sin t, b cos t + a sin t), t = 2 pi * positions[axis of the pair] * turns of the pair
- * in fp32.  Pair i of rotary_dim / 2 is the elements (2i, 2i + 1) (interleaved) or (i, i + rotary_dim / 2); elements from rotary_dim on are not turned.
- *   turns : round(2^64 * frequency / (2 pi)), the frequency in radians per position; angles are right to 2^-32 turns up to positions of 2^33, to position * 2^-65 turns
- *           behind, and rounded once, to fp32 (2^-26 turns)
+ * in fp32, finite rows of any size by the formula.  Pair i of rotary_dim / 2 is the elements (2i, 2i + 1) (interleaved) or (i, i + rotary_dim / 2); elements from rotary_dim on are not turned.
+ *   turns : round(2^64 * frequency / (2 pi)), the frequency in radians per position; an angle is off by less than position * 2^-65 + 2^-32 turns, and is then rounded
+ *           once, to fp32 (2^-26 turns)
  *   axis  : which of the n_axes positions a pair goes by; positions[axis * pos_stride_axis + b * pos_stride_b + l * pos_stride_l], int32 or int64
  *   weights : fp32 at [h * stride_h + d * stride_d] (a stride of 0 shares them), or NULL
  * (Infinity/infinity/models/basic.py:316-326: cosine attention and two-axis positions in front of the quantizer.) */

@@ -111,7 +111,7 @@ class PagedCache:
 
 
 def draft_tree(parents: torch.Tensor, kv_lens: torch.Tensor, q_starts: torch.Tensor, max_q: int) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Masks ``[tokens, ceil(max_q / 32)]`` for ``attend(tree=...)`` and positions ``[tokens]`` of drafted tokens, both int32.
+    """Masks ``[tokens, ceil(max_q / 32)]`` (of no more than ``tokens`` bits a row) for ``attend(tree=...)`` and positions ``[tokens]`` of drafted tokens, both int32.
 
     ``parents`` (int32 ``[tokens]``): the number of a token's parent among the drafted tokens of its sequence, smaller than its own, or -1 for a child of the
     sequence's last token before them.  ``kv_lens``, ``q_starts``, ``max_q`` as for ``attend``.  A mask has the bits of a token's ancestors and its own;

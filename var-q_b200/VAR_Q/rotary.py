@@ -41,7 +41,7 @@ class Rotary:
     Frequencies: ``base ** (-2i / rotary_dim)`` for pair i; with ``restart`` a section of n pairs has ``base ** (-2j / 2n)`` for its pair j, as if it were
     a rotary embedding of its own; or ``frequencies``, one for every pair.
 
-    A frequency is held as a 64-bit fraction of a turn: angles are right to 2^-32 turns for positions up to 2^33 (to position * 2^-65 turns behind them), and rounded once, to
+    A frequency (a double, ``frequencies``) is held as a 64-bit fraction of a turn: an angle is off by less than position * 2^-65 + 2^-32 turns, and is then rounded once, to
     fp32 (2^-26 turns), for sine and cosine."""
 
     def __init__(self, head_dim: int, base: float = 10000.0, sections: Optional[Sequence[int]] = None, interleaved: bool = False, restart: bool = False,

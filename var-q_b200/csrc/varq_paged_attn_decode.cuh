@@ -20,7 +20,8 @@
 // in which it has warps: four of them, each a chain of products, exponentials and unpacking.  Lengths that differ and parts cut by the longest leave an SM without warps for
 // another 6 % of the time.  One sequence of 1000 keys, 8 heads: 6.1 us, a chain of latencies (launch, lengths, pages, rows, two products, the cluster's merge).  Four tokens
 // over a window of 1024 (20 rows of a head) on 24 sequences: 26 us.  (Queries loaded and converted piece by piece in front of the first tile's copies, weights of a row's parts made for
-// every element: 7.4 and 30.)  With rows straight from the pages into registers, a tile ahead, instead of the ring: 290 us.
+// every element: 7.4 and 30.)  All queries asked for at once cost the form of 16 rows at 128 columns up to 76 bytes of spills where it had up to 40, and no time: 16 rows
+// of a head, 8 bits, 1 sequence of 1000 keys 11.1 -> 8.2 us, 24 of 500 to 3000 47.3 -> 41.5, 64 of 2000 to 8000 185 -> 165.  With rows straight from the pages into registers, a tile ahead, instead of the ring: 290 us.
 //
 // TREE: queries that are drafted tokens see, of one another, what their rows of bits say; in its own instantiations, the other kernels' registers being as full as they can be.
 // A tree of 16 over 1000 keys, 4 query heads to each of 8: 11.1 us; drafts of 1 to 32 on 24 sequences of up to 3000 keys, 12 heads x 64, 4 and 2 bits: 34 us: issue in 59 % of the

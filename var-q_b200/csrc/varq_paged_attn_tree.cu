@@ -12,7 +12,8 @@
 // What bounds it (B200): the softmax warps' chain, 2500 cycles for a tile of 64 keys (450 instructions; its 64 exponentials take 512 of them), which two warps on a scheduler
 // do not fill, and about 15000 cycles of a CTA around its tiles (lengths, queries, the first tile's copies and conversion, the output).  32 sequences, drafts of 64, 2000 to 8000
 // keys, 32 query / 8 cache heads x 128, 8 bits: 223 us, 765 TFLOP/s (102 us at the dense rate, 58 by bytes); the chunk kernel with masks looked up by each thread took 304.
-// Drafts of 26 of 16 sequences, window 1024, groups of five heads: 40 us (52); drafts of 32 (one tile of rows), 16 sequences of 1000 to 4000 keys: 63 us (78).
+// Drafts of 26 of 16 sequences, window 1024, groups of five heads: 40 us (52); drafts of 32 (one tile of rows), 16 sequences of 1000 to 4000 keys: 63 us (78).  (Times of replayed
+// graphs, without the masks' launch.  Called one by one, the masks among them, the first takes 236 to 250 us, 683 TFLOP/s, the second 42.)
 // On the way (us for the first and the second): two groups over one tile of rows, bits by lane 256 / 48; the form with masks a loop 233 / 43; queries by a thread per row
 // through their own places in shared memory 224 / 40 (by registers and shuffles 11000 cycles of a CTA, so 6000).  Turned down: equal pieces of all sequences' tiles
 // for 148 CTAs that stay, whatever the lengths, 283 / 81: the parts' store and merge and the list of a CTA's items cost more than the last wave; both chunks' scores first,

@@ -5,19 +5,21 @@
 //
 // for pairs (a, b) of neighbours or of elements half the rotary dimension apart, t = position on the pair's axis times its frequency.
 // Angles: a frequency is held as turns per position, a fraction of 64 bits; position times that, modulo 2^64, is the angle in turns with an error of
-// position * 2^-65 turns (a product in fp32 is off by whole radians from 10^7 on).  Its upper 32 bits, rounded to fp32 (2^-26 turns), go to sincospi.  Everything
-// behind is fp32, rounded once to the output's type, or to the code of the cache.
+// position * 2^-65 turns (a product in fp32 is off by whole radians from 10^7 on).  Its upper 32 bits (2^-32 turns more), rounded to fp32 (2^-26 turns), go to sincospi.
+// Everything behind is fp32, rounded once to the output's type, or to the code of the cache.
 //
 // D / 16 neighbouring lanes hold a row with two pieces of eight values each, chosen so that both values of a pair are in one lane.  The lanes of a
 // token share its angles, which the block computes once for all heads.  The next rows' pieces are on their way to shared memory (cp.async), three ahead, which keeps enough
 // bytes in flight without registers for them.
 //
-// What bounds it (B200): its bytes, as long as it only turns.  16384 tokens of 16 + 16 heads x 128, bf16, L2 norm: 268 MB in 45 us, 5.9 TB/s (41 us at the copy rate).  In front
-// of a cache issue: 16384 tokens of 32 + 8 + 8 heads, K in 8 bits, V in 4: 80 us, 55 by its bytes; some 260 instructions for a row and warp, where the quantized rows
-// take twice those of a query's.  A few tokens: a launch, 3.5 us for 16.  On the way (first case / last one): values one by one in registers, one row ahead 72 / 111 us;
-// pairs of fp32 in one instruction 53 / 111; rows copied ahead 46 / 109; a loop for each of q, k and v, with addresses by steps 46 / 89; registers for two blocks
-// on an SM instead of three where rows are quantized 46 / 82; two conversions in an instruction, one factor for a row 45 / 82; blocks of 128 threads 45 / 80.  fp32 rows, whose pieces such
-// copies would take half a sector at a time, are held one ahead: 36.9 us for 8192 tokens of 16 + 4 heads, 44 with copies.
+// What bounds it (B200): its bytes, as long as it only turns.  16384 tokens of 16 + 16 heads x 128, bf16, L2 norm: 268 MB in 46 us, 5.8 TB/s (41 us at the copy rate).  In front
+// of a cache no unit is full (issue 58 %, DRAM 46 %, 16 warps on an SM): 16384 tokens of 32 + 8 + 8 heads, K in 8 bits, V in 4: 82 us, 55 by its bytes; some 260 instructions
+// of a warp for its four rows, where quantized rows take twice those of a query's.  A few tokens: a launch, 3.5 us for 16.  16 bits to fp32 (the first case, in front of an image
+// schedule): 403 MB in 74 us, 61 at the copy rate; its 80 registers spill.
+// On the way (first case / append; without the test for rows of extreme sizes): values one by one in registers, one row ahead 72 / 111 us; pairs of fp32 in one instruction
+// 53 / 111; rows copied ahead 46 / 109; a loop for each of q, k and v, with addresses by steps 46 / 89; registers for two blocks on an SM instead of three where rows are
+// quantized 46 / 82; two conversions in an instruction, one factor for a row 45 / 82; blocks of 128 threads 45 / 80.  fp32 rows, whose pieces such copies would take half a
+// sector at a time, are held one ahead: 34.8 us for 8192 tokens of 16 + 4 heads (25.6 by its bytes), 44 with copies.
 #include <cstring>
 #include <type_traits>
 
